@@ -41,8 +41,12 @@ typedef enum sa2_status {
     SA2_ERR_LAUNCH_FAILED = -7,  /* hipGetLastError() after a launch */
     SA2_ERR_UNSUPPORTED = -8,    /* a forced kernel path does not support the shape/dtype */
     SA2_ERR_TOO_LARGE = -9,      /* an index would overflow the kernels' 32-bit grid */
-    SA2_ERR_STATIC_WORKSPACE = -10 /* sa2_backward_static_workspace: the problem does not fit
+    SA2_ERR_STATIC_WORKSPACE = -10, /* sa2_backward_static_workspace: the problem does not fit
                                       SA2_STATIC_WORKSPACE_BYTES, or the array's address is unavailable */
+    SA2_ERR_BAD_HEADS = -11,     /* query heads are not a multiple of the heads of keys and values */
+    SA2_ERR_BAD_ROTARY = -12,    /* rotary_dim is odd, < 2 or > D, or positions are neither 4 nor 8 bytes */
+    SA2_ERR_BAD_CACHE = -13,     /* page size, page count or table width < 1 */
+    SA2_ERR_BAD_TREE = -14       /* a tree of fewer than 1 or more than SA2_TREE_NODES nodes */
 } sa2_status;
 
 typedef enum sa2_dtype { SA2_F32 = 0, SA2_BF16 = 1, SA2_F16 = 2 } sa2_dtype;
@@ -169,6 +173,49 @@ int sa2_backward_static_workspace(const void* q, const void* k1, const void* k2,
  */
 int sa2_rowdot(const void* out, const void* dout, float* dsum,
                int B, int N, int H, int D, const int64_t* strides, int dtype, void* hip_stream);
+
+/* ======================================================================================================
+ * Ordinary attention layers, as they stand between 2-simplicial ones.  The rules above hold for these too.
+ * H query heads share HK heads of keys and values (H a multiple of HK; query head h reads head h / (H/HK)).
+ *
+ * Rows come as [B, N, heads, D] (cu_seqlens NULL), or packed: B = 1, N rows of `sequences` sequences one behind
+ * the other, sequence s in rows cu_seqlens[s] .. cu_seqlens[s+1]-1 (int32, DEVICE memory, sequences + 1
+ * non-decreasing entries between 0 and N).  Sequences may be empty.  Rows that belong to no sequence are described at each call.
+ */
+
+/*
+ * Rotary positions: q_out = a R(p f) q, and the same for k (NULL, with HK 0: q alone).
+ *   frequencies  [rotary_dim / 2] float64 (DEVICE), radians per position; pair j turns by position * frequencies[j]
+ *   positions    [B,N] int32 (position_bytes 4) or int64 (8), DEVICE, or NULL: a row's place in its sequence
+ *                (0 for a row of no sequence); any value is valid
+ *   interleaved  1: pair j is columns 2j and 2j+1; 0: columns j and j + rotary_dim/2.  Columns from rotary_dim on
+ *                are copied.
+ *   amplitude    a, on the rotated columns
+ *   inverse      1: turns by the opposite angle, which is the gradient of the same call with 0
+ *   strides      q, k, q_out, k_out (3 int64 each, HOST); outputs must not overlap inputs
+ */
+int sa2_rotary(const void* q, const void* k, void* q_out, void* k_out, const double* frequencies,
+               const void* positions, int position_bytes, const int32_t* cu_seqlens, int sequences,
+               int B, int N, int H, int HK, int D, int rotary_dim, const int64_t* strides,
+               float amplitude, int interleaved, int inverse, int dtype, void* hip_stream);
+
+/*
+ * New rows of keys and values into a cache of `pages` pieces of `page_size` rows ([pages, page_size, HK, D]).
+ *   page_table  [sequences, table_width] int32 (DEVICE): row r of sequence b lies in page page_table[b][r / page_size]
+ *               at r % page_size; NULL: in page b at r (a cache [sequences, capacity, HK, D])
+ *   lengths     [sequences] int32 (DEVICE): rows that the cache holds already; new row a goes to lengths[b] + a.
+ *               Not changed by the call.
+ *   k, v        [B,N,HK,D], or packed with cu_seqlens
+ *   rows        [B, nrows] int32 (DEVICE) or NULL, not with cu_seqlens: element a names the row of the sequence's N
+ *               that goes to lengths[b] + a; elements outside 0 .. N-1 are left out
+ *   strides     k, v, k_cache, v_cache (batch or page, row, head; HOST)
+ * A row is left out where its place lies beyond the table, or its page is not in 0 .. pages-1.  Places that two rows
+ * of one call share (a page listed twice) hold either.
+ */
+int sa2_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* lengths,
+                     const int32_t* page_table, const int32_t* rows, int nrows,
+                     const int32_t* cu_seqlens, int sequences, int B, int N, int HK, int D,
+                     int page_size, int pages, int table_width, const int64_t* strides, int dtype, void* hip_stream);
 
 #ifdef __cplusplus
 }

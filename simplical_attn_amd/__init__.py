@@ -12,6 +12,7 @@ from .simplicial_attn import (  # noqa: F401
 )
 
 from .compiled_op import two_simplicial_attention  # noqa: F401,E402
+from .layer_ops import cache_append, rotary_embedding, rotary_frequencies  # noqa: F401,E402
 
 __all__ = [
     "two_simplicial_attention",
@@ -23,6 +24,9 @@ __all__ = [
     "simplicial_forward",
     "simplicial_backward",
     "simplicial_rowdot",
+    "rotary_embedding",
+    "rotary_frequencies",
+    "cache_append",
 ]
 
 # Names the reference package exports (simplicial/__init__.py:12-27) that have no

@@ -3,7 +3,7 @@
     python -m simplical_attn_amd.build        # compile every source, link libsa2_hip.so and _sa2_torch.so
 
 One object per .hip file (hipcc for gfx950, compiled in parallel), linked into
-simplical_attn_amd/lib/libsa2_hip.so, and csrc/host/sa2_torch.cpp (host code against torch's C++ API) into
+simplical_attn_amd/lib/libsa2_hip.so, and csrc/host/*.cpp (host code against torch's C++ API) into
 simplical_attn_amd/lib/_sa2_torch.so.  Cross-compiles without a GPU.
 """
 import concurrent.futures
@@ -20,7 +20,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libsa2_hip.so")
-HOST_SRC = os.path.join(CSRC, "host", "sa2_torch.cpp")
+HOST_SRC = os.path.join(CSRC, "host")
 HOST_PATH = os.path.join(LIB_DIR, "_sa2_torch.so")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 
@@ -70,32 +70,42 @@ def _compile(src, extra):
     return obj, err
 
 
-def _build_host():
-    """The torch extension: no device code, so the host compiler builds it."""
+def _host_object(src):
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
     inc = [x for d in cpp_extension.include_paths("cuda") if os.path.isdir(d) for x in ("-isystem", d)]
-    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    tmp = HOST_PATH + ".tmp"
-    cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+    obj = os.path.join(OBJ_DIR, os.path.basename(src) + ".o")
+    cmd = ["g++", "-O2", "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            "-DTORCH_EXTENSION_NAME=_sa2_torch", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi()),
-           "-I", os.path.join(ROOT, "include"), *inc, "-isystem", sysconfig.get_paths()["include"], HOST_SRC, "-o", tmp,
-           "-L", lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+           "-I", os.path.join(ROOT, "include"), *inc, "-isystem", sysconfig.get_paths()["include"], "-c", src, "-o", obj]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError("building the host extension failed:\n" + res.stderr)
+        raise RuntimeError("building the host extension failed on %s:\n%s" % (src, res.stderr))
+    return obj
+
+
+def _link_host(objs):
+    """The torch extension: no device code, so the host compiler builds it."""
+    import torch
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = HOST_PATH + ".tmp"
+    res = subprocess.run(["g++", "-shared", *objs, "-o", tmp, "-L", lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python"],
+                         capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("linking the host extension failed:\n" + res.stderr)
     os.replace(tmp, HOST_PATH)
 
 
 def build_library(verbose=True, extra_flags=()):
     os.makedirs(OBJ_DIR, exist_ok=True)
     sources = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(sources) + 1)) as ex:
-        host = ex.submit(_build_host)
+    host_sources = sorted(glob.glob(os.path.join(HOST_SRC, "*.cpp")))
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(sources) + len(host_sources))) as ex:
+        host = [ex.submit(_host_object, s) for s in host_sources]
         results = list(ex.map(lambda s: _compile(s, list(extra_flags)), sources))
-        host.result()
+        _link_host([h.result() for h in host])
     for (obj, err), src in zip(results, sources):
         if verbose and err.strip():
             print("[%s]\n%s" % (os.path.basename(src), err), file=sys.stderr)

@@ -16,11 +16,13 @@
 #include <cmath>
 #include <optional>
 
-#include "sa2.h"
+#include "sa2_torch.h"
+
+decltype(&sa2_strerror) sa2_host::err_fn = nullptr;
 
 namespace {
 
-using at::Tensor;
+using namespace sa2_host;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -28,16 +30,6 @@ decltype(&sa2_forward_ws) fwd_fn = nullptr;
 decltype(&sa2_fwd_workspace_bytes) fwd_ws_fn = nullptr;
 decltype(&sa2_backward) bwd_fn = nullptr;
 decltype(&sa2_bwd_workspace_bytes) ws_fn = nullptr;
-decltype(&sa2_strerror) err_fn = nullptr;
-
-// A negative status of the C ABI; becomes simplical_attn_amd._lib.Sa2Error in Python
-struct Status : std::runtime_error {
-    int code;
-    explicit Status(int c) : std::runtime_error("sa2 error " + std::to_string(c) + ": " + err_fn(c)), code(c) {}
-};
-void check(int rc) {
-    if (rc != 0) throw Status(rc);
-}
 
 struct Args {
     int64_t w1, w2;
@@ -46,14 +38,6 @@ struct Args {
     unsigned flags;
 };
 
-int dtype_code(const Tensor& t) {
-    switch (t.scalar_type()) {
-        case at::kFloat: return SA2_F32;
-        case at::kBFloat16: return SA2_BF16;
-        case at::kHalf: return SA2_F16;
-        default: return -1;
-    }
-}
 bool same(const Tensor& t, const Tensor& q) {
     return t.defined() && t.scalar_type() == q.scalar_type() && t.sizes() == q.sizes() && t.device() == q.device();
 }
@@ -167,8 +151,6 @@ void refuse_inputs(const Tensor& q, const Tensor& k1, const Tensor& k2, const Te
 //    the allocation of the output only, and a replay would return uninitialised memory);
 //  - tensors of torch.func transforms and other wrappers, and active dispatch modes.
 PyObject* general_py = nullptr;
-bool plain(const Tensor& t) { return !t._fw_grad(0).defined() && !at::isTensorSubclassLike(t); }
-
 Tensor attention(const Tensor& q, const Tensor& k1, const Tensor& k2, const Tensor& v1, const Tensor& v2, int64_t w1, int64_t w2,
                  std::optional<double> scale, double k2_bias, double v2_bias, bool inclusive, unsigned flags) {
     if (!inputs_ok(q, k1, k2, v1, v2)) refuse_inputs(q, k1, k2, v1, v2);
@@ -241,4 +223,5 @@ PYBIND11_MODULE(_sa2_torch, m) {
     m.def("attention", &attention);
     m.def("forward", &forward);
     m.def("backward", &backward);
+    sa2_host::define_layers(m);
 }

@@ -1,0 +1,220 @@
+// Host path of the operators of ordinary attention layers (rotary positions, causal attention over prompts, rows of a
+// cache, drafted trees): checks, outputs, workspaces, the calls of the C ABI and the autograd formulas.
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+
+#include <cmath>
+#include <optional>
+
+#include "sa2_torch.h"
+
+namespace sa2_host {
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> Maybe;
+
+decltype(&sa2_rotary) rotary_fn = nullptr;
+decltype(&sa2_cache_append) append_fn = nullptr;
+
+// ---- checks ----------------------------------------------------------------------------------------------------------
+// The first tensor of a call: [batch, rows, heads, head_dim], or packed [rows, heads, head_dim]
+void check_first(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.dim() == 4 || t.dim() == 3, name, ": expected [batch, seq_len, heads, head_dim] or packed [rows, heads, head_dim], got ", t.sizes());
+    TORCH_CHECK_TYPE(dtype_code(t) >= 0, name, ": unsupported dtype ", t.scalar_type(), " (float32, bfloat16, float16)");
+}
+// One that goes with it: same leading sizes, head_dim, dtype and device
+void check_beside(const Tensor& t, const char* name, const Tensor& q, const char* first) {
+    TORCH_CHECK_VALUE(t.dim() == q.dim() && t.size(-1) == q.size(-1) && t.size(0) == q.size(0) && (q.dim() == 3 || t.size(1) == q.size(1)), name, ": ",
+                      t.sizes(), " does not go with ", first, " ", q.sizes());
+    TORCH_CHECK_VALUE(t.scalar_type() == q.scalar_type() && t.device() == q.device(), name, " must match ", first, " in dtype and device");
+}
+void check_heads(const Tensor& q, const Tensor& k) {
+    TORCH_CHECK_VALUE(k.size(-2) >= 1 && q.size(-2) % k.size(-2) == 0, "the ", q.size(-2), " query heads are not a multiple of the ", k.size(-2), " heads of keys and values");
+}
+void check_ints(const Maybe& t, const char* name, const Tensor& q, int64_t dim) {
+    if (!t) return;
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == dim, name, " must be an int32 tensor of ", dim, " dimension(s), got ", t->scalar_type(), " ", t->sizes());
+    TORCH_CHECK_VALUE(t->device() == q.device(), name, " must be on the device of the other tensors");
+}
+void check_cu(const Maybe& cu, const Tensor& q) {
+    check_ints(cu, "cu_seqlens", q, 1);
+    TORCH_CHECK_VALUE(!cu || (q.dim() == 3 && cu->numel() >= 2), "cu_seqlens needs packed [rows, heads, head_dim] tensors and at least two entries");
+}
+void check_place(const char* op, std::initializer_list<Tensor> ts) {
+    for (const Tensor& t : ts) {
+        TORCH_CHECK(t.is_cuda(), op, " runs on the GPU only; got a ", t.device(), " tensor");
+        TORCH_CHECK(plain(t), op, " takes plain tensors: no forward-mode derivatives, torch.func transforms or tensor subclasses");
+    }
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), op, " cannot be recorded by torch.jit.trace");
+}
+
+// ---- tensors as the C ABI takes them -----------------------------------------------------------------------------------
+// Unit stride along head_dim and positive strides on every axis longer than 1; anything else is copied
+bool strided(const Tensor& t) {
+    bool ok = t.stride(-1) == 1 || t.size(-1) == 1;
+    for (int64_t a = 0; a + 1 < t.dim(); ++a) ok = ok && (t.stride(a) > 0 || t.size(a) == 1);
+    return ok;
+}
+Tensor rows(const Tensor& t) { return strided(t) ? t : t.contiguous(); }
+void put_strides(int64_t* s, const Tensor& t) {
+    const bool batched = t.dim() == 4;
+    s[0] = batched ? t.stride(0) : 0;
+    s[1] = t.stride(batched ? 1 : 0);
+    s[2] = t.stride(batched ? 2 : 1);
+}
+struct Sizes {
+    int B, N, H, D;
+};
+Sizes sizes(const Tensor& t) {
+    const bool batched = t.dim() == 4;
+    TORCH_CHECK_VALUE(t.numel() <= (int64_t)1 << 40 && t.size(0) < ((int64_t)1 << 31) && t.size(1) < ((int64_t)1 << 31) && t.size(-2) < ((int64_t)1 << 31), "sizes beyond 2^31: ", t.sizes());
+    return {batched ? (int)t.size(0) : 1, (int)t.size(batched ? 1 : 0), (int)t.size(-2), (int)t.size(-1)};
+}
+Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous)); }
+void* stream(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+const int32_t* ints(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
+Tensor dense(const Maybe& t) { return t ? t->contiguous() : Tensor(); }
+
+// ---- rotary ----------------------------------------------------------------------------------------------------------
+struct Angles {
+    Tensor frequencies, positions, cu;         // the last two may be undefined
+    double amplitude;
+    bool interleaved;
+};
+
+std::pair<Tensor, Tensor> run_rotary(const Tensor& q_, const Tensor& k_, const Angles& a, bool inverse) {
+    const Tensor q = rows(q_), k = k_.defined() ? rows(k_) : Tensor();
+    const c10::DeviceGuard guard(q.device());
+    Tensor q2 = like(q), k2 = k.defined() ? like(k) : Tensor();
+    const Sizes z = sizes(q);
+    const int hk = k.defined() ? sizes(k).H : 0;
+    if (z.B == 0 || z.N == 0 || z.D == 0 || (z.H == 0 && hk == 0)) return {q2, k2};
+    int64_t s[12] = {};
+    put_strides(s, q);
+    put_strides(s + 6, q2);
+    if (hk) {
+        put_strides(s + 3, k);
+        put_strides(s + 9, k2);
+    }
+    check(rotary_fn(q.const_data_ptr(), hk ? k.const_data_ptr() : nullptr, q2.data_ptr(), hk ? k2.data_ptr() : nullptr, a.frequencies.const_data_ptr<double>(),
+                    a.positions.defined() ? a.positions.const_data_ptr() : nullptr, a.positions.defined() ? (int)a.positions.element_size() : 0, ints(a.cu),
+                    a.cu.defined() ? (int)a.cu.numel() - 1 : 0, z.B, z.N, z.H, hk, z.D, (int)(2 * a.frequencies.numel()), s, (float)a.amplitude, a.interleaved, inverse,
+                    dtype_code(q), stream(q)));
+    return {q2, k2};
+}
+
+struct RotaryFormula : torch::autograd::Function<RotaryFormula> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Maybe& k, Angles a) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({a.frequencies, a.positions, a.cu});
+        ctx->saved_data["amplitude"] = a.amplitude;
+        ctx->saved_data["interleaved"] = a.interleaved;
+        auto [q2, k2] = run_rotary(q, k ? *k : Tensor(), a, false);
+        return k2.defined() ? variable_list{q2, k2} : variable_list{q2};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const auto s = ctx->get_saved_variables();
+        const Angles a{s[0], s[1], s[2], ctx->saved_data["amplitude"].toDouble(), ctx->saved_data["interleaved"].toBool()};
+        Tensor dq = ctx->needs_input_grad(0) ? grads[0] : Tensor(), dk = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
+        if (dq.defined()) std::tie(dq, dk) = run_rotary(dq, dk, a, true);
+        else if (dk.defined()) dk = run_rotary(dk, Tensor(), a, true).first;
+        return {dq, dk, Tensor()};
+    }
+};
+
+std::pair<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& frequencies, const Maybe& positions, const Maybe& cu, bool interleaved, double amplitude) {
+    check_first(q, "q");
+    if (k) check_beside(*k, "k", q, "q");
+    TORCH_CHECK_VALUE(q.size(-1) <= 256, "head_dim ", q.size(-1), " is above 256");
+    TORCH_CHECK_VALUE(frequencies.dim() == 1 && frequencies.scalar_type() == at::kDouble && frequencies.device() == q.device(), "frequencies must be a float64 vector on q's device");
+    TORCH_CHECK_VALUE(frequencies.numel() >= 1 && 2 * frequencies.numel() <= q.size(-1), "frequencies turn ", 2 * frequencies.numel(), " columns, head_dim is ", q.size(-1));
+    TORCH_CHECK_VALUE(!frequencies.requires_grad(), "rotary_embedding has no gradient for frequencies");
+    check_cu(cu, q);
+    if (positions) {
+        TORCH_CHECK_VALUE(!cu, "give positions or cu_seqlens, not both");
+        TORCH_CHECK_VALUE(positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong, "positions must be int32 or int64");
+        TORCH_CHECK_VALUE(positions->sizes() == q.sizes().slice(0, q.dim() - 2) && positions->device() == q.device(), "positions ", positions->sizes(), " must have q's leading sizes and device");
+    }
+    check_place("rotary_embedding", {q});
+    if (k) check_place("rotary_embedding", {*k});
+    const Angles a{frequencies.contiguous(), dense(positions), dense(cu), amplitude, interleaved};
+    py::gil_scoped_release nogil;
+    if (at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()))) {
+        auto r = RotaryFormula::apply(q, k, a);
+        return {r[0], k ? Maybe(r[1]) : Maybe()};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [q2, k2] = run_rotary(q, k ? *k : Tensor(), a, false);
+    return {q2, k ? Maybe(k2) : Maybe()};
+}
+
+// ---- cache -----------------------------------------------------------------------------------------------------------
+// A cache's two tensors and what finds rows in them; `beside` has the rows' heads and head_dim
+struct CacheView {
+    Tensor k, v, lengths, table;
+    int page_size, pages, width;
+};
+CacheView check_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths, const Maybe& table, const Tensor& k, int64_t sequences) {
+    for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(k_cache, "k_cache"), {v_cache, "v_cache"}}) {
+        TORCH_CHECK_VALUE(t.dim() == 4 && t.size(2) == k.size(-2) && t.size(3) == k.size(-1) && t.sizes() == k_cache.sizes(), name,
+                          ": expected [pages, page_size, ", k.size(-2), ", ", k.size(-1), "], got ", t.sizes());
+        TORCH_CHECK_VALUE(t.scalar_type() == k.scalar_type() && t.device() == k.device(), name, " must match k in dtype and device");
+        TORCH_CHECK_VALUE(strided(t), name, " needs unit stride along head_dim and positive strides: it is used in place");
+        TORCH_CHECK_VALUE(t.size(0) >= 1 && t.size(1) >= 1 && t.size(0) < ((int64_t)1 << 31) && t.size(1) < ((int64_t)1 << 31), name, ": a cache needs at least one page of one row, got ", t.sizes());
+    }
+    check_ints(lengths, "lengths", k, 1);
+    TORCH_CHECK_VALUE(lengths.numel() == sequences, "lengths has ", lengths.numel(), " entries for ", sequences, " sequences");
+    check_ints(table, "page_table", k, 2);
+    TORCH_CHECK_VALUE(!table || (table->size(0) == sequences && table->size(1) >= 1), "page_table ", table ? table->sizes() : at::IntArrayRef(), " must be [", sequences, ", pages of a sequence]");
+    if (!table) TORCH_CHECK_VALUE(k_cache.size(0) == sequences, "without a page_table the cache is [sequences, capacity, heads, head_dim]: got ", k_cache.size(0), " pieces for ", sequences, " sequences");
+    return {k_cache, v_cache, lengths.contiguous(), dense(table), (int)k_cache.size(1), (int)k_cache.size(0), table ? (int)table->size(1) : 1};
+}
+
+void append(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths, const Maybe& table, const Maybe& chosen, const Maybe& cu) {
+    check_first(k_, "k");
+    check_beside(v_, "v", k_, "k");
+    TORCH_CHECK_VALUE(k_.size(-2) == v_.size(-2), "k and v differ in heads: ", k_.sizes(), ", ", v_.sizes());
+    TORCH_CHECK_VALUE(k_.size(-1) >= 1 && k_.size(-1) <= 256 && k_.size(-2) >= 1, "heads and head_dim must be at least 1, head_dim at most 256: ", k_.sizes());
+    check_cu(cu, k_);
+    TORCH_CHECK_VALUE(k_.dim() == 4 || cu, "packed rows need cu_seqlens");
+    const int64_t sequences = cu ? cu->numel() - 1 : k_.size(0);
+    check_ints(chosen, "rows", k_, 2);
+    if (chosen) TORCH_CHECK_VALUE(!cu && chosen->size(0) == sequences, "rows must be [batch, any] and go with [batch, seq_len, heads, head_dim] tensors");
+    const CacheView c = check_cache(k_cache, v_cache, lengths, table, k_, sequences);
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (k_.requires_grad() || v_.requires_grad() || k_cache.requires_grad() || v_cache.requires_grad())),
+                "cache_append has no gradient: call it under torch.no_grad() or on detached tensors");
+    check_place("cache_append", {k_, v_, k_cache, v_cache});
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor k = rows(k_), v = rows(v_), pick = dense(chosen), ends = dense(cu);
+    const c10::DeviceGuard guard(k.device());
+    const Sizes z = sizes(k);
+    if (z.B == 0 || z.N == 0 || (pick.defined() && pick.numel() == 0)) return;
+    int64_t s[12];
+    put_strides(s, k);
+    put_strides(s + 3, v);
+    put_strides(s + 6, c.k);
+    put_strides(s + 9, c.v);
+    check(append_fn(k.const_data_ptr(), v.const_data_ptr(), c.k.data_ptr(), c.v.data_ptr(), ints(c.lengths), ints(c.table), ints(pick), pick.defined() ? (int)pick.size(1) : 0, ints(ends),
+                    ends.defined() ? (int)ends.numel() - 1 : 0, z.B, z.N, z.H, z.D, c.page_size, c.pages, c.width, s, dtype_code(k), stream(k)));
+    torch::autograd::impl::bump_version(c.k);
+    torch::autograd::impl::bump_version(c.v);
+}
+
+}  // namespace
+
+void define_layers(py::module_& m) {
+    m.def("bind_layers", [](uintptr_t rotary, uintptr_t append) {
+        rotary_fn = (decltype(rotary_fn))rotary;
+        append_fn = (decltype(append_fn))append;
+    });
+    m.def("rotary", &rotary);
+    m.def("cache_append", &append);
+}
+
+}  // namespace sa2_host

@@ -235,6 +235,10 @@ const char* sa2_strerror(int status) {
         case SA2_ERR_TOO_LARGE: return "problem too large for the kernels' 32-bit grid (B*H*N must be < 2^31)";
         case SA2_ERR_STATIC_WORKSPACE: return "the problem needs more workspace than the library's own SA2_STATIC_WORKSPACE_BYTES, or "
                                               "the address of that array could not be obtained on this device";
+        case SA2_ERR_BAD_HEADS: return "the number of query heads must be a multiple of the number of key heads";
+        case SA2_ERR_BAD_ROTARY: return "rotary_dim must be even and in 2 .. D, positions int32 or int64";
+        case SA2_ERR_BAD_CACHE: return "a cache needs a page size, a page count and a table width of at least 1";
+        case SA2_ERR_BAD_TREE: return "a drafted tree must have 1 to 64 nodes";
     }
     return "unknown sa2 status";
 }

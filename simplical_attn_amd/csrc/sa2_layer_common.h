@@ -1,0 +1,126 @@
+// Shared declarations of the kernels of ordinary attention layers (rotary positions, causal attention over prompts,
+// cache rows, drafted trees).
+#pragma once
+
+#include "sa2_common.h"
+#include "sa2_mfma_common.h"
+
+namespace sa2 {
+
+// Rows of a problem: B sequences of N rows each, or (cu != nullptr) B = 1 and `sequences` packed ones, sequence s in
+// the rows cu[s] .. cu[s+1]-1 of the N.  The bounds lie in device memory: kernels clamp them to 0 .. N.
+struct Rows {
+    int B, N;
+    const int32_t* cu;
+    int sequences;
+};
+
+// One call of causal attention.  H query heads share HK heads of keys and values, G = H / HK neighbours one.
+struct Causal {
+    Rows rows;
+    int H, HK, G, D;
+    float scale;
+    Tensor q, k, v, out, dout, dq, dk, dv;     // gradients with p == nullptr: not requested
+    float* lse;                                // [B,H,N]
+    float* delta;                              // [B,H,N]  sum_d dout*out
+    float* part;                               // partial sums (path specific)
+};
+
+struct Rotary {
+    Rows rows;
+    int H, HK, D, rot;
+    Tensor q, k, q_out, k_out;
+    const double* frequencies;                 // [rot / 2], radians per position
+    const void* positions;                     // [B,N] of position_bytes each, or nullptr: the row's place in its sequence
+    int position_bytes;
+    float amplitude;
+    int interleaved, inverse;
+};
+
+// A cache of keys and values: `pages` pieces of `page_size` rows (sn: from row to row, sb: from page to page).  Row r of
+// sequence b lies in page table[b * width + r / page_size], or without a table in page b.
+struct Cache {
+    Tensor k, v;
+    const int32_t* table;
+    const int32_t* lengths;                    // [B] rows that are there
+    int page_size, pages, width;
+};
+
+struct Append {
+    Cache cache;
+    Rows rows;                                 // of the new rows
+    int HK, D;
+    Tensor k, v;
+    const int32_t* chosen;                     // [B, nchosen] rows of the sequence's N to take, or nullptr: all
+    int nchosen;
+};
+
+struct Tree {
+    Cache cache;
+    int B, T, H, HK, G, D;
+    float scale;
+    Tensor q, k, v, out;
+    const int32_t* parents;                    // [B,T], or nullptr: a chain
+    float* part;                               // partial outputs, see sa2_tree.hip
+    int nsplit;
+};
+
+int launch_rotary(const Rotary& p, int dtype, hipStream_t st);
+int launch_append(const Append& p, int dtype, hipStream_t st);
+
+namespace {
+
+// The memory of V elements as 32-bit floats and back
+template <class T, int V>
+__device__ __forceinline__ void load_floats(const T* p, float (&x)[V]) {
+    if constexpr (V * sizeof(T) == 16 && sizeof(T) == 4) {
+        const float4 u = *(const float4*)p;
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    } else if constexpr (V * sizeof(T) == 16) {
+        union { uint4 u; T e[8]; } w;
+        w.u = *(const uint4*)p;
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = to_float(w.e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = to_float(p[i]);
+    }
+}
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, bf16_t*) { return ElemBF16::pack(a, b); }
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, f16_t*) { return ElemF16::pack(a, b); }
+template <class T, int V>
+__device__ __forceinline__ void store_floats(T* p, const float (&x)[V]) {
+    if constexpr (V * sizeof(T) == 16 && sizeof(T) == 4) {
+        *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+    } else if constexpr (V * sizeof(T) == 16) {
+        *(uint4*)p = make_uint4(pack_pair(x[0], x[1], p), pack_pair(x[2], x[3], p), pack_pair(x[4], x[5], p), pack_pair(x[6], x[7], p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) from_float(x[i], p + i);
+    }
+}
+
+// The sequence of packed row n, -1 where none holds it (cu is non-decreasing)
+__device__ __forceinline__ int sequence_of(const Rows& r, int n) {
+    int lo = 0, hi = r.sequences;                       // cu[lo] <= n < cu[hi], once both are checked
+    if (n < r.cu[0] || n >= r.cu[hi]) return -1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (r.cu[mid] <= n) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// All pointers and strides that a kernel's 16-byte accesses need
+inline bool aligned16(const Tensor& t, int64_t size, bool batched) {
+    return !((uintptr_t)t.p & 15u) && (t.sn * size) % 16 == 0 && (t.sh * size) % 16 == 0 && (!batched || (t.sb * size) % 16 == 0);
+}
+
+template <class F>
+int for_type(int dtype, F&& f) {
+    return dtype == SA2_F32 ? f((float*)nullptr) : dtype == SA2_BF16 ? f((bf16_t*)nullptr) : f((f16_t*)nullptr);
+}
+
+}  // namespace
+}  // namespace sa2

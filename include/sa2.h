@@ -217,6 +217,49 @@ int sa2_cache_append(const void* k, const void* v, void* k_cache, void* v_cache,
                      const int32_t* cu_seqlens, int sequences, int B, int N, int HK, int D,
                      int page_size, int pages, int table_width, const int64_t* strides, int dtype, void* hip_stream);
 
+/*
+ * Causal attention over whole prompts: query i of a sequence attends to its keys 0 .. i.
+ *   S = scale q k^T, out = softmax(S) v, lse = log sum e^S (natural), [B,H,N] fp32 (packed: [H,N])
+ *   strides      q, k, v, out
+ * Rows of no sequence: out 0, lse -infinity.  An infinity or NaN in k or v reaches the queries that attend to it only.
+ * flags: SA2_FLAG_AUTO, or SA2_FLAG_FORCE_GENERIC for the kernels with fp32 products whatever the type.
+ */
+int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, float* lse,
+                       const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                       const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream);
+
+/*
+ * Its gradients: out and lse are what the forward gave for these inputs.  A NULL gradient is not wanted; every other one
+ * is fully overwritten (rows of no sequence: 0).  dk and dv are sums over the query heads that share a head.
+ *   workspace    sa2_causal_bwd_workspace_bytes(...) bytes, 256-byte aligned; contents on entry ignored
+ *   strides      q, k, v, out, dout, dq, dk, dv
+ * No atomics: two calls on the same inputs give identical bits.
+ */
+size_t sa2_causal_bwd_workspace_bytes(int B, int N, int H, int HK, int D, int dtype, unsigned flags);
+int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+                        void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                        const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                        const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream);
+
+/*
+ * T drafted tokens per sequence (1 .. SA2_TREE_NODES; one: a decoding step) over a cache as at sa2_cache_append, which
+ * does not hold them yet.  Node i attends to the cached rows 0 .. lengths[b]-1, to itself and to its ancestors.
+ *   q, out       [B,T,H,D]; k, v [B,T,HK,D]: the drafted tokens'
+ *   parents      [B,T] int32 (DEVICE): the node before it, smaller than its own number, or -1 on the cached rows.  A node
+ *                whose chain does not end at -1 (-2 marks a place that is not used) attends to nothing: its output is 0.
+ *                NULL: a chain, node i behind node i-1.
+ *   lengths      clamped to 0 .. capacity; rows in pages that are not in 0 .. pages-1 are not there
+ *   workspace    sa2_tree_workspace_bytes(...) bytes, 256-byte aligned (0 bytes: may be NULL); contents on entry ignored
+ *   strides      q, k, v, k_cache, v_cache, out
+ */
+#define SA2_TREE_NODES 64
+size_t sa2_tree_workspace_bytes(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype, unsigned flags);
+int sa2_tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out,
+                       const int32_t* parents, const int32_t* lengths, const int32_t* page_table,
+                       void* workspace, size_t workspace_bytes, int B, int T, int H, int HK, int D,
+                       int page_size, int pages, int table_width, const int64_t* strides, float scale,
+                       int dtype, unsigned flags, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,7 +12,15 @@ from .simplicial_attn import (  # noqa: F401
 )
 
 from .compiled_op import two_simplicial_attention  # noqa: F401,E402
-from .layer_ops import cache_append, rotary_embedding, rotary_frequencies  # noqa: F401,E402
+from .layer_ops import (  # noqa: F401,E402
+    cache_append,
+    causal_attention,
+    causal_attention_backward,
+    causal_attention_forward,
+    rotary_embedding,
+    rotary_frequencies,
+    tree_attention,
+)
 
 __all__ = [
     "two_simplicial_attention",
@@ -27,6 +35,10 @@ __all__ = [
     "rotary_embedding",
     "rotary_frequencies",
     "cache_append",
+    "causal_attention",
+    "causal_attention_forward",
+    "causal_attention_backward",
+    "tree_attention",
 ]
 
 # Names the reference package exports (simplicial/__init__.py:12-27) that have no

@@ -10,7 +10,8 @@ LIB_PATH = os.environ.get("SA2_LIBRARY", os.path.join(_PKG, "lib", "libsa2_hip.s
 EXPORTED_SYMBOLS = (
     "sa2_version", "sa2_strerror", "sa2_uses_mfma", "sa2_forward", "sa2_forward_ws", "sa2_fwd_workspace_bytes",
     "sa2_bwd_workspace_bytes", "sa2_backward", "sa2_backward_static_workspace", "sa2_rowdot",
-    "sa2_rotary", "sa2_cache_append",
+    "sa2_rotary", "sa2_cache_append", "sa2_causal_forward", "sa2_causal_bwd_workspace_bytes", "sa2_causal_backward",
+    "sa2_tree_workspace_bytes", "sa2_tree_attention",
 )
 STATIC_WORKSPACE_BYTES = 64 << 20
 
@@ -70,6 +71,16 @@ def load():
     lib.sa2_rotary.argtypes = ([c_void_p] * 6 + [c_int, c_void_p, c_int] + [c_int] * 6 + [i64p, c_float] + [c_int] * 3 + [c_void_p])
     lib.sa2_cache_append.restype = c_int
     lib.sa2_cache_append.argtypes = ([c_void_p] * 7 + [c_int, c_void_p, c_int] + [c_int] * 7 + [i64p, c_int, c_void_p])
+    lib.sa2_causal_forward.restype = c_int
+    lib.sa2_causal_forward.argtypes = [c_void_p] * 6 + [c_int] * 6 + [i64p, c_float, c_int, c_uint, c_void_p]
+    lib.sa2_causal_bwd_workspace_bytes.restype = c_size_t
+    lib.sa2_causal_bwd_workspace_bytes.argtypes = [c_int] * 6 + [c_uint]
+    lib.sa2_causal_backward.restype = c_int
+    lib.sa2_causal_backward.argtypes = ([c_void_p] * 10 + [c_size_t, c_void_p] + [c_int] * 6 + [i64p, c_float, c_int, c_uint, c_void_p])
+    lib.sa2_tree_workspace_bytes.restype = c_size_t
+    lib.sa2_tree_workspace_bytes.argtypes = [c_int] * 8 + [c_uint]
+    lib.sa2_tree_attention.restype = c_int
+    lib.sa2_tree_attention.argtypes = ([c_void_p] * 10 + [c_size_t] + [c_int] * 8 + [i64p, c_float, c_int, c_uint, c_void_p])
     _lib = lib
     return lib
 
@@ -94,7 +105,7 @@ def host():
         module.bind(address(lib.sa2_forward_ws), address(lib.sa2_fwd_workspace_bytes), address(lib.sa2_backward),
                     address(lib.sa2_bwd_workspace_bytes), address(lib.sa2_strerror), simplicial_attn._check_inputs, simplicial_attn._check_saved, Sa2Error,
                     simplicial_attn.TwoSimplicialAttentionFunction.apply)
-        module.bind_layers(address(lib.sa2_rotary), address(lib.sa2_cache_append))
+        module.bind_layers(*[address(getattr(lib, name)) for name in EXPORTED_SYMBOLS[EXPORTED_SYMBOLS.index("sa2_rotary"):]])
         _host = module
     return _host
 

@@ -18,6 +18,11 @@ typedef std::optional<Tensor> Maybe;
 
 decltype(&sa2_rotary) rotary_fn = nullptr;
 decltype(&sa2_cache_append) append_fn = nullptr;
+decltype(&sa2_causal_forward) causal_fwd_fn = nullptr;
+decltype(&sa2_causal_bwd_workspace_bytes) causal_ws_fn = nullptr;
+decltype(&sa2_causal_backward) causal_bwd_fn = nullptr;
+decltype(&sa2_tree_workspace_bytes) tree_ws_fn = nullptr;
+decltype(&sa2_tree_attention) tree_fn = nullptr;
 
 // ---- checks ----------------------------------------------------------------------------------------------------------
 // The first tensor of a call: [batch, rows, heads, head_dim], or packed [rows, heads, head_dim]
@@ -206,15 +211,171 @@ void append(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Ten
     torch::autograd::impl::bump_version(c.v);
 }
 
+// ---- causal attention --------------------------------------------------------------------------------------------------
+struct Prompt {
+    Tensor cu;                                 // may be undefined
+    double scale;
+    unsigned flags;
+};
+Tensor workspace(const Tensor& q, size_t bytes) { return at::empty({(int64_t)bytes}, q.options().dtype(at::kByte).requires_grad(false)); }
+
+std::pair<Tensor, Tensor> run_causal_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Prompt& a) {
+    const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
+    const c10::DeviceGuard guard(q.device());
+    const Sizes z = sizes(q);
+    const auto fp32 = q.options().dtype(at::kFloat).requires_grad(false);
+    Tensor out = like(q), lse = q.dim() == 4 ? at::empty({z.B, z.H, z.N}, fp32) : at::empty({z.H, z.N}, fp32);
+    if (out.numel() == 0) return {out, lse};
+    int64_t s[12];
+    put_strides(s, q);
+    put_strides(s + 3, k);
+    put_strides(s + 6, v);
+    put_strides(s + 9, out);
+    check(causal_fwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(), (float*)lse.data_ptr(), ints(a.cu), a.cu.defined() ? (int)a.cu.numel() - 1 : 0,
+                        z.B, z.N, z.H, (int)k.size(-2), z.D, s, (float)a.scale, dtype_code(q), a.flags, stream(q)));
+    return {out, lse};
+}
+
+// `needs`: bit t set = gradient t of (q, k, v) is wanted; the others stay undefined
+std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& out_, const Tensor& lse, const Tensor& dout_, unsigned needs, const Prompt& a) {
+    const Tensor q = rows(q_), k = rows(k_), v = rows(v_), out = rows(out_), dout = rows(dout_);
+    const c10::DeviceGuard guard(q.device());
+    const Sizes z = sizes(q);
+    const int hk = (int)k.size(-2);
+    std::array<Tensor, 3> g;
+    const Tensor* const of[3] = {&q, &k, &v};
+    for (int i = 0; i < 3; ++i)
+        if (needs >> i & 1) g[i] = like(*of[i]);
+    if (q.numel() == 0) return g;
+    const size_t bytes = causal_ws_fn(z.B, z.N, z.H, hk, z.D, dtype_code(q), a.flags);
+    const Tensor ws = workspace(q, std::max<size_t>(bytes, 256));
+    int64_t s[24];
+    const Tensor* const t[8] = {&q, &k, &v, &out, &dout, g[0].defined() ? &g[0] : &q, g[1].defined() ? &g[1] : &k, g[2].defined() ? &g[2] : &v};
+    for (int i = 0; i < 8; ++i) put_strides(s + 3 * i, *t[i]);
+    auto ptr = [&](int i) { return g[i].defined() ? g[i].data_ptr() : nullptr; };
+    check(causal_bwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.const_data_ptr(), dout.const_data_ptr(), (const float*)lse.const_data_ptr(), ptr(0), ptr(1), ptr(2),
+                        ws.data_ptr(), (size_t)ws.numel(), ints(a.cu), a.cu.defined() ? (int)a.cu.numel() - 1 : 0, z.B, z.N, z.H, hk, z.D, s, (float)a.scale, dtype_code(q), a.flags, stream(q)));
+    return g;
+}
+
+struct CausalFormula : torch::autograd::Function<CausalFormula> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, Prompt a) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [out, lse] = run_causal_forward(q, k, v, a);
+        ctx->save_for_backward({q, k, v, out, lse, a.cu});
+        ctx->saved_data["scale"] = a.scale;
+        ctx->saved_data["flags"] = (int64_t)a.flags;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const auto s = ctx->get_saved_variables();
+        const Prompt a{s[5], ctx->saved_data["scale"].toDouble(), (unsigned)ctx->saved_data["flags"].toInt()};
+        unsigned needs = 0;
+        for (int i = 0; i < 3; ++i) needs |= (ctx->needs_input_grad(i) ? 1u : 0u) << i;
+        auto g = run_causal_backward(s[0], s[1], s[2], s[3], s[4], grads[0], needs, a);
+        return {g[0], g[1], g[2], Tensor()};
+    }
+};
+
+Prompt check_causal(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, const std::optional<double>& scale, unsigned flags) {
+    check_first(q, "q");
+    check_beside(k, "k", q, "q");
+    check_beside(v, "v", q, "q");
+    TORCH_CHECK_VALUE(k.size(-2) == v.size(-2), "k and v differ in heads: ", k.sizes(), ", ", v.sizes());
+    check_heads(q, k);
+    TORCH_CHECK_VALUE(q.size(-1) >= 1 && q.size(-1) <= 256, "head_dim must be 1 to 256, got ", q.size(-1));
+    check_cu(cu, q);
+    TORCH_CHECK_VALUE(q.dim() == 4 || cu, "packed rows need cu_seqlens");
+    check_place("causal_attention", {q, k, v});
+    return {dense(cu), scale ? *scale : 1.0 / std::sqrt((double)q.size(-1)), flags};
+}
+
+Tensor causal(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, std::optional<double> scale, unsigned flags) {
+    const Prompt a = check_causal(q, k, v, cu, scale, flags);
+    py::gil_scoped_release nogil;
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) return CausalFormula::apply(q, k, v, a);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return run_causal_forward(q, k, v, a).first;
+}
+
+std::pair<Tensor, Tensor> causal_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, std::optional<double> scale, unsigned flags) {
+    const Prompt a = check_causal(q, k, v, cu, scale, flags);
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    return run_causal_forward(q, k, v, a);
+}
+
+std::tuple<Maybe, Maybe, Maybe> causal_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse, const Tensor& dout, const Maybe& cu,
+                                                std::optional<double> scale, unsigned needs, unsigned flags) {
+    const Prompt a = check_causal(q, k, v, cu, scale, flags);
+    for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(out, "out"), {dout, "dout"}})
+        TORCH_CHECK_VALUE(t.sizes() == q.sizes() && t.scalar_type() == q.scalar_type() && t.device() == q.device(), name, " must match q in shape, dtype and device");
+    const bool batched = q.dim() == 4;
+    TORCH_CHECK_VALUE(lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.is_contiguous() && lse.dim() == q.dim() - 1 && lse.size(-1) == q.size(-3) && lse.size(-2) == q.size(-2) &&
+                          (!batched || lse.size(0) == q.size(0)), "lse must be the contiguous float32 tensor that the forward returned, got ", lse.scalar_type(), " ", lse.sizes());
+    check_place("causal_attention", {out, lse, dout});
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto g = run_causal_backward(q, k, v, out, lse, dout, needs, a);
+    auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
+    return {maybe(g[0]), maybe(g[1]), maybe(g[2])};
+}
+
+// ---- drafted trees -----------------------------------------------------------------------------------------------------
+Tensor tree(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Maybe& parents, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths, const Maybe& table,
+            std::optional<double> scale, unsigned flags) {
+    TORCH_CHECK_VALUE(q_.dim() == 4, "q: expected [batch, nodes, heads, head_dim], got ", q_.sizes());
+    check_first(q_, "q");
+    check_beside(k_, "k", q_, "q");
+    check_beside(v_, "v", q_, "q");
+    TORCH_CHECK_VALUE(k_.size(-2) == v_.size(-2), "k and v differ in heads: ", k_.sizes(), ", ", v_.sizes());
+    check_heads(q_, k_);
+    TORCH_CHECK_VALUE(q_.size(-1) >= 1 && q_.size(-1) <= 256, "head_dim must be 1 to 256, got ", q_.size(-1));
+    TORCH_CHECK_VALUE(q_.size(1) >= 1 && q_.size(1) <= SA2_TREE_NODES, "a drafted tree has 1 to ", SA2_TREE_NODES, " nodes, got ", q_.size(1));
+    check_ints(parents, "parents", q_, 2);
+    TORCH_CHECK_VALUE(!parents || (parents->size(0) == q_.size(0) && parents->size(1) == q_.size(1)), "parents must be [batch, nodes]");
+    const CacheView c = check_cache(k_cache, v_cache, lengths, table, k_, q_.size(0));
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (q_.requires_grad() || k_.requires_grad() || v_.requires_grad() || k_cache.requires_grad() || v_cache.requires_grad())),
+                "tree_attention has no gradient: call it under torch.no_grad() or on detached tensors");
+    check_place("tree_attention", {q_, k_, v_, k_cache, v_cache});
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor q = rows(q_), k = rows(k_), v = rows(v_), up = dense(parents);
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = like(q);
+    if (out.numel() == 0) return out;
+    const Sizes z = sizes(q);
+    const int hk = (int)k.size(2);
+    const size_t bytes = tree_ws_fn(z.B, z.N, z.H, hk, z.D, c.page_size, c.width, dtype_code(q), flags);
+    const Tensor ws = bytes ? workspace(q, bytes) : Tensor();
+    int64_t s[18];
+    const Tensor* const t[6] = {&q, &k, &v, &c.k, &c.v, &out};
+    for (int i = 0; i < 6; ++i) put_strides(s + 3 * i, *t[i]);
+    check(tree_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), c.k.const_data_ptr(), c.v.const_data_ptr(), out.data_ptr(), ints(up), ints(c.lengths), ints(c.table),
+                  bytes ? ws.data_ptr() : nullptr, bytes, z.B, z.N, z.H, hk, z.D, c.page_size, c.pages, c.width, s, (float)(scale ? *scale : 1.0 / std::sqrt((double)z.D)), dtype_code(q),
+                  flags, stream(q)));
+    return out;
+}
+
 }  // namespace
 
 void define_layers(py::module_& m) {
-    m.def("bind_layers", [](uintptr_t rotary, uintptr_t append) {
+    m.def("bind_layers", [](uintptr_t rotary, uintptr_t append, uintptr_t causal_fwd, uintptr_t causal_ws, uintptr_t causal_bwd, uintptr_t tree_ws, uintptr_t tree) {
         rotary_fn = (decltype(rotary_fn))rotary;
         append_fn = (decltype(append_fn))append;
+        causal_fwd_fn = (decltype(causal_fwd_fn))causal_fwd;
+        causal_ws_fn = (decltype(causal_ws_fn))causal_ws;
+        causal_bwd_fn = (decltype(causal_bwd_fn))causal_bwd;
+        tree_ws_fn = (decltype(tree_ws_fn))tree_ws;
+        tree_fn = (decltype(tree_fn))tree;
     });
     m.def("rotary", &rotary);
     m.def("cache_append", &append);
+    m.def("causal", &causal);
+    m.def("causal_forward", &causal_forward);
+    m.def("causal_backward", &causal_backward);
+    m.def("tree", &tree);
 }
 
 }  // namespace sa2_host

@@ -25,6 +25,33 @@ int check_rows(int B, int N, int H, int D, const int32_t* cu, int sequences, int
     return SA2_OK;
 }
 
+int make_causal(Causal& p, const int32_t* cu, int sequences, int B, int N, int H, int HK, int D, float scale, int dtype) {
+    const int rc = check_rows(B, N, H, D, cu, sequences, dtype);
+    if (rc != SA2_OK) return rc;
+    if (HK < 1 || H % HK) return SA2_ERR_BAD_HEADS;
+    memset(&p, 0, sizeof(p));
+    p.rows = Rows{B, N, cu, sequences};
+    p.H = H; p.HK = HK; p.G = H / HK; p.D = D;
+    p.scale = scale;
+    return SA2_OK;
+}
+size_t delta_bytes(const Causal& p) { return ((size_t)p.rows.B * p.H * p.rows.N * sizeof(float) + 255) / 256 * 256; }
+
+int check_tree(int B, int T, int H, int HK, int D, int dtype) {
+    const int rc = check_rows(B, T, H, D, nullptr, 0, dtype);
+    if (rc != SA2_OK) return rc;
+    if (HK < 1 || H % HK) return SA2_ERR_BAD_HEADS;
+    return T > SA2_TREE_NODES ? SA2_ERR_BAD_TREE : SA2_OK;
+}
+// Workgroups that share a sequence's keys: two per CU over the chip, each with at least eight tiles of 32 keys of what a
+// sequence may hold, at most 64 (how many it does hold is known on the device only)
+int tree_splits(int B, int T, int H, int HK, int D, int page_size, int table_width) {
+    const int64_t streams = (int64_t)B * HK * ((T * (H / HK) + 31) / 32), tiles = ((int64_t)page_size * table_width + 31) / 32;
+    int64_t n = (2 * CUS + streams - 1) / streams;
+    if (n > tiles / 8) n = tiles / 8;
+    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+}
+
 }  // namespace
 
 extern "C" {
@@ -90,6 +117,87 @@ int sa2_cache_append(const void* k, const void* v, void* k_cache, void* v_cache,
     for (const Tensor* t : {&p.cache.k, &p.cache.v})
         if (!stride_ok(*t, pages, page_size, HK)) return SA2_ERR_BAD_STRIDE;
     return launch_append(p, dtype, (hipStream_t)hip_stream);
+}
+
+int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, float* lse,
+                       const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                       const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream) {
+    if (!q || !k || !v || !out || !lse || !strides) return SA2_ERR_NULL_POINTER;
+    Causal p;
+    const int rc = make_causal(p, cu_seqlens, sequences, B, N, H, HK, D, scale, dtype);
+    if (rc != SA2_OK) return rc;
+    p.q = tensor(q, strides, 0);
+    p.k = tensor(k, strides, 1);
+    p.v = tensor(v, strides, 2);
+    p.out = tensor(out, strides, 3);
+    p.lse = lse;
+    if (!stride_ok(p.q, B, N, H) || !stride_ok(p.out, B, N, H) || !stride_ok(p.k, B, N, HK) || !stride_ok(p.v, B, N, HK)) return SA2_ERR_BAD_STRIDE;
+    return launch_causal_f32_fwd(p, dtype, (hipStream_t)hip_stream);
+}
+
+size_t sa2_causal_bwd_workspace_bytes(int B, int N, int H, int HK, int D, int dtype, unsigned flags) {
+    Causal p;
+    if (make_causal(p, nullptr, 0, B, N, H, HK, D, 1.f, dtype) != SA2_OK) return 0;
+    return delta_bytes(p);
+}
+
+int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+                        void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                        const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                        const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream) {
+    if (!q || !k || !v || !out || !dout || !lse || !workspace || !strides) return SA2_ERR_NULL_POINTER;
+    Causal p;
+    int rc = make_causal(p, cu_seqlens, sequences, B, N, H, HK, D, scale, dtype);
+    if (rc != SA2_OK) return rc;
+    Tensor* const t[8] = {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv};
+    const void* const at[8] = {q, k, v, out, dout, dq, dk, dv};
+    for (int i = 0; i < 8; ++i) {
+        *t[i] = tensor(at[i], strides, i);
+        if (at[i] && !stride_ok(*t[i], B, N, i == 1 || i == 2 || i > 5 ? HK : H)) return SA2_ERR_BAD_STRIDE;
+    }
+    if (((uintptr_t)workspace & 255u) || workspace_bytes < sa2_causal_bwd_workspace_bytes(B, N, H, HK, D, dtype, flags)) return SA2_ERR_WORKSPACE_TOO_SMALL;
+    p.lse = const_cast<float*>(lse);
+    p.delta = (float*)workspace;
+    p.part = (float*)((char*)workspace + delta_bytes(p));
+    const hipStream_t st = (hipStream_t)hip_stream;
+    if (!dq && !dk && !dv) return SA2_OK;
+    if (dq || dk) rc = launch_rowdot(p.out, p.dout, p.delta, B, N, H, D, dtype, st);
+    return rc == SA2_OK ? launch_causal_f32_bwd(p, dtype, st) : rc;
+}
+
+size_t sa2_tree_workspace_bytes(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype, unsigned flags) {
+    if (check_tree(B, T, H, HK, D, dtype) != SA2_OK || page_size < 1 || table_width < 1) return 0;
+    return tree_part_bytes(B, T, H, D, tree_splits(B, T, H, HK, D, page_size, table_width));
+}
+
+int sa2_tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out,
+                       const int32_t* parents, const int32_t* lengths, const int32_t* page_table,
+                       void* workspace, size_t workspace_bytes, int B, int T, int H, int HK, int D,
+                       int page_size, int pages, int table_width, const int64_t* strides, float scale,
+                       int dtype, unsigned flags, void* hip_stream) {
+    if (!q || !k || !v || !k_cache || !v_cache || !out || !lengths || !strides) return SA2_ERR_NULL_POINTER;
+    const int rc = check_tree(B, T, H, HK, D, dtype);
+    if (rc != SA2_OK) return rc;
+    if (page_size < 1 || pages < 1 || table_width < 1 || (!page_table && (pages < B || table_width != 1)) || (int64_t)page_size * table_width > 0x7fffffff - 64)
+        return SA2_ERR_BAD_CACHE;
+    Tree p;
+    memset(&p, 0, sizeof(p));
+    p.B = B; p.T = T; p.H = H; p.HK = HK; p.G = H / HK; p.D = D;
+    p.scale = scale;
+    p.q = tensor(q, strides, 0);
+    p.k = tensor(k, strides, 1);
+    p.v = tensor(v, strides, 2);
+    p.cache = Cache{tensor(k_cache, strides, 3), tensor(v_cache, strides, 4), page_table, lengths, page_size, pages, table_width};
+    p.out = tensor(out, strides, 5);
+    if (!stride_ok(p.q, B, T, H) || !stride_ok(p.out, B, T, H) || !stride_ok(p.k, B, T, HK) || !stride_ok(p.v, B, T, HK) ||
+        !stride_ok(p.cache.k, pages, page_size, HK) || !stride_ok(p.cache.v, pages, page_size, HK))
+        return SA2_ERR_BAD_STRIDE;
+    p.parents = parents;
+    p.nsplit = tree_splits(B, T, H, HK, D, page_size, table_width);
+    p.part = (float*)workspace;
+    if (p.nsplit > 1 && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < tree_part_bytes(B, T, H, D, p.nsplit)))
+        return SA2_ERR_WORKSPACE_TOO_SMALL;
+    return launch_tree_f32(p, dtype, (hipStream_t)hip_stream);
 }
 
 }  // extern "C"

@@ -55,18 +55,30 @@ struct Append {
     int nchosen;
 };
 
+// Nodes of drafted trees over a cache: the G query heads of a key head and the T nodes make R = T * G rows that read the
+// same keys; row r is node r / G, head r % G of the G.  The cached keys of a sequence are shared by `nsplit` workgroups, whose
+// outputs, not yet divided by their sums, lie in `part`: [nsplit][B*HK][R] pairs (reference point, sum), then
+// [nsplit][B*HK][R][width] values.
 struct Tree {
     Cache cache;
     int B, T, H, HK, G, D;
     float scale;
     Tensor q, k, v, out;
     const int32_t* parents;                    // [B,T], or nullptr: a chain
-    float* part;                               // partial outputs, see sa2_tree.hip
+    float* part;
     int nsplit;
 };
+constexpr int TREE_NODES = 64;
+__host__ __device__ constexpr int tree_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+inline size_t tree_part_bytes(int B, int T, int H, int D, int nsplit) {
+    return nsplit > 1 ? (size_t)nsplit * B * T * H * (tree_width(D) + 2) * sizeof(float) : 0;
+}
 
 int launch_rotary(const Rotary& p, int dtype, hipStream_t st);
 int launch_append(const Append& p, int dtype, hipStream_t st);
+int launch_causal_f32_fwd(const Causal& p, int dtype, hipStream_t st);
+int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st);
+int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
 
 namespace {
 

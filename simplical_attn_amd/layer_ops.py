@@ -77,3 +77,48 @@ def cache_append(k, v, k_cache, v_cache, lengths, page_table=None, rows=None, cu
 
     Rows whose place lies beyond the capacity, or whose page is not one of the cache's, are left out."""
     _lib.host().cache_append(k, v, k_cache, v_cache, lengths, page_table, rows, cu_seqlens)
+
+
+def causal_attention(q, k, v, cu_seqlens=None, scale=None):
+    """softmax(scale q k^T) v, query i of a sequence over its keys 0 .. i; differentiable in q, k and v.
+
+    q        [batch, seq_len, heads, head_dim], or packed [rows, heads, head_dim] with cu_seqlens; head_dim up to 256
+    k, v     as q, with heads that divide q's: query head h reads head h // (heads / key heads)
+    scale    1 / sqrt(head_dim) if None
+
+    Returns a tensor like q, zero in rows of no sequence.  bf16 and fp16 with a head_dim up to 128 that is a multiple of 8 and rows on
+    the 16-byte grid run on the 16-bit matrix pipes (softmax weights rounded to the type, sums in fp32), everything else
+    with fp32 products."""
+    return _lib.host().causal(q, k, v, cu_seqlens, scale, _lib.FLAG_AUTO)
+
+
+def causal_attention_forward(q, k, v, cu_seqlens=None, scale=None, flags=_lib.FLAG_AUTO):
+    """(out, lse) without autograd: lse is log sum e^(scale q k), [batch, heads, seq_len] or packed [heads, rows], float32,
+    -infinity in rows of no sequence.  flags: _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products."""
+    return _lib.host().causal_forward(q, k, v, cu_seqlens, scale, int(flags))
+
+
+def causal_attention_backward(q, k, v, out, lse, dout, cu_seqlens=None, scale=None, needs=(True, True, True),
+                              flags=_lib.FLAG_AUTO):
+    """(dq, dk, dv) in the inputs' type, None where ``needs`` is False.  ``out`` and ``lse`` are what
+    causal_attention_forward returned for the same inputs and arguments.  Deterministic."""
+    if len(needs) != 3:
+        raise ValueError("needs must have three entries (dq, dk, dv), got %d" % len(needs))
+    mask = sum(1 << t for t, need in enumerate(needs) if need)
+    return _lib.host().causal_backward(q, k, v, out, lse, dout, cu_seqlens, scale, mask, int(flags))
+
+
+def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None, scale=None):
+    """Attention of drafted tokens over a cache: node i of a sequence attends to the ``lengths`` rows that the cache holds, to
+    itself and to its ancestors in the draft.  One node is a decoding step.
+
+    q                 [batch, nodes, heads, head_dim], 1 to 64 nodes
+    k, v              [batch, nodes, key heads, head_dim]: the drafted tokens' own, not yet in the cache
+    parents           int32 [batch, nodes]: the node that node i follows, smaller than i, or -1 for the last cached token; -2
+                      (or any chain that does not end at -1) marks a place that is not used, whose output is zero.
+                      None: a chain, each node behind the one before it
+    k_cache, v_cache, lengths, page_table   as at cache_append, which brings the accepted nodes into the cache
+    scale             1 / sqrt(head_dim) if None
+
+    No gradients.  Returns a tensor like q."""
+    return _lib.host().tree(q, k, v, parents, k_cache, v_cache, lengths, page_table, scale, _lib.FLAG_AUTO)

@@ -1,0 +1,237 @@
+"""causal_attention against the definition in 64 bits (bounds: causal_util.py): types, head layouts, lengths from one row on,
+packed sequences with empty ones and rows behind the last, views, values that must not reach rows which do not see them,
+gradients against differences, other streams, graphs."""
+import math
+
+import pytest
+import torch
+
+import simplical_attn_amd as sa
+from simplical_attn_amd import _lib
+from tests.causal_util import check, exact
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _inputs(lead, H, HK, D, dtype, seed, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(*lead, h, D, generator=g) * s).to(dtype).to(DEV) for h, s in ((H, std), (HK, std), (HK, 1.0), (H, 1.0))]
+
+
+def _rounded(dtype, flags=0):
+    return dtype != FP32 and not flags
+
+
+def _compare(q, k, v, dout, out, lse, grads, spans, scale, dtype, flags):
+    """spans: (index of the rows, index of the lse) of each sequence."""
+    H, HK = q.shape[-2], k.shape[-2]
+    G = H // HK
+    for rows, lrows in spans:
+        for hk in range(HK):
+            hs = slice(hk * G, hk * G + G)
+            want = exact(q[rows][:, hs], k[rows][:, hk], v[rows][:, hk], dout[rows][:, hs], scale, dtype, _rounded(dtype, flags))
+            check(out[rows][:, hs], want["out"], "out")
+            check(lse[lrows][..., :][hs].transpose(0, 1), want["lse"], "lse")
+            if grads is not None:
+                check(grads[0][rows][:, hs], want["dq"], "dq")
+                check(grads[1][rows][:, hk:hk + 1], want["dk"], "dk")
+                check(grads[2][rows][:, hk:hk + 1], want["dv"], "dv")
+
+
+def _all(q, k, v, dout, flags, cu=None, scale=None):
+    out, lse = sa.causal_attention_forward(q, k, v, cu, scale, flags=flags)
+    return out, lse, sa.causal_attention_backward(q, k, v, out, lse, dout, cu, scale, flags=flags)
+
+
+SHAPES = [(1, 1, 1, 1, 64), (2, 2, 2, 1, 64), (1, 31, 3, 3, 32), (1, 33, 4, 2, 128), (2, 64, 2, 2, 64), (1, 65, 8, 1, 128),
+          (1, 127, 2, 1, 80), (1, 129, 6, 2, 128), (2, 200, 4, 4, 64), (1, 257, 4, 1, 128), (1, 300, 2, 1, 96), (1, 511, 2, 2, 128),
+          (1, 1000, 2, 1, 64), (1, 777, 3, 1, 128), (1, 70, 2, 1, 8), (1, 40, 2, 1, 256), (1, 77, 2, 2, 136), (1, 50, 1, 1, 33), (1, 45, 2, 1, 1)]
+
+
+@pytest.mark.parametrize("flags", [_lib.FLAG_AUTO, _lib.FLAG_FORCE_GENERIC])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("B,N,H,HK,D", SHAPES)
+def test_batches(B, N, H, HK, D, dtype, flags):
+    if dtype == FP32 and flags:
+        pytest.skip("the same kernels")
+    q, k, v, dout = _inputs((B, N), H, HK, D, dtype, B + N + D)
+    out, lse, grads = _all(q, k, v, dout, flags)
+    _compare(q, k, v, dout, out, lse, grads, [((b,), (b,)) for b in range(B)], D ** -0.5, dtype, flags)
+
+
+PACKED = [[0, 5], [0, 1, 2, 3], [0, 0, 64, 64, 65, 200], [3, 40, 40, 168, 297], [0, 300, 301, 900]]
+
+
+@pytest.mark.parametrize("dtype,H,HK,D", [(BF16, 4, 2, 128), (FP16, 2, 1, 64), (FP32, 3, 3, 64), (BF16, 2, 2, 40), (FP32, 2, 1, 128), (BF16, 1, 1, 256)])
+@pytest.mark.parametrize("ends", PACKED)
+def test_packed(ends, dtype, H, HK, D):
+    T = ends[-1] + 9
+    q, k, v, dout = _inputs((T,), H, HK, D, dtype, T + D)
+    for x in (q, k, v, dout):                                # rows of no sequence hold anything
+        x[:ends[0]] = math.nan
+        x[ends[-1]:] = math.inf
+    cu = torch.tensor(ends, dtype=torch.int32, device=DEV)
+    out, lse, grads = _all(q, k, v, dout, 0, cu)
+    spans = [((slice(a, b),), (slice(None), slice(a, b))) for a, b in zip(ends, ends[1:]) if b > a]
+    _compare(q, k, v, dout, out, lse, grads, spans, D ** -0.5, dtype, 0)
+    for x in (out, *grads):
+        assert x[:ends[0]].count_nonzero() == 0 and x[ends[-1]:].count_nonzero() == 0
+    assert (lse[:, ends[-1]:] == -math.inf).all() and (lse[:, :ends[0]] == -math.inf).all()
+
+
+def test_many_short_sequences():
+    """More sequences than a wavefront has lanes, some empty."""
+    g = torch.Generator().manual_seed(2)
+    lens = torch.randint(0, 9, (200,), generator=g).tolist()
+    ends = [0]
+    for n in lens:
+        ends.append(ends[-1] + n)
+    q, k, v, dout = _inputs((ends[-1],), 2, 1, 64, BF16, 7)
+    out, lse, grads = _all(q, k, v, dout, 0, torch.tensor(ends, dtype=torch.int32, device=DEV))
+    spans = [((slice(a, b),), (slice(None), slice(a, b))) for a, b in zip(ends, ends[1:]) if b > a]
+    _compare(q, k, v, dout, out, lse, grads, spans, 64 ** -0.5, BF16, 0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("flags", [0, _lib.FLAG_FORCE_GENERIC])
+@pytest.mark.parametrize("D", [64, 128])
+def test_hidden_rows_may_hold_anything(dtype, flags, D):
+    """An infinity or NaN in row j of k, v, q or dout changes nothing that row j is hidden from."""
+    N, at = 150, 70
+    q, k, v, dout = _inputs((1, N), 2, 1, D, dtype, 5)
+
+    def same(a, b):
+        # sums of at most 2 N terms in another order: 2 (2 N + 16) e of magnitudes that stay below 64, then one rounding each
+        return ((a.double() - b.double()).abs() <= torch.finfo(a.dtype).eps * b.double().abs() + 2 * (2 * N + 16) * 2.0 ** -24 * 64).all()
+
+    base = _all(q, k, v, dout, flags)
+    for bad in (math.nan, math.inf, -math.inf):
+        k2, v2 = k.clone(), v.clone()
+        k2[:, at, :, 3], v2[:, at, :, 5] = bad, bad
+        out, lse, (dq, _, _) = _all(q, k2, v2, dout, flags)
+        assert same(out[:, :at], base[0][:, :at]) and same(lse[..., :at], base[1][..., :at]) and same(dq[:, :at], base[2][0][:, :at])
+        assert not torch.isfinite(out[:, at:]).all(-1).any()
+        q2, d2 = q.clone(), dout.clone()
+        q2[:, at, :, 3], d2[:, at, :, 5] = bad, bad
+        _, _, (_, dk, dv) = _all(q2, k, v, d2, flags)
+        assert same(dk[:, at + 1:], base[2][1][:, at + 1:]) and same(dv[:, at + 1:], base[2][2][:, at + 1:])
+        assert not torch.isfinite(dv[:, :at + 1].float()).all(-1).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_views_broadcasts_and_odd_rows(dtype):
+    g = torch.Generator().manual_seed(11)
+    fused = torch.randn(2, 90, 8, 64, generator=g).to(dtype).to(DEV)
+    q, k, v = fused[:, :, :4], fused[:, :, 4:6], fused[:, :, 6:8]
+    dout = torch.randn(2, 4, 90, 64, generator=g).to(dtype).to(DEV).transpose(1, 2)
+    want = _all(q.contiguous(), k.contiguous(), v.contiguous(), dout.contiguous(), 0)
+    got = _all(q, k, v, dout, 0)
+    for a, b in zip((*got[:2], *got[2]), (*want[:2], *want[2])):
+        assert torch.equal(a, b)
+    # a head shared by expansion, a gradient expanded over rows, rows off the 16-byte grid
+    wide = torch.randn(1, 70, 2, 70, generator=g).to(dtype).to(DEV)
+    q, k = wide[..., 3:67], wide[:, :, :1, 5:69].expand(1, 70, 2, 64)
+    dout = torch.ones(1, 1, 1, 1, dtype=dtype, device=DEV).expand(1, 70, 2, 64)
+    got = _all(q, k, k, dout, 0)
+    # (rows off the grid run on the kernels with fp32 products)
+    _compare(q, k, k, dout, got[0], got[1], got[2], [((0,), (0,))], 0.125, dtype, 0)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, 0.5, 2.0])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_scales(scale, dtype):
+    q, k, v, dout = _inputs((1, 140), 2, 2, 64, dtype, 3)
+    out, lse, grads = _all(q, k, v, dout, 0, scale=scale)
+    _compare(q, k, v, dout, out, lse, grads, [((0,), (0,))], scale, dtype, 0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_large_scores(dtype):
+    """Scores of several hundred: the running maximum moves, weights underflow."""
+    q, k, v, dout = _inputs((1, 300), 2, 1, 128, dtype, 13, std=6.0)
+    out, lse, grads = _all(q, k, v, dout, 0)
+    _compare(q, k, v, dout, out, lse, grads, [((0,), (0,))], 128 ** -0.5, dtype, 0)
+
+
+def test_only_wanted_gradients_and_determinism():
+    q, k, v, dout = _inputs((1, 400), 4, 2, 64, BF16, 17)
+    out, lse, grads = _all(q, k, v, dout, 0)
+    for mask in range(8):
+        needs = [bool(mask >> i & 1) for i in range(3)]
+        got = sa.causal_attention_backward(q, k, v, out, lse, dout, needs=needs)
+        for need, a, b in zip(needs, got, grads):
+            assert torch.equal(a, b) if need else a is None
+    leaf = v.clone().requires_grad_(True)
+    (dv,) = torch.autograd.grad(sa.causal_attention(q, k, leaf), leaf, dout)
+    assert torch.equal(dv, grads[2])
+
+
+def test_gradients_against_differences():
+    q, k, v, dout = _inputs((1, 40), 4, 2, 64, FP32, 19)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(sa.causal_attention(*leaves), leaves, dout)
+    f = lambda *x: (sa.causal_attention(*x).double() * dout.double()).sum().item()
+    g = torch.Generator().manual_seed(20)
+    for i, grad in enumerate(grads):
+        step = torch.randn(leaves[i].shape, generator=g).to(DEV)
+        h = 2.0 ** -6
+        moved = [[(t + s * h * step).detach() if j == i else t.detach() for j, t in enumerate(leaves)] for s in (1, -1)]
+        slope = (f(*moved[0]) - f(*moved[1])) / (2 * h)
+        # third derivatives are of the order of the gradient itself: h^2; rounding of 10^4 outputs: 10^2 * 2^-24 / h
+        size = (grad.double().abs() * step.double().abs()).sum().item()
+        assert abs(slope - (grad.double() * step.double()).sum().item()) <= 4 * h * h * size + 1e-3
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2^31 and more elements into a packed tensor."""
+    D, H = 128, 1
+    T = (1 << 31) // (8 * D) + 300
+    big = torch.zeros(T, 8, D, dtype=BF16, device=DEV)                    # head 0 of 8: rows 1024 elements apart
+    q, k, v, dout = _inputs((260,), 1, 1, D, BF16, 23)
+    for i, x in enumerate((q, k, v, dout)):
+        big[T - 260:, i] = x[:, 0]
+    views = [big[:, i:i + 1] for i in range(4)]
+    cu = torch.tensor([T - 260, T], dtype=torch.int32, device=DEV)
+    out, lse, grads = _all(*views, 0, cu)
+    want = _all(q, k, v, dout, 0, torch.tensor([0, 260], dtype=torch.int32, device=DEV))
+    for a, b in zip((out, *grads), (want[0], *want[2])):
+        assert torch.equal(a[T - 260:], b) and a[:T - 260].count_nonzero() == 0
+    assert torch.equal(lse[:, T - 260:], want[1])
+
+
+def test_other_stream_and_replayed_graph():
+    q, k, v, dout = _inputs((100,), 4, 2, 128, BF16, 29)
+    cu = torch.tensor([0, 30, 100], dtype=torch.int32, device=DEV)
+    want = _all(q, k, v, dout, 0, cu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _all(q, k, v, dout, 0, cu)
+    side.synchronize()
+    for a, b in zip((*got[:2], *got[2]), (*want[:2], *want[2])):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = _all(q, k, v, dout, 0, cu)
+    g = torch.Generator().manual_seed(31)
+    for ends in ([0, 1, 100], [0, 64, 64], [50, 80, 99]):
+        cu.copy_(torch.tensor(ends, dtype=torch.int32))
+        for x in (q, k, v, dout):
+            x.copy_(torch.randn(x.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (*captured[:2], *captured[2])]
+        eager = _all(q, k, v, dout, 0, cu)
+        for a, b in zip(got, (*eager[:2], *eager[2])):
+            assert torch.equal(a, b)
+
+
+def test_empty():
+    q = torch.zeros(2, 0, 4, 64, dtype=BF16, device=DEV, requires_grad=True)
+    k = torch.zeros(2, 0, 2, 64, dtype=BF16, device=DEV)
+    out = sa.causal_attention(q, k, k)
+    assert out.shape == q.shape
+    assert torch.autograd.grad(out, q, torch.zeros_like(out))[0].shape == q.shape

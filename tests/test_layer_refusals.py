@@ -88,6 +88,52 @@ def test_append(lib, error, kw):
         _append(**kw)
 
 
+@pytest.mark.parametrize("error,call", [
+    (ValueError, lambda: sa.causal_attention(t(2, 8), t(2, 8), t(2, 8))),
+    (TypeError, lambda: sa.causal_attention(*[t(1, 2, 3, 8, dtype=torch.int32)] * 3)),
+    (ValueError, lambda: sa.causal_attention(t(1, 2, 4, 8), t(1, 3, 4, 8), t(1, 2, 4, 8))),
+    (ValueError, lambda: sa.causal_attention(t(1, 2, 4, 8), t(1, 2, 4, 8), t(1, 2, 2, 8))),
+    (ValueError, lambda: sa.causal_attention(t(1, 2, 4, 8), t(1, 2, 3, 8), t(1, 2, 3, 8))),
+    (ValueError, lambda: sa.causal_attention(t(1, 2, 4, 8), t(1, 2, 4, 8), t(1, 2, 4, 8, dtype=torch.float16))),
+    (ValueError, lambda: sa.causal_attention(*[t(1, 2, 4, 257)] * 3)),
+    (ValueError, lambda: sa.causal_attention(*[t(5, 4, 8)] * 3)),
+    (ValueError, lambda: sa.causal_attention(*[t(1, 5, 4, 8)] * 3, cu_seqlens=ints(0, 5))),
+    (ValueError, lambda: sa.causal_attention(*[t(5, 4, 8)] * 3, cu_seqlens=ints(0, 5).long())),
+    (RuntimeError, lambda: sa.causal_attention(*[t(5, 4, 8)] * 3, cu_seqlens=ints(0, 5))),
+    (ValueError, lambda: sa.causal_attention_backward(*[t(1, 5, 4, 8)] * 3, t(1, 5, 4, 8), t(1, 4, 5), t(1, 5, 4, 8), needs=(True,))),
+])
+def test_causal(lib, error, call):
+    with pytest.raises(error):
+        call()
+
+
+def _tree(q=(2, 3, 4, 8), k=(2, 3, 2, 8), parents=ints(-1, 0, 1, -1, -1, 0).view(2, 3), kc=(4, 16, 2, 8), lengths=ints(0, 0),
+          table=ints(0, 1, 2, 3).view(2, 2), v=None):
+    make = lambda x: x if isinstance(x, torch.Tensor) else t(*x)
+    return sa.tree_attention(make(q), make(k), make(v or k), parents, make(kc), make(kc), lengths, table)
+
+
+@pytest.mark.parametrize("error,kw", [
+    (ValueError, dict(q=(6, 4, 8))),
+    (ValueError, dict(q=(2, 65, 4, 8), k=(2, 65, 2, 8), parents=None)),
+    (ValueError, dict(q=(2, 0, 4, 8), k=(2, 0, 2, 8), parents=None)),
+    (ValueError, dict(q=(2, 3, 3, 8))),
+    (ValueError, dict(v=(2, 3, 4, 8))),
+    (ValueError, dict(q=(2, 3, 4, 260), k=(2, 3, 2, 260), kc=(4, 16, 2, 260))),
+    (ValueError, dict(parents=ints(-1, 0, 1))),
+    (ValueError, dict(parents=ints(-1, 0).view(1, 2))),
+    (ValueError, dict(parents=ints(-1, 0, 1, -1, -1, 0).view(2, 3).long())),
+    (ValueError, dict(kc=(4, 16, 4, 8))),
+    (ValueError, dict(table=None)),
+    (ValueError, dict(lengths=ints(0, 0, 0))),
+    (RuntimeError, dict(q=t(2, 3, 4, 8).requires_grad_(True))),
+    (RuntimeError, dict()),
+])
+def test_tree(lib, error, kw):
+    with pytest.raises(error):
+        _tree(**kw)
+
+
 def test_c_abi(lib):
     st = _lib.stride_array([(1024, 128, 64)] * 4)
 
@@ -109,5 +155,32 @@ def test_c_abi(lib):
     assert append(N=0) == -3 and append(rows=ONE) == -3 and append(rows=ONE, nrows=2, B=1, cu=ONE, seqs=2) == -3
     assert append(page=0) == -13 and append(pages=0) == -13 and append(width=0) == -13 and append(table=None, pages=1) == -13
     assert append(strides=_lib.stride_array([(1024, 0, 64)] * 4)) == -4
+
+    st = _lib.stride_array([(1024, 128, 64)] * 8)
+
+    def causal(q=ONE, cu=None, seqs=0, B=1, N=8, H=2, HK=2, D=64, strides=st, dtype=1):
+        return lib.sa2_causal_forward(q, ONE, ONE, ONE, ONE, cu, seqs, B, N, H, HK, D, strides, 0.1, dtype, 0, None)
+
+    assert causal(q=None) == -1 and causal(dtype=5) == -2 and causal(N=0) == -3 and causal(D=257) == -3 and causal(B=2, cu=ONE, seqs=3) == -3
+    assert causal(HK=3) == -11 and causal(HK=0) == -11 and causal(N=1 << 30) == -9
+    assert causal(strides=_lib.stride_array([(1024, 128, 0)] * 8)) == -4
+    need = lib.sa2_causal_bwd_workspace_bytes(1, 8, 2, 2, 64, 1, 0)
+    assert need >= 2 * 8 * 4 and lib.sa2_causal_bwd_workspace_bytes(1, 8, 3, 2, 64, 1, 0) == 0
+
+    def backward(workspace=ONE, size=need, dq=ONE, H=2):
+        return lib.sa2_causal_backward(ONE, ONE, ONE, ONE, ONE, ONE, dq, None, None, workspace, size, None, 0, 1, 8, H, 2, 64, st, 0.1, 1, 0, None)
+
+    assert backward(workspace=None) == -1 and backward(size=need - 1) == -6 and backward(workspace=ctypes.c_void_p(264)) == -6 and backward(H=3) == -11
+    assert backward(dq=None) == 0                         # no gradient is wanted: nothing is launched
+
+    def tree(q=ONE, lengths=ONE, table=ONE, B=2, T=4, H=4, HK=2, D=64, page=16, pages=4, width=2, strides=st, dtype=1):
+        return lib.sa2_tree_attention(q, ONE, ONE, ONE, ONE, ONE, None, lengths, table, None, 0, B, T, H, HK, D, page, pages, width, strides, 0.1, dtype, 0, None)
+
+    assert tree(q=None) == -1 and tree(lengths=None) == -1 and tree(dtype=-1) == -2 and tree(B=0) == -3
+    assert tree(HK=3) == -11 and tree(T=65) == -14 and tree(page=0) == -13 and tree(pages=0) == -13 and tree(table=None) == -13
+    assert tree(table=None, pages=1, width=1) == -13 and tree(page=1 << 20, width=1 << 12) == -13
+    assert tree(strides=_lib.stride_array([(1024, -1, 64)] * 8)) == -4
+    assert lib.sa2_tree_workspace_bytes(1, 1, 8, 2, 128, 64, 512, 1, 0) > 0 and tree(page=64, pages=512, width=512) == -6
+    assert lib.sa2_tree_workspace_bytes(1, 65, 8, 2, 128, 64, 512, 1, 0) == 0
     seen = {lib.sa2_strerror(code) for code in range(-14, 0)}
     assert len(seen) == 14 and not any(b"unknown sa2" in m for m in seen)

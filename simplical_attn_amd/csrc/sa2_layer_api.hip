@@ -132,6 +132,8 @@ int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, f
     p.out = tensor(out, strides, 3);
     p.lse = lse;
     if (!stride_ok(p.q, B, N, H) || !stride_ok(p.out, B, N, H) || !stride_ok(p.k, B, N, HK) || !stride_ok(p.v, B, N, HK)) return SA2_ERR_BAD_STRIDE;
+    if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out}))
+        return launch_causal16_fwd(p, dtype, (hipStream_t)hip_stream);
     return launch_causal_f32_fwd(p, dtype, (hipStream_t)hip_stream);
 }
 

@@ -2,6 +2,8 @@
 // cache rows, drafted trees).
 #pragma once
 
+#include <initializer_list>
+
 #include "sa2_common.h"
 #include "sa2_mfma_common.h"
 
@@ -78,6 +80,10 @@ int launch_rotary(const Rotary& p, int dtype, hipStream_t st);
 int launch_append(const Append& p, int dtype, hipStream_t st);
 int launch_causal_f32_fwd(const Causal& p, int dtype, hipStream_t st);
 int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st);
+// bf16 and fp16 with a head_dim up to 128 that is a multiple of 8, rows on the 16-byte grid
+bool causal16_supported(int D, int dtype);
+bool causal16_layout(const Causal& p, std::initializer_list<const Tensor*> ts);
+int launch_causal16_fwd(const Causal& p, int dtype, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
 
 namespace {

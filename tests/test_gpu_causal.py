@@ -195,10 +195,11 @@ def test_offsets_beyond_32_bits():
     views = [big[:, i:i + 1] for i in range(4)]
     cu = torch.tensor([T - 260, T], dtype=torch.int32, device=DEV)
     out, lse, grads = _all(*views, 0, cu)
-    want = _all(q, k, v, dout, 0, torch.tensor([0, 260], dtype=torch.int32, device=DEV))
-    for a, b in zip((out, *grads), (want[0], *want[2])):
-        assert torch.equal(a[T - 260:], b) and a[:T - 260].count_nonzero() == 0
-    assert torch.equal(lse[:, T - 260:], want[1])
+    # (a call on the 260 rows alone may take other kernels, so the definition is what the bits are compared with)
+    for a in (out, *grads):
+        assert a[:T - 260].count_nonzero() == 0
+    _compare(q, k, v, dout, out[T - 260:], lse[:, T - 260:].contiguous(), [x[T - 260:] for x in grads],
+             [((slice(None),), (slice(None),))], D ** -0.5, BF16, 0)
 
 
 def test_other_stream_and_replayed_graph():

@@ -12,112 +12,16 @@
 // sweep.  Rounding weights to 16 bits costs half a step of each, whatever m; a unit whose sum passes REF_LIMIT has the workgroup
 // sweep its keys a second time, with the running maximum.
 // K and V come by direct global->LDS loads into three buffers of 64 keys, so that one barrier per 64 keys is enough.
-#include "sa2_causal_common.h"
-#include "sa2_mfma_lone.h"
+#include "sa2_causal16.h"
 
 namespace sa2 {
 namespace {
 
-constexpr int THREADS = 256, WAVES = 4, SUB = 32, KEYS = 2 * SUB, BUFFERS = 3;
+constexpr int BUFFERS = 3;
 
 template <class E> struct RefLimit;
 template <> struct RefLimit<ElemBF16> { static constexpr float value = 1.152921504606847e18f; };   // 2^60
 template <> struct RefLimit<ElemF16> { static constexpr float value = 32768.f; };                  // below 65504
-
-template <int D>
-struct Buffer {                                             // K and V of KEYS keys: two QuadTiles each
-    static constexpr int K = 0, V = 2 * QuadTile<D>::BYTES, BYTES = 4 * QuadTile<D>::BYTES;
-};
-
-// KEYS rows of K and of V to LDS; each wavefront brings a quarter.  Rows from `len` on and columns from p.D on: zeros.
-template <int D>
-struct Fetch {
-    using T = QuadTile<D>;
-    static constexpr int INSTR = KEYS / T::RPW / WAVES;     // per tensor and wavefront
-    const char *k, *v;                                      // row 0 of the sequence
-    int64_t ks, vs;                                         // bytes from row to row
-    uint32_t koff[INSTR], voff[INSTR];                      // of the lane's rows in a tile
-    int row[INSTR];
-    bool pad;                                               // the lane's columns lie behind the row
-    __device__ __forceinline__ void init(const Causal& p, const Span& s, int hk) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        k = (const char*)p.k.p + row_offset(p.k, s, 0, hk) * 2;
-        v = (const char*)p.v.p + row_offset(p.v, s, 0, hk) * 2;
-        ks = p.k.sn * 2;
-        vs = p.v.sn * 2;
-        const int chunk = T::dma_chunk(lane);
-        pad = chunk * 8 >= p.D;
-#pragma unroll
-        for (int i = 0; i < INSTR; ++i) {
-            row[i] = (wave * INSTR + i) * T::RPW + T::dma_row(lane);
-            koff[i] = (uint32_t)(row[i] * ks) + chunk * 16;
-            voff[i] = (uint32_t)(row[i] * vs) + chunk * 16;
-        }
-    }
-    __device__ __forceinline__ void request(int first, int len, uint32_t buffer, bool padded) const {
-        const int wave = threadIdx.x >> 6;
-        const char *kb = k + first * ks, *vb = v + first * vs;
-        if (first + KEYS <= len && !padded) {
-#pragma unroll
-            for (int i = 0; i < INSTR; ++i) {
-                const int g = wave * INSTR + i;             // group of RPW rows
-                lds_request(kb, koff[i], buffer + Buffer<D>::K + g * T::GROUP);
-                lds_request(vb, voff[i], buffer + Buffer<D>::V + g * T::GROUP);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < INSTR; ++i) {
-                const int g = wave * INSTR + i;
-                const bool there = first + row[i] < len && !pad;
-                lds_request(there ? kb + koff[i] : (const char*)zero_chunk, buffer + Buffer<D>::K + g * T::GROUP);
-                lds_request(there ? vb + voff[i] : (const char*)zero_chunk, buffer + Buffer<D>::V + g * T::GROUP);
-            }
-        }
-    }
-};
-// (groups of the two QuadTiles of a buffer follow one another)
-static_assert(QuadTile<64>::BYTES == QuadTile<64>::NGROUP * QuadTile<64>::GROUP && QuadTile<128>::BYTES == QuadTile<128>::NGROUP * QuadTile<128>::GROUP, "");
-
-// An infinity or NaN among eight 16-bit values
-template <class E>
-__device__ __forceinline__ bool not_finite(const typename E::x8& x) {
-    constexpr uint32_t EXP = E::DTYPE == SA2_BF16 ? 0x7f80u : 0x7c00u;
-    union { typename E::x8 v; uint32_t u[4]; } w;
-    w.v = x;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) odd = odd || (w.u[i] & EXP) == EXP || (w.u[i] >> 16 & EXP) == EXP;
-    return odd;
-}
-// Sums S0 .. += V^T w one key at a time and on the vector ALU, into the queries that see the key: a weight of zero would not keep an
-// infinity or NaN out.  `tile`: the V tile in LDS
-template <class E, class L, int S0, int D, class F>
-__device__ __forceinline__ void guarded_output(uint32_t tile, const typename E::x8 (&w)[2], F&& visible) {
-    using T = QuadTile<D>;
-    const int half = (threadIdx.x & 63) >> 5;
-    union { typename E::x8 v[2]; uint32_t u[8]; } x;
-    x.v[0] = w[0];
-    x.v[1] = w[1];
-#pragma unroll 1
-    for (int key = 0; key < 32; ++key) {
-        const int at = 8 * (key / 16) + 4 * (key % 16 / 8) + key % 4;      // of the half that holds the key's weight
-        uint32_t pair = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pair = at / 2 == i ? x.u[i] : pair;
-        const float held = at & 1 ? E::hi(pair) : E::lo(pair), other = other_half(held), weight = (key / 4 & 1) == half ? held : other;
-        const bool sees = visible(key);
-        const uint32_t row = tile + (uint32_t)((key / T::RPW) * T::GROUP + key % T::RPW * 64), flip = (uint32_t)T::flip(key);
-        static_for<D / 8>([&](auto C) __attribute__((always_inline)) {
-            constexpr int ch = decltype(C)::value, r = S0 + 4 * ch;
-            typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-            const u2 v = *(const u2 __attribute__((address_space(3)))*)(uintptr_t)(row + ch / 4 * T::BLOCK + ((ch % 4) ^ flip) * 16 + half * 8);
-            const float4 o = L::template get_regs<r>();
-            auto plus = [&](float o, float v) { return __float_as_uint(sees ? fmaf(weight, v, o) : o); };
-            L::template set_regs<r>(plus(o.x, E::lo(v.x)), plus(o.y, E::hi(v.x)), plus(o.z, E::lo(v.y)), plus(o.w, E::hi(v.y)));
-        });
-    }
-    asm volatile("s_nop 7" ::: "memory");
-}
 
 template <class E, int D, int NQ>
 __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(Causal p, bool padded) {
@@ -143,10 +47,10 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(
     }
     const int q0 = ((s.len + BLOCK - 1) / BLOCK - 1 - s.block) * BLOCK, mine = q0 + wave * ROWS;
     const int last = q0 + BLOCK < s.len ? q0 + BLOCK : s.len;              // the workgroup's keys: 0 .. last - 1
-    const int tiles = (last + KEYS - 1) / KEYS;
+    const int tiles = (last + TILE_ROWS - 1) / TILE_ROWS;
 
     Fetch<D> fetch;
-    fetch.init(p, s, hk);
+    fetch.init(p.k, p.v, s, hk, p.D);
 
     // queries, second operand of the logits; a negative scale is taken out of them, so that the largest logit has the largest weight
     const float c = fabsf(p.scale) * LOG2E;
@@ -177,12 +81,12 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(
     X8 kf[KK], vf[2][DT];                                                  // a piece's operands, shared by its blocks
     // (one address per piece, the rest are offsets of the reads)
     auto keys_at = [&](uint32_t buf, int sub) {
-        uint32_t at = buf + row_lane + (uint32_t)(Buffer<D>::K + sub * T::BYTES);
+        uint32_t at = buf + row_lane + (uint32_t)(Buffer<D>::FIRST + sub * T::BYTES);
         stays(at);
         return at;
     };
     auto values_at = [&](uint32_t buf, int sub) {
-        uint32_t at = buf + column_lane + (uint32_t)(Buffer<D>::V + sub * T::BYTES);
+        uint32_t at = buf + column_lane + (uint32_t)(Buffer<D>::SECOND + sub * T::BYTES);
         stays(at);
         return at;
     };
@@ -292,7 +196,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(
     int released;                                                          // tiles 0 .. released are in LDS
     uint32_t arriving;                                                     // the buffer that the next request fills
     auto request = [&](int t) {
-        fetch.request(t * KEYS, last, arriving, padded);
+        fetch.request(t * TILE_ROWS, last, arriving, padded);
         arriving = after(arriving);
     };
     auto arrive = [&]() {                                                  // the next one too; its successor is on its way
@@ -332,13 +236,13 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(
                 float sum;
                 weights(st[0], at, sum, w[0], std::true_type{}, seen);
                 l[n] += sum;
-                if (odd) guarded_output<E, L, O0 + n * DT * 16, D>(buf + (uint32_t)(Buffer<D>::V + sub * T::BYTES), w[0], [&](int key) { return key <= seen; });
+                if (odd) guarded_sum<E, L, O0 + n * DT * 16, D>(buf + (uint32_t)(Buffer<D>::SECOND + sub * T::BYTES), w[0], [&](int key) { return key <= seen; });
                 else output(N, w[0]);
             }
         });
     };
     const bool active = mine < s.len;
-    const int full = active ? mine / KEYS : 0;                             // tiles that all of the wavefront's queries see
+    const int full = active ? mine / TILE_ROWS : 0;                             // tiles that all of the wavefront's queries see
     constexpr int LOOK = NQ == 1 ? 2 : 1;                                  // tiles ahead that a round of steps reads keys of
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
@@ -407,7 +311,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(
             if (active && t <= full) {
 #pragma unroll 1
                 for (int sub = t == done / 2 ? done % 2 : 0; sub < 2; ++sub) {
-                    const int first = t * KEYS + sub * SUB;
+                    const int first = t * TILE_ROWS + sub * SUB;
                     if (first < mine + ROWS) piece(here, sub, first);
                 }
             }

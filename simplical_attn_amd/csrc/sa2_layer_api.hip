@@ -1,5 +1,6 @@
 // extern "C" boundary of the operators of ordinary attention layers: argument validation and kernel choice.
 // No allocation, no synchronisation, no state.
+#include <math.h>
 #include <string.h>
 
 #include "sa2_layer_common.h"
@@ -140,7 +141,8 @@ int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, f
 size_t sa2_causal_bwd_workspace_bytes(int B, int N, int H, int HK, int D, int dtype, unsigned flags) {
     Causal p;
     if (make_causal(p, nullptr, 0, B, N, H, HK, D, 1.f, dtype) != SA2_OK) return 0;
-    return delta_bytes(p);
+    if ((flags & SA2_FLAG_FORCE_GENERIC) || !causal16_supported(D, dtype)) return delta_bytes(p);
+    return 2 * delta_bytes(p) + CAUSAL16_TOPS * sizeof(float) + causal16_part_bytes(B, N, HK, p.G, D);
 }
 
 int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
@@ -160,9 +162,16 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
     if (((uintptr_t)workspace & 255u) || workspace_bytes < sa2_causal_bwd_workspace_bytes(B, N, H, HK, D, dtype, flags)) return SA2_ERR_WORKSPACE_TOO_SMALL;
     p.lse = const_cast<float*>(lse);
     p.delta = (float*)workspace;
-    p.part = (float*)((char*)workspace + delta_bytes(p));
     const hipStream_t st = (hipStream_t)hip_stream;
     if (!dq && !dk && !dv) return SA2_OK;
+    // (-lse / scale is one of the 16-bit kernels' operands)
+    if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv}) &&
+        fabsf(scale) > 1e-20f) {
+        float* const minus_lse = (float*)((char*)workspace + delta_bytes(p));
+        float* const tops = (float*)((char*)minus_lse + delta_bytes(p));
+        p.part = tops + CAUSAL16_TOPS;
+        return launch_causal16_bwd(p, dtype, minus_lse, tops, st);
+    }
     if (dq || dk) rc = launch_rowdot(p.out, p.dout, p.delta, B, N, H, D, dtype, st);
     return rc == SA2_OK ? launch_causal_f32_bwd(p, dtype, st) : rc;
 }

@@ -84,6 +84,12 @@ int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st);
 bool causal16_supported(int D, int dtype);
 bool causal16_layout(const Causal& p, std::initializer_list<const Tensor*> ts);
 int launch_causal16_fwd(const Causal& p, int dtype, hipStream_t st);
+// their backward: p.delta receives -delta, minus_lse [B,H,N] -lse / scale, tops the largest |dout| of up to CAUSAL16_TOPS parts
+constexpr int CAUSAL16_TOPS = 1024;
+int causal16_splits(int B, int N, int HK, int G);
+size_t causal16_part_bytes(int B, int N, int HK, int G, int D);
+int launch_causal16_bwd(const Causal& p, int dtype, float* minus_lse, float* tops, hipStream_t st);
+int launch_causal16_dq(const Causal& p, int dtype, const float* tops, int ntops, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
 
 namespace {

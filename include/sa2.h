@@ -220,23 +220,25 @@ int sa2_cache_append(const void* k, const void* v, void* k_cache, void* v_cache,
 /*
  * Causal attention over whole prompts: query i of a sequence attends to its keys 0 .. i.
  *   S = scale q k^T, out = softmax(S) v, lse = log sum e^S (natural), [B,H,N] fp32 (packed: [H,N])
+ *   out_low      NULL, or (16-bit types) a tensor laid out as out that receives what rounding out left, for the backward:
+ *                with it delta = sum_d dout*out is formed from 16 to 22 bits of out instead of 8 to 11 (fp32: not used)
  *   strides      q, k, v, out
- * Rows of no sequence: out 0, lse -infinity.  An infinity or NaN in k or v reaches the queries that attend to it only.
+ * Rows of no sequence: out 0 (out_low is not written), lse -infinity.  An infinity or NaN in k or v reaches the queries that attend to it only.
  * flags: SA2_FLAG_AUTO, or SA2_FLAG_FORCE_GENERIC for the kernels with fp32 products whatever the type.
  */
-int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, float* lse,
+int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, void* out_low, float* lse,
                        const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
                        const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream);
 
 /*
- * Its gradients: out and lse are what the forward gave for these inputs.  A NULL gradient is not wanted; every other one
+ * Its gradients: out, out_low (or NULL) and lse are what the forward gave for these inputs.  A NULL gradient is not wanted; every other one
  * is fully overwritten (rows of no sequence: 0).  dk and dv are sums over the query heads that share a head.
  *   workspace    sa2_causal_bwd_workspace_bytes(...) bytes, 256-byte aligned; contents on entry ignored
  *   strides      q, k, v, out, dout, dq, dk, dv
  * No atomics: two calls on the same inputs give identical bits.
  */
 size_t sa2_causal_bwd_workspace_bytes(int B, int N, int H, int HK, int D, int dtype, unsigned flags);
-int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* out_low, const void* dout, const float* lse,
                         void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                         const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
                         const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream);

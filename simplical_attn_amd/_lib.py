@@ -72,11 +72,11 @@ def load():
     lib.sa2_cache_append.restype = c_int
     lib.sa2_cache_append.argtypes = ([c_void_p] * 7 + [c_int, c_void_p, c_int] + [c_int] * 7 + [i64p, c_int, c_void_p])
     lib.sa2_causal_forward.restype = c_int
-    lib.sa2_causal_forward.argtypes = [c_void_p] * 6 + [c_int] * 6 + [i64p, c_float, c_int, c_uint, c_void_p]
+    lib.sa2_causal_forward.argtypes = [c_void_p] * 7 + [c_int] * 6 + [i64p, c_float, c_int, c_uint, c_void_p]
     lib.sa2_causal_bwd_workspace_bytes.restype = c_size_t
     lib.sa2_causal_bwd_workspace_bytes.argtypes = [c_int] * 6 + [c_uint]
     lib.sa2_causal_backward.restype = c_int
-    lib.sa2_causal_backward.argtypes = ([c_void_p] * 10 + [c_size_t, c_void_p] + [c_int] * 6 + [i64p, c_float, c_int, c_uint, c_void_p])
+    lib.sa2_causal_backward.argtypes = ([c_void_p] * 11 + [c_size_t, c_void_p] + [c_int] * 6 + [i64p, c_float, c_int, c_uint, c_void_p])
     lib.sa2_tree_workspace_bytes.restype = c_size_t
     lib.sa2_tree_workspace_bytes.argtypes = [c_int] * 8 + [c_uint]
     lib.sa2_tree_attention.restype = c_int

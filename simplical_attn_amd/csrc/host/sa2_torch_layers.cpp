@@ -219,25 +219,28 @@ struct Prompt {
 };
 Tensor workspace(const Tensor& q, size_t bytes) { return at::empty({(int64_t)bytes}, q.options().dtype(at::kByte).requires_grad(false)); }
 
-std::pair<Tensor, Tensor> run_causal_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Prompt& a) {
+// `low`: receives what rounding the output left, for a backward (16-bit types)
+std::pair<Tensor, Tensor> run_causal_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Prompt& a, Tensor* low = nullptr) {
     const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
     const c10::DeviceGuard guard(q.device());
     const Sizes z = sizes(q);
     const auto fp32 = q.options().dtype(at::kFloat).requires_grad(false);
     Tensor out = like(q), lse = q.dim() == 4 ? at::empty({z.B, z.H, z.N}, fp32) : at::empty({z.H, z.N}, fp32);
     if (out.numel() == 0) return {out, lse};
+    if (low && dtype_code(q) != SA2_F32) *low = like(q);
     int64_t s[12];
     put_strides(s, q);
     put_strides(s + 3, k);
     put_strides(s + 6, v);
     put_strides(s + 9, out);
-    check(causal_fwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(), (float*)lse.data_ptr(), ints(a.cu), a.cu.defined() ? (int)a.cu.numel() - 1 : 0,
-                        z.B, z.N, z.H, (int)k.size(-2), z.D, s, (float)a.scale, dtype_code(q), a.flags, stream(q)));
+    check(causal_fwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(), low && low->defined() ? low->data_ptr() : nullptr, (float*)lse.data_ptr(), ints(a.cu),
+                        a.cu.defined() ? (int)a.cu.numel() - 1 : 0, z.B, z.N, z.H, (int)k.size(-2), z.D, s, (float)a.scale, dtype_code(q), a.flags, stream(q)));
     return {out, lse};
 }
 
 // `needs`: bit t set = gradient t of (q, k, v) is wanted; the others stay undefined
-std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& out_, const Tensor& lse, const Tensor& dout_, unsigned needs, const Prompt& a) {
+std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& out_, const Tensor& low, const Tensor& lse, const Tensor& dout_, unsigned needs,
+                                           const Prompt& a) {
     const Tensor q = rows(q_), k = rows(k_), v = rows(v_), out = rows(out_), dout = rows(dout_);
     const c10::DeviceGuard guard(q.device());
     const Sizes z = sizes(q);
@@ -253,7 +256,7 @@ std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, co
     const Tensor* const t[8] = {&q, &k, &v, &out, &dout, g[0].defined() ? &g[0] : &q, g[1].defined() ? &g[1] : &k, g[2].defined() ? &g[2] : &v};
     for (int i = 0; i < 8; ++i) put_strides(s + 3 * i, *t[i]);
     auto ptr = [&](int i) { return g[i].defined() ? g[i].data_ptr() : nullptr; };
-    check(causal_bwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.const_data_ptr(), dout.const_data_ptr(), (const float*)lse.const_data_ptr(), ptr(0), ptr(1), ptr(2),
+    check(causal_bwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.const_data_ptr(), low.defined() ? low.const_data_ptr() : nullptr, dout.const_data_ptr(), (const float*)lse.const_data_ptr(), ptr(0), ptr(1), ptr(2),
                         ws.data_ptr(), (size_t)ws.numel(), ints(a.cu), a.cu.defined() ? (int)a.cu.numel() - 1 : 0, z.B, z.N, z.H, hk, z.D, s, (float)a.scale, dtype_code(q), a.flags, stream(q)));
     return g;
 }
@@ -261,8 +264,9 @@ std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, co
 struct CausalFormula : torch::autograd::Function<CausalFormula> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, Prompt a) {
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [out, lse] = run_causal_forward(q, k, v, a);
-        ctx->save_for_backward({q, k, v, out, lse, a.cu});
+        Tensor low;
+        auto [out, lse] = run_causal_forward(q, k, v, a, &low);
+        ctx->save_for_backward({q, k, v, out, lse, a.cu, low});
         ctx->saved_data["scale"] = a.scale;
         ctx->saved_data["flags"] = (int64_t)a.flags;
         return out;
@@ -273,7 +277,7 @@ struct CausalFormula : torch::autograd::Function<CausalFormula> {
         const Prompt a{s[5], ctx->saved_data["scale"].toDouble(), (unsigned)ctx->saved_data["flags"].toInt()};
         unsigned needs = 0;
         for (int i = 0; i < 3; ++i) needs |= (ctx->needs_input_grad(i) ? 1u : 0u) << i;
-        auto g = run_causal_backward(s[0], s[1], s[2], s[3], s[4], grads[0], needs, a);
+        auto g = run_causal_backward(s[0], s[1], s[2], s[3], s[6], s[4], grads[0], needs, a);
         return {g[0], g[1], g[2], Tensor()};
     }
 };
@@ -317,7 +321,7 @@ std::tuple<Maybe, Maybe, Maybe> causal_backward(const Tensor& q, const Tensor& k
     check_place("causal_attention", {out, lse, dout});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
-    auto g = run_causal_backward(q, k, v, out, lse, dout, needs, a);
+    auto g = run_causal_backward(q, k, v, out, Tensor(), lse, dout, needs, a);
     auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
     return {maybe(g[0]), maybe(g[1]), maybe(g[2])};
 }

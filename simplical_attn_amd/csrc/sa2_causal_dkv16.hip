@@ -22,6 +22,8 @@ constexpr int BUFFERS = 4, BLOCK = SUB * WAVES;            // keys per workgroup
 constexpr int STATS = 2 * TILE_ROWS * 4;                    // bytes of the row terms of a tile
 
 // ---- row terms: delta = sum_d dO O, stored as -delta, and -lse / scale ----------------------------------------------
+// O with what its rounding left, where the forward wrote that: from the rounded output alone delta carries half a step of every
+// value, which in sequences of up to a hundred rows makes dQ and dK 1.5 to 2.3 times as far off as their own rounding does.
 template <class E, int LANES>                               // lanes per row, 16 bytes each
 __global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, float* minus_lse, float* tops) {
     const int lane = threadIdx.x % LANES, per = THREADS / LANES;
@@ -45,12 +47,12 @@ __global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, float* 
             if (lane * 8 < p.D) {
                 const uint4 x = *(const uint4*)((const uint16_t*)p.out.p + p.out.off(b, n, h) + lane * 8);
                 const uint4 y = *(const uint4*)((const uint16_t*)p.dout.p + p.dout.off(b, n, h) + lane * 8);
-                const uint32_t* xs = &x.x;
-                const uint32_t* ys = &y.x;
+                const uint4 z = p.out_low ? *(const uint4*)((const uint16_t*)p.out_low + p.out.off(b, n, h) + lane * 8) : make_uint4(0, 0, 0, 0);
+                const uint32_t *xs = &x.x, *ys = &y.x, *zs = &z.x;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float y0 = E::lo(ys[i]), y1 = E::hi(ys[i]);
-                    sum = fmaf(E::lo(xs[i]), y0, fmaf(E::hi(xs[i]), y1, sum));
+                    sum = fmaf(E::lo(xs[i]) + E::lo(zs[i]), y0, fmaf(E::hi(xs[i]) + E::hi(zs[i]), y1, sum));
                     large = fmaxf(large, fmaxf(fabsf(y0), fabsf(y1)));
                 }
             }
@@ -248,7 +250,8 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, cons
         __builtin_amdgcn_sched_barrier(0);
     };
     auto rest = [&]() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); };
-    // A piece by itself: queries `q0` .. + 31, some of which do not see the wavefront's keys
+    // A piece by itself: queries `q0` .. + 31, some of which do not see the wavefront's keys.  dS goes in as two 16-bit parts here: in
+    // sequences of a few rows, whose sums cancel, its rounding alone took dK to 1.7 times the error that its own rounding leaves
     auto piece = [&](uint32_t buf, int sub, int q0) {
         const uint32_t sat = stats_at(buf, sub), rat = rows_at(buf, sub), cat = cols_at(buf, sub);
         static_for<8>([&](auto X) __attribute__((always_inline)) { load_stat(X, sat, st[0], dp[0]); });
@@ -258,7 +261,7 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, cons
         asm volatile("s_nop 15\n\ts_nop 15" : "+v"(st[0]));
         asm volatile("s_nop 15\n\ts_nop 15" : "+v"(dp[0]));
         const bool masked = q0 < mine + SUB - 1 || q0 == 0;
-        union { uint32_t u[8]; X8 v[2]; } zp, zd;
+        union { uint32_t u[8]; X8 v[2]; } zp, zd, zl;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float e[2], ds[2];
@@ -274,6 +277,7 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, cons
             }
             zp.u[i] = pack2<E>(e[0], e[1]);
             zd.u[i] = pack2<E>(ds[0], ds[1]);
+            zl.u[i] = pack2<E>(ds[0] - E::lo(zd.u[i]), ds[1] - E::hi(zd.u[i]));
         }
         static_for<4 * DT>([&](auto C) __attribute__((always_inline)) { load_col(C, cat); });
         bool odd = false;
@@ -285,9 +289,11 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, cons
             const uint32_t tile = buffer(buf) + (uint32_t)(sub * T::BYTES);
             guarded_sum<E, L, V0, D>(tile + Buffer<D>::SECOND, zp.v, [&](int i) { return q0 + i >= key; });
             guarded_sum<E, L, K0, D>(tile + Buffer<D>::FIRST, zd.v, [&](int i) { return q0 + i >= key && q0 + i > 0; });
+            guarded_sum<E, L, K0, D>(tile + Buffer<D>::FIRST, zl.v, [&](int i) { return q0 + i >= key && q0 + i > 0; });
         } else {
-            asm volatile("s_nop 3" : "+v"(zp.v[0]), "+v"(zp.v[1]), "+v"(zd.v[0]), "+v"(zd.v[1]));
+            asm volatile("s_nop 3" : "+v"(zp.v[0]), "+v"(zp.v[1]), "+v"(zd.v[0]), "+v"(zd.v[1]), "+v"(zl.v[0]), "+v"(zl.v[1]));
             static_for<4 * DT>([&](auto C) __attribute__((always_inline)) { second_mfma(C, zp.v, zd.v); });
+            static_for<2 * DT>([&](auto C) __attribute__((always_inline)) { second_mfma(LONE_C(decltype(C)::value + 2 * DT), zp.v, zl.v); });
             rest();
         }
     };

@@ -115,9 +115,9 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dq16_kernel(Causal p, const
         static_for<2 * DT>([&](auto J) __attribute__((always_inline)) { second_mfma(N, J, x); });
         rest();
     };
-    // dS of a unit; masked: the lane's query sees the piece's keys 0 .. seen
-    auto weigh = [&](const floatx16& x, const floatx16& y, int n, X8 (&z)[2], auto masked, int seen) {
-        union { uint32_t u[8]; X8 v[2]; } o;
+    // dS of a unit, and what its rounding left (for the pieces of the own tile: see sa2_causal_dkv16.hip); masked: the lane's query sees the piece's keys 0 .. seen
+    auto weigh = [&](const floatx16& x, const floatx16& y, int n, X8 (&z)[2], X8 (&rest)[2], auto masked, int seen) {
+        union { uint32_t u[8]; X8 v[2]; } o, low;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float e[2];
@@ -129,9 +129,12 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dq16_kernel(Causal p, const
                 if constexpr (decltype(masked)::value) e[j] = 8 * (r / 4) + 4 * half + r % 4 <= seen ? e[j] : 0.f;
             }
             o.u[i] = pack2<E>(e[0], e[1]);
+            low.u[i] = pack2<E>(e[0] - E::lo(o.u[i]), e[1] - E::hi(o.u[i]));
         }
         z[0] = o.v[0];
         z[1] = o.v[1];
+        rest[0] = low.v[0];
+        rest[1] = low.v[1];
     };
     // One step: first products of unit V + 2, second product of unit V, dS of unit V + 1; operands of the units after those, as
     // soon as the ones before have been read for the last time (two MFMAs later)
@@ -203,9 +206,15 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dq16_kernel(Causal p, const
                 // (the first query of a sequence has one weight, 1, whose gradient is zero)
                 const int at = mine + 32 * n + (lane & 31), seen = at ? at - from : -1;
                 first(N, st[0], dp[0]);
-                weigh(st[0], dp[0], n, w[0], std::true_type{}, seen);
-                if (odd) guarded_sum<E, L, S0 + n * DT * 16, D>(buf + (uint32_t)(Buffer<D>::FIRST + sub * T::BYTES), w[0], [&](int key) { return key <= seen; });
-                else second(N, w[0]);
+                weigh(st[0], dp[0], n, w[0], w[1], std::true_type{}, seen);
+                if (odd) {
+                    const uint32_t tile = buf + (uint32_t)(Buffer<D>::FIRST + sub * T::BYTES);
+                    guarded_sum<E, L, S0 + n * DT * 16, D>(tile, w[0], [&](int key) { return key <= seen; });
+                    guarded_sum<E, L, S0 + n * DT * 16, D>(tile, w[1], [&](int key) { return key <= seen; });
+                } else {
+                    second(N, w[0]);
+                    second(N, w[1]);
+                }
             }
         });
     };
@@ -231,7 +240,8 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dq16_kernel(Causal p, const
             load_rows(rows_at(base, 1));
         }
         load_cols(cols_at(base, 0));
-        weigh(st[0], dp[0], 0, w[0], no, 0);
+        X8 unused[2];
+        weigh(st[0], dp[0], 0, w[0], unused, no, 0);
         asm volatile("s_nop 3" : "+v"(w[0][0]), "+v"(w[0][1]));
         int t = 0;
         for (; t + LOOK < full; ++t) {
@@ -252,7 +262,7 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dq16_kernel(Causal p, const
         }
         rest();
         second(LONE_C(0), w[0]);
-        weigh(st[1], dp[1], NQ - 1, w[1], no, 0);
+        weigh(st[1], dp[1], NQ - 1, w[1], unused, no, 0);
         if constexpr (NQ == 1) load_cols(cols_at(here, 1));
         second(LONE_C(NQ - 1), w[1]);
         done = 2 * t + (NQ == 1 ? 2 : 1);

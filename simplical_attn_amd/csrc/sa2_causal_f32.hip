@@ -133,8 +133,38 @@ __global__ __launch_bounds__(THREADS) void causal_f32_fwd_kernel(Causal p, int t
         else weighted_rows<DP, DP, false>(vt, 0, w, acc, sees);
     }
     l += other_half(l);
-    store_own<T, DP>(p.out, s, qi, h, 0, p.D, wide, acc, l > 0.f || l != l ? 1.f / l : 0.f);
+    const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+    store_own<T, DP>(p.out, s, qi, h, 0, p.D, wide, acc, f);
+    if constexpr (sizeof(T) == 2)
+        if (p.out_low) {
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    T rounded;
+                    from_float(acc[i][j] * f, &rounded);
+                    acc[i][j] = acc[i][j] * f - to_float(rounded);
+                }
+            Tensor low = p.out;
+            low.p = p.out_low;
+            store_own<T, DP>(low, s, qi, h, 0, p.D, wide, acc, 1.f);
+        }
     if (half == 0 && qi < s.len) lse[qi] = l == 0.f ? -INFINITY : fmaf(m, fabsf(p.scale), logf(l));
+}
+
+// delta = sum_d dO O, O with what its rounding left: a wavefront per row
+template <class T>
+__global__ __launch_bounds__(THREADS) void causal_f32_delta_kernel(Causal p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+    if (r >= (int64_t)p.rows.B * p.rows.N * p.H) return;
+    const int h = (int)(r % p.H), n = (int)(r / p.H % p.rows.N), b = (int)(r / p.H / p.rows.N);
+    const int64_t at = p.out.off(b, n, h);
+    const T *out = (const T*)p.out.p + at, *low = p.out_low ? (const T*)p.out_low + at : nullptr, *dout = (const T*)p.dout.p + p.dout.off(b, n, h);
+    float sum = 0.f;
+    for (int d = lane; d < p.D; d += 64) sum = fmaf(to_float(out[d]) + (low ? to_float(low[d]) : 0.f), to_float(dout[d]), sum);
+    sum = wave_sum(sum);
+    if (lane == 0) p.delta[((int64_t)b * p.H + h) * p.rows.N + n] = sum;
 }
 
 // dQ: the wavefront owns 32 queries and sweeps the keys they see
@@ -307,6 +337,11 @@ int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st) {
         return for_width(p.D, [&](auto w) {
             constexpr int DP = decltype(w)::value, DO = DP > 128 ? 128 : DP;
             int rc = SA2_OK;
+            if (p.dq.p || p.dk.p) {
+                const int64_t blocks = ((int64_t)p.rows.B * p.rows.N * p.H + WAVES - 1) / WAVES;
+                causal_f32_delta_kernel<T><<<dim3((unsigned)blocks), dim3(THREADS), 0, st>>>(p);
+                if (hipGetLastError() != hipSuccess) return (int)SA2_ERR_LAUNCH_FAILED;
+            }
             if (p.dk.p || p.dv.p)
                 rc = launch(causal_f32_dkv_kernel<T, DP, DO>, p, (int64_t)p.rows.B * p.HK * (DP / DO), 2 * TILE * Pitch<DP>::value + 64, wide, st);
             if (rc == SA2_OK && p.dq.p) rc = launch(causal_f32_dq_kernel<T, DP>, p, (int64_t)p.rows.B * p.H, 2 * TILE * Pitch<DP>::value, wide, st);

@@ -325,11 +325,17 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(
         const int at = mine + 32 * n + (lane & 31);
         if (at < s.len) {
             uint16_t* row = (uint16_t*)p.out.p + row_offset(p.out, s, at, h);
+            uint16_t* low = p.out_low ? (uint16_t*)p.out_low + row_offset(p.out, s, at, h) : nullptr;
             static_for<4 * DT>([&](auto X) __attribute__((always_inline)) {
                 constexpr int x = decltype(X)::value;
                 const float4 o = L::template get_regs<O0 + n * DT * 16 + 4 * x>();
                 const int col = 8 * x + 4 * half;
-                if (col < p.D) *(uint2*)(row + col) = make_uint2(pack2<E>(o.x * f, o.y * f), pack2<E>(o.z * f, o.w * f));
+                if (col < p.D) {
+                    const float4 y = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+                    const uint2 r = make_uint2(pack2<E>(y.x, y.y), pack2<E>(y.z, y.w));
+                    *(uint2*)(row + col) = r;
+                    if (low) *(uint2*)(low + col) = make_uint2(pack2<E>(y.x - E::lo(r.x), y.y - E::hi(r.x)), pack2<E>(y.z - E::lo(r.y), y.w - E::hi(r.y)));
+                }
             });
             if (half == 0) lse[at] = fmaf(m[n], fabsf(p.scale), logf(sum));
         }

@@ -120,7 +120,7 @@ int sa2_cache_append(const void* k, const void* v, void* k_cache, void* v_cache,
     return launch_append(p, dtype, (hipStream_t)hip_stream);
 }
 
-int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, float* lse,
+int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, void* out_low, float* lse,
                        const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
                        const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream) {
     if (!q || !k || !v || !out || !lse || !strides) return SA2_ERR_NULL_POINTER;
@@ -131,9 +131,10 @@ int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, f
     p.k = tensor(k, strides, 1);
     p.v = tensor(v, strides, 2);
     p.out = tensor(out, strides, 3);
+    p.out_low = dtype == SA2_F32 ? nullptr : out_low;
     p.lse = lse;
     if (!stride_ok(p.q, B, N, H) || !stride_ok(p.out, B, N, H) || !stride_ok(p.k, B, N, HK) || !stride_ok(p.v, B, N, HK)) return SA2_ERR_BAD_STRIDE;
-    if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out}))
+    if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out}) && !((uintptr_t)out_low & 15u))
         return launch_causal16_fwd(p, dtype, (hipStream_t)hip_stream);
     return launch_causal_f32_fwd(p, dtype, (hipStream_t)hip_stream);
 }
@@ -145,13 +146,13 @@ size_t sa2_causal_bwd_workspace_bytes(int B, int N, int H, int HK, int D, int dt
     return 2 * delta_bytes(p) + CAUSAL16_TOPS * sizeof(float) + causal16_part_bytes(B, N, HK, p.G, D);
 }
 
-int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* out_low, const void* dout, const float* lse,
                         void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                         const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
                         const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream) {
     if (!q || !k || !v || !out || !dout || !lse || !workspace || !strides) return SA2_ERR_NULL_POINTER;
     Causal p;
-    int rc = make_causal(p, cu_seqlens, sequences, B, N, H, HK, D, scale, dtype);
+    const int rc = make_causal(p, cu_seqlens, sequences, B, N, H, HK, D, scale, dtype);
     if (rc != SA2_OK) return rc;
     Tensor* const t[8] = {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv};
     const void* const at[8] = {q, k, v, out, dout, dq, dk, dv};
@@ -160,20 +161,20 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
         if (at[i] && !stride_ok(*t[i], B, N, i == 1 || i == 2 || i > 5 ? HK : H)) return SA2_ERR_BAD_STRIDE;
     }
     if (((uintptr_t)workspace & 255u) || workspace_bytes < sa2_causal_bwd_workspace_bytes(B, N, H, HK, D, dtype, flags)) return SA2_ERR_WORKSPACE_TOO_SMALL;
+    p.out_low = dtype == SA2_F32 ? nullptr : const_cast<void*>(out_low);
     p.lse = const_cast<float*>(lse);
     p.delta = (float*)workspace;
     const hipStream_t st = (hipStream_t)hip_stream;
     if (!dq && !dk && !dv) return SA2_OK;
     // (-lse / scale is one of the 16-bit kernels' operands)
     if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv}) &&
-        fabsf(scale) > 1e-20f) {
+        fabsf(scale) > 1e-20f && !((uintptr_t)out_low & 15u)) {
         float* const minus_lse = (float*)((char*)workspace + delta_bytes(p));
         float* const tops = (float*)((char*)minus_lse + delta_bytes(p));
         p.part = tops + CAUSAL16_TOPS;
         return launch_causal16_bwd(p, dtype, minus_lse, tops, st);
     }
-    if (dq || dk) rc = launch_rowdot(p.out, p.dout, p.delta, B, N, H, D, dtype, st);
-    return rc == SA2_OK ? launch_causal_f32_bwd(p, dtype, st) : rc;
+    return launch_causal_f32_bwd(p, dtype, st);
 }
 
 size_t sa2_tree_workspace_bytes(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype, unsigned flags) {

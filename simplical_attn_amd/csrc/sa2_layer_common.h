@@ -23,8 +23,9 @@ struct Causal {
     int H, HK, G, D;
     float scale;
     Tensor q, k, v, out, dout, dq, dk, dv;     // gradients with p == nullptr: not requested
+    void* out_low;                             // laid out as out, or nullptr: what rounding out to 16 bits left
     float* lse;                                // [B,H,N]
-    float* delta;                              // [B,H,N]  sum_d dout*out
+    float* delta;                              // [B,H,N]  sum_d dout*(out + out_low)
     float* part;                               // partial sums (path specific)
 };
 

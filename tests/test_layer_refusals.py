@@ -159,7 +159,7 @@ def test_c_abi(lib):
     st = _lib.stride_array([(1024, 128, 64)] * 8)
 
     def causal(q=ONE, cu=None, seqs=0, B=1, N=8, H=2, HK=2, D=64, strides=st, dtype=1):
-        return lib.sa2_causal_forward(q, ONE, ONE, ONE, ONE, cu, seqs, B, N, H, HK, D, strides, 0.1, dtype, 0, None)
+        return lib.sa2_causal_forward(q, ONE, ONE, ONE, None, ONE, cu, seqs, B, N, H, HK, D, strides, 0.1, dtype, 0, None)
 
     assert causal(q=None) == -1 and causal(dtype=5) == -2 and causal(N=0) == -3 and causal(D=257) == -3 and causal(B=2, cu=ONE, seqs=3) == -3
     assert causal(HK=3) == -11 and causal(HK=0) == -11 and causal(N=1 << 30) == -9
@@ -168,7 +168,7 @@ def test_c_abi(lib):
     assert need >= 2 * 8 * 4 and lib.sa2_causal_bwd_workspace_bytes(1, 8, 3, 2, 64, 1, 0) == 0
 
     def backward(workspace=ONE, size=need, dq=ONE, H=2):
-        return lib.sa2_causal_backward(ONE, ONE, ONE, ONE, ONE, ONE, dq, None, None, workspace, size, None, 0, 1, 8, H, 2, 64, st, 0.1, 1, 0, None)
+        return lib.sa2_causal_backward(ONE, ONE, ONE, ONE, None, ONE, ONE, dq, None, None, workspace, size, None, 0, 1, 8, H, 2, 64, st, 0.1, 1, 0, None)
 
     assert backward(workspace=None) == -1 and backward(size=need - 1) == -6 and backward(workspace=ctypes.c_void_p(264)) == -6 and backward(H=3) == -11
     assert backward(dq=None) == 0                         # no gradient is wanted: nothing is launched

@@ -209,6 +209,7 @@ int sa2_tree_attention(const void* q, const void* k, const void* v, const void* 
     p.part = (float*)workspace;
     if (p.nsplit > 1 && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < tree_part_bytes(B, T, H, D, p.nsplit)))
         return SA2_ERR_WORKSPACE_TOO_SMALL;
+    if (!(flags & SA2_FLAG_FORCE_GENERIC) && tree16_supported(p, dtype)) return launch_tree16(p, dtype, (hipStream_t)hip_stream);
     return launch_tree_f32(p, dtype, (hipStream_t)hip_stream);
 }
 

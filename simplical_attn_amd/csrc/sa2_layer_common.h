@@ -92,6 +92,8 @@ size_t causal16_part_bytes(int B, int N, int HK, int G, int D);
 int launch_causal16_bwd(const Causal& p, int dtype, float* minus_lse, float* tops, hipStream_t st);
 int launch_causal16_dq(const Causal& p, int dtype, const float* tops, int ntops, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
+bool tree16_supported(const Tree& p, int dtype);
+int launch_tree16(const Tree& p, int dtype, hipStream_t st);
 
 namespace {
 

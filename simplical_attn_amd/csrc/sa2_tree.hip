@@ -100,7 +100,7 @@ __global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, i
         l += sum;
         m = m2;
         auto visible = [&](int j) { return (sees >> j & 1) != 0; };
-        if (drafted || __any(!seen && row < R)) weighted_rows<DP, DP, true>(vt, 0, w, acc, visible);
+        if (drafted) weighted_rows<DP, DP, true>(vt, 0, w, acc, visible);
         else weighted_rows<DP, DP, false>(vt, 0, w, acc, visible);
     }
     l += other_half(l);
@@ -127,6 +127,7 @@ __global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, i
         for (int x = 0; x < WAVES; ++x) {
             const float mx = stats[x * 64 + col], f = mx == -INFINITY ? (stats[x * 64 + 32 + col] == 0.f ? 0.f : 1.f) : exp2f((mx - top) * c);
             const float4 y = *(const float4*)(lds + x * 2 * TILE * PITCH + col * PITCH + d);
+            if (stats[x * 64 + 32 + col] == 0.f) continue;                 // nothing seen: its values may be anything
             sum += f * stats[x * 64 + 32 + col];
             o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
         }

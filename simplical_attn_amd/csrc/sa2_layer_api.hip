@@ -44,12 +44,13 @@ int check_tree(int B, int T, int H, int HK, int D, int dtype) {
     if (HK < 1 || H % HK) return SA2_ERR_BAD_HEADS;
     return T > SA2_TREE_NODES ? SA2_ERR_BAD_TREE : SA2_OK;
 }
-// Workgroups that share a sequence's keys: two per CU over the chip, each with at least eight tiles of 32 keys of what a
-// sequence may hold, at most 64 (how many it does hold is known on the device only)
-int tree_splits(int B, int T, int H, int HK, int D, int page_size, int table_width) {
-    const int64_t streams = (int64_t)B * HK * ((T * (H / HK) + 31) / 32), tiles = ((int64_t)page_size * table_width + 31) / 32;
-    int64_t n = (2 * CUS + streams - 1) / streams;
-    if (n > tiles / 8) n = tiles / 8;
+// Workgroups that share a sequence's keys: as many as are on the chip at once, one per CU, each with at least four tiles of 32
+// keys (one per wavefront) of what a sequence may hold, at most 64 (how many it does hold is known on the device only)
+int tree_splits(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype) {
+    const int rows = T * (H / HK), block = dtype == SA2_F32 || rows <= 32 ? 32 : 64;
+    const int64_t streams = (int64_t)B * HK * ((rows + block - 1) / block), tiles = ((int64_t)page_size * table_width + 31) / 32;
+    int64_t n = CUS / streams;
+    if (n > tiles / 4) n = tiles / 4;
     return n < 1 ? 1 : n > 64 ? 64 : (int)n;
 }
 
@@ -179,7 +180,7 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
 
 size_t sa2_tree_workspace_bytes(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype, unsigned flags) {
     if (check_tree(B, T, H, HK, D, dtype) != SA2_OK || page_size < 1 || table_width < 1) return 0;
-    return tree_part_bytes(B, T, H, D, tree_splits(B, T, H, HK, D, page_size, table_width));
+    return tree_part_bytes(B, T, H, D, tree_splits(B, T, H, HK, D, page_size, table_width, dtype));
 }
 
 int sa2_tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out,
@@ -205,7 +206,7 @@ int sa2_tree_attention(const void* q, const void* k, const void* v, const void* 
         !stride_ok(p.cache.k, pages, page_size, HK) || !stride_ok(p.cache.v, pages, page_size, HK))
         return SA2_ERR_BAD_STRIDE;
     p.parents = parents;
-    p.nsplit = tree_splits(B, T, H, HK, D, page_size, table_width);
+    p.nsplit = tree_splits(B, T, H, HK, D, page_size, table_width, dtype);
     p.part = (float*)workspace;
     if (p.nsplit > 1 && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < tree_part_bytes(B, T, H, D, p.nsplit)))
         return SA2_ERR_WORKSPACE_TOO_SMALL;

@@ -30,55 +30,61 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
     const int units = p.nsplit * p.B * p.HK, group = blockIdx.x / (8 * blocks), in = blockIdx.x - group * 8 * blocks;
     const int left = units - 8 * group < 8 ? units - 8 * group : 8, block = in / left, id = 8 * group + in - block * left;
     const int split = id % p.nsplit, stream = id / p.nsplit, b = stream / p.HK, hk = stream % p.HK;
+    // (a short table as a whole: its reads do not wait for the sequence's length)
+    const bool whole = p.cache.width <= 4 * THREADS;
+    if (p.cache.table && whole)
+        for (int i = threadIdx.x; i < p.cache.width; i += THREADS) pages[i] = p.cache.table[(int64_t)b * p.cache.width + i];
     const int held = tree_held(p, b), cached = (held + 31) / 32, all = cached + (p.T + 31) / 32;
     const int lo = (int)((int64_t)all * split / p.nsplit), hi = (int)((int64_t)all * (split + 1) / p.nsplit);
 
     // the share's part of the page table
-    const int page_size = p.cache.page_size, page0 = (int)((unsigned)(lo * 32) / (unsigned)page_size);
+    const int page_size = p.cache.page_size;
+    int page0 = 0;
     if (p.cache.table) {
-        const int end = (hi < cached ? hi * 32 : held) - 1, last = end < 0 ? -1 : (int)((unsigned)end / (unsigned)page_size);
-        for (int i = threadIdx.x; page0 + i <= last; i += THREADS) pages[i] = p.cache.table[(int64_t)b * p.cache.width + page0 + i];
+        if (!whole) {
+            page0 = (int)((unsigned)(lo * 32) / (unsigned)page_size);
+            const int end = (hi < cached ? hi * 32 : held) - 1, last = end < 0 ? -1 : (int)((unsigned)end / (unsigned)page_size);
+            for (int i = threadIdx.x; page0 + i <= last; i += THREADS) pages[i] = p.cache.table[(int64_t)b * p.cache.width + page0 + i];
+        }
         __syncthreads();
     }
-    // K and V rows of tile t to a buffer; returns which of its 32 rows are there (the others are zeros)
+    // K and V rows of tile t to a buffer; returns which of its 32 rows are there (the others are zeros).  One instruction brings RPW
+    // rows; where these lie in one page, one behind the other, their address is scalar arithmetic, elsewhere every lane asks the
+    // lane that found its row.
+    const int chunk = T::dma_chunk(lane), sub = T::dma_row(lane);
+    const bool pad = chunk * 8 >= p.D, together = p.D == D && (!p.cache.table || page_size % T::RPW == 0);
     auto request = [&](int t, uint32_t to) {
-        const int r = (t < cached ? t : t - cached) * 32 + (lane & 31);
-        const char *k = nullptr, *v = nullptr;
-        bool there;
-        if (t < cached) {
-            there = r < held;
-            int page = b, at = r;
-            if (p.cache.table && there) {
-                const int i = (int)((unsigned)r / (unsigned)page_size);
-                page = pages[i - page0];
-                at = r - i * page_size;
-                there = page >= 0 && page < p.cache.pages;
-            }
-            if (there) {
-                k = (const char*)p.cache.k.p + p.cache.k.off(page, at, hk) * 2;
-                v = (const char*)p.cache.v.p + p.cache.v.off(page, at, hk) * 2;
-            }
-        } else {
-            there = r < p.T;
-            if (there) {
-                k = (const char*)p.k.p + p.k.off(b, r, hk) * 2;
-                v = (const char*)p.v.p + p.v.off(b, r, hk) * 2;
-            }
+        const bool drafted = t >= cached;
+        const int r = (drafted ? t - cached : t) * 32 + (lane & 31);
+        const Tensor &K = drafted ? p.k : p.cache.k, &V = drafted ? p.v : p.cache.v;
+        int page = b, at = r;
+        bool there = r < (drafted ? p.T : held);
+        if (!drafted && p.cache.table && there) {
+            const int i = (int)((unsigned)r / (unsigned)page_size);
+            page = pages[i - page0];
+            at = r - i * page_size;
+            there = page >= 0 && page < p.cache.pages;
         }
-        const uint64_t ka = (uint64_t)(uintptr_t)k, va = (uint64_t)(uintptr_t)v;
-        const int chunk = T::dma_chunk(lane);
-        const bool pad = chunk * 8 >= p.D;
+        const uint32_t mask = (uint32_t)__ballot(there);
+        const uint32_t koff = (uint32_t)(sub * K.sn * 2) + chunk * 16, voff = (uint32_t)(sub * V.sn * 2) + chunk * 16;
+        const char *kb = (const char*)K.p + (int64_t)hk * K.sh * 2, *vb = (const char*)V.p + (int64_t)hk * V.sh * 2;
 #pragma unroll
         for (int g = 0; g < T::NGROUP; ++g) {
-            const int from = g * T::RPW + T::dma_row(lane);
-            auto take = [&](uint64_t a) {
-                const uint64_t x = (uint64_t)(uint32_t)__shfl((int)(a >> 32), from) << 32 | (uint32_t)__shfl((int)a, from);
-                return x && !pad ? (const void*)(uintptr_t)(x + chunk * 16) : (const void*)zero_chunk;
-            };
-            lds_request(take(ka), to + g * T::GROUP);
-            lds_request(take(va), to + T::BYTES + g * T::GROUP);
+            constexpr uint32_t FULL = (1u << T::RPW) - 1;
+            const uint32_t kto = to + g * T::GROUP, vto = kto + T::BYTES;
+            if (together && (mask >> (g * T::RPW) & FULL) == FULL) {
+                const int64_t pg = __builtin_amdgcn_readlane(page, g * T::RPW), row = __builtin_amdgcn_readlane(at, g * T::RPW);
+                lds_request(kb + (pg * K.sb + row * K.sn) * 2, koff, kto);
+                lds_request(vb + (pg * V.sb + row * V.sn) * 2, voff, vto);
+            } else {
+                const int from = g * T::RPW + sub;
+                const int64_t pg = __shfl(page, from), row = __shfl(at, from);
+                const bool ok = (mask >> from & 1) && !pad;
+                lds_request(ok ? (const void*)(kb + (pg * K.sb + row * K.sn) * 2 + chunk * 16) : (const void*)zero_chunk, kto);
+                lds_request(ok ? (const void*)(vb + (pg * V.sb + row * V.sn) * 2 + chunk * 16) : (const void*)zero_chunk, vto);
+            }
         }
-        return (uint32_t)__ballot(there);
+        return mask;
     };
     int t = lo + wave;
     uint32_t there[2] = {0, 0};
@@ -295,7 +301,7 @@ int launch(const Tree& p, hipStream_t st) {
 bool tree16_supported(const Tree& p, int dtype) {
     if (dtype == SA2_F32 || p.D % 8 || p.D > 128) return false;
     for (const Tensor* t : {&p.q, &p.k, &p.v, &p.cache.k, &p.cache.v, &p.out})
-        if (!aligned16(*t, 2, true)) return false;
+        if (!aligned16(*t, 2, true) || t->sn >= 1 << 22) return false;     // (a group's rows within 2^31 bytes of its first)
     return !p.cache.table || (p.cache.width + p.nsplit - 1) / p.nsplit + 128 / p.cache.page_size + 3 <= ENTRIES;
 }
 

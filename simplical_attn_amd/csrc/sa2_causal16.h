@@ -69,17 +69,19 @@ struct Fetch {
 // (groups of the two QuadTiles of a buffer follow one another)
 static_assert(QuadTile<64>::BYTES == QuadTile<64>::NGROUP * QuadTile<64>::GROUP && QuadTile<128>::BYTES == QuadTile<128>::NGROUP * QuadTile<128>::GROUP, "");
 
-// An infinity or NaN among eight 16-bit values
+// Eight 16-bit values each of whose exponents of ones carries into the top bit of its half: `any_odd` of these ORed together tells
+// whether one was an infinity or NaN
 template <class E>
-__device__ __forceinline__ bool not_finite(const typename E::x8& x) {
-    constexpr uint32_t EXP = E::DTYPE == SA2_BF16 ? 0x7f80u : 0x7c00u;
+__device__ __forceinline__ uint32_t odd_bits(const typename E::x8& x) {
+    constexpr uint32_t EXP = E::DTYPE == SA2_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = E::DTYPE == SA2_BF16 ? 0x00800080u : 0x04000400u;
     union { typename E::x8 v; uint32_t u[4]; } w;
     w.v = x;
-    bool odd = false;
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) odd = odd || (w.u[i] & EXP) == EXP || (w.u[i] >> 16 & EXP) == EXP;
-    return odd;
+    for (int i = 0; i < 4; ++i) bits |= (w.u[i] & EXP) + ONE;
+    return bits;
 }
+__device__ __forceinline__ bool any_odd(uint32_t bits) { return __any((bits & 0x80008000u) != 0); }
 // Sums S0 .. += tile^T w one row of the tile (in LDS) at a time and on the vector ALU, for the lanes that see the row: a weight of
 // zero would not keep an infinity or NaN out
 template <class E, class L, int S0, int D, class F>

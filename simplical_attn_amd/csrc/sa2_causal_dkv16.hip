@@ -280,12 +280,12 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, cons
             zl.u[i] = pack2<E>(ds[0] - E::lo(zd.u[i]), ds[1] - E::hi(zd.u[i]));
         }
         static_for<4 * DT>([&](auto C) __attribute__((always_inline)) { load_col(C, cat); });
-        bool odd = false;
+        uint32_t bits = 0;
         if (masked) {
 #pragma unroll
-            for (int i = 0; i < 4 * DT; ++i) odd = odd || not_finite<E>(cols[i]);
+            for (int i = 0; i < 4 * DT; ++i) bits |= odd_bits<E>(cols[i]);
         }
-        if (__any(odd)) {
+        if (any_odd(bits)) {
             const uint32_t tile = buffer(buf) + (uint32_t)(sub * T::BYTES);
             guarded_sum<E, L, V0, D>(tile + Buffer<D>::SECOND, zp.v, [&](int i) { return q0 + i >= key; });
             guarded_sum<E, L, K0, D>(tile + Buffer<D>::FIRST, zd.v, [&](int i) { return q0 + i >= key && q0 + i > 0; });

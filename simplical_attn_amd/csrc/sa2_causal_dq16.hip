@@ -194,12 +194,12 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dq16_kernel(Causal p, const
         load_rows(rows_at(buf, sub));
         load_cols(cols_at(buf, sub));
         const bool masked = from + SUB - 1 > mine || from + mine == 0;
-        bool odd = false;
+        uint32_t bits = 0;
         if (masked) {
 #pragma unroll
-            for (int j = 0; j < 2 * DT; ++j) odd = odd || not_finite<E>(cols[j]);
+            for (int j = 0; j < 2 * DT; ++j) bits |= odd_bits<E>(cols[j]);
         }
-        odd = __any(odd);
+        const bool odd = any_odd(bits);
         static_for<NQ>([&](auto N) __attribute__((always_inline)) {
             constexpr int n = decltype(N)::value;
             if (from <= mine + 32 * n + 31) {

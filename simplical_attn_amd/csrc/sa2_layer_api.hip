@@ -45,12 +45,12 @@ int check_tree(int B, int T, int H, int HK, int D, int dtype) {
     return T > SA2_TREE_NODES ? SA2_ERR_BAD_TREE : SA2_OK;
 }
 // Workgroups that share a sequence's keys: as many as are on the chip at once, one per CU, each with at least four tiles of 32
-// keys (one per wavefront) of what a sequence may hold, at most 64 (how many it does hold is known on the device only)
+// keys (one per wavefront; eight where the wavefronts share them) of what a sequence may hold, at most 64 (how many it does hold is known on the device only)
 int tree_splits(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype) {
-    const int rows = T * (H / HK), block = dtype == SA2_F32 || rows <= 32 ? 32 : 64;
+    const int rows = T * (H / HK), block = dtype == SA2_F32 ? 32 : tree16_rows(rows), least = block > 64 ? 8 : 4;
     const int64_t streams = (int64_t)B * HK * ((rows + block - 1) / block), tiles = ((int64_t)page_size * table_width + 31) / 32;
     int64_t n = CUS / streams;
-    if (n > tiles / 4) n = tiles / 4;
+    if (n > tiles / least) n = tiles / least;
     return n < 1 ? 1 : n > 64 ? 64 : (int)n;
 }
 

@@ -92,6 +92,11 @@ size_t causal16_part_bytes(int B, int N, int HK, int G, int D);
 int launch_causal16_bwd(const Causal& p, int dtype, float* minus_lse, float* tops, hipStream_t st);
 int launch_causal16_dq(const Causal& p, int dtype, const float* tops, int ntops, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
+// 16-bit kernels: rows that a workgroup has of R; up to 64 its wavefronts share them and divide the keys, beyond it is the other
+// way round (16/4 heads, 4 x 65536 rows, head_dim 128: 64 rows XXX, YYY)
+inline int tree16_rows(int R) { return R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256; }
+constexpr int TREE16_ENTRIES = 4096;                       // of the page table that a workgroup keeps in LDS
+int launch_tree_rows16(const Tree& p, int dtype, hipStream_t st);
 bool tree16_supported(const Tree& p, int dtype);
 int launch_tree16(const Tree& p, int dtype, hipStream_t st);
 

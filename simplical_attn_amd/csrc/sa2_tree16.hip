@@ -14,8 +14,6 @@
 namespace sa2 {
 namespace {
 
-constexpr int ENTRIES = 4096;                              // of the page table that a workgroup keeps in LDS
-
 template <class E, int D, int NQ>
 __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) {
     using T = QuadTile<D>;
@@ -148,14 +146,14 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int d = 0; d < DT; ++d) vf[ks][d] = quad_tile_column<D, X8>(va, 0, d, ks);
-        bool odd = false;
+        uint32_t bits = 0;
         if (drafted) {
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int d = 0; d < DT; ++d) odd = odd || not_finite<E>(vf[ks][d]);
-            odd = __any(odd);
+                for (int d = 0; d < DT; ++d) bits |= odd_bits<E>(vf[ks][d]);
         }
+        const bool odd = any_odd(bits);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             const uint32_t sees = drafted ? (uint32_t)(seen[n] >> first) & here : seen[n] ? here : 0u;
@@ -291,7 +289,7 @@ int launch(const Tree& p, hipStream_t st) {
     const int64_t grid = (int64_t)blocks * p.nsplit * p.B * p.HK;
     if (grid > 0x7fffffff) return SA2_ERR_TOO_LARGE;
     if (!allow_full_lds((const void*)kernel)) return SA2_ERR_LAUNCH_FAILED;
-    kernel<<<dim3((unsigned)grid), dim3(THREADS), WAVES * 4 * QuadTile<D>::BYTES + ENTRIES * 4, st>>>(p, blocks);
+    kernel<<<dim3((unsigned)grid), dim3(THREADS), WAVES * 4 * QuadTile<D>::BYTES + TREE16_ENTRIES * 4, st>>>(p, blocks);
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 
@@ -302,17 +300,17 @@ bool tree16_supported(const Tree& p, int dtype) {
     if (dtype == SA2_F32 || p.D % 8 || p.D > 128) return false;
     for (const Tensor* t : {&p.q, &p.k, &p.v, &p.cache.k, &p.cache.v, &p.out})
         if (!aligned16(*t, 2, true) || t->sn >= 1 << 22) return false;     // (a group's rows within 2^31 bytes of its first)
-    return !p.cache.table || (p.cache.width + p.nsplit - 1) / p.nsplit + 128 / p.cache.page_size + 3 <= ENTRIES;
+    return !p.cache.table || (p.cache.width + p.nsplit - 1) / p.nsplit + 256 / p.cache.page_size + 3 <= TREE16_ENTRIES;
 }
 
 int launch_tree16(const Tree& p, int dtype, hipStream_t st) {
     auto of = [&](auto e) {
         using E = decltype(e);
-        const bool two = p.T * p.G > 32;
+        const bool two = p.T * p.G > 32;                     // (more than 64: see below)
         if (p.D <= 64) return two ? launch<E, 64, 2>(p, st) : launch<E, 64, 1>(p, st);
         return two ? launch<E, 128, 2>(p, st) : launch<E, 128, 1>(p, st);
     };
-    const int rc = dtype == SA2_F16 ? of(ElemF16{}) : of(ElemBF16{});
+    const int rc = tree16_rows(p.T * p.G) > 64 ? launch_tree_rows16(p, dtype, st) : dtype == SA2_F16 ? of(ElemF16{}) : of(ElemBF16{});
     return rc == SA2_OK && p.nsplit > 1 ? launch_tree_join(p, dtype, st) : rc;
 }
 

@@ -24,7 +24,7 @@ struct Stage {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = i * THREADS + threadIdx.x, r = c / (DP / 4), d = c % (DP / 4) * 4;
-            x[i] = first + r < s.len ? load4((const T*)t.p + row_offset(t, s, first + r, h), d, D, wide) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[i] = load4((const T*)t.p + row_offset(t, s, first + r < s.len ? first + r : 0, h), d, D, wide, first + r < s.len);
         }
     }
     __device__ __forceinline__ void put(float* lds) const {
@@ -35,16 +35,6 @@ struct Stage {
         }
     }
 };
-// The wavefront's own 32 rows as second operand: slot (4c + i, half) holds column 8c + 4 * half + i of row lane % 32
-template <class T, int DP>
-__device__ __forceinline__ void own_rows(float (&x)[DP / 2], const Tensor& t, const Span& s, int first, int h, int D, bool wide, float factor) {
-    const int lane = threadIdx.x & 63, r = first + (lane & 31), half = lane >> 5;
-#pragma unroll
-    for (int c = 0; c < DP / 8; ++c) {
-        const float4 v = r < s.len ? load4((const T*)t.p + row_offset(t, s, r, h), 8 * c + 4 * half, D, wide) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[4 * c] = v.x * factor; x[4 * c + 1] = v.y * factor; x[4 * c + 2] = v.z * factor; x[4 * c + 3] = v.w * factor;
-    }
-}
 template <class T, int DO>
 __device__ __forceinline__ void store_own(const Tensor& t, const Span& s, int at, int h, int first, int D, bool wide, const floatx16 (&acc)[DO / 32], float factor) {
     const int half = (threadIdx.x & 63) >> 5;
@@ -64,8 +54,9 @@ __device__ __forceinline__ void fill_rows(const Tensor& t, const Span& s, int h,
     for (int i = threadIdx.x; i < s.len * D; i += THREADS) from_float(0.f, (T*)t.p + row_offset(t, s, i / D, h) + i % D);
 }
 
-template <class T, int DP>
-__global__ __launch_bounds__(THREADS) void causal_f32_fwd_kernel(Causal p, int tiles, bool wide) {
+template <class T, int DP, bool WIDE>
+__global__ __launch_bounds__(THREADS) void causal_f32_fwd_kernel(Causal p, int tiles) {
+    constexpr bool wide = WIDE;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float *kt = lds, *vt = lds + TILE * Pitch<DP>::value;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -168,8 +159,9 @@ __global__ __launch_bounds__(THREADS) void causal_f32_delta_kernel(Causal p) {
 }
 
 // dQ: the wavefront owns 32 queries and sweeps the keys they see
-template <class T, int DP>
-__global__ __launch_bounds__(THREADS) void causal_f32_dq_kernel(Causal p, int tiles, bool wide) {
+template <class T, int DP, bool WIDE>
+__global__ __launch_bounds__(THREADS) void causal_f32_dq_kernel(Causal p, int tiles) {
+    constexpr bool wide = WIDE;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float *kt = lds, *vt = lds + TILE * Pitch<DP>::value;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -220,8 +212,9 @@ __global__ __launch_bounds__(THREADS) void causal_f32_dq_kernel(Causal p, int ti
 
 // dK and dV: the wavefront owns 32 keys and sweeps the queries of all G heads that see them.  Columns `first` .. + DO of the
 // gradients: at head_dim 256 two workgroups share them, each with all of the two first products (the registers hold no more).
-template <class T, int DP, int DO>
-__global__ __launch_bounds__(THREADS) void causal_f32_dkv_kernel(Causal p, int tiles, bool wide) {
+template <class T, int DP, int DO, bool WIDE>
+__global__ __launch_bounds__(THREADS) void causal_f32_dkv_kernel(Causal p, int tiles) {
+    constexpr bool wide = WIDE;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float *qt = lds, *dt = lds + TILE * Pitch<DP>::value, *stats = dt + TILE * Pitch<DP>::value;     // lse * log2(e), delta
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -309,11 +302,11 @@ bool wide_rows(const Causal& p, std::initializer_list<const Tensor*> ts, bool ba
     return ok;
 }
 template <class K>
-int launch(K kernel, const Causal& p, int64_t streams, int floats, bool wide, hipStream_t st) {
+int launch(K kernel, const Causal& p, int64_t streams, int floats, hipStream_t st) {
     const int64_t tiles = count_tiles(p.rows, BLOCK);
     if (streams * tiles > 0x7fffffff) return SA2_ERR_TOO_LARGE;
     if (!allow_full_lds((const void*)kernel)) return SA2_ERR_LAUNCH_FAILED;
-    kernel<<<dim3((unsigned)(streams * tiles)), dim3(THREADS), floats * sizeof(float), st>>>(p, (int)tiles, wide);
+    kernel<<<dim3((unsigned)(streams * tiles)), dim3(THREADS), floats * sizeof(float), st>>>(p, (int)tiles);
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 
@@ -323,10 +316,8 @@ int launch_causal_f32_fwd(const Causal& p, int dtype, hipStream_t st) {
     return for_type(dtype, [&](auto* e) {
         using T = std::remove_pointer_t<decltype(e)>;
         const bool wide = wide_rows<T>(p, {&p.q, &p.k, &p.v, &p.out}, p.rows.B > 1);
-        return for_width(p.D, [&](auto w) {
-            constexpr int DP = decltype(w)::value;
-            return launch(causal_f32_fwd_kernel<T, DP>, p, (int64_t)p.rows.B * p.H, 2 * TILE * Pitch<DP>::value, wide, st);
-        });
+        if (p.D <= 128) return launch_causal_f32_few_fwd(p, dtype, wide, st);
+        return launch(wide ? causal_f32_fwd_kernel<T, 256, true> : causal_f32_fwd_kernel<T, 256, false>, p, (int64_t)p.rows.B * p.H, 2 * TILE * Pitch<256>::value, st);
     });
 }
 
@@ -334,19 +325,18 @@ int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st) {
     return for_type(dtype, [&](auto* e) {
         using T = std::remove_pointer_t<decltype(e)>;
         const bool wide = wide_rows<T>(p, {&p.q, &p.k, &p.v, &p.dout, &p.dq, &p.dk, &p.dv}, p.rows.B > 1);
-        return for_width(p.D, [&](auto w) {
-            constexpr int DP = decltype(w)::value, DO = DP > 128 ? 128 : DP;
-            int rc = SA2_OK;
-            if (p.dq.p || p.dk.p) {
-                const int64_t blocks = ((int64_t)p.rows.B * p.rows.N * p.H + WAVES - 1) / WAVES;
-                causal_f32_delta_kernel<T><<<dim3((unsigned)blocks), dim3(THREADS), 0, st>>>(p);
-                if (hipGetLastError() != hipSuccess) return (int)SA2_ERR_LAUNCH_FAILED;
-            }
-            if (p.dk.p || p.dv.p)
-                rc = launch(causal_f32_dkv_kernel<T, DP, DO>, p, (int64_t)p.rows.B * p.HK * (DP / DO), 2 * TILE * Pitch<DP>::value + 64, wide, st);
-            if (rc == SA2_OK && p.dq.p) rc = launch(causal_f32_dq_kernel<T, DP>, p, (int64_t)p.rows.B * p.H, 2 * TILE * Pitch<DP>::value, wide, st);
-            return rc;
-        });
+        if (p.dq.p || p.dk.p) {
+            const int64_t blocks = ((int64_t)p.rows.B * p.rows.N * p.H + WAVES - 1) / WAVES;
+            causal_f32_delta_kernel<T><<<dim3((unsigned)blocks), dim3(THREADS), 0, st>>>(p);
+            if (hipGetLastError() != hipSuccess) return (int)SA2_ERR_LAUNCH_FAILED;
+        }
+        if (p.D <= 128) return launch_causal_f32_few_bwd(p, dtype, wide, st);
+        int rc = SA2_OK;
+        if (p.dk.p || p.dv.p)
+            rc = launch(wide ? causal_f32_dkv_kernel<T, 256, 128, true> : causal_f32_dkv_kernel<T, 256, 128, false>, p, (int64_t)p.rows.B * p.HK * 2, 2 * TILE * Pitch<256>::value + 64, st);
+        if (rc == SA2_OK && p.dq.p)
+            rc = launch(wide ? causal_f32_dq_kernel<T, 256, true> : causal_f32_dq_kernel<T, 256, false>, p, (int64_t)p.rows.B * p.H, 2 * TILE * Pitch<256>::value, st);
+        return rc;
     });
 }
 

@@ -8,8 +8,6 @@
 namespace sa2 {
 namespace {
 
-constexpr int AHEAD = 1;
-
 // The keys of a workgroup's block of queries, as the sweep takes them (sa2_sweep16.h)
 template <int D>
 struct CausalKeys {
@@ -76,7 +74,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(
     CausalKeys<D> keys{fetch, padded, mine < s.len, last, mine, ROWS, tiles, 0, 0};
     keys.full = keys.active ? mine / TILE_ROWS : 0;
     keys.pieces = keys.active ? (mine + ROWS) / SUB : 0;
-    sweep16<E, D, NQ, AHEAD>(keys, base, c, m, l);
+    sweep16<E, D, NQ>(keys, base, c, m, l);
     static_for<NQ>([&](auto N) __attribute__((always_inline)) {
         constexpr int n = decltype(N)::value;
         const float sum = l[n] + other_half(l[n]), f = 1.f / sum;
@@ -106,7 +104,7 @@ int launch(const Causal& p, hipStream_t st) {
     const int64_t grid = (int64_t)p.rows.B * p.H * count_tiles(p.rows, 32 * NQ * WAVES);
     if (grid > 0x7fffffff) return SA2_ERR_TOO_LARGE;
     if (!allow_full_lds((const void*)kernel)) return SA2_ERR_LAUNCH_FAILED;
-    kernel<<<dim3((unsigned)grid), dim3(THREADS), sweep_buffers(AHEAD) * Buffer<D>::BYTES, st>>>(p, p.D != D);
+    kernel<<<dim3((unsigned)grid), dim3(THREADS), BUFFERS * Buffer<D>::BYTES, st>>>(p, p.D != D);
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 

@@ -16,20 +16,25 @@ __device__ __forceinline__ floatx16 zero16() {
     return z;
 }
 
-// Columns d .. d+3 of a row of D, zeros behind it.  `wide`: rows on the 16-byte grid (fp32) or 8-byte grid, D a multiple of 4
+// Columns d .. d+3 of a row of D, zeros behind it and where the row is not `there` (`row` can be read all the same: as a branch around
+// every load this cost twice the time of the products).  `wide`: rows on the 16-byte grid (fp32) or 8-byte grid, D a multiple of 4
 template <class T>
-__device__ __forceinline__ float4 load4(const T* row, int d, int D, bool wide) {
+__device__ __forceinline__ float4 load4(const T* row, int d, int D, bool wide, bool there) {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (wide) {
-        if (d < D) {
-            if constexpr (sizeof(T) == 4) x = *(const float4*)(row + d);
-            else {
-                union { uint2 u; T e[4]; } w;
-                w.u = *(const uint2*)(row + d);
-                x = make_float4(to_float(w.e[0]), to_float(w.e[1]), to_float(w.e[2]), to_float(w.e[3]));
-            }
+        const bool ok = there && d < D;
+        const T* from = row + (d < D ? d : 0);
+        if constexpr (sizeof(T) == 4) x = *(const float4*)from;
+        else {
+            union { uint2 u; T e[4]; } w;
+            w.u = *(const uint2*)from;
+            x = make_float4(to_float(w.e[0]), to_float(w.e[1]), to_float(w.e[2]), to_float(w.e[3]));
         }
-    } else {
+        x.x = ok ? x.x : 0.f;
+        x.y = ok ? x.y : 0.f;
+        x.z = ok ? x.z : 0.f;
+        x.w = ok ? x.w : 0.f;
+    } else if (there) {
         float* y = &x.x;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -56,6 +61,17 @@ __device__ __forceinline__ void store4(T* row, int d, int D, bool wide, float4 x
 template <int DP>
 struct Pitch { static constexpr int value = DP + 4; };
 
+// The wavefront's own 32 rows as second operand: slot (4c + i, half) holds column 8c + 4 * half + i of row lane % 32
+template <class T, int DP>
+__device__ __forceinline__ void own_rows(float (&x)[DP / 2], const Tensor& t, const Span& s, int first, int h, int D, bool wide, float factor) {
+    const int lane = threadIdx.x & 63, r = first + (lane & 31), half = lane >> 5;
+    const T* row = (const T*)t.p + row_offset(t, s, r < s.len ? r : 0, h);
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+        const float4 v = load4(row, 8 * c + 4 * half, D, wide, r < s.len);
+        x[4 * c] = v.x * factor; x[4 * c + 1] = v.y * factor; x[4 * c + 2] = v.z * factor; x[4 * c + 3] = v.w * factor;
+    }
+}
 // [tile rows] x [own rows]: rows of the tile in the registers, own ones in the lanes
 template <int DP>
 __device__ __forceinline__ floatx16 tile_product(const float* lds, const float (&own)[DP / 2]) {

@@ -81,6 +81,9 @@ int launch_rotary(const Rotary& p, int dtype, hipStream_t st);
 int launch_append(const Append& p, int dtype, hipStream_t st);
 int launch_causal_f32_fwd(const Causal& p, int dtype, hipStream_t st);
 int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st);
+// the same for few rows, head_dim up to 128: the four wavefronts of a workgroup share its 32 rows and divide what these see
+int launch_causal_f32_few_fwd(const Causal& p, int dtype, bool wide, hipStream_t st);
+int launch_causal_f32_few_bwd(const Causal& p, int dtype, bool wide, hipStream_t st);
 // bf16 and fp16 with a head_dim up to 128 that is a multiple of 8, rows on the 16-byte grid
 bool causal16_supported(int D, int dtype);
 bool causal16_layout(const Causal& p, std::initializer_list<const Tensor*> ts);
@@ -93,7 +96,7 @@ int launch_causal16_bwd(const Causal& p, int dtype, float* minus_lse, float* top
 int launch_causal16_dq(const Causal& p, int dtype, const float* tops, int ntops, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
 // 16-bit kernels: rows that a workgroup has of R; up to 64 its wavefronts share them and divide the keys, beyond it is the other
-// way round (16/4 heads, 4 x 65536 rows, head_dim 128: 64 rows XXX, YYY)
+// way round (16/4 heads, 4 x 65536 cached rows, head_dim 128, 192 rows: 398 us dividing keys, 161 dividing rows; 64 rows: AAA, BBB)
 inline int tree16_rows(int R) { return R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256; }
 constexpr int TREE16_ENTRIES = 4096;                       // of the page table that a workgroup keeps in LDS
 int launch_tree_rows16(const Tree& p, int dtype, hipStream_t st);

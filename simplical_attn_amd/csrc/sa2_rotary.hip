@@ -4,8 +4,8 @@
 // pair is (2j, 2j+1) of the rotated part (interleaved) or (j, j + rot/2).  The gradient is the same rotation by the
 // opposite angle.  Columns from rot on are copied.
 //
-// Bound by memory: every element is read once and written once.  A thread keeps the cosines and sines of V pairs (one or
-// two 16-byte chunks of a row) and goes through heads of q and of k with them, so that the angles, which cost about 40
+// Bound by memory: every element is read once and written once.  A thread keeps the cosines and sines of the pairs of one
+// 16-byte chunk of a row (interleaved) or of two, half a rotated part apart, and goes through heads of q and of k with them, so that the angles, which cost about 40
 // instructions each, are shared by the heads and never lie in memory.  Angles: the product and its reduction to an eighth
 // of a turn in 64 bits (a position of 10^6 leaves 10^-10 of a radian), the series of sine and cosine in 32.
 #include "sa2_layer_common.h"
@@ -34,17 +34,23 @@ struct Split {
     int rows, share, units;
 };
 
+// Elements of a chunk V, pairs of a thread: an interleaved chunk holds V / 2 whole pairs
+template <int V, bool INTERLEAVED>
+constexpr int pairs_of() { return INTERLEAVED && V > 1 ? V / 2 : V; }
+
 template <class T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(THREADS) void rotary_kernel(Rotary p, Split sp) {
+    constexpr bool ONE = INTERLEAVED && V > 1;                              // one chunk, not two
+    constexpr int NP = pairs_of<V, INTERLEAVED>();
     const int64_t total = (int64_t)p.rows.B * p.rows.N;
-    const int per_row = sp.share * sp.units, turning = p.rot / 2 / V;
+    const int per_row = sp.share * sp.units, turning = p.rot / 2 / NP;
     for (int it = threadIdx.x; it < sp.rows * per_row; it += THREADS) {
         const int rl = it / per_row, rest = it - rl * per_row, first = rest / sp.units, unit = rest - first * sp.units;
         const int64_t row = (int64_t)blockIdx.x * sp.rows + rl;
         if (row >= total) break;
         const int b = p.rows.B == 1 ? 0 : (int)(row / p.rows.N), n = (int)(row - (int64_t)b * p.rows.N);
         const bool turns = unit < turning;
-        float c[V], s[V];
+        float c[NP], s[NP];
         int d0, d1;
         if (turns) {
             double pos;
@@ -54,26 +60,27 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(Rotary p, Split sp) {
                 pos = sq < 0 ? 0.0 : (double)(n - p.rows.cu[sq]);
             } else pos = (double)n;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                turn(pos, p.frequencies[unit * V + i], p.amplitude, c[i], s[i]);
+            for (int i = 0; i < NP; ++i) {
+                turn(pos, p.frequencies[unit * NP + i], p.amplitude, c[i], s[i]);
                 if (p.inverse) s[i] = -s[i];
             }
-            d0 = INTERLEAVED ? 2 * V * unit : V * unit;
-            d1 = INTERLEAVED ? d0 + V : d0 + p.rot / 2;
+            d0 = INTERLEAVED ? 2 * NP * unit : V * unit;
+            d1 = INTERLEAVED ? d0 + 1 : d0 + p.rot / 2;
         } else {
             d0 = d1 = p.rot + (unit - turning) * V;
         }
         constexpr int AHEAD = 4;                                            // heads with their loads under way together
         const int heads = p.H + p.HK;
         for (int h0 = first; h0 < heads; h0 += AHEAD * sp.share) {
-            float x[AHEAD][V], y[AHEAD][V];
+            float x[AHEAD][V], y[ONE ? 1 : AHEAD][V];
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 const int h = h0 + i * sp.share;
                 if (h < heads) {
                     const T* src = h < p.H ? (const T*)p.q.p + p.q.off(b, n, h) : (const T*)p.k.p + p.k.off(b, n, h - p.H);
                     load_floats<T, V>(src + d0, x[i]);
-                    if (turns) load_floats<T, V>(src + d1, y[i]);
+                    if constexpr (!ONE)
+                        if (turns) load_floats<T, V>(src + d1, y[i]);
                 }
             }
 #pragma unroll
@@ -82,38 +89,28 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(Rotary p, Split sp) {
                 if (h < heads) {
                     T* dst = h < p.H ? (T*)p.q_out.p + p.q_out.off(b, n, h) : (T*)p.k_out.p + p.k_out.off(b, n, h - p.H);
                     if (turns) {
-                        float u[V], w[V];
 #pragma unroll
-                        for (int j = 0; j < V; ++j) {
-                            // interleaved: the two chunks hold V pairs one behind the other
-                            float& a0 = INTERLEAVED ? (2 * j < V ? x[i][2 * j % V] : y[i][2 * j % V]) : x[i][j];
-                            float& a1 = INTERLEAVED ? (V == 1 ? y[i][0] : 2 * j < V ? x[i][(2 * j + 1) % V] : y[i][(2 * j + 1) % V]) : y[i][j];
+                        for (int j = 0; j < NP; ++j) {
+                            float& a0 = ONE ? x[i][2 * j % V] : x[i][j];
+                            float& a1 = ONE ? x[i][(2 * j + 1) % V] : y[ONE ? 0 : i][j];
                             const float r0 = fmaf(-a1, s[j], a0 * c[j]), r1 = fmaf(a0, s[j], a1 * c[j]);
-                            if constexpr (INTERLEAVED) {
-                                if (2 * j < V) u[2 * j % V] = r0; else w[2 * j % V] = r0;
-                                if (V == 1) w[0] = r1;
-                                else if (2 * j < V) u[(2 * j + 1) % V] = r1;
-                                else w[(2 * j + 1) % V] = r1;
-                            } else {
-                                u[j] = r0;
-                                w[j] = r1;
-                            }
+                            a0 = r0;
+                            a1 = r1;
                         }
-                        store_floats<T, V>(dst + d0, u);
-                        store_floats<T, V>(dst + d1, w);
-                    } else {
-                        store_floats<T, V>(dst + d0, x[i]);
                     }
+                    store_floats<T, V>(dst + d0, x[i]);
+                    if constexpr (!ONE)
+                        if (turns) store_floats<T, V>(dst + d1, y[i]);
                 }
             }
         }
     }
 }
 
-template <class T, int V>
+template <class T, int V, bool INTERLEAVED>
 int launch(const Rotary& p, hipStream_t st) {
     Split sp;
-    sp.units = p.rot / 2 / V + (p.D - p.rot) / V;
+    sp.units = p.rot / 2 / pairs_of<V, INTERLEAVED>() + (p.D - p.rot) / V;
     const int64_t rows = (int64_t)p.rows.B * p.rows.N;
     const int heads = p.H + p.HK;
     // Four heads per thread where that leaves the chip two wavefronts per SIMD, one where it does not
@@ -122,8 +119,7 @@ int launch(const Rotary& p, hipStream_t st) {
     sp.rows = per_row >= THREADS ? 1 : THREADS / per_row;
     const int64_t blocks = (rows + sp.rows - 1) / sp.rows;
     if (blocks > 0x7fffffff) return SA2_ERR_TOO_LARGE;
-    if (p.interleaved) rotary_kernel<T, V, true><<<dim3((unsigned)blocks), dim3(THREADS), 0, st>>>(p, sp);
-    else rotary_kernel<T, V, false><<<dim3((unsigned)blocks), dim3(THREADS), 0, st>>>(p, sp);
+    rotary_kernel<T, V, INTERLEAVED><<<dim3((unsigned)blocks), dim3(THREADS), 0, st>>>(p, sp);
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 
@@ -135,9 +131,10 @@ int launch_rotary(const Rotary& p, int dtype, hipStream_t st) {
         constexpr int V = 16 / sizeof(T), S = sizeof(T);
         const bool batched = p.rows.B > 1, k = p.HK > 0;
         // 16-byte chunks where no pair and no copied column straddles one, single elements elsewhere
-        const bool wide = p.rot % (2 * V) == 0 && p.D % V == 0 && aligned16(p.q, S, batched) && aligned16(p.q_out, S, batched) &&
+        const bool wide = p.rot % (p.interleaved ? V : 2 * V) == 0 && p.D % V == 0 && aligned16(p.q, S, batched) && aligned16(p.q_out, S, batched) &&
                           (!k || (aligned16(p.k, S, batched) && aligned16(p.k_out, S, batched)));
-        return wide ? launch<T, V>(p, st) : launch<T, 1>(p, st);
+        if (p.interleaved) return wide ? launch<T, V, true>(p, st) : launch<T, 1, true>(p, st);
+        return wide ? launch<T, V, false>(p, st) : launch<T, 1, false>(p, st);
     });
 }
 

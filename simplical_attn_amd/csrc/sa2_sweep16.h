@@ -18,7 +18,7 @@
 namespace sa2 {
 namespace {
 
-constexpr int sweep_buffers(int ahead) { return ahead + 2; }
+constexpr int BUFFERS = 3;
 
 template <class E> struct RefLimit;
 template <> struct RefLimit<ElemBF16> { static constexpr float value = 1.152921504606847e18f; };   // 2^60
@@ -37,15 +37,14 @@ struct SweepRegs : Lone<(D * NQ > 128 ? 192 : 96)> {
 //   sees(n, piece)              what the lane's row of block n sees of a piece, bit by key
 //   guarded(piece)              values that some row does not see may be infinite or NaN
 // Queries lie in their registers; outputs are left in theirs, in units of e^(scale m), with the lane's part of their sums in l.
-// AHEAD: tiles on their way beside the one that is waited for; LDS holds sweep_buffers(AHEAD) tiles from `base` on.
+// LDS holds BUFFERS tiles from `base` on (with a fourth, and requests two tiles ahead, times were the same).
 // c: |scale| log2(e).  All wavefronts of the workgroup call it.
-template <class E, int D, int NQ, int AHEAD, class SRC>
+template <class E, int D, int NQ, class SRC>
 __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, float (&m)[NQ], float (&l)[NQ]) {
     using T = QuadTile<D>;
     using X8 = typename E::x8;
     using L = SweepRegs<D, NQ>;
     constexpr int KK = D / 16, DT = D / 32, O0 = L::O0, Q0 = L::Q0;
-    constexpr int BUFFERS = sweep_buffers(AHEAD);
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const uint32_t row_lane = T::row_lane(lane), column_lane = T::column_lane(lane);
     auto after = [&](uint32_t buf) { return buf == base + (BUFFERS - 1) * Buffer<D>::BYTES ? base : buf + Buffer<D>::BYTES; };
@@ -176,13 +175,11 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
         src.request(t, arriving);
         arriving = after(arriving);
     };
-    auto arrive = [&]() {                                                  // the next one too; its successors are on their way
-        if (AHEAD == 2 && released + 2 < src.tiles) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Fetch<D>::INSTR) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0xc07f);                                // (lgkmcnt(0): what LDS gave has come)
-        __builtin_amdgcn_s_barrier();
+    auto arrive = [&]() {                                                  // the next one too; its successor is on its way
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
         ++released;
-        if (released + AHEAD < src.tiles) request(released + AHEAD);
+        if (released + 1 < src.tiles) request(released + 1);
     };
     // One piece of 32 keys by itself, with masks, and values that a weight of zero would not keep out.  Rows that have no reference point
     // take their maximum here; `safe`: all rows do, as the running one.  The weights of a block stand between the MFMAs of the other.
@@ -237,7 +234,6 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
         released = -1;
         arriving = base;
         request(0);
-        if (AHEAD == 2 && src.tiles > 1) request(1);
         arrive();
         rest();
         static_for<NQ * DT * 4>([&](auto X) __attribute__((always_inline)) { L::template set_regs<O0 + 4 * decltype(X)::value>(0u, 0u, 0u, 0u); });

@@ -13,8 +13,9 @@ namespace {
 template <int DP>
 constexpr int waves_of() { return DP > 128 ? 2 : 4; }      // (the tiles of four would not fit LDS)
 
-template <class T, int DP>
-__global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, int blocks, bool wide) {
+template <class T, int DP, bool WIDE>
+__global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, int blocks) {
+    constexpr bool wide = WIDE;
     constexpr int WAVES = waves_of<DP>(), PITCH = Pitch<DP>::value;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -35,7 +36,7 @@ __global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, i
     const float sign = p.scale < 0.f ? -1.f : 1.f, c = fabsf(p.scale) * LOG2E;
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) {
-        const float4 v = row < R ? load4((const T*)p.q.p + p.q.off(b, node, h), 8 * i + 4 * half, p.D, wide) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 v = load4((const T*)p.q.p + p.q.off(b, node, h), 8 * i + 4 * half, p.D, wide, row < R);
         q[4 * i] = v.x * sign; q[4 * i + 1] = v.y * sign; q[4 * i + 2] = v.z * sign; q[4 * i + 3] = v.w * sign;
     }
     floatx16 acc[DP / 32];
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, i
         const bool drafted = t >= cached;
         const int first = (drafted ? t - cached : t) * TILE, r = first + (lane & 31);
         bool there;
-        const T *krow = nullptr, *vrow = nullptr;
+        const T *krow = (const T*)p.q.p, *vrow = krow;                     // (can be read)
         if (drafted) {
             there = r < p.T;
             if (there) {
@@ -66,9 +67,8 @@ __global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, i
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i) {
             const int d = half * (DP / 2) + 4 * i;
-            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-            *(float4*)(kt + (lane & 31) * PITCH + d) = there ? load4(krow, d, p.D, wide) : z;
-            *(float4*)(vt + (lane & 31) * PITCH + d) = there ? load4(vrow, d, p.D, wide) : z;
+            *(float4*)(kt + (lane & 31) * PITCH + d) = load4(krow, d, p.D, wide, there);
+            *(float4*)(vt + (lane & 31) * PITCH + d) = load4(vrow, d, p.D, wide, there);
         }
         __threadfence_block();
         __builtin_amdgcn_wave_barrier();
@@ -208,9 +208,9 @@ int launch_tree_f32(const Tree& p, int dtype, hipStream_t st) {
             const int blocks = (p.T * p.G + TILE - 1) / TILE;
             const int64_t grid = (int64_t)blocks * p.nsplit * p.B * p.HK;
             if (grid > 0x7fffffff) return (int)SA2_ERR_TOO_LARGE;
-            const auto kernel = tree_f32_kernel<T, DP>;
+            const auto kernel = wide_tree<T>(p) ? tree_f32_kernel<T, DP, true> : tree_f32_kernel<T, DP, false>;
             if (!allow_full_lds((const void*)kernel)) return (int)SA2_ERR_LAUNCH_FAILED;
-            kernel<<<dim3((unsigned)grid), dim3(64 * WAVES), (WAVES * 2 * TILE * Pitch<DP>::value + WAVES * 64) * sizeof(float), st>>>(p, blocks, wide_tree<T>(p));
+            kernel<<<dim3((unsigned)grid), dim3(64 * WAVES), (WAVES * 2 * TILE * Pitch<DP>::value + WAVES * 64) * sizeof(float), st>>>(p, blocks);
             return (int)(hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED);
         });
     });

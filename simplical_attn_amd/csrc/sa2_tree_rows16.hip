@@ -9,8 +9,6 @@
 namespace sa2 {
 namespace {
 
-constexpr int AHEAD = 2;                                   // (one tile ahead, the memory's latency was what the sweep waited for: 161 us instead of XXX)
-
 template <int D, int NQ>
 struct TreeKeys {
     using T = QuadTile<D>;
@@ -78,7 +76,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree_rows16_kernel(Tree p, int blo
     using L = SweepRegs<D, NQ>;
     constexpr int KK = D / 16, DT = D / 32, ROWS = 32 * NQ, BLOCK = ROWS * WAVES;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    int32_t* const pages = (int32_t*)(lds + sweep_buffers(AHEAD) * Buffer<D>::BYTES);
+    int32_t* const pages = (int32_t*)(lds + BUFFERS * Buffer<D>::BYTES);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, R = p.T * p.G;
     // (stream, split) units, the blocks of rows of one of them on one XCD
     const int units = p.nsplit * p.B * p.HK, group = blockIdx.x / (8 * blocks), in = blockIdx.x - group * 8 * blocks;
@@ -144,7 +142,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree_rows16_kernel(Tree p, int blo
     });
     float m[NQ], l[NQ];
     if (keys.tiles > 0) {
-        sweep16<E, D, NQ, AHEAD>(keys, lds_address(lds), c, m, l);
+        sweep16<E, D, NQ>(keys, lds_address(lds), c, m, l);
     } else {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -181,7 +179,7 @@ int launch(const Tree& p, hipStream_t st) {
     const int64_t grid = (int64_t)blocks * p.nsplit * p.B * p.HK;
     if (grid > 0x7fffffff) return SA2_ERR_TOO_LARGE;
     if (!allow_full_lds((const void*)kernel)) return SA2_ERR_LAUNCH_FAILED;
-    kernel<<<dim3((unsigned)grid), dim3(THREADS), sweep_buffers(AHEAD) * Buffer<D>::BYTES + TREE16_ENTRIES * 4, st>>>(p, blocks);
+    kernel<<<dim3((unsigned)grid), dim3(THREADS), BUFFERS * Buffer<D>::BYTES + TREE16_ENTRIES * 4, st>>>(p, blocks);
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 

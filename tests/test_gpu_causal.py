@@ -155,6 +155,91 @@ def test_large_scores(dtype):
     _compare(q, k, v, dout, out, lse, grads, [((0,), (0,))], 128 ** -0.5, dtype, 0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("B,N,H,HK,D", [(1, 300, 128, 16, 128), (8, 513, 16, 4, 64), (4, 1100, 16, 16, 128), (3, 700, 32, 8, 80), (2, 1500, 24, 24, 64)])
+def test_many_rows(B, N, H, HK, D, dtype):
+    """Sizes at which a wavefront owns 64 queries; some heads are compared."""
+    q, k, v, dout = _inputs((B, N), H, HK, D, dtype, N + D)
+    out, lse, grads = _all(q, k, v, dout, 0)
+    G = H // HK
+    for b, hk in ((0, 0), (B - 1, HK - 1), (B // 2, HK // 2)):
+        hs, ks = slice(hk * G, hk * G + G), slice(hk, hk + 1)
+        part = lambda x, heads: x[b:b + 1][:, :, heads]
+        _compare(part(q, hs), part(k, ks), part(v, ks), part(dout, hs), part(out, hs), lse[b:b + 1, hs],
+                 [part(x, h) for x, h in zip(grads, (hs, ks, ks))], [((0,), (0,))], D ** -0.5, dtype, 0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("H,HK,D", [(2, 1, 64), (2, 2, 128), (96, 8, 64), (96, 8, 128)])
+def test_later_keys_far_above_the_first(H, HK, D, dtype):
+    """Scores that exceed the ones of a row's first 32 keys by e^60 and more: the workgroup sweeps its keys a second time."""
+    N = 600
+    q, k, v, dout = _inputs((1, N), H, HK, D, dtype, H + D, std=4.0)
+    k[:, :32] *= 0.01
+    out, lse, grads = _all(q, k, v, dout, 0)
+    G = H // HK
+    for hk in (0, HK - 1):
+        hs, ks = slice(hk * G, hk * G + G), slice(hk, hk + 1)
+        _compare(q[:, :, hs], k[:, :, ks], v[:, :, ks], dout[:, :, hs], out[:, :, hs], lse[:, hs], [grads[0][:, :, hs], grads[1][:, :, ks], grads[2][:, :, ks]],
+                 [((0,), (0,))], D ** -0.5, dtype, 0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_gradients_of_autograd(dtype):
+    """The training path, which also keeps what rounding the output left; expanded keys get the sum of their gradients."""
+    q, k, v, dout = _inputs((2, 150), 4, 2, 64, dtype, 43)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = sa.causal_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, dout)
+    _, lse = sa.causal_attention_forward(q.detach(), k.detach(), v.detach())
+    _compare(q.detach(), k.detach(), v.detach(), dout, out.detach(), lse, grads, [((b,), (b,)) for b in range(2)], 0.125, dtype, 0)
+    one = k.detach()[:, :, :1].clone().requires_grad_(True)
+    (shared,) = torch.autograd.grad(sa.causal_attention(q.detach(), one.expand(2, 150, 4, 64), v.detach()[:, :, :1].expand(2, 150, 4, 64)), one, dout)
+    (grouped,) = torch.autograd.grad(sa.causal_attention(q.detach(), one, v.detach()[:, :, :1].contiguous()), one, dout)
+    # the four heads' gradients, each rounded to the type and added in it, against the one sum: 8 half steps of their magnitudes
+    size = grouped.double().abs().amax()
+    assert (shared.double() - grouped.double()).abs().max() <= 8 * torch.finfo(dtype).eps / 2 * 4 * size + 1e-4
+
+
+def test_small_fp16_gradients():
+    """Gradients far below fp16's smallest normal number times the softmax weights keep their precision."""
+    q, k, v, dout = _inputs((1, 700), 2, 1, 64, FP16, 47)
+    out, lse, want = _all(q, k, v, dout, 0)
+    small = (dout.double() * 2.0 ** -9).half()                  # exact: a power of two, above the subnormal numbers for nearly all
+    got = sa.causal_attention_backward(q, k, v, out, lse, small)
+    for a, b in zip(got[:2], want[:2]):
+        # the same up to the rounding of results that are subnormal now (2^-25 each) and of inputs that are
+        assert ((a.double() * 2.0 ** 9 - b.double()).abs() <= 2.0 ** -10 * b.double().abs() + 2.0 ** -14 * b.double().abs().max() + 2.0 ** -15).all()
+
+
+def test_calls_at_once():
+    """Two streams, and two captured graphs replayed in turn, each with its own data."""
+    sets = [_inputs((1, 260), 4, 2, 64, BF16, 50 + i) for i in range(2)]
+    want = [_all(*x, 0) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        got = []
+        for st, x in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(_all(*x, 0))
+    torch.cuda.synchronize()
+    graphs, captured = [], []
+    for x in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            captured.append(_all(*x, 0))
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for results in (got, captured):
+        for r, w in zip(results, want):
+            for a, b in zip((*r[:2], *r[2]), (*w[:2], *w[2])):
+                assert torch.equal(a, b)
+
+
 def test_only_wanted_gradients_and_determinism():
     q, k, v, dout = _inputs((1, 400), 4, 2, 64, BF16, 17)
     out, lse, grads = _all(q, k, v, dout, 0)

@@ -108,6 +108,43 @@ def test_trees(B, T, H, HK, D, page, width, dtype, paged):
         _check(_run(*x), *x, D ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("B,T,H,HK,D,page,width", [
+    (1, 64, 16, 2, 128, 16, 260), (2, 48, 16, 4, 128, 64, 40), (1, 33, 4, 2, 64, 7, 300), (3, 64, 4, 2, 64, 32, 30), (2, 20, 20, 1, 80, 3, 700), (1, 64, 3, 1, 128, 5, 999)])
+def test_many_rows(B, T, H, HK, D, page, width, dtype):
+    """More than 64 rows per key head: the wavefronts of a workgroup divide the rows and share the keys."""
+    x = _case(B, T, H, HK, D, page, width, dtype, T + D + page)
+    _check(_run(*x), *x, D ** -0.5)
+    lengths, table, kc = x[6], x[7], x[4]
+    for n in (0, 63, 64, 65, page * width):
+        lengths.fill_(min(n, page * width))
+        _check(_run(*x), *x, D ** -0.5)
+    table[0, width // 2], table[-1, 0] = -1, kc.shape[0]       # pages that are none
+    _check(_run(*x), *x, D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,H,D", [(64, 4, 64), (64, 4, 128), (40, 2, 128), (3, 2, 64)])
+def test_later_keys_far_above_the_first(T, H, D, dtype):
+    x = _case(1, T, H, 1, D, 64, 40, dtype, 61, std=8.0)
+    x[6].fill_(64 * 40)
+    x[4][x[7][0, 0].long()] *= 0.01
+    _check(_run(*x, 0.5), *x, 0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_long_tables(dtype):
+    """One long cache shared by 64 workgroups; a table longer than a workgroup keeps in LDS."""
+    x = _case(1, 2, 4, 1, 64, 16, 2100, dtype, 71)
+    x[6].fill_(16 * 2100 - 5)
+    _check(_run(*x), *x, 0.125)
+    x = _case(64, 1, 8, 4, 64, 1, 4500, dtype, 73)
+    out = _run(*x)
+    part = lambda t, b: t[b:b + 1]
+    for b in (0, 40, 63):
+        _check(part(out, b), *(part(t, b) for t in x[:4]), x[4], x[5], part(x[6], b), part(x[7], b), 0.125)
+
+
 def test_chain_and_bad_parents():
     q, k, v, _, kc, vc, lengths, table = _case(2, 7, 4, 2, 64, 16, 6, BF16, 3)
     chain = torch.arange(-1, 6, dtype=torch.int32).expand(2, 7).contiguous()

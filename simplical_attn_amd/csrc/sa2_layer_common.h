@@ -59,9 +59,9 @@ struct Append {
 };
 
 // Nodes of drafted trees over a cache: the G query heads of a key head and the T nodes make R = T * G rows that read the
-// same keys; row r is node r / G, head r % G of the G.  The cached keys of a sequence are shared by `nsplit` workgroups, whose
-// outputs, not yet divided by their sums, lie in `part`: [nsplit][B*HK][R] pairs (reference point, sum), then
-// [nsplit][B*HK][R][width] values.
+// same keys; row r is node r / G, head r % G of the G.  The keys of the B sequences are cut into shares, nsplit * B units in all
+// (sa2_tree_common.h), whose outputs, not yet divided by their sums, lie in `part`: [units][HK][R] pairs (reference point, sum),
+// then [units][HK][R][width] values.
 struct Tree {
     Cache cache;
     int B, T, H, HK, G, D;
@@ -70,8 +70,8 @@ struct Tree {
     const int32_t* parents;                    // [B,T], or nullptr: a chain
     float* part;
     int nsplit;
+    bool dealt;                                // shares by the sequences' lengths
 };
-constexpr int TREE_NODES = 64;
 __host__ __device__ constexpr int tree_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 inline size_t tree_part_bytes(int B, int T, int H, int D, int nsplit) {
     return nsplit > 1 ? (size_t)nsplit * B * T * H * (tree_width(D) + 2) * sizeof(float) : 0;
@@ -96,7 +96,7 @@ int launch_causal16_bwd(const Causal& p, int dtype, float* minus_lse, float* top
 int launch_causal16_dq(const Causal& p, int dtype, const float* tops, int ntops, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
 // 16-bit kernels: rows that a workgroup has of R; up to 64 its wavefronts share them and divide the keys, beyond it is the other
-// way round (16/4 heads, 4 x 65536 cached rows, head_dim 128, 192 rows: 398 us dividing keys, 161 dividing rows; 64 rows: AAA, BBB)
+// way round (16/4 heads, 4 x 65536 cached rows, head_dim 128, 192 rows: 398 us dividing keys, 161 dividing rows)
 inline int tree16_rows(int R) { return R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256; }
 constexpr int TREE16_ENTRIES = 4096;                       // of the page table that a workgroup keeps in LDS
 int launch_tree_rows16(const Tree& p, int dtype, hipStream_t st);

@@ -24,13 +24,16 @@ __global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, i
     int id = blockIdx.x;
     const int block = id % blocks;
     id /= blocks;
-    const int split = id % p.nsplit, stream = id / p.nsplit, b = stream / p.HK, hk = stream % p.HK;
+    const int unit = id / p.HK, hk = id % p.HK;
+    TreeShare share;
+    if (!tree_share(p, unit, share)) return;
+    const int b = share.b;
     const int row = block * TILE + (lane & 31), node = row < R ? row / p.G : 0, h = hk * p.G + (row < R ? row - node * p.G : 0);
     uint64_t seen = tree_ancestors(p, b);
     seen = (uint64_t)__shfl((uint32_t)(seen >> 32), node) << 32 | __shfl((uint32_t)seen, node);
     if (row >= R) seen = 0;
     const int held = tree_held(p, b), cached = (held + TILE - 1) / TILE, all = cached + (p.T + TILE - 1) / TILE;
-    const int lo = (int)((int64_t)all * split / p.nsplit), hi = (int)((int64_t)all * (split + 1) / p.nsplit);
+    const int lo = (int)((int64_t)all * share.split / share.count), hi = (int)((int64_t)all * (share.split + 1) / share.count);
 
     float q[DP / 2];
     const float sign = p.scale < 0.f ? -1.f : 1.f, c = fabsf(p.scale) * LOG2E;
@@ -132,8 +135,8 @@ __global__ __launch_bounds__(64 * waves_of<DP>()) void tree_f32_kernel(Tree p, i
             o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
         }
         if (p.nsplit > 1) {
-            if (d == 0) *tree_stat(p, split, stream, to) = TreePart{top, sum};
-            *(float4*)(tree_values(p, split, stream, to, tree_width(p.D)) + d) = o;
+            if (d == 0) *tree_stat(p, unit, hk, to) = TreePart{top, sum};
+            *(float4*)(tree_values(p, unit, hk, to, tree_width(p.D)) + d) = o;
         } else {
             const float f = sum == 0.f ? 0.f : 1.f / sum;
             store4((T*)p.out.p + p.out.off(b, to / p.G, hk * p.G + to % p.G), d, p.D, wide, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
@@ -149,15 +152,18 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p, bool wide) {
     constexpr int GROUPS = 1024 / W, EACH = 64 / GROUPS;      // at most 64 splits
     __shared__ float4 sums[GROUPS][W / 4];
     const int64_t R = p.T * p.G, row = blockIdx.x, stream = row / R;
+    const int hk = (int)(stream % p.HK), b = (int)(stream / p.HK);
+    TreeShare share;
+    tree_shares_of(p, b, share);
     const int r = (int)(row - stream * R), lane = threadIdx.x & 63, group = threadIdx.x / (W / 4), d = threadIdx.x % (W / 4) * 4;
     const float c = fabsf(p.scale) * LOG2E;
     float4 y[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const int split = i * GROUPS + group;
-        y[i] = split < p.nsplit ? *(const float4*)(tree_values(p, split, stream, r, W) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        y[i] = split < share.count ? *(const float4*)(tree_values(p, share.first + split, hk, r, W) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const TreePart s = lane < p.nsplit ? *tree_stat(p, lane, stream, r) : TreePart{-INFINITY, 0.f};
+    const TreePart s = lane < share.count ? *tree_stat(p, share.first + lane, hk, r) : TreePart{-INFINITY, 0.f};
     const float top = wave_max(s.top), f = s.sum == 0.f ? 0.f : s.top == -INFINITY ? 1.f : exp2f((s.top - top) * c), sum = wave_sum(f * s.sum);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p, bool wide) {
         o.x += z.x; o.y += z.y; o.z += z.z; o.w += z.w;
     }
     const float g = sum == 0.f ? 0.f : 1.f / sum;
-    store4((T*)p.out.p + p.out.off((int)(stream / p.HK), r / p.G, (int)(stream % p.HK) * p.G + r % p.G), d, p.D, wide, make_float4(o.x * g, o.y * g, o.z * g, o.w * g));
+    store4((T*)p.out.p + p.out.off(b, r / p.G, hk * p.G + r % p.G), d, p.D, wide, make_float4(o.x * g, o.y * g, o.z * g, o.w * g));
 }
 
 template <class T>

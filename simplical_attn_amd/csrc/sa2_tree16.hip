@@ -24,10 +24,10 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
     const uint32_t mine = lds_address(lds) + wave * 2 * STAGE;
     int32_t* const pages = (int32_t*)(lds + WAVES * 2 * STAGE);
     const int R = p.T * p.G;
-    // (stream, split) units, the blocks of rows of one of them on one XCD
-    const int units = p.nsplit * p.B * p.HK, group = blockIdx.x / (8 * blocks), in = blockIdx.x - group * 8 * blocks;
-    const int left = units - 8 * group < 8 ? units - 8 * group : 8, block = in / left, id = 8 * group + in - block * left;
-    const int split = id % p.nsplit, stream = id / p.nsplit, b = stream / p.HK, hk = stream % p.HK;
+    // the blocks of rows of a unit's key head on one XCD
+    const int all_units = p.nsplit * p.B * p.HK, group = blockIdx.x / (8 * blocks), in = blockIdx.x - group * 8 * blocks;
+    const int left = all_units - 8 * group < 8 ? all_units - 8 * group : 8, block = in / left, id = 8 * group + in - block * left;
+    const int unit = id / p.HK, hk = id % p.HK, b = unit / p.nsplit, split = unit - b * p.nsplit;
     // (a short table as a whole: its reads do not wait for the sequence's length)
     const bool whole = p.cache.width <= 4 * THREADS;
     if (p.cache.table && whole)
@@ -272,8 +272,8 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
                 y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
             }
             if (p.nsplit > 1) {
-                if (d == 0) *tree_stat(p, split, stream, to) = TreePart{top, total};
-                *(float4*)(tree_values(p, split, stream, to, D) + d) = y;
+                if (d == 0) *tree_stat(p, unit, hk, to) = TreePart{top, total};
+                *(float4*)(tree_values(p, unit, hk, to, D) + d) = y;
             } else if (d < p.D) {
                 const float f = total == 0.f ? 0.f : 1.f / total;
                 *(uint2*)((uint16_t*)p.out.p + p.out.off(b, to / p.G, hk * p.G + to % p.G) + d) = make_uint2(pack2<E>(y.x * f, y.y * f), pack2<E>(y.z * f, y.w * f));

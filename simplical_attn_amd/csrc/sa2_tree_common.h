@@ -49,17 +49,75 @@ __device__ __forceinline__ bool tree_place(const Cache& c, int b, int r, int& pa
     return page >= 0 && page < c.pages;
 }
 
-// Result (nsplit 1) or partial result of a row: `sum` and values in units of e^top
+// How the workgroups of a key head are dealt to the sequences: a unit is one share of one sequence's keys.  Either every sequence has
+// nsplit of them, or (`dealt`) of nsplit * B units every sequence gets one and its part of the others by its keys, at most 64 in
+// all.  Lengths lie in device memory, so every wavefront counts for itself, which takes about 4 us of a call: dealt are the shares
+// of the kernels whose time is products, and from eight per sequence on (one empty cache and three of 33000 to 65000 rows, 48
+// nodes: 160 us with 16 each, 130 dealt; single tokens of 8 x 4096 rows 22.6 us with 8 each, 23.2 dealt; of 32 x 2048 rows, two
+// each, 37 and 49).
+struct TreeShare {
+    int b, split, count, first;                            // sequence, which of its shares, how many it has, the first one's unit
+};
+template <class F>
+__device__ __forceinline__ bool tree_deal(const Tree& p, F&& is, TreeShare& s) {
+    const int lane = threadIdx.x & 63;
+    auto keys = [&](int i) { return i < p.B ? (double)tree_held(p, i) + p.T : 0.0; };
+    double total = 0.0;
+    for (int c = 0; c < p.B; c += 64) total += keys(c + lane);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    // (a little less than its part, so that rounding never deals more units than there are)
+    const double each = (double)(p.nsplit - 1) * p.B / total * (1.0 - 1e-9);
+    int before = 0;
+    for (int c = 0; c < p.B; c += 64) {
+        int mine = 1 + (int)(keys(c + lane) * each);
+        mine = c + lane >= p.B ? 0 : mine < 64 ? mine : 64;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(sum, o);
+            if (lane >= o) sum += up;
+        }
+        const uint64_t hit = __ballot(mine > 0 && is(c + lane, before + sum - mine, before + sum));
+        if (hit) {
+            const int l = __ffsll((unsigned long long)hit) - 1;
+            s.b = c + l;
+            s.count = __builtin_amdgcn_readfirstlane(__shfl(mine, l));
+            s.first = before + __builtin_amdgcn_readfirstlane(__shfl(sum - mine, l));
+            s.split = 0;
+            return true;
+        }
+        before += __builtin_amdgcn_readfirstlane(__shfl(sum, 63));
+    }
+    return false;
+}
+// The share that a unit is; false: none
+__device__ __forceinline__ bool tree_share(const Tree& p, int unit, TreeShare& s) {
+    if (!p.dealt) {
+        const int b = unit / p.nsplit;
+        s = TreeShare{b, unit - b * p.nsplit, p.nsplit, b * p.nsplit};
+        return true;
+    }
+    const bool any = tree_deal(p, [&](int, int from, int to) { return from <= unit && unit < to; }, s);
+    s.split = unit - s.first;
+    return any;
+}
+// The shares of a sequence
+__device__ __forceinline__ void tree_shares_of(const Tree& p, int b, TreeShare& s) {
+    if (!p.dealt) s = TreeShare{b, 0, p.nsplit, b * p.nsplit};
+    else tree_deal(p, [&](int i, int, int) { return i == b; }, s);
+}
+
+// Partial result of a row of a unit: `sum` and values in units of e^top
 struct TreePart {
     float top, sum;
 };
-__device__ __forceinline__ TreePart* tree_stat(const Tree& p, int split, int64_t stream, int row) {
-    const int R = p.T * p.G;
-    return (TreePart*)p.part + ((int64_t)split * p.B * p.HK + stream) * R + row;
+__device__ __forceinline__ TreePart* tree_stat(const Tree& p, int unit, int hk, int row) {
+    return (TreePart*)p.part + ((int64_t)unit * p.HK + hk) * (p.T * p.G) + row;
 }
-__device__ __forceinline__ float* tree_values(const Tree& p, int split, int64_t stream, int row, int width) {
-    const int64_t R = p.T * p.G, rows = (int64_t)p.B * p.HK * R;
-    return p.part + 2 * rows * p.nsplit + ((int64_t)split * rows + stream * R + row) * width;
+__device__ __forceinline__ float* tree_values(const Tree& p, int unit, int hk, int row, int width) {
+    const int64_t R = p.T * p.G, slots = (int64_t)p.nsplit * p.B * p.HK * R;
+    return p.part + 2 * slots + (((int64_t)unit * p.HK + hk) * R + row) * width;
 }
 
 }  // namespace

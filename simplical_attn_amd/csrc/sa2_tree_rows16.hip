@@ -78,12 +78,16 @@ __global__ __launch_bounds__(THREADS, 1) void tree_rows16_kernel(Tree p, int blo
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int32_t* const pages = (int32_t*)(lds + BUFFERS * Buffer<D>::BYTES);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, R = p.T * p.G;
-    // (stream, split) units, the blocks of rows of one of them on one XCD
-    const int units = p.nsplit * p.B * p.HK, group = blockIdx.x / (8 * blocks), in = blockIdx.x - group * 8 * blocks;
-    const int left = units - 8 * group < 8 ? units - 8 * group : 8, block = in / left, id = 8 * group + in - block * left;
-    const int split = id % p.nsplit, stream = id / p.nsplit, b = stream / p.HK, hk = stream % p.HK;
-    const int held = tree_held(p, b), cached = (held + TILE_ROWS - 1) / TILE_ROWS, all = cached + 1;
-    const int lo = (int)((int64_t)all * split / p.nsplit), hi = (int)((int64_t)all * (split + 1) / p.nsplit);
+    // the blocks of rows of a unit's key head on one XCD
+    const int all_units = p.nsplit * p.B * p.HK, group = blockIdx.x / (8 * blocks), in = blockIdx.x - group * 8 * blocks;
+    const int left = all_units - 8 * group < 8 ? all_units - 8 * group : 8, block = in / left, id = 8 * group + in - block * left;
+    const int unit = id / p.HK, hk = id % p.HK;
+    TreeShare share;
+    if (!tree_share(p, unit, share)) return;
+    const auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };       // in all lanes, which the compiler does not see
+    const int b = same(share.b);
+    const int held = same(tree_held(p, b)), cached = (held + TILE_ROWS - 1) / TILE_ROWS, all = cached + 1;
+    const int lo = same((int)((int64_t)all * share.split / share.count)), hi = same((int)((int64_t)all * (share.split + 1) / share.count));
 
     TreeKeys<D, NQ> keys{p, pages};
     keys.b = b;
@@ -157,7 +161,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree_rows16_kernel(Tree p, int blo
         const bool any = keys.seen[n] && keys.tiles > 0 && both != 0.f;
         const float sum = any ? both : 0.f, f = any ? 1.f / sum : 0.f;
         if (row < R) {
-            float* const part = p.nsplit > 1 ? tree_values(p, split, stream, row, D) : nullptr;
+            float* const part = p.nsplit > 1 ? tree_values(p, unit, hk, row, D) : nullptr;
             uint16_t* const out = (uint16_t*)p.out.p + p.out.off(b, node[n], head[n]);
             static_for<4 * DT>([&](auto X) __attribute__((always_inline)) {
                 constexpr int x = decltype(X)::value;
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree_rows16_kernel(Tree p, int blo
                 if (part) *(float4*)(part + col) = o;
                 else if (col < p.D) *(uint2*)(out + col) = make_uint2(pack2<E>(o.x * f, o.y * f), pack2<E>(o.z * f, o.w * f));
             });
-            if (part && half == 0) *tree_stat(p, split, stream, row) = TreePart{any ? m[n] : -INFINITY, sum};
+            if (part && half == 0) *tree_stat(p, unit, hk, row) = TreePart{any ? m[n] : -INFINITY, sum};
         }
     });
 }

@@ -47,7 +47,8 @@ int check_tree(int B, int T, int H, int HK, int D, int dtype) {
 // Workgroups that share a sequence's keys: as many as are on the chip at once, one per CU, each with at least four tiles of 32
 // keys (one per wavefront; eight where the wavefronts share them) of what a sequence may hold, at most 64 (how many it does hold is known on the device only)
 int tree_splits(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype) {
-    const int rows = T * (H / HK), block = dtype == SA2_F32 ? 32 : tree16_rows(rows), least = block > 64 ? 8 : 4;
+    const int64_t keys = (int64_t)B * HK * page_size * table_width;
+    const int rows = T * (H / HK), block = dtype == SA2_F32 ? 32 : tree16_rows(rows, keys), least = block > 64 ? 8 : 4;
     const int64_t streams = (int64_t)B * HK * ((rows + block - 1) / block), tiles = ((int64_t)page_size * table_width + 31) / 32;
     int64_t n = CUS / streams;
     if (n > tiles / least) n = tiles / least;
@@ -211,7 +212,7 @@ int sa2_tree_attention(const void* q, const void* k, const void* v, const void* 
     if (p.nsplit > 1 && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < tree_part_bytes(B, T, H, D, p.nsplit)))
         return SA2_ERR_WORKSPACE_TOO_SMALL;
     const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && tree16_supported(p, dtype);
-    p.dealt = B > 1 && p.nsplit >= 8 && (!narrow || tree16_rows(T * p.G) > 64);     // (sa2_tree16.hip takes equal shares)
+    p.dealt = B > 1 && p.nsplit >= 8 && (!narrow || tree16_rows(p) > 64);      // (sa2_tree16.hip takes equal shares)
     if (narrow) return launch_tree16(p, dtype, (hipStream_t)hip_stream);
     return launch_tree_f32(p, dtype, (hipStream_t)hip_stream);
 }

@@ -96,8 +96,11 @@ int launch_causal16_bwd(const Causal& p, int dtype, float* minus_lse, float* top
 int launch_causal16_dq(const Causal& p, int dtype, const float* tops, int ntops, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
 // 16-bit kernels: rows that a workgroup has of R; up to 64 its wavefronts share them and divide the keys, beyond it is the other
-// way round (16/4 heads, 4 x 65536 cached rows, head_dim 128, 192 rows: 398 us dividing keys, 161 dividing rows)
-inline int tree16_rows(int R) { return R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256; }
+// way round (16/4 heads, 4 x 65536 cached rows, head_dim 128, 192 rows: 398 us dividing keys, 161 dividing rows).  From 33 to 64
+// it is the other way round too where a CU has 1024 keys or more (64 rows of head_dim 128: 4 x 65536 rows 148 us and 98, 32 x 2048
+// 63 and 54; 8 x 2048 26.5 and 27.6, 512 rows 19 and 23).  `keys`: those that the cache may hold, of all sequences and key heads.
+inline int tree16_rows(int R, int64_t keys) { return R <= 32 ? 32 : R <= 64 && keys < 1024 * CUS ? 64 : R <= 128 ? 128 : 256; }
+inline int tree16_rows(const Tree& p) { return tree16_rows(p.T * p.G, (int64_t)p.B * p.HK * p.cache.page_size * p.cache.width); }
 constexpr int TREE16_ENTRIES = 4096;                       // of the page table that a workgroup keeps in LDS
 int launch_tree_rows16(const Tree& p, int dtype, hipStream_t st);
 bool tree16_supported(const Tree& p, int dtype);

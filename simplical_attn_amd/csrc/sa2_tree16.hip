@@ -300,17 +300,19 @@ bool tree16_supported(const Tree& p, int dtype) {
     if (dtype == SA2_F32 || p.D % 8 || p.D > 128) return false;
     for (const Tensor* t : {&p.q, &p.k, &p.v, &p.cache.k, &p.cache.v, &p.out})
         if (!aligned16(*t, 2, true) || t->sn >= 1 << 22) return false;     // (a group's rows within 2^31 bytes of its first)
-    return !p.cache.table || (p.cache.width + p.nsplit - 1) / p.nsplit + 256 / p.cache.page_size + 3 <= TREE16_ENTRIES;
+    // (of nsplit shares for each, a sequence has at least nsplit - 1 where they are dealt and its cache is full)
+    const int shares = p.nsplit > 1 ? p.nsplit - 1 : 1;
+    return !p.cache.table || (p.cache.width + shares - 1) / shares + 256 / p.cache.page_size + 3 <= TREE16_ENTRIES;
 }
 
 int launch_tree16(const Tree& p, int dtype, hipStream_t st) {
     auto of = [&](auto e) {
         using E = decltype(e);
-        const bool two = p.T * p.G > 32;                     // (more than 64: see below)
+        const bool two = p.T * p.G > 32;
         if (p.D <= 64) return two ? launch<E, 64, 2>(p, st) : launch<E, 64, 1>(p, st);
         return two ? launch<E, 128, 2>(p, st) : launch<E, 128, 1>(p, st);
     };
-    const int rc = tree16_rows(p.T * p.G) > 64 ? launch_tree_rows16(p, dtype, st) : dtype == SA2_F16 ? of(ElemF16{}) : of(ElemBF16{});
+    const int rc = tree16_rows(p) > 64 ? launch_tree_rows16(p, dtype, st) : dtype == SA2_F16 ? of(ElemF16{}) : of(ElemBF16{});
     return rc == SA2_OK && p.nsplit > 1 ? launch_tree_join(p, dtype, st) : rc;
 }
 

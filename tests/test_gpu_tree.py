@@ -145,6 +145,27 @@ def test_long_tables(dtype):
         _check(part(out, b), *(part(t, b) for t in x[:4]), x[4], x[5], part(x[6], b), part(x[7], b), 0.125)
 
 
+def test_shares_of_a_long_table_of_single_rows():
+    """Full caches behind pages of one row: shares that are longer than an eighth of the table."""
+    x = _case(2, 64, 32, 16, 64, 1, 30000, BF16, 79)
+    x[6].fill_(30000)
+    _check(_run(*x), *x, 0.125)
+    x[6][1] = 31
+    _check(_run(*x), *x, 0.125)
+
+
+@pytest.mark.parametrize("B,T,cap", [(4, 12, 65536), (32, 16, 2048), (3, 9, 40000)])
+def test_few_rows_over_many_keys(B, T, cap):
+    x = _case(B, T, 16, 4, 128, 64, cap // 64, BF16, 83)
+    x[6].fill_(cap - 9)
+    x[6][0] = 0
+    x[6][B // 2] = cap // 3
+    out = _run(*x)
+    for b in (0, B // 2, B - 1):
+        part = lambda t: t[b:b + 1]
+        _check(part(out), *(part(t) for t in x[:4]), x[4], x[5], part(x[6]), part(x[7]), 128 ** -0.5)
+
+
 def test_chain_and_bad_parents():
     q, k, v, _, kc, vc, lengths, table = _case(2, 7, 4, 2, 64, 16, 6, BF16, 3)
     chain = torch.arange(-1, 6, dtype=torch.int32).expand(2, 7).contiguous()

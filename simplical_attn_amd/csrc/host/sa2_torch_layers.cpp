@@ -87,10 +87,10 @@ Tensor dense(const Maybe& t) { return t ? t->contiguous() : Tensor(); }
 struct Angles {
     Tensor frequencies, positions, cu;         // the last two may be undefined
     double amplitude;
-    bool interleaved;
+    bool interleaved, inverse;
 };
 
-std::pair<Tensor, Tensor> run_rotary(const Tensor& q_, const Tensor& k_, const Angles& a, bool inverse) {
+std::pair<Tensor, Tensor> run_rotary(const Tensor& q_, const Tensor& k_, const Angles& a) {
     const Tensor q = rows(q_), k = k_.defined() ? rows(k_) : Tensor();
     const c10::DeviceGuard guard(q.device());
     Tensor q2 = like(q), k2 = k.defined() ? like(k) : Tensor();
@@ -106,11 +106,14 @@ std::pair<Tensor, Tensor> run_rotary(const Tensor& q_, const Tensor& k_, const A
     }
     check(rotary_fn(q.const_data_ptr(), hk ? k.const_data_ptr() : nullptr, q2.data_ptr(), hk ? k2.data_ptr() : nullptr, a.frequencies.const_data_ptr<double>(),
                     a.positions.defined() ? a.positions.const_data_ptr() : nullptr, a.positions.defined() ? (int)a.positions.element_size() : 0, ints(a.cu),
-                    a.cu.defined() ? (int)a.cu.numel() - 1 : 0, z.B, z.N, z.H, hk, z.D, (int)(2 * a.frequencies.numel()), s, (float)a.amplitude, a.interleaved, inverse,
+                    a.cu.defined() ? (int)a.cu.numel() - 1 : 0, z.B, z.N, z.H, hk, z.D, (int)(2 * a.frequencies.numel()), s, (float)a.amplitude, a.interleaved, a.inverse,
                     dtype_code(q), stream(q)));
     return {q2, k2};
 }
 
+std::pair<Tensor, Tensor> turn(const Tensor& q, const Tensor& k, const Angles& a);
+
+// (its backward is the same operator, so it has derivatives of every order)
 struct RotaryFormula : torch::autograd::Function<RotaryFormula> {
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const Maybe& k, Angles a) {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -118,19 +121,29 @@ struct RotaryFormula : torch::autograd::Function<RotaryFormula> {
         ctx->save_for_backward({a.frequencies, a.positions, a.cu});
         ctx->saved_data["amplitude"] = a.amplitude;
         ctx->saved_data["interleaved"] = a.interleaved;
-        auto [q2, k2] = run_rotary(q, k ? *k : Tensor(), a, false);
+        ctx->saved_data["inverse"] = a.inverse;
+        auto [q2, k2] = run_rotary(q, k ? *k : Tensor(), a);
         return k2.defined() ? variable_list{q2, k2} : variable_list{q2};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        at::AutoDispatchBelowADInplaceOrView below;
         const auto s = ctx->get_saved_variables();
-        const Angles a{s[0], s[1], s[2], ctx->saved_data["amplitude"].toDouble(), ctx->saved_data["interleaved"].toBool()};
+        const Angles a{s[0], s[1], s[2], ctx->saved_data["amplitude"].toDouble(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool()};
         Tensor dq = ctx->needs_input_grad(0) ? grads[0] : Tensor(), dk = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
-        if (dq.defined()) std::tie(dq, dk) = run_rotary(dq, dk, a, true);
-        else if (dk.defined()) dk = run_rotary(dk, Tensor(), a, true).first;
+        if (dq.defined()) std::tie(dq, dk) = turn(dq, dk, a);
+        else if (dk.defined()) dk = turn(dk, Tensor(), a).first;
         return {dq, dk, Tensor()};
     }
 };
+
+// `k` may be undefined
+std::pair<Tensor, Tensor> turn(const Tensor& q, const Tensor& k, const Angles& a) {
+    if (at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
+        auto r = RotaryFormula::apply(q, k.defined() ? Maybe(k) : Maybe(), a);
+        return {r[0], k.defined() ? r[1] : Tensor()};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    return run_rotary(q, k, a);
+}
 
 std::pair<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& frequencies, const Maybe& positions, const Maybe& cu, bool interleaved, double amplitude) {
     check_first(q, "q");
@@ -147,14 +160,9 @@ std::pair<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& f
     }
     check_place("rotary_embedding", {q});
     if (k) check_place("rotary_embedding", {*k});
-    const Angles a{frequencies.contiguous(), dense(positions), dense(cu), amplitude, interleaved};
+    const Angles a{frequencies.contiguous(), dense(positions), dense(cu), amplitude, interleaved, false};
     py::gil_scoped_release nogil;
-    if (at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()))) {
-        auto r = RotaryFormula::apply(q, k, a);
-        return {r[0], k ? Maybe(r[1]) : Maybe()};
-    }
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto [q2, k2] = run_rotary(q, k ? *k : Tensor(), a, false);
+    auto [q2, k2] = turn(q, k ? *k : Tensor(), a);
     return {q2, k ? Maybe(k2) : Maybe()};
 }
 
@@ -180,6 +188,16 @@ CacheView check_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor
     return {k_cache, v_cache, lengths.contiguous(), dense(table), (int)k_cache.size(1), (int)k_cache.size(0), table ? (int)table->size(1) : 1};
 }
 
+// Whether the memory from a tensor's first element to its last meets the other's
+bool meet(const Tensor& a, const Tensor& b) {
+    auto end = [](const Tensor& t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        return (const char*)t.const_data_ptr() + (last + 1) * t.element_size();
+    };
+    return (const char*)a.const_data_ptr() < end(b) && (const char*)b.const_data_ptr() < end(a);
+}
+
 void append(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths, const Maybe& table, const Maybe& chosen, const Maybe& cu) {
     check_first(k_, "k");
     check_beside(v_, "v", k_, "k");
@@ -196,10 +214,14 @@ void append(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Ten
     check_place("cache_append", {k_, v_, k_cache, v_cache});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor k = rows(k_), v = rows(v_), pick = dense(chosen), ends = dense(cu);
+    Tensor k = rows(k_), v = rows(v_);
+    const Tensor pick = dense(chosen), ends = dense(cu);
     const c10::DeviceGuard guard(k.device());
     const Sizes z = sizes(k);
     if (z.B == 0 || z.N == 0 || (pick.defined() && pick.numel() == 0)) return;
+    // rows that are a view of the cache (moved within it) are read before any is written
+    if (meet(k, c.k) || meet(k, c.v)) k = k.clone(at::MemoryFormat::Contiguous);
+    if (meet(v, c.k) || meet(v, c.v)) v = v.clone(at::MemoryFormat::Contiguous);
     int64_t s[12];
     put_strides(s, k);
     put_strides(s + 3, v);
@@ -249,7 +271,11 @@ std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, co
     const Tensor* const of[3] = {&q, &k, &v};
     for (int i = 0; i < 3; ++i)
         if (needs >> i & 1) g[i] = like(*of[i]);
-    if (q.numel() == 0) return g;
+    if (q.numel() == 0) {
+        for (Tensor& t : g)
+            if (t.defined()) t.zero_();        // (keys that no query head reads)
+        return g;
+    }
     const size_t bytes = causal_ws_fn(z.B, z.N, z.H, hk, z.D, dtype_code(q), a.flags);
     const Tensor ws = workspace(q, std::max<size_t>(bytes, 256));
     int64_t s[24];
@@ -272,6 +298,7 @@ struct CausalFormula : torch::autograd::Function<CausalFormula> {
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "causal_attention has first derivatives only: its backward cannot run with create_graph=True");
         at::AutoDispatchBelowADInplaceOrView below;
         const auto s = ctx->get_saved_variables();
         const Prompt a{s[5], ctx->saved_data["scale"].toDouble(), (unsigned)ctx->saved_data["flags"].toInt()};

@@ -54,7 +54,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, or
 
 def rotary_embedding(q, k, frequencies, positions=None, cu_seqlens=None, interleaved=False, amplitude=1.0):
     """(q', k'): the first 2 * len(frequencies) columns of every head turned by position * frequencies, the others copied;
-    differentiable in q and k (the gradient is the rotation by the opposite angle).
+    differentiable in q and k, to any order (the gradient is the rotation by the opposite angle).
 
     q, k         [batch, seq_len, heads, head_dim] or packed; k has heads of its own, or is None (then k' is None)
     frequencies  float64 vector (rotary_frequencies); the angles are formed in 64 bits, so positions may be far
@@ -75,12 +75,15 @@ def cache_append(k, v, k_cache, v_cache, lengths, page_table=None, rows=None, cu
     rows              int32 [batch, any]: which of a sequence's seq_len rows to take, in this order (accepted nodes of a
                       draft); entries outside 0 .. seq_len-1 are left out, their places stay as they are
 
-    Rows whose place lies beyond the capacity, or whose page is not one of the cache's, are left out."""
+    Rows whose place lies beyond the capacity, or whose page is not one of the cache's, are left out.  k and v may be views
+    of the cache itself: all rows are read before one is written.  Two rows of one call with the same place (a page that the
+    table names twice) leave either."""
     _lib.host().cache_append(k, v, k_cache, v_cache, lengths, page_table, rows, cu_seqlens)
 
 
 def causal_attention(q, k, v, cu_seqlens=None, scale=None):
-    """softmax(scale q k^T) v, query i of a sequence over its keys 0 .. i; differentiable in q, k and v.
+    """softmax(scale q k^T) v, query i of a sequence over its keys 0 .. i; differentiable in q, k and v (once: create_graph=True
+    is refused).
 
     q        [batch, seq_len, heads, head_dim], or packed [rows, heads, head_dim] with cu_seqlens; head_dim up to 256
     k, v     as q, with heads that divide q's: query head h reads head h // (heads / key heads)

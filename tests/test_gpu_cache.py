@@ -99,3 +99,15 @@ def test_replayed_graph():
         torch.cuda.synchronize()
         assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1])
         lengths += 3
+
+
+def test_rows_that_are_the_caches_own():
+    """Views of the cache as new rows, which the call's own places overlap: all are read first."""
+    g = torch.Generator().manual_seed(29)
+    kc, vc = (torch.randn(2, 600, 4, 64, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    want = [c.clone() for c in (kc, vc)]
+    for b, n in ((0, 7), (1, 200)):
+        for w, c in zip(want, (kc, vc)):
+            w[b, n:n + 400] = c[b, :400]
+    sa.cache_append(kc[:, :400], vc[:, :400], kc, vc, torch.tensor([7, 200], dtype=torch.int32, device=DEV))
+    assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])

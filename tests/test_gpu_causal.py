@@ -315,6 +315,21 @@ def test_other_stream_and_replayed_graph():
             assert torch.equal(a, b)
 
 
+def test_second_derivatives_are_refused():
+    q, k, v, dout = _inputs((1, 40), 2, 1, 64, BF16, 61)
+    q.requires_grad_(True)
+    out = sa.causal_attention(q, k, v)
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        torch.autograd.grad(out, q, dout, create_graph=True)
+
+
+def test_no_query_heads():
+    q = torch.zeros(1, 5, 0, 64, dtype=BF16, device=DEV)
+    k = torch.ones(1, 5, 2, 64, dtype=BF16, device=DEV, requires_grad=True)
+    out = sa.causal_attention(q, k, k)
+    assert out.shape == q.shape and torch.autograd.grad(out, k, q)[0].count_nonzero() == 0
+
+
 def test_empty():
     q = torch.zeros(2, 0, 4, 64, dtype=BF16, device=DEV, requires_grad=True)
     k = torch.zeros(2, 0, 2, 64, dtype=BF16, device=DEV)

@@ -134,3 +134,17 @@ def test_replayed_graph():
         got = [t.clone() for t in captured]
         for a, b in zip(got, sa.rotary_embedding(q, k, f, pos)):
             assert torch.equal(a, b)
+
+
+def test_second_derivatives():
+    """The gradient is linear in what comes back, and differentiable in it: turning forth and back again."""
+    g = torch.Generator().manual_seed(23)
+    q, k = (torch.randn(2, 9, h, 16, generator=g).to(DEV).requires_grad_(True) for h in (3, 1))
+    f = sa.rotary_frequencies(8, device=DEV)
+    a = [torch.randn(2, 9, h, 16, generator=g).to(DEV).requires_grad_(True) for h in (3, 1)]
+    grads = torch.autograd.grad(sa.rotary_embedding(q, k, f), (q, k), a, create_graph=True)
+    b = [torch.randn(x.shape, generator=g).to(DEV) for x in grads]
+    got = torch.autograd.grad(grads, a, b)
+    want = sa.rotary_embedding(*b, f)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)

@@ -7,6 +7,8 @@
 // Every product keeps the index that a wavefront owns (32 queries, or 32 keys) in the lane: S^T = K Q^T leaves lane l with
 // query l % 32 and the keys 8g + 4(l/32) + r in register 4g + r, so that softmax is arithmetic within a lane and one exchange
 // of halves, and these registers are, as they are, the second operand of the next product.
+// Here: the kernels for a head_dim above 128, whose accumulators leave no room for a wavefront to have tiles of its own (four share
+// each tile and have 32 rows apiece); the row terms; the choice.  Up to 128: sa2_causal_f32_narrow.hip.
 // Bound by the matrix pipe: an MFMA takes 64 cycles, for which one LDS read of 4 or 16 bytes per lane is enough.
 #include "sa2_f32_tiles.h"
 
@@ -316,7 +318,7 @@ int launch_causal_f32_fwd(const Causal& p, int dtype, hipStream_t st) {
     return for_type(dtype, [&](auto* e) {
         using T = std::remove_pointer_t<decltype(e)>;
         const bool wide = wide_rows<T>(p, {&p.q, &p.k, &p.v, &p.out}, p.rows.B > 1);
-        if (p.D <= 128) return launch_causal_f32_few_fwd(p, dtype, wide, st);
+        if (p.D <= 128) return launch_causal_f32_narrow_fwd(p, dtype, wide, st);
         return launch(wide ? causal_f32_fwd_kernel<T, 256, true> : causal_f32_fwd_kernel<T, 256, false>, p, (int64_t)p.rows.B * p.H, 2 * TILE * Pitch<256>::value, st);
     });
 }
@@ -330,7 +332,7 @@ int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st) {
             causal_f32_delta_kernel<T><<<dim3((unsigned)blocks), dim3(THREADS), 0, st>>>(p);
             if (hipGetLastError() != hipSuccess) return (int)SA2_ERR_LAUNCH_FAILED;
         }
-        if (p.D <= 128) return launch_causal_f32_few_bwd(p, dtype, wide, st);
+        if (p.D <= 128) return launch_causal_f32_narrow_bwd(p, dtype, wide, st);
         int rc = SA2_OK;
         if (p.dk.p || p.dv.p)
             rc = launch(wide ? causal_f32_dkv_kernel<T, 256, 128, true> : causal_f32_dkv_kernel<T, 256, 128, false>, p, (int64_t)p.rows.B * p.HK * 2, 2 * TILE * Pitch<256>::value + 64, st);

@@ -81,9 +81,9 @@ int launch_rotary(const Rotary& p, int dtype, hipStream_t st);
 int launch_append(const Append& p, int dtype, hipStream_t st);
 int launch_causal_f32_fwd(const Causal& p, int dtype, hipStream_t st);
 int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st);
-// the same for few rows, head_dim up to 128: the four wavefronts of a workgroup share its 32 rows and divide what these see
-int launch_causal_f32_few_fwd(const Causal& p, int dtype, bool wide, hipStream_t st);
-int launch_causal_f32_few_bwd(const Causal& p, int dtype, bool wide, hipStream_t st);
+// the same, head_dim up to 128: the four wavefronts of a workgroup share its 32 rows and divide what these see
+int launch_causal_f32_narrow_fwd(const Causal& p, int dtype, bool wide, hipStream_t st);
+int launch_causal_f32_narrow_bwd(const Causal& p, int dtype, bool wide, hipStream_t st);
 // bf16 and fp16 with a head_dim up to 128 that is a multiple of 8, rows on the 16-byte grid
 bool causal16_supported(int D, int dtype);
 bool causal16_layout(const Causal& p, std::initializer_list<const Tensor*> ts);

@@ -6,7 +6,7 @@
 // and a piece of 32 keys: D / 8 MFMAs, and 16 weights per lane.  The units run in a pipeline of three: while the vector ALU makes
 // the weights of unit u, the matrix pipe has the logits of u+1 and the output of u-1, MFMA by MFMA between them (sa2_mfma_lone.h:
 // outputs and queries stay in accumulation registers that the kernel owns; left to the compiler they moved to and fro, 280
-// instructions more per 64 MFMAs, and the MFMAs stood in rows: 583 us instead of 327 at B1 N8192 H16/4 D128).
+// instructions more per 64 MFMAs, and the MFMAs stood in rows: 583 us instead of 302 at B1 N8192 H16/4 D128).
 // The weights are e^(s - m) with m the row's maximum over its first 32 keys: no maximum and no scaling of the output in the
 // sweep.  Rounding weights to 16 bits costs half a step of each, whatever m; a unit whose sum passes REF_LIMIT has the workgroup
 // sweep its keys a second time, with the running maximum.

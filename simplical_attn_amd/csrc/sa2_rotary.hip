@@ -115,7 +115,6 @@ int launch(const Rotary& p, hipStream_t st) {
     sp.units = p.rot / 2 / pairs_of<V, INTERLEAVED>() + (p.D - p.rot) / V;
     const int64_t rows = (int64_t)p.rows.B * p.rows.N;
     const int heads = p.H + p.HK;
-    // Four heads per thread where that leaves the chip two wavefronts per SIMD, one where it does not
     // Eight heads per thread where that leaves the chip eight wavefronts per SIMD (16384 rows of 20 heads, half of head_dim 128, interleaved:
     // 37 us, 44 with four), four where it leaves two, one elsewhere
     sp.share = rows * sp.units * ((heads + 7) / 8) >= 8 * 4 * 64 * CUS ? (heads + 7) / 8 : rows * sp.units * ((heads + 3) / 4) >= 2 * 4 * 64 * CUS ? (heads + 3) / 4 : heads;

@@ -3,7 +3,7 @@
 // Small calls are bound by the longest chain of tiles: a quarter of it here.  Every tile is read by as many workgroups as
 // have rows that see it, four times as many as with 128 rows each, from L2.  Against 128 rows per workgroup: 323 rows in four
 // sequences, 4/2 heads, head_dim 64, forward and backward 244 -> 80 us; B1 N8192 H4/1 D128 1779 -> 950 us forward (72 TFLOP/s of
-// the 153 that a large product reaches: an exponential and its mask for every two columns of products), 14.2 -> 5.9 ms backward.
+// the 153 that a large product reaches: an exponential and its mask for every two columns of products), 14.2 -> 3.9 ms backward.
 #include "sa2_f32_tiles.h"
 
 namespace sa2 {
@@ -181,14 +181,13 @@ __global__ __launch_bounds__(THREADS) void causal_f32_narrow_fwd_kernel(Causal p
 }
 
 template <class T, int DP, bool WIDE>
-__global__ __launch_bounds__(THREADS) void causal_f32_narrow_dq_kernel(Causal p) {
+__device__ __forceinline__ void queries_gradient(const Causal& p, int id, float* lds) {
     constexpr bool wide = WIDE;
     constexpr int REGION = 2 * TILE * Pitch<DP>::value;
-    extern __shared__ __attribute__((aligned(16))) float lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     float *kt = lds + wave * REGION, *vt = kt + TILE * Pitch<DP>::value;
     int stream, tile;
-    order(blockIdx.x, p.rows.B * p.H, stream, tile);
+    order(id, p.rows.B * p.H, stream, tile);
     const int b = stream / p.H, h = stream % p.H, hk = h / p.G;
     Span s;
     if (!find_tile(p.rows, b, tile, TILE, s)) return;
@@ -232,18 +231,15 @@ __global__ __launch_bounds__(THREADS) void causal_f32_narrow_dq_kernel(Causal p)
     add_up<T, DP>(lds, REGION, p.dq, s, q0, h, p.D, wide, p.scale);
 }
 
-// KEYS, VALUES: which of dK and dV a launch makes.  Both at once at head_dim up to 64; one after the other at 128, with the logits twice
-// (five products instead of four), because keys, values and both sums take 256 registers and what did not fit went to memory
-// (N 8192, 4/1 heads: 5.8 ms together, 4.7 apart).
+// KEYS, VALUES: which of dK and dV a workgroup makes
 template <class T, int DP, bool WIDE, bool KEYS, bool VALUES>
-__global__ __launch_bounds__(THREADS) void causal_f32_narrow_dkv_kernel(Causal p) {
+__device__ __forceinline__ void keys_gradients(const Causal& p, int id, float* lds) {
     constexpr bool wide = WIDE;
     constexpr int REGION = 2 * TILE * Pitch<DP>::value;
-    extern __shared__ __attribute__((aligned(16))) float lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     float *qt = lds + wave * REGION, *dt = qt + TILE * Pitch<DP>::value, *stats = lds + WAVES * REGION + wave * 64;
     int stream, tile;
-    order(blockIdx.x, p.rows.B * p.HK, stream, tile);
+    order(id, p.rows.B * p.HK, stream, tile);
     const int b = stream / p.HK, hk = stream % p.HK;
     Span s;
     if (!find_tile(p.rows, b, tile, TILE, s)) return;
@@ -311,12 +307,26 @@ __global__ __launch_bounds__(THREADS) void causal_f32_narrow_dkv_kernel(Causal p
     if (VALUES && p.dv.p) add_up<T, DP>(lds + TILE * Pitch<DP>::value, REGION, p.dv, s, j0, hk, p.D, wide, 1.f);
 }
 
-template <class K>
-int launch(K kernel, const Causal& p, int heads, int DP, hipStream_t st) {
-    const int64_t grid = (int64_t)p.rows.B * heads * count_tiles(p.rows, TILE);
+// All gradients in one launch, so that one's workgroups fill the CUs that the other's last ones leave (323 rows in four sequences: dK and
+// dV 38 us, dQ 19, one after the other): `keys` workgroups for dK and dV (APART: for dK), `values` for dV, the others for dQ.
+// APART: dK and dV from workgroups of their own, with the logits twice (five products instead of four).  At head_dim 128 always, because
+// keys, values and both sums take 256 registers and what did not fit went to memory (N 8192, 4/1 heads: 5.8 ms together, 4.7 apart);
+// below where there are CUs for both (217 rows of 4/2 heads of 64: 41 us together, 32 apart; B2 N1024 H8/8: 156 and 181).
+template <class T, int DP, bool WIDE, bool APART>
+__global__ __launch_bounds__(THREADS) void causal_f32_narrow_bwd_kernel(Causal p, int keys, int values) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int id = blockIdx.x;
+    if (id < keys) keys_gradients<T, DP, WIDE, true, !APART>(p, id, lds);
+    else if (APART && id < keys + values) keys_gradients<T, DP, WIDE, false, true>(p, id - keys, lds);
+    else queries_gradient<T, DP, WIDE>(p, id - keys - values, lds);
+}
+
+template <class K, class... A>
+int launch(K kernel, const Causal& p, int64_t streams, int DP, hipStream_t st, A... more) {
+    const int64_t grid = (int64_t)p.rows.B * streams * count_tiles(p.rows, TILE);
     if (grid > 0x7fffffff) return SA2_ERR_TOO_LARGE;
     if (!allow_full_lds((const void*)kernel)) return SA2_ERR_LAUNCH_FAILED;
-    kernel<<<dim3((unsigned)grid), dim3(THREADS), (WAVES * 2 * TILE * (DP + 4) + WAVES * 64) * sizeof(float), st>>>(p);
+    kernel<<<dim3((unsigned)grid), dim3(THREADS), (WAVES * 2 * TILE * (DP + 4) + WAVES * 64) * sizeof(float), st>>>(p, more...);
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 template <class F>
@@ -343,17 +353,14 @@ int launch_causal_f32_narrow_bwd(const Causal& p, int dtype, bool wide, hipStrea
         using T = std::remove_pointer_t<decltype(e)>;
         return for_narrow_width(p.D, [&](auto w) {
             constexpr int DP = decltype(w)::value;
-            int rc = SA2_OK;
-            if constexpr (DP < 128) {
-                if (p.dk.p || p.dv.p)
-                    rc = launch(wide ? causal_f32_narrow_dkv_kernel<T, DP, true, true, true> : causal_f32_narrow_dkv_kernel<T, DP, false, true, true>, p, p.HK, DP, st);
-            } else {
-                if (p.dk.p) rc = launch(wide ? causal_f32_narrow_dkv_kernel<T, DP, true, true, false> : causal_f32_narrow_dkv_kernel<T, DP, false, true, false>, p, p.HK, DP, st);
-                if (rc == SA2_OK && p.dv.p)
-                    rc = launch(wide ? causal_f32_narrow_dkv_kernel<T, DP, true, false, true> : causal_f32_narrow_dkv_kernel<T, DP, false, false, true>, p, p.HK, DP, st);
-            }
-            if (rc == SA2_OK && p.dq.p) rc = launch(wide ? causal_f32_narrow_dq_kernel<T, DP, true> : causal_f32_narrow_dq_kernel<T, DP, false>, p, p.H, DP, st);
-            return rc;
+            const int64_t each = (int64_t)p.rows.B * p.HK * count_tiles(p.rows, TILE);
+            const bool any = p.dk.p || p.dv.p, apart = DP == 128 || 2 * each <= CUS;
+            const int streams = (apart ? (p.dk.p ? p.HK : 0) + (p.dv.p ? p.HK : 0) : any ? p.HK : 0) + (p.dq.p ? p.H : 0);
+            const int keys = (apart ? p.dk.p != nullptr : any) ? (int)each : 0, values = apart && p.dv.p ? (int)each : 0;
+            if (streams == 0) return (int)SA2_OK;
+            if constexpr (DP < 128)
+                if (!apart) return launch(wide ? causal_f32_narrow_bwd_kernel<T, DP, true, false> : causal_f32_narrow_bwd_kernel<T, DP, false, false>, p, streams, DP, st, keys, values);
+            return launch(wide ? causal_f32_narrow_bwd_kernel<T, DP, true, true> : causal_f32_narrow_bwd_kernel<T, DP, false, true>, p, streams, DP, st, keys, values);
         });
     });
 }

@@ -8,13 +8,13 @@
 // Keys, values and both sums live in accumulation registers (sa2_mfma_lone.h); 32 queries are D / 4 MFMAs.  They run in a pipeline
 // of three: the first products of the next 32 queries and the second products of the last between the vector instructions of
 // these.  Every operand of an MFMA comes from LDS for it alone (128 bytes per cycle and CU at the full rate of the MFMAs, which is
-// what LDS gives), read four MFMAs of its kind ahead.
+// what LDS gives), read three or four MFMAs of its kind ahead.
 // The queries of the G heads that share the keys are one stream, of which `nsplit` workgroups take shares where the key blocks are
 // few or uneven (the first keys are seen by all queries, the last by few); their fp32 sums meet in a last launch, in order.
 // fp16: dS is multiplied by the power of two that takes the largest |dO| to 1 .. 2, so that small gradients do not fall below its
 // smallest numbers; it comes off the sum.
 // Measured: B1 N8192 H16/4 D128 bf16 512 us with row terms (18) and sums (14), 1145 TFLOP/s of its four products in the kernel's own 480; N16384 H8/2 fp16
-// 1065, B2 N2048 H8 D64 50.  MFMAs are busy 50 % of the time; LDS reads and the exponentials share the rest.
+// 1065, B2 N2048 H8 D64 44.  MFMAs are busy 50 % of the time; LDS reads and the exponentials share the rest.
 #include "sa2_causal16.h"
 
 namespace sa2 {
@@ -208,7 +208,9 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, cons
     };
     // One step: first products of piece u + 1 (FIRST), weights of u, second products of u - 1 (SECOND), u of parity PAR; operands of
     // the pieces after those
-    constexpr int SLOTS = 4 * KK, LEAD = 4, LAG = SLOTS == 32 ? 20 : 11;
+    // (LEAD: operands ahead; with three the kernel of 64 columns has two wavefronts per SIMD, dK and dV of B1 N8192 H16 285 us, with four one,
+    // 306)
+    constexpr int SLOTS = 4 * KK, LEAD = D == 64 ? 3 : 4, LAG = SLOTS == 32 ? 20 : 11;
     auto step = [&](auto PP, auto FF, auto SS, uint32_t rat, uint32_t rnext, uint32_t snext, uint32_t cat, uint32_t cnext) __attribute__((always_inline)) {
         constexpr int PAR = decltype(PP)::value;
         constexpr bool FIRST = decltype(FF)::value, SECOND = decltype(SS)::value;

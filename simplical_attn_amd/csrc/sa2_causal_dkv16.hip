@@ -15,7 +15,7 @@
 // smallest numbers; it comes off the sum.
 // Measured: B1 N8192 H16/4 D128 bf16 512 us with row terms (18) and sums (14), 1145 TFLOP/s of its four products in the kernel's own 480; N16384 H8/2 fp16
 // 1065, B2 N2048 H8 D64 44.  MFMAs are busy 50 % of the time; LDS reads and the exponentials share the rest.
-#include "sa2_causal16.h"
+#include "sa2_causal_dq16.h"
 
 namespace sa2 {
 namespace {
@@ -81,18 +81,17 @@ __global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, float* 
 
 // ---- dK, dV ------------------------------------------------------------------------------------------------------------
 template <class E, int D>
-__global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, const float* minus_lse, const float* tops, int ntops, int nsplit, bool padded) {
+__device__ __forceinline__ void keys_gradients16(const Causal& p, const float* minus_lse, const float* tops, int ntops, int nsplit, bool padded, int id, char* lds) {
     using T = QuadTile<D>;
     using X8 = typename E::x8;
     using L = Lone<(D == 128 ? 192 : 96)>;
     constexpr int KK = D / 16, DT = D / 32;
     constexpr int V0 = 0, K0 = DT * 16, KEY0 = 2 * DT * 16, VALUE0 = KEY0 + KK * 4;      // sums of dV and dK, keys, values
-    extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t base = lds_address(lds), stats = base + BUFFERS * Buffer<D>::BYTES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const float f = E::DTYPE == SA2_F16 ? gradient_factor(tops, ntops, (float*)lds) : 1.f;
     int stream, tile;
-    order(blockIdx.x, p.rows.B * p.HK * nsplit, stream, tile);
+    order(id, p.rows.B * p.HK * nsplit, stream, tile);
     const int split = stream % nsplit;
     stream /= nsplit;
     const int b = stream / p.HK, hk = stream % p.HK;
@@ -381,6 +380,20 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, cons
     }
 }
 
+template <class E, int D>
+__global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, const float* minus_lse, const float* tops, int ntops, int nsplit, bool padded) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    keys_gradients16<E, D>(p, minus_lse, tops, ntops, nsplit, padded, blockIdx.x, lds);
+}
+// All gradients in one launch where there are few workgroups, so that one's fill the CUs that the other's short ones leave: `queries`
+// workgroups for dQ, whose longest chains are the longest of all, then those for dK and dV.
+template <class E, int D>
+__global__ __launch_bounds__(THREADS, 1) void causal_bwd16_kernel(Causal p, const float* minus_lse, const float* tops, int ntops, int nsplit, int queries, bool padded) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if ((int)blockIdx.x < queries) queries_gradient16<E, D, 1>(p, tops, ntops, padded, blockIdx.x, lds);
+    else keys_gradients16<E, D>(p, minus_lse, tops, ntops, nsplit, padded, blockIdx.x - queries, lds);
+}
+
 // Sums of the shares in their order: part[split][dK, dV][row][D]
 template <class E>
 __global__ __launch_bounds__(THREADS) void causal_sums_kernel(Causal p, int nsplit) {
@@ -415,15 +428,19 @@ int launch(const Causal& p, float* minus_lse, float* tops, hipStream_t st) {
     if (lanes == 16) causal_terms_kernel<E, 16><<<dim3(blocks), dim3(THREADS), 0, st>>>(p, minus_lse, tops);
     else causal_terms_kernel<E, 8><<<dim3(blocks), dim3(THREADS), 0, st>>>(p, minus_lse, tops);
     if (hipGetLastError() != hipSuccess) return SA2_ERR_LAUNCH_FAILED;
+    const bool together = p.dq.p && (p.dk.p || p.dv.p) && !causal16_two(p);
     if (p.dk.p || p.dv.p) {
         const int nsplit = causal16_splits(p.rows.B, p.rows.N, p.HK, p.G);
         auto of = [&](auto w) {
             constexpr int D = decltype(w)::value;
-            const auto kernel = causal_dkv16_kernel<E, D>;
-            const int64_t grid = (int64_t)p.rows.B * p.HK * nsplit * count_tiles(p.rows, BLOCK);
-            if (grid > 0x7fffffff) return (int)SA2_ERR_TOO_LARGE;
-            if (!allow_full_lds((const void*)kernel)) return (int)SA2_ERR_LAUNCH_FAILED;
-            kernel<<<dim3((unsigned)grid), dim3(THREADS), BUFFERS * (Buffer<D>::BYTES + STATS), st>>>(p, minus_lse, tops, blocks, nsplit, p.D != D);
+            const int64_t keys = (int64_t)p.rows.B * p.HK * nsplit * count_tiles(p.rows, BLOCK), queries = together ? (int64_t)p.rows.B * p.H * count_tiles(p.rows, BLOCK) : 0;
+            constexpr int LDS = BUFFERS * (Buffer<D>::BYTES + STATS);
+            static_assert(LDS >= DQ_BUFFERS * Buffer<D>::BYTES, "");
+            if (keys + queries > 0x7fffffff) return (int)SA2_ERR_TOO_LARGE;
+            const dim3 grid((unsigned)(keys + queries)), block(THREADS);
+            if (!allow_full_lds(together ? (const void*)causal_bwd16_kernel<E, D> : (const void*)causal_dkv16_kernel<E, D>)) return (int)SA2_ERR_LAUNCH_FAILED;
+            if (together) causal_bwd16_kernel<E, D><<<grid, block, LDS, st>>>(p, minus_lse, tops, blocks, nsplit, (int)queries, p.D != D);
+            else causal_dkv16_kernel<E, D><<<grid, block, LDS, st>>>(p, minus_lse, tops, blocks, nsplit, p.D != D);
             return (int)(hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED);
         };
         const int rc = p.D <= 64 ? of(std::integral_constant<int, 64>{}) : of(std::integral_constant<int, 128>{});
@@ -434,7 +451,7 @@ int launch(const Causal& p, float* minus_lse, float* tops, hipStream_t st) {
             if (hipGetLastError() != hipSuccess) return SA2_ERR_LAUNCH_FAILED;
         }
     }
-    return p.dq.p ? launch_causal16_dq(p, E::DTYPE, tops, blocks, st) : SA2_OK;
+    return p.dq.p && !together ? launch_causal16_dq(p, E::DTYPE, tops, blocks, st) : SA2_OK;
 }
 
 }  // namespace

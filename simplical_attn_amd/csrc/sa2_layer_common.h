@@ -87,6 +87,8 @@ int launch_causal_f32_narrow_bwd(const Causal& p, int dtype, bool wide, hipStrea
 // bf16 and fp16 with a head_dim up to 128 that is a multiple of 8, rows on the 16-byte grid
 bool causal16_supported(int D, int dtype);
 bool causal16_layout(const Causal& p, std::initializer_list<const Tensor*> ts);
+// whether a wavefront owns two blocks of 32 queries (forward, dQ)
+bool causal16_two(const Causal& p);
 int launch_causal16_fwd(const Causal& p, int dtype, hipStream_t st);
 // their backward: p.delta receives -delta, minus_lse [B,H,N] -lse / scale, tops the largest |dout| of up to CAUSAL16_TOPS parts
 constexpr int CAUSAL16_TOPS = 1024;

@@ -386,7 +386,9 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, cons
     keys_gradients16<E, D>(p, minus_lse, tops, ntops, nsplit, padded, blockIdx.x, lds);
 }
 // All gradients in one launch where there are few workgroups, so that one's fill the CUs that the other's short ones leave: `queries`
-// workgroups for dQ, whose longest chains are the longest of all, then those for dK and dV.
+// workgroups for dQ, whose longest chains are the longest of all, then those for dK and dV (B2 N2048 H8 D64 80 us apart, 59 together; B4 N1024
+// H16/4 D128 133 and 126; with as many blocks of 256 queries as would give every CU two, B1 N8192 H16/4 D128, 921 and 967: there
+// a wavefront with 64 queries saves more).
 template <class E, int D>
 __global__ __launch_bounds__(THREADS, 1) void causal_bwd16_kernel(Causal p, const float* minus_lse, const float* tops, int ntops, int nsplit, int queries, bool padded) {
     extern __shared__ __attribute__((aligned(16))) char lds[];

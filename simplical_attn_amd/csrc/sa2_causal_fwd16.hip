@@ -125,7 +125,6 @@ bool causal16_layout(const Causal& p, std::initializer_list<const Tensor*> ts) {
 int launch_causal16_fwd(const Causal& p, int dtype, hipStream_t st) {
     auto of = [&](auto e) {
         using E = decltype(e);
-        // two blocks of queries per wavefront halve what LDS has to deliver; one where the workgroups would leave CUs idle
         const bool two = causal16_two(p);
         if (p.D <= 64) return two ? launch<E, 64, 2>(p, st) : launch<E, 64, 1>(p, st);
         return two ? launch<E, 128, 2>(p, st) : launch<E, 128, 1>(p, st);

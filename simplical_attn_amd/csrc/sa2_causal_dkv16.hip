@@ -458,7 +458,7 @@ int launch(const Causal& p, float* minus_lse, float* tops, hipStream_t st) {
 
 }  // namespace
 
-// Shares of a key block's stream: four workgroups per CU over the chip, where the stream is that long (packed sequences: as if
+// Shares of a key block's stream: two workgroups per CU over the chip, where the stream is that long (packed sequences: as if
 // they were one, the bound that the host knows)
 int causal16_splits(int B, int N, int HK, int G) {
     const int64_t blocks = (int64_t)B * HK * ((N + BLOCK - 1) / BLOCK), tiles = (int64_t)G * ((N + TILE_ROWS - 1) / TILE_ROWS);

@@ -184,6 +184,57 @@ def test_later_keys_far_above_the_first(H, HK, D, dtype):
                  [((0,), (0,))], D ** -0.5, dtype, 0)
 
 
+# blocks of 256 queries: two or more per CU, so that a wavefront owns 64 of them
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("B,N,H,HK,D", [(1, 300, 256, 16, 128), (16, 513, 12, 4, 64), (8, 1100, 16, 16, 128), (6, 700, 32, 8, 80), (4, 1500, 24, 24, 64), (1, 1023, 144, 8, 64)])
+def test_two_blocks_per_wavefront(B, N, H, HK, D, dtype):
+    test_many_rows(B, N, H, HK, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("H,HK,D", [(192, 8, 64), (192, 8, 128)])
+def test_two_blocks_and_later_keys_far_above_the_first(H, HK, D, dtype):
+    test_later_keys_far_above_the_first(H, HK, D, dtype)
+
+
+# fp32: more blocks of 32 keys than CUs, which make dK and dV together up to head_dim 64
+@pytest.mark.parametrize("B,N,H,HK,D", [(4, 600, 8, 4, 64), (2, 700, 16, 8, 32), (3, 450, 8, 4, 50), (2, 600, 8, 4, 128)])
+def test_many_rows_of_fp32(B, N, H, HK, D):
+    test_many_rows(B, N, H, HK, D, FP32)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_two_blocks_and_hidden_rows(D, dtype):
+    """Packed, with rows of no sequence that hold NaN and infinities, and NaN in the last keys and values of each sequence."""
+    ends, rows, H, HK = [40, 340, 341, 341, 1100], 1200, 128, 4
+    q, k, v, dout = _inputs((rows,), H, HK, D, dtype, 67 + D)
+    clean = [t.clone() for t in (q, k, v, dout)]
+    for t in (q, k, v, dout):
+        t[:40] = math.nan
+        t[1100:] = math.inf
+    for t in (k, v):
+        t[339] = math.nan
+        t[1099] = math.inf
+    cu = torch.tensor(ends, dtype=torch.int32, device=DEV)
+
+    def same(a, b):
+        # as in test_hidden_rows_may_hold_anything, with sequences of up to 759 rows
+        return ((a.double() - b.double()).abs() <= torch.finfo(a.dtype).eps * b.double().abs() + 2 * (2 * 759 + 16) * 2.0 ** -24 * 64).all()
+
+    out, lse = sa.causal_attention_forward(q, k, v, cu)
+    want, want_lse = sa.causal_attention_forward(*clean[:3], cu)
+    for lo, hi in ((40, 339), (340, 341), (341, 1099)):
+        assert same(out[lo:hi], want[lo:hi]) and same(lse[:, lo:hi], want_lse[:, lo:hi])
+    for x in (out[:40], out[1100:]):
+        assert x.count_nonzero() == 0
+    # gradients of the queries before those keys
+    grads = sa.causal_attention_backward(q, k, v, want, want_lse, clean[3], cu)
+    clear = sa.causal_attention_backward(*clean[:3], want, want_lse, clean[3], cu)
+    for lo, hi in ((40, 339), (340, 341), (341, 1099)):
+        assert same(grads[0][lo:hi], clear[0][lo:hi])
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 def test_gradients_of_autograd(dtype):
     """The training path, which also keeps what rounding the output left; expanded keys get the sum of their gradients."""

@@ -25,7 +25,8 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, or
     "base"    the base raised to base * factor ** (rotary_dim / (rotary_dim - 2)): the slowest pair is divided by
               factor, the fastest stays
     "parts"   pairs that make at most slow_turns turns over original_length positions are divided by factor, those that
-              make fast_turns or more stay, between them the pair's number decides linearly
+              make fast_turns or more stay, between them the pair's number decides linearly ("NTK-by-parts" of the YaRN
+              paper, Peng et al. 2023, with its ends of the ramp: whole pair numbers, 0 at least and rotary_dim - 1 at most)
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_dim must be even and at least 2, got %r" % (rotary_dim,))
@@ -42,10 +43,12 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, or
     elif scaling == "parts":
         if not original_length or not 0 < slow_turns < fast_turns:
             raise ValueError('scaling="parts" needs original_length and 0 < slow_turns < fast_turns')
-        # the pair, as a real number, that makes t turns over the original length
+        # the pair, as a real number, that makes t turns over the original length; the last one may make more than slow_turns,
+        # so that the ramp ends behind it
         pair = lambda t: rotary_dim * math.log(original_length / (2 * math.pi * t)) / (2 * math.log(base))
-        first, last = max(0, math.floor(pair(fast_turns))), min(rotary_dim // 2 - 1, math.ceil(pair(slow_turns)))
+        first, last = max(0, math.floor(pair(fast_turns))), min(rotary_dim - 1, math.ceil(pair(slow_turns)))
         kept = 1 - ((pairs - first) / max(last - first, 1e-3)).clamp(0, 1)
+        kept[pairs >= last] = 0
         f = f * kept + f / factor * (1 - kept)
     elif scaling not in (None, "base"):
         raise ValueError('unknown scaling %r (None, "linear", "base", "parts")' % (scaling,))

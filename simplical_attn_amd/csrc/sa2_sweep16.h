@@ -8,8 +8,8 @@
 // outputs and queries stay in accumulation registers that the kernel owns; left to the compiler they moved to and fro, 280
 // instructions more per 64 MFMAs, and the MFMAs stood in rows: 583 us instead of 302 at B1 N8192 H16/4 D128).
 // The weights are e^(s - m) with m the row's maximum over its first 32 keys: no maximum and no scaling of the output in the
-// sweep.  Rounding weights to 16 bits costs half a step of each, whatever m; a unit whose sum passes REF_LIMIT has the workgroup
-// sweep its keys a second time, with the running maximum.
+// sweep.  Rounding weights to 16 bits costs half a step of each, whatever m; a unit whose sum passes RefLimit, or first keys whose scores
+// are all minus infinity, have the workgroup sweep its keys a second time, with the running maximum.
 // K and V come by direct global->LDS loads into three buffers of 64 keys, so that one barrier per 64 keys is enough.
 #pragma once
 
@@ -252,7 +252,10 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
                 logits(N, st[n]);
                 ready(st[n]);
                 m[n] = top_of(st[n], ~0u);
-                m[n] = m[n] == -INFINITY ? 0.f : m[n];
+                if (m[n] == -INFINITY) {                                   // (scores of minus infinity say nothing about the others)
+                    m[n] = 0.f;
+                    worst = INFINITY;
+                }
             });
             if constexpr (NQ == 1) {
                 load_keys(keys_at(base, 1));

@@ -1,0 +1,69 @@
+"""Causal attention and large drafted trees where a row's first 32 keys say little about the others: first keys whose scores are minus
+infinity."""
+import math
+
+import pytest
+import torch
+
+import simplical_attn_amd as sa
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, FP16 = torch.bfloat16, torch.float16
+E = 2.0 ** -24
+
+
+def _rows(heads, N, D, dtype, seed):
+    """q [1, N, heads, D], k, v [1, N, 1, D]; scores of scale 1 / 8: column 0 of q is 8, so that column 0 of k is added to them."""
+    g = torch.Generator().manual_seed(seed)
+    q, k, v = (torch.randn(1, N, h, D, generator=g).to(DEV) for h in (heads, 1, 1))
+    q[..., 0] = 8
+    k[..., 0] = 0
+    return [x.to(dtype) for x in (q, k, v)]
+
+
+def _check(out, q, k, v, rows, scale, seen=None):
+    """Bounds as in causal_util.py, of rows `rows` of one sequence (seen: their masks, else causal)."""
+    t = torch.finfo(out.dtype).eps / 2
+    Q, K, V, D = q[rows].double(), k.double(), v.double(), q.shape[-1]
+    n = len(K)
+    M = seen if seen is not None else torch.arange(n, device=DEV)[None] <= torch.arange(n, device=DEV)[rows, None]
+    S = (Q @ K.T * scale).masked_fill(~M, -math.inf)
+    P = torch.softmax(S, 1)
+    r = ((D + 4) * E * scale * (Q.abs() @ K.abs().nan_to_num(posinf=0).T)).masked_fill(~M, 0).amax(1, keepdim=True)
+    want = P @ V
+    low = 2.0 ** -25 if out.dtype == FP16 else 0.0
+    bound = (P @ V.abs()) * (2 * r + t + (n + 16) * E) + low * (M.double() @ V.abs()) + t * want.abs() + 2.0 ** -24
+    x = out[rows].double()
+    assert torch.isfinite(x).all()
+    assert ((x - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("heads,D", [(2, 64), (2, 128), (192, 128)])
+def test_first_keys_without_a_score(heads, D, dtype):
+    """The first 32 keys' scores are minus infinity, the others' far below zero."""
+    q, k, v = _rows(heads, 600, D, dtype, D + 1)
+    k[..., 0] = -300
+    k[:, :32, :, 0] = -math.inf
+    out = sa.causal_attention(q, k, v, scale=0.125)
+    for h in (0, heads - 1):
+        _check(out[0, :, h], q[0, :, h], k[0, :, 0], v[0, :, 0], slice(32, None), 0.125)
+
+
+def _tree(q, k, v, T, **kw):
+    """The last T rows of q as a chain of drafted nodes over the other rows of k and v."""
+    n = k.shape[1] - T
+    cut = lambda x, a, b: x[:, a:b].contiguous()
+    lengths = torch.tensor([n], dtype=torch.int32, device=DEV)
+    return sa.tree_attention(cut(q, n, n + T), cut(k, n, n + T), cut(v, n, n + T), None, cut(k, 0, n), cut(v, 0, n), lengths, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_first_keys_without_a_score_in_trees(dtype):
+    q, k, v = _rows(4, 40 + 2000, 128, dtype, 4)
+    k[..., 0] = -300
+    k[:, :700, :, 0] = -math.inf
+    out = _tree(q, k, v, 40, scale=0.125)
+    for h in (0, 3):
+        _check(torch.cat((out[0, :1, h].expand(2000, 128), out[0, :, h])), q[0, :, h], k[0, :, 0], v[0, :, 0], slice(2000, None), 0.125)

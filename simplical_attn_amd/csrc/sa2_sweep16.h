@@ -9,7 +9,8 @@
 // instructions more per 64 MFMAs, and the MFMAs stood in rows: 583 us instead of 302 at B1 N8192 H16/4 D128).
 // The weights are e^(s - m) with m the row's maximum over its first 32 keys: no maximum and no scaling of the output in the
 // sweep.  Rounding weights to 16 bits costs half a step of each, whatever m; a unit whose sum passes RefLimit, or first keys whose scores
-// are all minus infinity, have the workgroup sweep its keys a second time, with the running maximum.
+// are all minus infinity, have the workgroup sweep its keys a second time, with the running maximum; in bf16, whose values reach the end
+// of fp32's range, an output that is no number does so too once weights are above 1.
 // K and V come by direct global->LDS loads into three buffers of 64 keys, so that one barrier per 64 keys is enough.
 #pragma once
 
@@ -23,6 +24,7 @@ constexpr int BUFFERS = 3;
 template <class E> struct RefLimit;
 template <> struct RefLimit<ElemBF16> { static constexpr float value = 1.152921504606847e18f; };   // 2^60
 template <> struct RefLimit<ElemF16> { static constexpr float value = 32768.f; };                  // below 65504
+constexpr float OUTPUT_CHECK = 64.f;                        // sum of a unit (16 weights of a lane) up to which outputs are not looked at
 
 // Accumulation registers: outputs of block n and columns 32 d .. from O0 + (n * D/32 + d) * 16 on, queries from Q0 + (n * D/16 + kk) * 4
 template <int D, int NQ>
@@ -309,7 +311,20 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
             for (int sub = t == done / 2 ? done % 2 : 0; sub < 2; ++sub)
                 if (2 * t + sub < src.pieces) piece(here, sub, 2 * t + sub, pass != 0);
         }
-        if (!__syncthreads_or(worst > RefLimit<E>::value)) break;
+        bool again = worst > RefLimit<E>::value;
+        if constexpr (E::DTYPE == SA2_BF16) {
+            // (with smaller weights a second sweep would come no further; fp16 values times weights up to the limit are far from fp32's end)
+            if (pass == 0 && __any(worst > OUTPUT_CHECK)) {
+                rest();
+                uint32_t bits = 0;
+                static_for<NQ * DT * 4>([&](auto X) __attribute__((always_inline)) {
+                    const float4 o = L::template get_regs<O0 + 4 * decltype(X)::value>();
+                    for (const float y : {o.x, o.y, o.z, o.w}) bits |= (__float_as_uint(y) & 0x7f800000u) + 0x00800000u;
+                });
+                again = again || bits >> 31;
+            }
+        }
+        if (!__syncthreads_or(again)) break;
     }
     rest();
 }

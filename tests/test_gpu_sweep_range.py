@@ -1,5 +1,5 @@
-"""Causal attention and large drafted trees where a row's first 32 keys say little about the others: first keys whose scores are minus
-infinity."""
+"""Causal attention and large drafted trees where a row's first 32 keys say little about the others: values so large that weights above
+1 take the sums out of fp32's range, first keys whose scores are minus infinity."""
 import math
 
 import pytest
@@ -39,6 +39,20 @@ def _check(out, q, k, v, rows, scale, seen=None):
     assert ((x - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("size", [90, 120])
+@pytest.mark.parametrize("rise", [3.0, 8.0, 40.0])
+@pytest.mark.parametrize("heads,D", [(2, 64), (2, 128), (192, 64), (192, 128)])
+def test_large_values(heads, D, rise, size):
+    """bf16 values of 2^size and keys from the 300th on with scores `rise` above the first ones'."""
+    q, k, v = _rows(heads, 700, D, BF16, D)
+    k[:, 300:, :, 0] = rise
+    v = (v.double().clamp(-4, 4) * 2.0 ** size).to(BF16)
+    out = sa.causal_attention(q, k, v, scale=0.125)
+    # (with weights of at most 1, 700 values of up to 2^122 are in range)
+    for h in (0, heads - 1):
+        _check(out[0, :, h], q[0, :, h], k[0, :, 0], v[0, :, 0], slice(None), 0.125)
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("heads,D", [(2, 64), (2, 128), (192, 128)])
 def test_first_keys_without_a_score(heads, D, dtype):
@@ -57,6 +71,18 @@ def _tree(q, k, v, T, **kw):
     cut = lambda x, a, b: x[:, a:b].contiguous()
     lengths = torch.tensor([n], dtype=torch.int32, device=DEV)
     return sa.tree_attention(cut(q, n, n + T), cut(k, n, n + T), cut(v, n, n + T), None, cut(k, 0, n), cut(v, 0, n), lengths, **kw)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rise", [8.0, 40.0])
+@pytest.mark.parametrize("size", [100, 120])
+def test_large_values_in_trees(D, rise, size):
+    q, k, v = _rows(4, 40 + 3000, D, BF16, D + 2)
+    k[:, 200:, :, 0] = rise
+    v = (v.double().clamp(-4, 4) * 2.0 ** size).to(BF16)
+    out = _tree(q, k, v, 40, scale=0.125)
+    for h in (0, 3):
+        _check(torch.cat((out[0, :1, h].expand(3000, D), out[0, :, h])), q[0, :, h], k[0, :, 0], v[0, :, 0], slice(3000, None), 0.125)
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])

@@ -8,7 +8,8 @@
 // outputs and queries stay in accumulation registers that the kernel owns; left to the compiler they moved to and fro, 280
 // instructions more per 64 MFMAs, and the MFMAs stood in rows: 583 us instead of 302 at B1 N8192 H16/4 D128).
 // The weights are e^(s - m) with m the row's maximum over its first 32 keys: no maximum and no scaling of the output in the
-// sweep.  Rounding weights to 16 bits costs half a step of each, whatever m; a unit whose sum passes RefLimit, or first keys whose scores
+// sweep.  Rounding weights to bf16 costs half a step of each, whatever m, to fp16 half a step or 2^-25, which is why there m is lower than
+// that (lowered_by).  A unit whose sum passes RefLimit, or first keys whose scores
 // are all minus infinity, have the workgroup sweep its keys a second time, with the running maximum; in bf16, whose values reach the end
 // of fp32's range, an output that is no number does so too once weights are above 1.
 // K and V come by direct global->LDS loads into three buffers of 64 keys, so that one barrier per 64 keys is enough.
@@ -24,6 +25,17 @@ constexpr int BUFFERS = 3;
 template <class E> struct RefLimit;
 template <> struct RefLimit<ElemBF16> { static constexpr float value = 1.152921504606847e18f; };   // 2^60
 template <> struct RefLimit<ElemF16> { static constexpr float value = 32768.f; };                  // below 65504
+// Many keys far below the first ones add up, and in fp16 all weights under 2^-25 would be lost.  Of `keys` keys rounding takes less than
+// 2^-15 of the largest weight where weights are 2^lift times as large, that is, the reference point lift / c lower (c: |scale| log2(e)).
+// More would leave less room for scores above the first keys' (lift 4 at 16384 keys: e^7.6; with 6, scores of standard deviation 2 would
+// take half of the workgroups through a second sweep).
+template <class E>
+__device__ __forceinline__ float lowered_by(int keys, float c) {
+    if (E::DTYPE != SA2_F16 || keys <= 1024) return 0.f;
+    const int lift = 32 - __clz(keys - 1) - 10;
+    const float by = c > 1e-20f ? (float)(lift < 8 ? lift : 8) / c : 0.f;
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(by)));       // (the same in all lanes)
+}
 constexpr float OUTPUT_CHECK = 64.f;                        // sum of a unit (16 weights of a lane) up to which outputs are not looked at
 
 // Accumulation registers: outputs of block n and columns 32 d .. from O0 + (n * D/32 + d) * 16 on, queries from Q0 + (n * D/16 + kk) * 4
@@ -38,6 +50,7 @@ struct SweepRegs : Lone<(D * NQ > 128 ? 192 : 96)> {
 //   pieces                      pieces of 32 keys that it needs at all
 //   sees(n, piece)              what the lane's row of block n sees of a piece, bit by key
 //   guarded(piece)              values that some row does not see may be infinite or NaN
+//   lower                       lowered_by of the keys
 // Queries lie in their registers; outputs are left in theirs, in units of e^(scale m), with the lane's part of their sums in l.
 // LDS holds BUFFERS tiles from `base` on (with a fourth, and requests two tiles ahead, times were the same).
 // c: |scale| log2(e).  All wavefronts of the workgroup call it.
@@ -202,7 +215,7 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
             constexpr int n = decltype(N)::value;
             const uint32_t seen = src.sees(n, which);
             if (safe || __any(m[n] == -INFINITY)) {
-                const float top = top_of(st[n], seen);
+                const float top = top_of(st[n], seen) - src.lower;
                 if (safe) {
                     const float now = fmaxf(m[n], top), f = m[n] == -INFINITY ? 0.f : exp2f((m[n] - now) * c);
                     l[n] *= f;
@@ -253,7 +266,7 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
                 constexpr int n = decltype(N)::value;
                 logits(N, st[n]);
                 ready(st[n]);
-                m[n] = top_of(st[n], ~0u);
+                m[n] = top_of(st[n], ~0u) - src.lower;
                 if (m[n] == -INFINITY) {                                   // (scores of minus infinity say nothing about the others)
                     m[n] = 0.f;
                     worst = INFINITY;

@@ -18,6 +18,7 @@ struct TreeKeys {
     const int32_t* pages;                                  // of the share, the first of them page0
     const char *kc, *vc, *kd, *vd;                         // cache and drafted rows of the key head
     int b, page0, held, cached, lo, tiles, full, pieces, chunk, sub;
+    float lower;
     bool pad, together;
     uint64_t seen[NQ];                                     // drafted nodes that the lane's rows see (0: a row that is not there)
 
@@ -123,6 +124,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree_rows16_kernel(Tree p, int blo
 
     const uint64_t ancestors = tree_ancestors(p, b);
     const float c = fabsf(p.scale) * LOG2E;
+    keys.lower = lowered_by<E>(held + p.T, c);
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
     int node[NQ], head[NQ];
     static_for<NQ>([&](auto N) __attribute__((always_inline)) {

@@ -1,5 +1,5 @@
 """Causal attention and large drafted trees where a row's first 32 keys say little about the others: values so large that weights above
-1 take the sums out of fp32's range, first keys whose scores are minus infinity."""
+1 take the sums out of fp32's range, first keys whose scores are minus infinity, fp16 weights below 2^-25 of the largest."""
 import math
 
 import pytest
@@ -32,7 +32,9 @@ def _check(out, q, k, v, rows, scale, seen=None):
     P = torch.softmax(S, 1)
     r = ((D + 4) * E * scale * (Q.abs() @ K.abs().nan_to_num(posinf=0).T)).masked_fill(~M, 0).amax(1, keepdim=True)
     want = P @ V
-    low = 2.0 ** -25 if out.dtype == FP16 else 0.0
+    # fp16: of the keys up to the row's own at most 2^-25 each, less by the power of two that their number brings (2^10: 1, up to 2^8)
+    keys = M.sum(1, keepdim=True).double().clamp(min=1)
+    low = 2.0 ** (-25 - (keys.log2().ceil() - 10).clamp(0, 8)) if out.dtype == FP16 else 0.0
     bound = (P @ V.abs()) * (2 * r + t + (n + 16) * E) + low * (M.double() @ V.abs()) + t * want.abs() + 2.0 ** -24
     x = out[rows].double()
     assert torch.isfinite(x).all()
@@ -93,3 +95,37 @@ def test_first_keys_without_a_score_in_trees(dtype):
     out = _tree(q, k, v, 40, scale=0.125)
     for h in (0, 3):
         _check(torch.cat((out[0, :1, h].expand(2000, 128), out[0, :, h])), q[0, :, h], k[0, :, 0], v[0, :, 0], slice(2000, None), 0.125)
+
+
+@pytest.mark.parametrize("T", [1, 12, 40])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_cached_key_far_above_all_others(D, T):
+    """fp16: the first key's weight is 2^25 times every other one's, whose sum still counts."""
+    N = 40000
+    g = torch.Generator().manual_seed(D)
+    v = 32 * (torch.randn(1, N + T, 1, D, generator=g).to(DEV).half().abs() + 1)
+    v[:, 0] = -0.01
+    k = torch.zeros(1, N + T, 1, D, dtype=FP16, device=DEV)
+    q = torch.zeros(1, N + T, 4, D, dtype=FP16, device=DEV)
+    q[..., 0], k[:, 0, :, 0] = 1, 17.5
+    out = _tree(q, k, v, T, scale=1.0)
+    for h in (0, 3):
+        _check(torch.cat((out[0, :1, h].expand(N, D), out[0, :, h])), q[0, :, h], k[0, :, 0], v[0, :, 0], slice(N, None), 1.0)
+
+
+def test_a_key_far_above_all_others():
+    """fp16: the first key's weight is 2^25 times every other one's, whose sum still counts."""
+    N, D = 24000, 64
+    g = torch.Generator().manual_seed(33)
+    v = 32 * (torch.randn(1, N, 1, D, generator=g).to(DEV).half().abs() + 1)
+    v[:, 0] = -0.01
+    k = torch.zeros(1, N, 1, D, dtype=FP16, device=DEV)
+    q = torch.zeros(1, N, 2, D, dtype=FP16, device=DEV)
+    q[..., 0], k[:, 0, :, 0] = 1, 17.5
+    out, lse = sa.causal_attention_forward(q, k, v, scale=1.0)
+    for h in (0, 1):
+        rows = slice(N - 2000, None, 7)
+        _check(out[0, :, h], q[0, :, h], k[0, :, 0], v[0, :, 0], rows, 1.0)
+        n = torch.arange(N, device=DEV).double()
+        # the score is exact; a logarithm and a product in 32 bits, sums of n terms
+        assert ((lse[0, h].double() - (math.exp(17.5) + n).log()).abs() <= (n + 64) * E).all()

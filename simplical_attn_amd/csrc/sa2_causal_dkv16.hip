@@ -11,8 +11,7 @@
 // what LDS gives), read three or four MFMAs of its kind ahead.
 // The queries of the G heads that share the keys are one stream, of which `nsplit` workgroups take shares where the key blocks are
 // few or uneven (the first keys are seen by all queries, the last by few); their fp32 sums meet in a last launch, in order.
-// fp16: dS is multiplied by the power of two that takes the largest |dO| to 1 .. 2, so that small gradients do not fall below its
-// smallest numbers; it comes off the sum.
+// fp16: dS is multiplied by a power of two of its key's own (sa2_causal16.h), which comes off the sum.
 // Measured: B1 N8192 H16/4 D128 bf16 512 us with row terms (18) and sums (14), 1145 TFLOP/s of its four products in the kernel's own 480; N16384 H8/2 fp16
 // 1065, B2 N2048 H8 D64 44.  MFMAs are busy 50 % of the time; LDS reads and the exponentials share the rest.
 #include "sa2_causal_dq16.h"
@@ -22,12 +21,13 @@ namespace {
 
 constexpr int BUFFERS = 4, BLOCK = SUB * WAVES;            // keys per workgroup
 constexpr int STATS = 2 * TILE_ROWS * 4;                    // bytes of the row terms of a tile
+constexpr int TERMS_BLOCKS = 1024;
 
 // ---- row terms: delta = sum_d dO O, stored as -delta, and -lse / scale ----------------------------------------------
 // O with what its rounding left, where the forward wrote that: from the rounded output alone delta carries half a step of every
 // value, which in sequences of up to a hundred rows makes dQ and dK 1.5 to 2.3 times as far off as their own rounding does.
 template <class E, int LANES>                               // lanes per row, 16 bytes each
-__global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, float* minus_lse, float* tops) {
+__global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, Causal16Terms terms) {
     const int lane = threadIdx.x % LANES, per = THREADS / LANES;
     const int64_t rows = (int64_t)p.rows.B * p.rows.N * p.H;
     const float over = -1.f / p.scale;
@@ -36,10 +36,9 @@ __global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, float* 
         lo = p.rows.cu[0];
         hi = p.rows.cu[p.rows.sequences];
     }
-    float top = 0.f;
     for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < rows; r0 += (int64_t)gridDim.x * per) {
         const int64_t r = r0 + threadIdx.x / LANES;
-        float sum = 0.f, large = 0.f;
+        float sum = 0.f, square = 0.f;
         int h = 0, n = 0, b = 0;
         if (r < rows) {
             h = (int)(r % p.H);
@@ -55,33 +54,113 @@ __global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, float* 
                 for (int i = 0; i < 4; ++i) {
                     const float y0 = E::lo(ys[i]), y1 = E::hi(ys[i]);
                     sum = fmaf(E::lo(xs[i]) + E::lo(zs[i]), y0, fmaf(E::hi(xs[i]) + E::hi(zs[i]), y1, sum));
-                    large = fmaxf(large, fmaxf(fabsf(y0), fabsf(y1)));
+                    if (E::DTYPE == SA2_F16) square = fmaf(y0, y0, fmaf(y1, y1, square));
                 }
             }
         }
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        if (r < rows && n >= lo && n < hi) {
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            sum += __shfl_xor(sum, o);
+            if (E::DTYPE == SA2_F16) square += __shfl_xor(square, o);
+        }
+        if (r < rows && n >= lo && n < hi && lane == 0) {
             const int64_t at = ((int64_t)b * p.H + h) * p.rows.N + n;
-            if (lane == 0) {
-                p.delta[at] = -sum;
-                minus_lse[at] = p.lse[at] * over;
-            }
-            top = fmaxf(top, large);
+            p.delta[at] = -sum;
+            terms.minus_lse[at] = p.lse[at] * over;
+            if (E::DTYPE == SA2_F16) terms.dout[at] = sqrtf(square);
         }
     }
-    if (E::DTYPE == SA2_F16) {
-        __shared__ float tops_of[WAVES];
-        top = wave_max(top);
-        if ((threadIdx.x & 63) == 0) tops_of[threadIdx.x >> 6] = top;
-        __syncthreads();
-        if (threadIdx.x == 0) tops[blockIdx.x] = fmaxf(fmaxf(tops_of[0], tops_of[1]), fmaxf(tops_of[2], tops_of[3]));
+    if constexpr (E::DTYPE == SA2_F16) {
+        const int64_t values = (int64_t)p.rows.B * p.rows.N * p.HK;
+        for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < values; r0 += (int64_t)gridDim.x * per) {
+            const int64_t r = r0 + threadIdx.x / LANES;
+            const int h = (int)(r % p.HK), n = (int)(r / p.HK % p.rows.N), b = (int)(r / p.HK / p.rows.N);
+            float square = 0.f;
+            if (r < values && lane * 8 < p.D) {
+                const uint4 x = *(const uint4*)((const uint16_t*)p.v.p + p.v.off(b, n, h) + lane * 8);
+                const uint32_t* xs = &x.x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) square = fmaf(E::lo(xs[i]), E::lo(xs[i]), fmaf(E::hi(xs[i]), E::hi(xs[i]), square));
+            }
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) square += __shfl_xor(square, o);
+            if (r < values && lane == 0) terms.v[((int64_t)b * p.HK + h) * p.rows.N + n] = sqrtf(square);
+        }
     }
+}
+
+// The factor of the lane's key j0 + 32 * wave + lane % 32 for shares lo .. hi-1 of the stream of tiles (`per` of each head, from row j0 on).
+// `lds`: 2 * WAVES + 2 * BLOCK floats.  Every thread calls it
+__device__ __forceinline__ float key_factor(const Causal& p, const Causal16Terms& terms, const Span& s, int hk, int j0, int per, int lo, int hi, float* lds) {
+    constexpr int OWN = BLOCK / TILE_ROWS, AHEAD = 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t first = ((int64_t)s.b * p.H + hk * p.G) * p.rows.N + s.first + j0;
+    // rows behind the block: each wavefront every fourth tile, loads of four under way
+    float dout = 0.f, delta = 0.f;
+    int g = (lo + wave) / per, i = lo + wave - g * per;
+    for (int x = lo + wave; x < hi;) {
+        float a[AHEAD], b[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int row = i * TILE_ROWS + lane;
+            const bool there = x < hi && i >= OWN && j0 + row < s.len;
+            const int64_t at = first + (there ? (int64_t)g * p.rows.N + row : 0);
+            a[k] = there ? terms.dout[at] : 0.f;
+            b[k] = there ? p.delta[at] : 0.f;
+            x += WAVES;
+            i += WAVES;
+            while (i >= per) {
+                i -= per;
+                ++g;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            dout = fmaxf(dout, finite_or_zero(a[k]));
+            delta = fmaxf(delta, finite_or_zero(b[k]));
+        }
+    }
+    dout = wave_max(dout);
+    delta = wave_max(delta);
+    // rows of the block: the largest of a row's heads
+    const int t = threadIdx.x;
+    if (t < BLOCK) {
+        float a = 0.f, b = 0.f;
+        if (j0 + t < s.len && lo < hi)
+            for (int head = lo / per; head <= (hi - 1) / per; ++head) {
+                const int x = head * per + t / TILE_ROWS;
+                if (x < lo || x >= hi) continue;
+                const int64_t at = first + (int64_t)head * p.rows.N + t;
+                a = fmaxf(a, finite_or_zero(terms.dout[at]));
+                b = fmaxf(b, finite_or_zero(p.delta[at]));
+            }
+        lds[2 * WAVES + t] = a;
+        lds[2 * WAVES + BLOCK + t] = b;
+    }
+    if (lane == 0) {
+        lds[wave] = dout;
+        lds[WAVES + wave] = delta;
+    }
+    __syncthreads();
+    const int key = 32 * wave + (lane & 31);
+    float reach[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const float* const own = lds + 2 * WAVES + w * BLOCK;
+        float later = 0.f;
+#pragma unroll
+        for (int k = 0; k < BLOCK / 64; ++k) later = fmaxf(later, 64 * k + lane >= 32 * wave + 32 ? own[64 * k + lane] : 0.f);
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) later = fmaxf(later, lds[w * WAVES + k]);
+        reach[w] = fmaxf(wave_max(later), largest_from(own[key]));
+    }
+    const float v = j0 + key < s.len ? terms.v[((int64_t)s.b * p.HK + hk) * p.rows.N + s.first + j0 + key] : 0.f;
+    return gradient_factor(fmaf(reach[0], v, reach[1]));
 }
 
 // ---- dK, dV ------------------------------------------------------------------------------------------------------------
 template <class E, int D>
-__device__ __forceinline__ void keys_gradients16(const Causal& p, const float* minus_lse, const float* tops, int ntops, int nsplit, bool padded, int id, char* lds) {
+__device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16Terms& terms, int nsplit, bool padded, int id, char* lds) {
     using T = QuadTile<D>;
     using X8 = typename E::x8;
     using L = Lone<(D == 128 ? 192 : 96)>;
@@ -89,7 +168,6 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const float* m
     constexpr int V0 = 0, K0 = DT * 16, KEY0 = 2 * DT * 16, VALUE0 = KEY0 + KK * 4;      // sums of dV and dK, keys, values
     const uint32_t base = lds_address(lds), stats = base + BUFFERS * Buffer<D>::BYTES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const float f = E::DTYPE == SA2_F16 ? gradient_factor(tops, ntops, (float*)lds) : 1.f;
     int stream, tile;
     order(id, p.rows.B * p.HK * nsplit, stream, tile);
     const int split = stream % nsplit;
@@ -108,6 +186,11 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const float* m
     }
     const int j0 = s.block * BLOCK, mine = j0 + wave * SUB, key = mine + (lane & 31);
     const float c = p.scale * LOG2E;
+    // the stream: tiles of 64 queries, from the one with the block's first key on, of one head after the other
+    const int t0 = j0 / TILE_ROWS, per = (s.len + TILE_ROWS - 1) / TILE_ROWS - t0;
+    const int64_t all = (int64_t)per * p.G;
+    const int lo = (int)(all * split / nsplit), hi = (int)(all * (split + 1) / nsplit);
+    const float f = E::DTYPE == SA2_F16 ? key_factor(p, terms, s, hk, j0, per, lo, hi, (float*)lds) : 1.f;
 
     static_for<2>([&](auto W) __attribute__((always_inline)) {
         const Tensor& t = decltype(W)::value ? p.v : p.k;
@@ -126,10 +209,6 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const float* m
     });
     static_for<8 * DT>([&](auto X) __attribute__((always_inline)) { L::template set_regs<4 * decltype(X)::value>(0u, 0u, 0u, 0u); });
 
-    // the stream: tiles of 64 queries, from the one with the block's first key on, of one head after the other
-    const int t0 = j0 / TILE_ROWS, per = (s.len + TILE_ROWS - 1) / TILE_ROWS - t0;
-    const int64_t all = (int64_t)per * p.G;
-    const int lo = (int)(all * split / nsplit), hi = (int)(all * (split + 1) / nsplit);
     int rg = lo / per, rt = lo - rg * per;                                 // head and tile of the next request
     Fetch<D> fetch;
     fetch.init(p.q, p.dout, s, hk * p.G + rg, p.D);
@@ -142,7 +221,7 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const float* m
         const int first = (t0 + rt) * TILE_ROWS;
         fetch.request(first, s.len, buffer(arriving), padded);
         if (wave < 2) {
-            const float* src = (wave ? p.delta : minus_lse) + stat_row + (int64_t)(hk * p.G + rg) * p.rows.N + first + lane;
+            const float* src = (wave ? p.delta : terms.minus_lse) + stat_row + (int64_t)(hk * p.G + rg) * p.rows.N + first + lane;
             lds_request4(first + lane < s.len ? (const void*)src : (const void*)zero_chunk, stats + arriving * STATS + wave * TILE_ROWS * 4);
         }
         arriving = after(arriving);
@@ -301,7 +380,7 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const float* m
         }
     };
     if (lo < hi) {
-        if (E::DTYPE == SA2_F16) __syncthreads();                          // (the factor's reduction has left LDS)
+        if (E::DTYPE == SA2_F16) __syncthreads();                          // (the factors have left LDS)
         request();
         arrive();
         constexpr int OWN = BLOCK / TILE_ROWS;                             // a head's first tiles hold the block's own rows
@@ -381,19 +460,19 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const float* m
 }
 
 template <class E, int D>
-__global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, const float* minus_lse, const float* tops, int ntops, int nsplit, bool padded) {
+__global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, Causal16Terms terms, int nsplit, bool padded) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    keys_gradients16<E, D>(p, minus_lse, tops, ntops, nsplit, padded, blockIdx.x, lds);
+    keys_gradients16<E, D>(p, terms, nsplit, padded, blockIdx.x, lds);
 }
 // All gradients in one launch where there are few workgroups, so that one's fill the CUs that the other's short ones leave: `queries`
 // workgroups for dQ, whose longest chains are the longest of all, then those for dK and dV (B2 N2048 H8 D64 80 us apart, 59 together; B4 N1024
 // H16/4 D128 133 and 126; with as many blocks of 256 queries as would give every CU two, B1 N8192 H16/4 D128, 921 and 967: there
 // a wavefront with 64 queries saves more).
 template <class E, int D>
-__global__ __launch_bounds__(THREADS, 1) void causal_bwd16_kernel(Causal p, const float* minus_lse, const float* tops, int ntops, int nsplit, int queries, bool padded) {
+__global__ __launch_bounds__(THREADS, 1) void causal_bwd16_kernel(Causal p, Causal16Terms terms, int nsplit, int queries, bool padded) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    if ((int)blockIdx.x < queries) queries_gradient16<E, D, 1>(p, tops, ntops, padded, blockIdx.x, lds);
-    else keys_gradients16<E, D>(p, minus_lse, tops, ntops, nsplit, padded, blockIdx.x - queries, lds);
+    if ((int)blockIdx.x < queries) queries_gradient16<E, D, 1>(p, terms, padded, blockIdx.x, lds);
+    else keys_gradients16<E, D>(p, terms, nsplit, padded, blockIdx.x - queries, lds);
 }
 
 // Sums of the shares in their order: part[split][dK, dV][row][D]
@@ -422,13 +501,13 @@ __global__ __launch_bounds__(THREADS) void causal_sums_kernel(Causal p, int nspl
 }
 
 template <class E>
-int launch(const Causal& p, float* minus_lse, float* tops, hipStream_t st) {
+int launch(const Causal& p, const Causal16Terms& terms, hipStream_t st) {
     const int64_t rows = (int64_t)p.rows.B * p.rows.N * p.H;
     const int lanes = p.D > 64 ? 16 : 8;
     const int64_t want = (rows + THREADS / lanes - 1) / (THREADS / lanes);
-    const int blocks = (int)(want < CAUSAL16_TOPS ? want : CAUSAL16_TOPS);
-    if (lanes == 16) causal_terms_kernel<E, 16><<<dim3(blocks), dim3(THREADS), 0, st>>>(p, minus_lse, tops);
-    else causal_terms_kernel<E, 8><<<dim3(blocks), dim3(THREADS), 0, st>>>(p, minus_lse, tops);
+    const int blocks = (int)(want < TERMS_BLOCKS ? want : TERMS_BLOCKS);
+    if (lanes == 16) causal_terms_kernel<E, 16><<<dim3(blocks), dim3(THREADS), 0, st>>>(p, terms);
+    else causal_terms_kernel<E, 8><<<dim3(blocks), dim3(THREADS), 0, st>>>(p, terms);
     if (hipGetLastError() != hipSuccess) return SA2_ERR_LAUNCH_FAILED;
     const bool together = p.dq.p && (p.dk.p || p.dv.p) && !causal16_two(p);
     if (p.dk.p || p.dv.p) {
@@ -441,8 +520,8 @@ int launch(const Causal& p, float* minus_lse, float* tops, hipStream_t st) {
             if (keys + queries > 0x7fffffff) return (int)SA2_ERR_TOO_LARGE;
             const dim3 grid((unsigned)(keys + queries)), block(THREADS);
             if (!allow_full_lds(together ? (const void*)causal_bwd16_kernel<E, D> : (const void*)causal_dkv16_kernel<E, D>)) return (int)SA2_ERR_LAUNCH_FAILED;
-            if (together) causal_bwd16_kernel<E, D><<<grid, block, LDS, st>>>(p, minus_lse, tops, blocks, nsplit, (int)queries, p.D != D);
-            else causal_dkv16_kernel<E, D><<<grid, block, LDS, st>>>(p, minus_lse, tops, blocks, nsplit, p.D != D);
+            if (together) causal_bwd16_kernel<E, D><<<grid, block, LDS, st>>>(p, terms, nsplit, (int)queries, p.D != D);
+            else causal_dkv16_kernel<E, D><<<grid, block, LDS, st>>>(p, terms, nsplit, p.D != D);
             return (int)(hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED);
         };
         const int rc = p.D <= 64 ? of(std::integral_constant<int, 64>{}) : of(std::integral_constant<int, 128>{});
@@ -453,7 +532,7 @@ int launch(const Causal& p, float* minus_lse, float* tops, hipStream_t st) {
             if (hipGetLastError() != hipSuccess) return SA2_ERR_LAUNCH_FAILED;
         }
     }
-    return p.dq.p && !together ? launch_causal16_dq(p, E::DTYPE, tops, blocks, st) : SA2_OK;
+    return p.dq.p && !together ? launch_causal16_dq(p, E::DTYPE, terms, st) : SA2_OK;
 }
 
 }  // namespace
@@ -471,8 +550,8 @@ size_t causal16_part_bytes(int B, int N, int HK, int G, int D) {
     return n > 1 ? (size_t)n * 2 * B * HK * N * D * sizeof(float) : 0;
 }
 
-int launch_causal16_bwd(const Causal& p, int dtype, float* minus_lse, float* tops, hipStream_t st) {
-    return dtype == SA2_F16 ? launch<ElemF16>(p, minus_lse, tops, st) : launch<ElemBF16>(p, minus_lse, tops, st);
+int launch_causal16_bwd(const Causal& p, int dtype, const Causal16Terms& terms, hipStream_t st) {
+    return dtype == SA2_F16 ? launch<ElemF16>(p, terms, st) : launch<ElemBF16>(p, terms, st);
 }
 
 }  // namespace sa2

@@ -5,7 +5,7 @@
 // The forward's sweep (sa2_causal_fwd16.hip) with dP beside the logits and dS K in the place of P V: a wavefront owns NQ blocks of 32
 // queries, whose rows of Q and dO and sums of dQ fill the accumulation registers (256 at head_dim 128 and NQ 2).  A piece of keys
 // is read three times from LDS: rows of K, rows of V, columns of K.  dS is rounded to 16 bits before the last product (half a step
-// of each); fp16: with the power of two of sa2_causal_dkv16.hip.
+// of each); fp16: times a power of two of its row's own (sa2_causal16.h).
 // Measured: B1 N8192 H16/4 D128 bf16 356 us with row terms (18), 1220 TFLOP/s of its three products in the kernel's own 338; N16384
 // H8/2 fp16 714, B2 N2048 H8 D64 38.  MFMAs are busy 57 % of the time.
 #pragma once
@@ -17,9 +17,46 @@ namespace {
 
 constexpr int DQ_BUFFERS = 3;
 
+// The factors of the lane's NQ rows, whose workgroup starts at row q0 of the sequence; `lds`: 2 * WAVES floats.  Every thread calls it
+template <int NQ>
+__device__ __forceinline__ void query_factors(const Causal& p, const Causal16Terms& terms, const Span& s, int h, int q0, float (&f)[NQ], float* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = q0 + wave * 32 * NQ;
+    const float* const v = terms.v + ((int64_t)s.b * p.HK + h / p.G) * p.rows.N + s.first;
+    const int64_t stat = ((int64_t)s.b * p.H + h) * p.rows.N + s.first;
+    // keys before the block, eight loads under way; those of the block by themselves
+    float before = 0.f;
+    for (int i = threadIdx.x; i < q0; i += 8 * THREADS)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) before = fmaxf(before, finite_or_zero(v[i + j * THREADS < q0 ? i + j * THREADS : i]));
+    float own[NQ], dout[NQ], delta[NQ], all = 0.f;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int at = mine + 32 * n + (lane & 31);
+        own[n] = at < s.len ? finite_or_zero(v[at]) : 0.f;
+        all = fmaxf(all, own[n]);
+        dout[n] = at < s.len ? terms.dout[stat + at] : 0.f;
+        delta[n] = at < s.len ? p.delta[stat + at] : 0.f;
+    }
+    before = wave_max(before);
+    all = wave_max(all);
+    if (lane == 0) {
+        lds[wave] = before;
+        lds[WAVES + wave] = all;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) before = fmaxf(before, fmaxf(lds[w], w < wave ? lds[WAVES + w] : 0.f));
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const float seen = fmaxf(before, largest_up_to(own[n]));
+        f[n] = gradient_factor(fmaf(dout[n], seen, fabsf(delta[n])));
+        before = __shfl(seen, 31, 32);
+    }
+}
+
 // Workgroup `id`; all of LDS is its own
 template <class E, int D, int NQ>
-__device__ __forceinline__ void queries_gradient16(const Causal& p, const float* tops, int ntops, bool padded, int id, char* lds) {
+__device__ __forceinline__ void queries_gradient16(const Causal& p, const Causal16Terms& terms, bool padded, int id, char* lds) {
     using T = QuadTile<D>;
     using X8 = typename E::x8;
     using L = Lone<(D * NQ > 128 ? 256 : D * NQ > 64 ? 192 : 96)>;
@@ -27,7 +64,6 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const float*
     constexpr int S0 = 0, Q0 = NQ * DT * 16, G0 = Q0 + NQ * KK * 4;        // accumulation registers of dQ, Q and dO
     const uint32_t base = lds_address(lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const float f = E::DTYPE == SA2_F16 ? gradient_factor(tops, ntops, (float*)lds) : 1.f;
     int stream, tile;
     order(id, p.rows.B * p.H, stream, tile);
     const int b = stream / p.H, h = stream % p.H, hk = h / p.G;
@@ -45,7 +81,8 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const float*
     fetch.init(p.k, p.v, s, hk, p.D);
 
     const float c = p.scale * LOG2E;
-    float lse2[NQ], delta[NQ];
+    float lse2[NQ], f[NQ], df[NQ];                                         // f: the rows' factors, df: delta times them
+    if constexpr (E::DTYPE == SA2_F16) query_factors<NQ>(p, terms, s, h, q0, f, (float*)lds);
     static_for<2 * NQ>([&](auto N) __attribute__((always_inline)) {
         constexpr int n = decltype(N)::value / 2, grad = decltype(N)::value % 2;
         const Tensor& t = grad ? p.dout : p.q;
@@ -63,7 +100,7 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const float*
             L::template set_regs<(grad ? G0 : Q0) + (n * KK + kk) * 4>(x[kk].x, x[kk].y, x[kk].z, x[kk].w);
         });
         const int64_t stat = ((int64_t)s.b * p.H + h) * p.rows.N + s.first + at;
-        if (grad) delta[n] = at < s.len ? -p.delta[stat] : 0.f;
+        if (grad) df[n] = at < s.len ? -p.delta[stat] * (E::DTYPE == SA2_F16 ? f[n] : 1.f) : 0.f;
         else lse2[n] = at < s.len ? p.lse[stat] * LOG2E : 0.f;
     });
     static_for<NQ * DT * 4>([&](auto X) __attribute__((always_inline)) { L::template set_regs<S0 + 4 * decltype(X)::value>(0u, 0u, 0u, 0u); });
@@ -128,8 +165,7 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const float*
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int r = 2 * i + j;
-                e[j] = fast_exp2(fmaf(x[r], c, -lse2[n])) * (y[r] - delta[n]);
-                if constexpr (E::DTYPE == SA2_F16) e[j] *= f;
+                e[j] = fast_exp2(fmaf(x[r], c, -lse2[n])) * (E::DTYPE == SA2_F16 ? fmaf(y[r], f[n], -df[n]) : y[r] - df[n]);
                 if constexpr (decltype(masked)::value) e[j] = 8 * (r / 4) + 4 * half + r % 4 <= seen ? e[j] : 0.f;
             }
             o.u[i] = pack2<E>(e[0], e[1]);
@@ -162,8 +198,8 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const float*
             deal<16, i - 1, LAG>([&](auto X) __attribute__((always_inline)) { e[decltype(X)::value] = fmaf(x[decltype(X)::value], c, -lse2[mid]); });
             deal<16, i - 2, LAG>([&](auto X) __attribute__((always_inline)) {
                 e[decltype(X)::value] = fast_exp2(e[decltype(X)::value]);
-                d[decltype(X)::value] = y[decltype(X)::value] - delta[mid];
-                if constexpr (E::DTYPE == SA2_F16) d[decltype(X)::value] *= f;
+                if constexpr (E::DTYPE == SA2_F16) d[decltype(X)::value] = fmaf(y[decltype(X)::value], f[mid], -df[mid]);
+                else d[decltype(X)::value] = y[decltype(X)::value] - df[mid];
             });
             deal<16, i - 3, LAG>([&](auto X) __attribute__((always_inline)) {
                 constexpr int j = decltype(X)::value;
@@ -222,7 +258,7 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const float*
             }
         });
     };
-    if (E::DTYPE == SA2_F16) __syncthreads();                              // (the factor's reduction has left LDS)
+    if (E::DTYPE == SA2_F16) __syncthreads();                              // (the factors have left LDS)
     request(0);
     arrive();
     const bool active = mine < s.len;
@@ -283,10 +319,10 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const float*
         }
     }
     rest();
-    const float to = p.scale / f;
     static_for<NQ>([&](auto N) __attribute__((always_inline)) {
         constexpr int n = decltype(N)::value;
         const int at = mine + 32 * n + (lane & 31);
+        const float to = E::DTYPE == SA2_F16 ? p.scale / f[n] : p.scale;
         if (at < s.len) {
             uint16_t* row = (uint16_t*)p.dq.p + row_offset(p.dq, s, at, h);
             static_for<4 * DT>([&](auto X) __attribute__((always_inline)) {

@@ -36,7 +36,8 @@ int make_causal(Causal& p, const int32_t* cu, int sequences, int B, int N, int H
     p.scale = scale;
     return SA2_OK;
 }
-size_t delta_bytes(const Causal& p) { return ((size_t)p.rows.B * p.H * p.rows.N * sizeof(float) + 255) / 256 * 256; }
+size_t row_bytes(const Causal& p, int heads) { return ((size_t)p.rows.B * heads * p.rows.N * sizeof(float) + 255) / 256 * 256; }
+size_t delta_bytes(const Causal& p) { return row_bytes(p, p.H); }
 
 int check_tree(int B, int T, int H, int HK, int D, int dtype) {
     const int rc = check_rows(B, T, H, D, nullptr, 0, dtype);
@@ -145,7 +146,7 @@ size_t sa2_causal_bwd_workspace_bytes(int B, int N, int H, int HK, int D, int dt
     Causal p;
     if (make_causal(p, nullptr, 0, B, N, H, HK, D, 1.f, dtype) != SA2_OK) return 0;
     if ((flags & SA2_FLAG_FORCE_GENERIC) || !causal16_supported(D, dtype)) return delta_bytes(p);
-    return 2 * delta_bytes(p) + CAUSAL16_TOPS * sizeof(float) + causal16_part_bytes(B, N, HK, p.G, D);
+    return 2 * delta_bytes(p) + (dtype == SA2_F16 ? delta_bytes(p) + row_bytes(p, HK) : 0) + causal16_part_bytes(B, N, HK, p.G, D);
 }
 
 int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* out_low, const void* dout, const float* lse,
@@ -171,10 +172,15 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
     // (-lse / scale is one of the 16-bit kernels' operands)
     if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv}) &&
         fabsf(scale) > 1e-20f && !((uintptr_t)out_low & 15u)) {
-        float* const minus_lse = (float*)((char*)workspace + delta_bytes(p));
-        float* const tops = (float*)((char*)minus_lse + delta_bytes(p));
-        p.part = tops + CAUSAL16_TOPS;
-        return launch_causal16_bwd(p, dtype, minus_lse, tops, st);
+        char* at = (char*)workspace + delta_bytes(p);
+        auto next = [&](size_t bytes) { char* const here = at; at += bytes; return (float*)here; };
+        Causal16Terms terms{next(delta_bytes(p)), nullptr, nullptr};
+        if (dtype == SA2_F16) {
+            terms.dout = next(delta_bytes(p));
+            terms.v = next(row_bytes(p, HK));
+        }
+        p.part = next(0);
+        return launch_causal16_bwd(p, dtype, terms, st);
     }
     return launch_causal_f32_bwd(p, dtype, st);
 }

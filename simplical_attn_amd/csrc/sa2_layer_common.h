@@ -90,12 +90,16 @@ bool causal16_layout(const Causal& p, std::initializer_list<const Tensor*> ts);
 // whether a wavefront owns two blocks of 32 queries (forward, dQ)
 bool causal16_two(const Causal& p);
 int launch_causal16_fwd(const Causal& p, int dtype, hipStream_t st);
-// their backward: p.delta receives -delta, minus_lse [B,H,N] -lse / scale, tops the largest |dout| of up to CAUSAL16_TOPS parts
-constexpr int CAUSAL16_TOPS = 1024;
+// Their backward.  Row terms: p.delta receives -delta; fp16: the Euclidean norms of rows bound dS
+struct Causal16Terms {
+    float* minus_lse;                          // [B,H,N]  -lse / scale
+    float* dout;                               // [B,H,N]  |dout|, fp16 only
+    float* v;                                  // [B,HK,N] |v|, fp16 only
+};
 int causal16_splits(int B, int N, int HK, int G);
 size_t causal16_part_bytes(int B, int N, int HK, int G, int D);
-int launch_causal16_bwd(const Causal& p, int dtype, float* minus_lse, float* tops, hipStream_t st);
-int launch_causal16_dq(const Causal& p, int dtype, const float* tops, int ntops, hipStream_t st);
+int launch_causal16_bwd(const Causal& p, int dtype, const Causal16Terms& terms, hipStream_t st);
+int launch_causal16_dq(const Causal& p, int dtype, const Causal16Terms& terms, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
 // 16-bit kernels: rows that a workgroup has of R; up to 64 its wavefronts share them and divide the keys, beyond it is the other
 // way round (16/4 heads, 4 x 65536 cached rows, head_dim 128, 192 rows: 398 us dividing keys, 161 dividing rows).  From 33 to 64

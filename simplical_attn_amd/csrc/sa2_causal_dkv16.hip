@@ -11,7 +11,8 @@
 // what LDS gives), read three or four MFMAs of its kind ahead.
 // The queries of the G heads that share the keys are one stream, of which `nsplit` workgroups take shares where the key blocks are
 // few or uneven (the first keys are seen by all queries, the last by few); their fp32 sums meet in a last launch, in order.
-// fp16: dS is multiplied by a power of two of its key's own (sa2_causal16.h), which comes off the sum.
+// fp16: dS is multiplied by a power of two of its key's own (sa2_causal16.h), which comes off the sum; so are the weights in dV, by 2^15
+// (they are 1 at most, and in a long or peaked row most are below fp16's smallest normal number): -lse / scale is higher by that.
 // Measured: B1 N8192 H16/4 D128 bf16 512 us with row terms (18) and sums (14), 1145 TFLOP/s of its four products in the kernel's own 480; N16384 H8/2 fp16
 // 1065, B2 N2048 H8 D64 44.  MFMAs are busy 50 % of the time; LDS reads and the exponentials share the rest.
 #include "sa2_causal_dq16.h"
@@ -22,6 +23,8 @@ namespace {
 constexpr int BUFFERS = 4, BLOCK = SUB * WAVES;            // keys per workgroup
 constexpr int STATS = 2 * TILE_ROWS * 4;                    // bytes of the row terms of a tile
 constexpr int TERMS_BLOCKS = 1024;
+template <class E>
+constexpr int LIFT = E::DTYPE == SA2_F16 ? 15 : 0;          // weights in dV are 2^LIFT times as large
 
 // ---- row terms: delta = sum_d dO O, stored as -delta, and -lse / scale ----------------------------------------------
 // O with what its rounding left, where the forward wrote that: from the rounded output alone delta carries half a step of every
@@ -30,7 +33,7 @@ template <class E, int LANES>                               // lanes per row, 16
 __global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, Causal16Terms terms) {
     const int lane = threadIdx.x % LANES, per = THREADS / LANES;
     const int64_t rows = (int64_t)p.rows.B * p.rows.N * p.H;
-    const float over = -1.f / p.scale;
+    const float over = -1.f / p.scale, lift = LIFT<E> / (p.scale * LOG2E);
     int lo = 0, hi = p.rows.N;
     if (p.rows.cu) {
         lo = p.rows.cu[0];
@@ -66,7 +69,7 @@ __global__ __launch_bounds__(THREADS) void causal_terms_kernel(Causal p, Causal1
         if (r < rows && n >= lo && n < hi && lane == 0) {
             const int64_t at = ((int64_t)b * p.H + h) * p.rows.N + n;
             p.delta[at] = -sum;
-            terms.minus_lse[at] = p.lse[at] * over;
+            terms.minus_lse[at] = fmaf(p.lse[at], over, lift);
             if (E::DTYPE == SA2_F16) terms.dout[at] = sqrtf(square);
         }
     }
@@ -191,6 +194,7 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
     const int64_t all = (int64_t)per * p.G;
     const int lo = (int)(all * split / nsplit), hi = (int)(all * (split + 1) / nsplit);
     const float f = E::DTYPE == SA2_F16 ? key_factor(p, terms, s, hk, j0, per, lo, hi, (float*)lds) : 1.f;
+    const float fd = f * (1.f / (1 << LIFT<E>));                           // what takes a lifted weight times dP - delta to dS times f
 
     static_for<2>([&](auto W) __attribute__((always_inline)) {
         const Tensor& t = decltype(W)::value ? p.v : p.k;
@@ -305,7 +309,7 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
             deal<16, i - 3, LAG>([&](auto X) __attribute__((always_inline)) {
                 constexpr int j = decltype(X)::value;
                 float ds = e[j] * y[j];
-                if constexpr (E::DTYPE == SA2_F16) ds *= f;
+                if constexpr (E::DTYPE == SA2_F16) ds *= fd;
                 if constexpr (j % 2) {
                     zp.u[j / 2] = pack2<E>(e[j - 1], e[j]);
                     zd.u[j / 2] = pack2<E>(d0, ds);
@@ -351,7 +355,7 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
             for (int j = 0; j < 2; ++j) {
                 const int r = 2 * i + j, query = q0 + 8 * (r / 4) + 4 * half + r % 4;
                 e[j] = fast_exp2(st[0][r] * c);
-                ds[j] = e[j] * dp[0][r] * f;
+                ds[j] = e[j] * dp[0][r] * fd;
                 if (masked) {
                     if (query < key) e[j] = ds[j] = 0.f;
                     if (query == 0) ds[j] = 0.f;             // a first query has one weight, 1, whose gradient is zero
@@ -442,9 +446,9 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
         static_for<4 * DT>([&](auto X) __attribute__((always_inline)) {
             constexpr int x = decltype(X)::value;
             const int col = 8 * x + 4 * half;
-            const float4 v = L::template get_regs<V0 + 4 * x>();
-            float4 k = L::template get_regs<K0 + 4 * x>();
-            const float to = p.scale / f;
+            float4 v = L::template get_regs<V0 + 4 * x>(), k = L::template get_regs<K0 + 4 * x>();
+            const float to = p.scale / f, off = 1.f / (1 << LIFT<E>);
+            v.x *= off; v.y *= off; v.z *= off; v.w *= off;
             k.x *= to; k.y *= to; k.z *= to; k.w *= to;
             if (col < p.D) {
                 if (nsplit > 1) {

@@ -92,7 +92,7 @@ bool causal16_two(const Causal& p);
 int launch_causal16_fwd(const Causal& p, int dtype, hipStream_t st);
 // Their backward.  Row terms: p.delta receives -delta; fp16: the Euclidean norms of rows bound dS
 struct Causal16Terms {
-    float* minus_lse;                          // [B,H,N]  -lse / scale
+    float* minus_lse;                          // [B,H,N]  -lse / scale; fp16: what weights are lifted by added (sa2_causal_dkv16.hip)
     float* dout;                               // [B,H,N]  |dout|, fp16 only
     float* v;                                  // [B,HK,N] |v|, fp16 only
 };

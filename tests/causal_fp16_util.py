@@ -4,7 +4,7 @@ Beside the roundings that causal_util.py counts (scores r, weights and dS half a
 by up to 2^-25 when it is rounded to fp16.  The kernels multiply what they round by powers of two first:
   out   weights by 2^L, L = log2(n) - 10, rounded up, from 0 to 8, over a reference point no higher than the row's maximum: off by
         2^-(25 + L) of the largest weight
-  dv    weights as they are
+  dv    weights by 2^15: 2^-40
   dq    dS of row i so that a bound of it, b_i = |dO_i| max_j |v_j| + |delta_i| over the keys that it sees, becomes 2^13 to 2^14: 2^-38 b_i
   dk    dS of key j the same with b_j = max_i |dO_i| |v_j| + max_i |delta_i| over the rows that see it, of all heads: 2^-38 b_j
 (|.| of rows: Euclidean norms.)  dS in two parts is off by less than dS in one."""
@@ -54,7 +54,7 @@ def exact(q, k, v, dout, scale):
         dk += scale * (dS.T @ Q[:, g])
         bk += abs(scale) * (b.T @ Q[:, g].abs() + (n * G + 16) * E * (dS.abs().T @ Q[:, g].abs()))
         dv += P.T @ dO[:, g]
-        bv += ((rel_P + T) * P + 2.0 ** -25 * mask).T @ dO[:, g].abs() + (n * G + 16) * E * (P.T @ dO[:, g].abs())
+        bv += ((rel_P + T) * P + 2.0 ** -40 * mask).T @ dO[:, g].abs() + (n * G + 16) * E * (P.T @ dO[:, g].abs())
     both = {name: tuple(torch.stack(x, 1) for x in zip(*pairs)) for name, pairs in res.items()}
     both["dk"] = (dk, bk + T * (dk.abs() + bk) + TINY)
     both["dv"] = (dv, bv + T * (dv.abs() + bv) + TINY)

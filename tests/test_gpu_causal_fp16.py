@@ -1,5 +1,5 @@
 """Causal attention in fp16 where its narrow range shows: values far from 1, rows and sequences whose gradients differ by many powers of
-two.  Bounds: causal_fp16_util.py."""
+two, weights far below a row's largest.  Bounds: causal_fp16_util.py."""
 import math
 
 import pytest
@@ -108,3 +108,28 @@ def test_rows_behind_an_infinity(bad):
         hs = slice(2 * hk, 2 * hk + 2)
         value, bound = exact(q[:, hs], k[:, hk], v[:, hk], dout[:, hs], 0.125)["dq"]
         assert ((dq[:270, hs].double() - value[:270]).abs() <= bound[:270]).all()
+
+
+@pytest.mark.parametrize("N,H,HK,D", [(4096, 1, 1, 64), (2000, 2, 1, 128), (3000, 48, 6, 64)])
+def test_values_of_small_weights(N, H, HK, D):
+    """Peaked scores: weights far below fp16's smallest normal number add up in dV."""
+    q, k, v, dout = _half(*_inputs(N, H, HK, D, 21, std=1.5))
+    got = _train(q, k, v, dout, torch.tensor([0, N], dtype=torch.int32, device=DEV))
+    if HK > 1:
+        G = H // HK
+        q, dout, got = q[:, -G:], dout[:, -G:], (got[0][:, -G:], got[1][:, -G:], got[2][:, -1:], got[3][:, -1:])
+        k, v = k[:, -1:], v[:, -1:]
+    _compare(q, k, v, dout, got, [0, N])
+
+
+@pytest.mark.parametrize("N,D,H", [(4096, 64, 2), (2500, 128, 3)])
+def test_values_of_vanishing_weights(N, D, H):
+    """A key whose weights are all below 2^-25 has a gradient of its value all the same."""
+    g = torch.Generator().manual_seed(D)
+    q = torch.zeros(N, H, D, dtype=FP16, device=DEV)
+    k = torch.zeros(N, 1, D, dtype=FP16, device=DEV)
+    q[..., 0], k[40::60, :, 0] = 1, -11
+    v, dout = (torch.randn(N, h, D, generator=g).to(DEV).half() for h in (1, H))
+    dout = 32 * (dout.abs() + 1)
+    got = _train(q, k, v, dout, torch.tensor([0, N], dtype=torch.int32, device=DEV), 1.0)
+    _compare(q, k, v, dout, got, [0, N], names=("dv",), scale=1.0)

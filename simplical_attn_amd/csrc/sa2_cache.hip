@@ -25,7 +25,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(Append p, int size, int
         n = a;
         b = sequence_of(p.rows, n);
         if (b < 0) return;
-        a = n - p.rows.cu[b];
+        a = place_of(p.rows, b, n);
         sb = 0;
     } else if (p.chosen) {
         n = p.chosen[item];

@@ -155,6 +155,11 @@ __device__ __forceinline__ int sequence_of(const Rows& r, int n) {
     }
     return lo;
 }
+// The place of packed row n in that sequence (a first bound below zero, down to the smallest int, is zero)
+__device__ __forceinline__ int place_of(const Rows& r, int sequence, int n) {
+    const int first = r.cu[sequence];
+    return first < 0 ? n : n - first;
+}
 
 // All pointers and strides that a kernel's 16-byte accesses need
 inline bool aligned16(const Tensor& t, int64_t size, bool batched) {

@@ -59,7 +59,7 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(Rotary p, Split sp) {
             if (p.positions) pos = p.position_bytes == 8 ? (double)((const int64_t*)p.positions)[row] : (double)((const int32_t*)p.positions)[row];
             else if (p.rows.cu) {
                 const int sq = sequence_of(p.rows, n);
-                pos = sq < 0 ? 0.0 : (double)(n - p.rows.cu[sq]);
+                pos = sq < 0 ? 0.0 : (double)place_of(p.rows, sq, n);
             } else pos = (double)n;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {

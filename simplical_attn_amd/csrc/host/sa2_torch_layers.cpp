@@ -1,6 +1,7 @@
 // Host path of the operators of ordinary attention layers (rotary positions, causal attention over prompts, rows of a
 // cache, drafted trees): checks, outputs, workspaces, the calls of the C ABI and the autograd formulas.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -48,10 +49,20 @@ void check_cu(const Maybe& cu, const Tensor& q) {
     check_ints(cu, "cu_seqlens", q, 1);
     TORCH_CHECK_VALUE(!cu || (q.dim() == 3 && cu->numel() >= 2), "cu_seqlens needs packed [rows, heads, head_dim] tensors and at least two entries");
 }
+// While the operators work.  They are no dispatcher operators: a dispatch mode of the user (FLOP counting, selective checkpointing) sees
+// nothing of them, neither a call nor what is allocated inside.  Modes that record or fake operators would miss the kernels: refused.
+struct Unseen {
+    explicit Unseen(const char* op) : guard(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot})) {
+        using Key = c10::impl::TorchDispatchModeKey;
+        for (const Key key : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL})
+            TORCH_CHECK(!c10::impl::TorchDispatchModeTLS::get_mode(key), op, " cannot run under fake tensors, make_fx or functionalization: no dispatcher operator stands for it");
+    }
+    c10::impl::ExcludeDispatchKeyGuard guard;
+};
 void check_place(const char* op, std::initializer_list<Tensor> ts) {
     for (const Tensor& t : ts) {
         TORCH_CHECK(t.is_cuda(), op, " runs on the GPU only; got a ", t.device(), " tensor");
-        TORCH_CHECK(plain(t), op, " takes plain tensors: no forward-mode derivatives, torch.func transforms or tensor subclasses");
+        TORCH_CHECK(!t._fw_grad(0).defined() && (t.key_set() & at::kTensorSubclassLike).empty(), op, " takes plain tensors: no forward-mode derivatives, torch.func transforms or tensor subclasses");
     }
     TORCH_CHECK(!torch::jit::tracer::isTracing(), op, " cannot be recorded by torch.jit.trace");
 }
@@ -91,6 +102,7 @@ struct Angles {
 };
 
 std::pair<Tensor, Tensor> run_rotary(const Tensor& q_, const Tensor& k_, const Angles& a) {
+    const Unseen unseen("rotary_embedding");
     const Tensor q = rows(q_), k = k_.defined() ? rows(k_) : Tensor();
     const c10::DeviceGuard guard(q.device());
     Tensor q2 = like(q), k2 = k.defined() ? like(k) : Tensor();
@@ -214,6 +226,7 @@ void append(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Ten
     check_place("cache_append", {k_, v_, k_cache, v_cache});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
+    const Unseen unseen("cache_append");
     Tensor k = rows(k_), v = rows(v_);
     const Tensor pick = dense(chosen), ends = dense(cu);
     const c10::DeviceGuard guard(k.device());
@@ -243,6 +256,7 @@ Tensor workspace(const Tensor& q, size_t bytes) { return at::empty({(int64_t)byt
 
 // `low`: receives what rounding the output left, for a backward (16-bit types)
 std::pair<Tensor, Tensor> run_causal_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Prompt& a, Tensor* low = nullptr) {
+    const Unseen unseen("causal_attention");
     const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
     const c10::DeviceGuard guard(q.device());
     const Sizes z = sizes(q);
@@ -263,6 +277,7 @@ std::pair<Tensor, Tensor> run_causal_forward(const Tensor& q_, const Tensor& k_,
 // `needs`: bit t set = gradient t of (q, k, v) is wanted; the others stay undefined
 std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& out_, const Tensor& low, const Tensor& lse, const Tensor& dout_, unsigned needs,
                                            const Prompt& a) {
+    const Unseen unseen("causal_attention");
     const Tensor q = rows(q_), k = rows(k_), v = rows(v_), out = rows(out_), dout = rows(dout_);
     const c10::DeviceGuard guard(q.device());
     const Sizes z = sizes(q);
@@ -372,6 +387,7 @@ Tensor tree(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Maybe& p
     check_place("tree_attention", {q_, k_, v_, k_cache, v_cache});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
+    const Unseen unseen("tree_attention");
     const Tensor q = rows(q_), k = rows(k_), v = rows(v_), up = dense(parents);
     const c10::DeviceGuard guard(q.device());
     Tensor out = like(q);

@@ -84,18 +84,19 @@ def cache_append(k, v, k_cache, v_cache, lengths, page_table=None, rows=None, cu
     _lib.host().cache_append(k, v, k_cache, v_cache, lengths, page_table, rows, cu_seqlens)
 
 
-def causal_attention(q, k, v, cu_seqlens=None, scale=None):
+def causal_attention(q, k, v, cu_seqlens=None, scale=None, flags=_lib.FLAG_AUTO):
     """softmax(scale q k^T) v, query i of a sequence over its keys 0 .. i; differentiable in q, k and v (once: create_graph=True
     is refused).
 
     q        [batch, seq_len, heads, head_dim], or packed [rows, heads, head_dim] with cu_seqlens; head_dim up to 256
     k, v     as q, with heads that divide q's: query head h reads head h // (heads / key heads)
     scale    1 / sqrt(head_dim) if None
+    flags    _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products whatever the type, gradients too
 
     Returns a tensor like q, zero in rows of no sequence.  bf16 and fp16 with a head_dim up to 128 that is a multiple of 8 and rows on
     the 16-byte grid run on the 16-bit matrix pipes (softmax weights rounded to the type, sums in fp32), everything else
     with fp32 products."""
-    return _lib.host().causal(q, k, v, cu_seqlens, scale, _lib.FLAG_AUTO)
+    return _lib.host().causal(q, k, v, cu_seqlens, scale, int(flags))
 
 
 def causal_attention_forward(q, k, v, cu_seqlens=None, scale=None, flags=_lib.FLAG_AUTO):
@@ -114,7 +115,7 @@ def causal_attention_backward(q, k, v, out, lse, dout, cu_seqlens=None, scale=No
     return _lib.host().causal_backward(q, k, v, out, lse, dout, cu_seqlens, scale, mask, int(flags))
 
 
-def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None, scale=None):
+def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None, scale=None, flags=_lib.FLAG_AUTO):
     """Attention of drafted tokens over a cache: node i of a sequence attends to the ``lengths`` rows that the cache holds, to
     itself and to its ancestors in the draft.  One node is a decoding step.
 
@@ -125,6 +126,8 @@ def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None,
                       None: a chain, each node behind the one before it
     k_cache, v_cache, lengths, page_table   as at cache_append, which brings the accepted nodes into the cache
     scale             1 / sqrt(head_dim) if None
+    flags             _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products whatever the type
 
-    No gradients.  Returns a tensor like q."""
-    return _lib.host().tree(q, k, v, parents, k_cache, v_cache, lengths, page_table, scale, _lib.FLAG_AUTO)
+    No gradients.  Returns a tensor like q.  bf16 and fp16 with a head_dim up to 128 that is a multiple of 8 and rows on the 16-byte
+    grid run on the 16-bit matrix pipes (softmax weights rounded to the type, sums in fp32), everything else with fp32 products."""
+    return _lib.host().tree(q, k, v, parents, k_cache, v_cache, lengths, page_table, scale, int(flags))

@@ -262,8 +262,8 @@ std::pair<Tensor, Tensor> run_causal_forward(const Tensor& q_, const Tensor& k_,
     const Sizes z = sizes(q);
     const auto fp32 = q.options().dtype(at::kFloat).requires_grad(false);
     Tensor out = like(q), lse = q.dim() == 4 ? at::empty({z.B, z.H, z.N}, fp32) : at::empty({z.H, z.N}, fp32);
-    if (out.numel() == 0) return {out, lse};
     if (low && dtype_code(q) != SA2_F32) *low = like(q);
+    if (out.numel() == 0) return {out, lse};
     int64_t s[12];
     put_strides(s, q);
     put_strides(s + 3, k);
@@ -275,10 +275,12 @@ std::pair<Tensor, Tensor> run_causal_forward(const Tensor& q_, const Tensor& k_,
 }
 
 // `needs`: bit t set = gradient t of (q, k, v) is wanted; the others stay undefined
-std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& out_, const Tensor& low, const Tensor& lse, const Tensor& dout_, unsigned needs,
+std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& out_, const Tensor& low_, const Tensor& lse, const Tensor& dout_, unsigned needs,
                                            const Prompt& a) {
     const Unseen unseen("causal_attention");
-    const Tensor q = rows(q_), k = rows(k_), v = rows(v_), out = rows(out_), dout = rows(dout_);
+    const Tensor q = rows(q_), k = rows(k_), v = rows(v_), dout = rows(dout_);
+    const bool alike = !low_.defined() || low_.strides() == out_.strides();       // (the ABI has the strides of one for both)
+    const Tensor out = alike ? rows(out_) : out_.contiguous(), low = !low_.defined() ? low_ : alike ? rows(low_) : low_.contiguous();
     const c10::DeviceGuard guard(q.device());
     const Sizes z = sizes(q);
     const int hk = (int)k.size(-2);
@@ -345,15 +347,19 @@ Tensor causal(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu
     return run_causal_forward(q, k, v, a).first;
 }
 
-std::pair<Tensor, Tensor> causal_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, std::optional<double> scale, unsigned flags) {
+std::tuple<Tensor, Tensor, Maybe> causal_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, std::optional<double> scale, unsigned flags, bool keep_low) {
     const Prompt a = check_causal(q, k, v, cu, scale, flags);
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
-    return run_causal_forward(q, k, v, a);
+    Tensor low;
+    auto [out, lse] = run_causal_forward(q, k, v, a, keep_low ? &low : nullptr);
+    return {out, lse, low.defined() ? Maybe(low) : Maybe()};
 }
 
 std::tuple<Maybe, Maybe, Maybe> causal_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse, const Tensor& dout, const Maybe& cu,
-                                                std::optional<double> scale, unsigned needs, unsigned flags) {
+                                                std::optional<double> scale, unsigned needs, unsigned flags, const Maybe& low) {
+    TORCH_CHECK_VALUE(!low || dtype_code(q) != SA2_F32, "out_low goes with 16-bit tensors");
+    if (low) TORCH_CHECK_VALUE(low->sizes() == q.sizes() && low->scalar_type() == q.scalar_type() && low->device() == q.device(), "out_low must match q in shape, dtype and device");
     const Prompt a = check_causal(q, k, v, cu, scale, flags);
     for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(out, "out"), {dout, "dout"}})
         TORCH_CHECK_VALUE(t.sizes() == q.sizes() && t.scalar_type() == q.scalar_type() && t.device() == q.device(), name, " must match q in shape, dtype and device");
@@ -361,9 +367,10 @@ std::tuple<Maybe, Maybe, Maybe> causal_backward(const Tensor& q, const Tensor& k
     TORCH_CHECK_VALUE(lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.is_contiguous() && lse.dim() == q.dim() - 1 && lse.size(-1) == q.size(-3) && lse.size(-2) == q.size(-2) &&
                           (!batched || lse.size(0) == q.size(0)), "lse must be the contiguous float32 tensor that the forward returned, got ", lse.scalar_type(), " ", lse.sizes());
     check_place("causal_attention", {out, lse, dout});
+    if (low) check_place("causal_attention", {*low});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
-    auto g = run_causal_backward(q, k, v, out, Tensor(), lse, dout, needs, a);
+    auto g = run_causal_backward(q, k, v, out, low ? *low : Tensor(), lse, dout, needs, a);
     auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
     return {maybe(g[0]), maybe(g[1]), maybe(g[2])};
 }

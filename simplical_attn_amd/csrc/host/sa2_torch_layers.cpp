@@ -1,6 +1,7 @@
 // Host path of the operators of ordinary attention layers (rotary positions, causal attention over prompts, rows of a
 // cache, drafted trees): checks, outputs, workspaces, the calls of the C ABI and the autograd formulas.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -223,6 +224,7 @@ void append(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Ten
     const CacheView c = check_cache(k_cache, v_cache, lengths, table, k_, sequences);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (k_.requires_grad() || v_.requires_grad() || k_cache.requires_grad() || v_cache.requires_grad())),
                 "cache_append has no gradient: call it under torch.no_grad() or on detached tensors");
+    TORCH_CHECK(c10::InferenceMode::is_enabled() || !(k_cache.is_inference() || v_cache.is_inference()), "cache_append changes the cache in place, which inference tensors allow in inference mode only");
     check_place("cache_append", {k_, v_, k_cache, v_cache});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;

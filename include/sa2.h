@@ -210,7 +210,7 @@ int sa2_rotary(const void* q, const void* k, void* q_out, void* k_out, const dou
  *               that goes to lengths[b] + a; elements outside 0 .. N-1 are left out
  *   strides     k, v, k_cache, v_cache (batch or page, row, head; HOST)
  * A row is left out where its place lies beyond the table, or its page is not in 0 .. pages-1.  Places that two rows
- * of one call share (a page listed twice) hold either.
+ * of one call share (a page listed twice) hold either or a mixture of both: rows are moved in pieces of up to 16 bytes.
  */
 int sa2_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* lengths,
                      const int32_t* page_table, const int32_t* rows, int nrows,

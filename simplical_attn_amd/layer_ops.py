@@ -80,7 +80,7 @@ def cache_append(k, v, k_cache, v_cache, lengths, page_table=None, rows=None, cu
 
     Rows whose place lies beyond the capacity, or whose page is not one of the cache's, are left out.  k and v may be views
     of the cache itself: all rows are read before one is written.  Two rows of one call with the same place (a page that the
-    table names twice) leave either."""
+    table names twice) leave either or a mixture of both there: rows are moved in pieces."""
     _lib.host().cache_append(k, v, k_cache, v_cache, lengths, page_table, rows, cu_seqlens)
 
 

@@ -57,7 +57,7 @@ __device__ __forceinline__ void fill_rows(const Tensor& t, const Span& s, int h,
 }
 
 template <class T, int DP, bool WIDE>
-__global__ __launch_bounds__(THREADS) void causal_f32_fwd_kernel(Causal p, int tiles) {
+__global__ __launch_bounds__(THREADS) void causal_f32_fwd_kernel(Causal p) {
     constexpr bool wide = WIDE;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float *kt = lds, *vt = lds + TILE * Pitch<DP>::value;
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(THREADS) void causal_f32_delta_kernel(Causal p) {
 
 // dQ: the wavefront owns 32 queries and sweeps the keys they see
 template <class T, int DP, bool WIDE>
-__global__ __launch_bounds__(THREADS) void causal_f32_dq_kernel(Causal p, int tiles) {
+__global__ __launch_bounds__(THREADS) void causal_f32_dq_kernel(Causal p) {
     constexpr bool wide = WIDE;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float *kt = lds, *vt = lds + TILE * Pitch<DP>::value;
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(THREADS) void causal_f32_dq_kernel(Causal p, int ti
 // dK and dV: the wavefront owns 32 keys and sweeps the queries of all G heads that see them.  Columns `first` .. + DO of the
 // gradients: at head_dim 256 two workgroups share them, each with all of the two first products (the registers hold no more).
 template <class T, int DP, int DO, bool WIDE>
-__global__ __launch_bounds__(THREADS) void causal_f32_dkv_kernel(Causal p, int tiles) {
+__global__ __launch_bounds__(THREADS) void causal_f32_dkv_kernel(Causal p) {
     constexpr bool wide = WIDE;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float *qt = lds, *dt = lds + TILE * Pitch<DP>::value, *stats = dt + TILE * Pitch<DP>::value;     // lse * log2(e), delta
@@ -308,7 +308,7 @@ int launch(K kernel, const Causal& p, int64_t streams, int floats, hipStream_t s
     const int64_t tiles = count_tiles(p.rows, BLOCK);
     if (streams * tiles > 0x7fffffff) return SA2_ERR_TOO_LARGE;
     if (!allow_full_lds((const void*)kernel)) return SA2_ERR_LAUNCH_FAILED;
-    kernel<<<dim3((unsigned)(streams * tiles)), dim3(THREADS), floats * sizeof(float), st>>>(p, (int)tiles);
+    kernel<<<dim3((unsigned)(streams * tiles)), dim3(THREADS), floats * sizeof(float), st>>>(p);
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 

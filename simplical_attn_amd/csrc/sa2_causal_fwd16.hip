@@ -16,7 +16,7 @@ template <int D>
 struct CausalKeys {
     Fetch<D> fetch;
     bool padded, active;
-    int last, mine, rows, tiles, full, pieces;
+    int last, mine, tiles, full, pieces;
     float lower;
     __device__ __forceinline__ void request(int t, uint32_t buffer) const { fetch.request(t * TILE_ROWS, last, buffer, padded); }
     __device__ __forceinline__ bool guarded(int piece) const { return piece * SUB + SUB - 1 > mine; }
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(THREADS, D == 64 ? 2 : 1) void causal_fwd16_kernel(
         });
     });
     float m[NQ], l[NQ];
-    CausalKeys<D> keys{fetch, padded, mine < s.len, last, mine, ROWS, tiles, 0, 0, lowered_by<E>(last, c)};
+    CausalKeys<D> keys{fetch, padded, mine < s.len, last, mine, tiles, 0, 0, lowered_by<E>(last, c)};
     keys.full = keys.active ? mine / TILE_ROWS : 0;
     keys.pieces = keys.active ? (mine + ROWS) / SUB : 0;
     sweep16<E, D, NQ>(keys, base, c, m, l);

@@ -218,7 +218,7 @@ int sa2_tree_attention(const void* q, const void* k, const void* v, const void* 
     if (p.nsplit > 1 && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < tree_part_bytes(B, T, H, D, p.nsplit)))
         return SA2_ERR_WORKSPACE_TOO_SMALL;
     const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && tree16_supported(p, dtype);
-    p.dealt = B > 1 && p.nsplit >= 8 && (!narrow || tree16_rows(p) > 64);      // (sa2_tree16.hip takes equal shares)
+    p.dealt = B > 1 && p.nsplit >= 8 && (!narrow || tree16_rows(p) > 64);      // (sa2_tree16.hip takes equal shares; 32 sequences at most)
     if (narrow) return launch_tree16(p, dtype, (hipStream_t)hip_stream);
     return launch_tree_f32(p, dtype, (hipStream_t)hip_stream);
 }

@@ -58,38 +58,31 @@ __device__ __forceinline__ bool tree_place(const Cache& c, int b, int r, int& pa
 struct TreeShare {
     int b, split, count, first;                            // sequence, which of its shares, how many it has, the first one's unit
 };
+// A lane counts for one sequence: with eight shares each there are 32 at most (tree_splits).
 template <class F>
 __device__ __forceinline__ bool tree_deal(const Tree& p, F&& is, TreeShare& s) {
     const int lane = threadIdx.x & 63;
-    auto keys = [&](int i) { return i < p.B ? (double)tree_held(p, i) + p.T : 0.0; };
-    double total = 0.0;
-    for (int c = 0; c < p.B; c += 64) total += keys(c + lane);
+    const double keys = lane < p.B ? (double)tree_held(p, lane) + p.T : 0.0;
+    double total = keys;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
     // (a little less than its part, so that rounding never deals more units than there are)
     const double each = (double)(p.nsplit - 1) * p.B / total * (1.0 - 1e-9);
-    int before = 0;
-    for (int c = 0; c < p.B; c += 64) {
-        int mine = 1 + (int)(keys(c + lane) * each);
-        mine = c + lane >= p.B ? 0 : mine < 64 ? mine : 64;
-        int sum = mine;
+    int mine = 1 + (int)(keys * each);
+    mine = lane >= p.B ? 0 : mine < 64 ? mine : 64;
+    int sum = mine;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(sum, o);
-            if (lane >= o) sum += up;
-        }
-        const uint64_t hit = __ballot(mine > 0 && is(c + lane, before + sum - mine, before + sum));
-        if (hit) {
-            const int l = __ffsll((unsigned long long)hit) - 1;
-            s.b = c + l;
-            s.count = __builtin_amdgcn_readfirstlane(__shfl(mine, l));
-            s.first = before + __builtin_amdgcn_readfirstlane(__shfl(sum - mine, l));
-            s.split = 0;
-            return true;
-        }
-        before += __builtin_amdgcn_readfirstlane(__shfl(sum, 63));
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(sum, o);
+        if (lane >= o) sum += up;
     }
-    return false;
+    const uint64_t hit = __ballot(mine > 0 && is(lane, sum - mine, sum));
+    if (!hit) return false;
+    s.b = __ffsll((unsigned long long)hit) - 1;
+    s.count = __builtin_amdgcn_readfirstlane(__shfl(mine, s.b));
+    s.first = __builtin_amdgcn_readfirstlane(__shfl(sum - mine, s.b));
+    s.split = 0;
+    return true;
 }
 // The share that a unit is; false: none
 __device__ __forceinline__ bool tree_share(const Tree& p, int unit, TreeShare& s) {

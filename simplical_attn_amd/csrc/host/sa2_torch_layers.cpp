@@ -110,6 +110,7 @@ std::pair<Tensor, Tensor> run_rotary(const Tensor& q_, const Tensor& k_, const A
     const Sizes z = sizes(q);
     const int hk = k.defined() ? sizes(k).H : 0;
     if (z.B == 0 || z.N == 0 || z.D == 0 || (z.H == 0 && hk == 0)) return {q2, k2};
+    if (z.H == 0) return {q2, run_rotary(k, Tensor(), a).first};
     int64_t s[12] = {};
     put_strides(s, q);
     put_strides(s + 6, q2);

@@ -45,7 +45,7 @@ typedef enum sa2_status {
                                       SA2_STATIC_WORKSPACE_BYTES, or the array's address is unavailable */
     SA2_ERR_BAD_HEADS = -11,     /* query heads are not a multiple of the heads of keys and values */
     SA2_ERR_BAD_ROTARY = -12,    /* rotary_dim is odd, < 2 or > D, or positions are neither 4 nor 8 bytes */
-    SA2_ERR_BAD_CACHE = -13,     /* page size, page count or table width < 1 */
+    SA2_ERR_BAD_CACHE = -13,     /* page size, page count or table width < 1, or (trees) page size times width >= 2^31 - 64 */
     SA2_ERR_BAD_TREE = -14       /* a tree of fewer than 1 or more than SA2_TREE_NODES nodes */
 } sa2_status;
 
@@ -250,6 +250,7 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
  *   parents      [B,T] int32 (DEVICE): the node before it, smaller than its own number, or -1 on the cached rows.  A node
  *                whose chain does not end at -1 (-2 marks a place that is not used) attends to nothing: its output is 0.
  *                NULL: a chain, node i behind node i-1.
+ *   capacity     page_size * table_width < 2^31 - 64 rows; without a page table table_width is 1
  *   lengths      clamped to 0 .. capacity; rows in pages that are not in 0 .. pages-1 are not there
  *   workspace    sa2_tree_workspace_bytes(...) bytes, 256-byte aligned (0 bytes: may be NULL); contents on entry ignored
  *   strides      q, k, v, k_cache, v_cache, out

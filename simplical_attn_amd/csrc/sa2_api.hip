@@ -237,7 +237,8 @@ const char* sa2_strerror(int status) {
                                               "the address of that array could not be obtained on this device";
         case SA2_ERR_BAD_HEADS: return "the number of query heads must be a multiple of the number of key heads";
         case SA2_ERR_BAD_ROTARY: return "rotary_dim must be even and in 2 .. D, positions int32 or int64";
-        case SA2_ERR_BAD_CACHE: return "a cache needs a page size, a page count and a table width of at least 1";
+        case SA2_ERR_BAD_CACHE: return "a cache needs a page size, a page count and a table width of at least 1, and for tree attention "
+                                       "page size times table width below 2^31 - 64";
         case SA2_ERR_BAD_TREE: return "a drafted tree must have 1 to 64 nodes";
     }
     return "unknown sa2 status";

@@ -24,15 +24,15 @@ constexpr int BUFFERS = 3;
 
 template <class E> struct RefLimit;
 template <> struct RefLimit<ElemBF16> { static constexpr float value = 1.152921504606847e18f; };   // 2^60
-template <> struct RefLimit<ElemF16> { static constexpr float value = 32768.f; };                  // below 65504
+template <> struct RefLimit<ElemF16> { static constexpr float value = 65504.f; };                  // (no weight of a unit is above its sum)
 // Many keys far below the first ones add up, and in fp16 all weights under 2^-25 would be lost.  Of `keys` keys rounding takes less than
-// 2^-15 of the largest weight where weights are 2^lift times as large, that is, the reference point lift / c lower (c: |scale| log2(e)).
-// More would leave less room for scores above the first keys' (lift 4 at 16384 keys: e^7.6; with 6, scores of standard deviation 2 would
-// take half of the workgroups through a second sweep).
+// 2^-11 of the largest weight, as the result's own rounding does, where weights are 2^lift times as large, that is, the reference point
+// lift / c lower (c: |scale| log2(e)).  More would leave less room for scores above the first keys': with a lift of 3 at 8192 keys scores
+// of standard deviation 2 send most workgroups through a second sweep (B1 N8192 H16/4 D128 270 -> 880 us; as it is those of 3 do, 960).
 template <class E>
 __device__ __forceinline__ float lowered_by(int keys, float c) {
-    if (E::DTYPE != SA2_F16 || keys <= 1024) return 0.f;
-    const int lift = 32 - __clz(keys - 1) - 10;
+    if (E::DTYPE != SA2_F16 || keys <= 16384) return 0.f;
+    const int lift = 32 - __clz(keys - 1) - 14;
     const float by = c > 1e-20f ? (float)(lift < 8 ? lift : 8) / c : 0.f;
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(by)));       // (the same in all lanes)
 }

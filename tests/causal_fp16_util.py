@@ -2,7 +2,7 @@
 
 Beside the roundings that causal_util.py counts (scores r, weights and dS half a step w, sums (n + 16) e), a number below 2^-14 is off
 by up to 2^-25 when it is rounded to fp16.  The kernels multiply what they round by powers of two first:
-  out   weights by 2^L, L = log2(n) - 10, rounded up, from 0 to 8, over a reference point no higher than the row's maximum: off by
+  out   weights by 2^L, L = log2(n) - 14, rounded up, from 0 to 8, over a reference point no higher than the row's maximum: off by
         2^-(25 + L) of the largest weight
   dv    weights by 2^15: 2^-40
   dq    dS of row i so that a bound of it, b_i = |dO_i| max_j |v_j| + |delta_i| over the keys that it sees, becomes 2^13 to 2^14: 2^-38 b_i
@@ -23,7 +23,7 @@ def exact(q, k, v, dout, scale):
     mask = torch.ones(n, n, dtype=torch.bool, device=q.device).tril()
     norm_v = V.norm(dim=-1)
     seen_v = norm_v.cummax(0).values
-    low_out = 2.0 ** (-25 - ((torch.arange(n, device=q.device) + 1.0).log2().ceil() - 10).clamp(0, 8)).double()[:, None]
+    low_out = 2.0 ** (-25 - ((torch.arange(n, device=q.device) + 1.0).log2().ceil() - 14).clamp(0, 8)).double()[:, None]
     res = {"out": [], "dq": []}
     rows, dk, dv, bk, bv = [], torch.zeros_like(K), torch.zeros_like(V), torch.zeros_like(K), torch.zeros_like(V)
     for g in range(G):

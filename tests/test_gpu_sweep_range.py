@@ -32,9 +32,9 @@ def _check(out, q, k, v, rows, scale, seen=None):
     P = torch.softmax(S, 1)
     r = ((D + 4) * E * scale * (Q.abs() @ K.abs().nan_to_num(posinf=0).T)).masked_fill(~M, 0).amax(1, keepdim=True)
     want = P @ V
-    # fp16: of the keys up to the row's own at most 2^-25 each, less by the power of two that their number brings (2^10: 1, up to 2^8)
+    # fp16: of the keys up to the row's own at most 2^-25 each, less by the power of two that their number brings (2^15: 1, up to 2^8)
     keys = M.sum(1, keepdim=True).double().clamp(min=1)
-    low = 2.0 ** (-25 - (keys.log2().ceil() - 10).clamp(0, 8)) if out.dtype == FP16 else 0.0
+    low = 2.0 ** (-25 - (keys.log2().ceil() - 14).clamp(0, 8)) if out.dtype == FP16 else 0.0
     bound = (P @ V.abs()) * (2 * r + t + (n + 16) * E) + low * (M.double() @ V.abs()) + t * want.abs() + 2.0 ** -24
     x = out[rows].double()
     assert torch.isfinite(x).all()

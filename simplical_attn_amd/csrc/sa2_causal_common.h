@@ -18,7 +18,8 @@ inline int64_t count_tiles(const Rows& r, int rows) {
 }
 // The `tile`-th one; false: none.  Packed sequences are counted by every wavefront for itself, 64 at a time: a prefix sum of
 // their tiles, no launch and no table before the kernel (about 1 us where 64 lanes hold all sequences).  Rows that no
-// sequence holds come last.
+// sequence holds come last.  Tiles are numbered sequence by sequence: callers put the longest of a sequence first, but a long
+// sequence behind others starts late.
 __device__ __forceinline__ bool find_tile(const Rows& r, int b, int tile, int rows, Span& s) {
     if (!r.cu) {
         s = Span{b, 0, r.N, tile, false};
@@ -64,8 +65,8 @@ __device__ __forceinline__ bool find_tile(const Rows& r, int b, int tile, int ro
     s.len = hi - s.first < rows ? hi - s.first : rows;
     return s.len > 0;
 }
-// Workgroup pid of streams * tiles: a stream is a (batch entry, head) pair.  Tiles run in the outer order, so that the longest
-// ones, which callers put first, start first; with a multiple of eight streams every XCD keeps its own (its L2 their keys).
+// Workgroup pid of streams * tiles: a stream is a (batch entry, head) pair.  Tiles run in the outer order, so that in a batch the longest
+// ones, which callers put first, start first (packed: each sequence's, one sequence after the other); with a multiple of eight streams every XCD keeps its own (its L2 their keys).
 __device__ __forceinline__ void order(int pid, int streams, int& stream, int& tile) {
     if (streams % 8 == 0) {
         const int each = streams / 8, i = pid >> 3;

@@ -13,8 +13,9 @@
 // few or uneven (the first keys are seen by all queries, the last by few); their fp32 sums meet in a last launch, in order.
 // fp16: dS is multiplied by a power of two of its key's own (sa2_causal16.h), which comes off the sum; so are the weights in dV, by 2^15
 // (they are 1 at most, and in a long or peaked row most are below fp16's smallest normal number): -lse / scale is higher by that.
-// Measured: B1 N8192 H16/4 D128 bf16 512 us with row terms (18) and sums (14), 1145 TFLOP/s of its four products in the kernel's own 480; N16384 H8/2 fp16
-// 1065, B2 N2048 H8 D64 44.  MFMAs are busy 50 % of the time; LDS reads and the exponentials share the rest.
+// Measured: B1 N8192 H16/4 D128 bf16 495 us (1110 TFLOP/s of its four products, MFMAs busy 52 % of the time at 2.0 GHz; LDS reads and the
+// exponentials share the rest), row terms 20, sums 14; all gradients of B2 N2048 H8 D64 57, of which one launch for dQ, dK and dV 44; fp16 N16384
+// H8/2, all gradients 1760 (bf16 1580).
 #include "sa2_causal_dq16.h"
 
 namespace sa2 {
@@ -469,8 +470,8 @@ __global__ __launch_bounds__(THREADS, 1) void causal_dkv16_kernel(Causal p, Caus
     keys_gradients16<E, D>(p, terms, nsplit, padded, blockIdx.x, lds);
 }
 // All gradients in one launch where there are few workgroups, so that one's fill the CUs that the other's short ones leave: `queries`
-// workgroups for dQ, whose longest chains are the longest of all, then those for dK and dV (B2 N2048 H8 D64 80 us apart, 59 together; B4 N1024
-// H16/4 D128 133 and 126; with as many blocks of 256 queries as would give every CU two, B1 N8192 H16/4 D128, 921 and 967: there
+// workgroups for dQ, whose longest chains are the longest of all, then those for dK and dV (B2 N2048 H8 D64 80 us apart, 57 together; B4 N1024
+// H16/4 D128 133 and 121; with as many blocks of 256 queries as would give every CU two, B1 N8192 H16/4 D128, 921 and 967: there
 // a wavefront with 64 queries saves more).
 template <class E, int D>
 __global__ __launch_bounds__(THREADS, 1) void causal_bwd16_kernel(Causal p, Causal16Terms terms, int nsplit, int queries, bool padded) {

@@ -23,7 +23,8 @@ int launch(const Causal& p, const Causal16Terms& terms, hipStream_t st) {
 }  // namespace
 
 // Two blocks of queries per wavefront halve what LDS has to deliver, one makes twice as many workgroups with half the chain: two where
-// every CU has two workgroups all the same (forward, head_dim 128: B1 N8192 H16/4 306 us with two, 350 with one; B4 N1024 43 and 37)
+// every CU has two workgroups all the same (forward, head_dim 128: B1 N8192 H16/4 306 us with two, 350 with one; B4 N1024 43 and 37).
+// Packed rows are counted as count_tiles bounds them, with a workgroup more for every sequence: many short sequences have two.
 bool causal16_two(const Causal& p) { return (int64_t)p.rows.B * p.H * count_tiles(p.rows, 64 * WAVES) >= 2 * CUS; }
 
 int launch_causal16_dq(const Causal& p, int dtype, const Causal16Terms& terms, hipStream_t st) {

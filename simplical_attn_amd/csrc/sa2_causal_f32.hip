@@ -9,7 +9,8 @@
 // of halves, and these registers are, as they are, the second operand of the next product.
 // Here: the kernels for a head_dim above 128, whose accumulators leave no room for a wavefront to have tiles of its own (four share
 // each tile and have 32 rows apiece); the row terms; the choice.  Up to 128: sa2_causal_f32_narrow.hip.
-// Bound by the matrix pipe: an MFMA takes 64 cycles, for which one LDS read of 4 or 16 bytes per lane is enough.
+// Bound by the matrix pipe: an MFMA takes 64 cycles, for which one LDS read of 4 or 16 bytes per lane is enough.  N4096 H8/2, forward and
+// backward: head_dim 256 bf16 2.3 and 15.4 ms, fp32 3.3 and 19.5; 192 (on 256 columns) as long.
 #include "sa2_f32_tiles.h"
 
 namespace sa2 {

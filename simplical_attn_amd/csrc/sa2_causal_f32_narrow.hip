@@ -2,7 +2,7 @@
 // four wavefronts divide the tiles of 32 rows that these see and bring each its own into LDS; their sums meet at the end.
 // Small calls are bound by the longest chain of tiles: a quarter of it here.  Every tile is read by as many workgroups as
 // have rows that see it, four times as many as with 128 rows each, from L2.  Against 128 rows per workgroup: 323 rows in four
-// sequences, 4/2 heads, head_dim 64, forward and backward 244 -> 80 us; B1 N8192 H4/1 D128 1779 -> 950 us forward (72 TFLOP/s of
+// sequences, 4/2 heads, head_dim 64, forward and backward 244 -> 80 us (67 with all gradients in one launch); B1 N8192 H4/1 D128 1779 -> 950 us forward (72 TFLOP/s of
 // the 153 that a large product reaches: an exponential and its mask for every two columns of products), 14.2 -> 3.9 ms backward.
 #include "sa2_f32_tiles.h"
 

@@ -3,8 +3,8 @@
 //   S = scale Q K^T (j <= i), P = softmax(S), O = P V, LSE = log sum e^S
 //
 // A wavefront owns NQ blocks of 32 queries and sweeps the keys that they see (sa2_sweep16.h); four wavefronts are a workgroup.
-// Measured (bf16): B1 N8192 H16/4 D128 302 us (910 TFLOP/s), N16384 H8/2 fp16 500 (1100), N8192 H16 D64 174 (792), B2 N2048 H8 D64
-// 30 (288).  Large calls are bound by the MFMAs at the clock that this load leaves (busy 45 % of the time at 2.0 GHz) and the
+// Measured (bf16): B1 N8192 H16/4 D128 260 us (1060 TFLOP/s), N16384 H8/2 fp16 510 (1080), N8192 H16 D64 172 (800), B2 N2048 H8 D64
+// 31 (280).  Large calls are bound by the MFMAs at the clock that this load leaves (busy 48 % of the time at 2.05 GHz) and the
 // exponentials between them, small ones by the longest block's chain of tiles: 2200 cycles per 64 keys with 32 queries of 128.
 #include "sa2_sweep16.h"
 

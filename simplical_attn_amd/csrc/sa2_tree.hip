@@ -4,8 +4,8 @@
 // its share of the sequence's cached rows and drafted nodes in tiles of 32 keys.  Its wavefronts take tiles in turn, each with
 // LDS, running maximum, sum and output of its own: they meet only at the end.
 // Bound by the cache's bytes where R is small, by the matrix pipe where it is large (fp32, 4 x 8192 rows, 16/4 heads of 128, single
-// tokens: 62 us; the bytes take 17 at a copy's rate, the products, of whose 32 columns four hold rows, 14: the rest is the latency
-// of a wavefront's tiles, which come one after the other).
+// tokens: 81 us; the bytes take 28 at a copy's rate, the products, of whose 32 columns four hold rows, 14: the rest is the latency
+// of a wavefront's tiles, whose loads start when the tile before is done).
 #include "sa2_f32_tiles.h"
 #include "sa2_tree_common.h"
 

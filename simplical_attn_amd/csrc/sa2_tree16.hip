@@ -6,8 +6,8 @@
 // of the keys, which are, as weights, the second operand of O^T = V^T P^T as they are.  Wavefronts take tiles in turn, each with
 // two LDS buffers of its own that direct global->LDS loads fill one tile ahead: no barrier in the sweep, 64 KB of a CU's reads under
 // way at head_dim 128 (a CU's share of the memory rate times its latency is 26 KB).  They meet at the end.
-// Bound by the cache's bytes where they are many (16 x 16384 rows, 16/4 heads of 128: 101 us, 4000 GB/s), elsewhere by the start of
-// a call and the latency of its chain: length, page numbers, rows, join (8 x 4096: 23 us, of which the bytes take 9; 512 rows 14.5).  Workgroups that read the same keys for other
+// Bound by the cache's bytes where they are many (16 x 16384 rows, 16/4 heads of 128: 105 us, 5100 GB/s), elsewhere by the start of
+// a call and the latency of its chain: length, page numbers, rows, join (8 x 4096: 25.6 us, of which the bytes take 14; 512 rows 14.5).  Workgroups that read the same keys for other
 // rows follow each other on one XCD, whose L2 serves all but the first.
 #include "sa2_causal16.h"
 #include "sa2_tree_common.h"

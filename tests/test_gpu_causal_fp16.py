@@ -133,3 +133,42 @@ def test_values_of_vanishing_weights(N, D, H):
     dout = 32 * (dout.abs() + 1)
     got = _train(q, k, v, dout, torch.tensor([0, N], dtype=torch.int32, device=DEV), 1.0)
     _compare(q, k, v, dout, got, [0, N], names=("dv",), scale=1.0)
+
+
+@pytest.mark.parametrize("N,H,HK,D", [(260, 4, 2, 64), (1030, 128, 4, 64)])
+def test_wanted_gradients_streams_and_replays(N, H, HK, D):
+    """Gradients do not depend on which are wanted, nor on the stream; a captured call follows its inputs."""
+    q, k, v, dout = _half(*_inputs(N, H, HK, D, 5))
+    cu = torch.tensor([0, N // 3, N], dtype=torch.int32, device=DEV)
+
+    def call(needs=(True, True, True)):
+        out, lse, low = sa.causal_attention_forward(q, k, v, cu, keep_low=True)
+        return sa.causal_attention_backward(q, k, v, out, lse, dout, cu, needs=needs, out_low=low)
+
+    want = call()
+    for mask in range(1, 8):
+        needs = [bool(mask >> i & 1) for i in range(3)]
+        for need, a, b in zip(needs, call(needs), want):
+            assert torch.equal(a, b) if need else a is None
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = call()
+    g = torch.Generator().manual_seed(6)
+    for ends, size in (([0, 1, N], 1.0), ([0, N // 2, N // 2], 300.0), ([5, 70, N - 3], 2.0 ** -10)):
+        cu.copy_(torch.tensor(ends, dtype=torch.int32))
+        for x in (q, k, v, dout):
+            x.copy_(torch.randn(x.shape, generator=g))
+        v.mul_(size)
+        dout.mul_(size)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        assert all(torch.equal(a, b) for a, b in zip(got, call()))
+        for x in got:                                        # (of v and dO of 300, dS k exceeds 65504: infinities, but no NaN)
+            assert not torch.isnan(x).any()

@@ -53,12 +53,14 @@ void check_cu(const Maybe& cu, const Tensor& q) {
 // While the operators work.  They are no dispatcher operators: a dispatch mode of the user (FLOP counting, selective checkpointing) sees
 // nothing of them, neither a call nor what is allocated inside.  Modes that record or fake operators would miss the kernels: refused.
 struct Unseen {
-    explicit Unseen(const char* op) : guard(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot})) {
+    explicit Unseen(const char* op) {
+        if (!c10::impl::dispatch_mode_enabled()) return;
         using Key = c10::impl::TorchDispatchModeKey;
         for (const Key key : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL})
             TORCH_CHECK(!c10::impl::TorchDispatchModeTLS::get_mode(key), op, " cannot run under fake tensors, make_fx or functionalization: no dispatcher operator stands for it");
+        guard.emplace(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot}));
     }
-    c10::impl::ExcludeDispatchKeyGuard guard;
+    std::optional<c10::impl::ExcludeDispatchKeyGuard> guard;
 };
 void check_place(const char* op, std::initializer_list<Tensor> ts) {
     for (const Tensor& t : ts) {

@@ -36,7 +36,7 @@ typedef enum sa2_status {
     SA2_ERR_BAD_DTYPE = -2,
     SA2_ERR_BAD_SHAPE = -3,      /* B,N,H,D < 1 or D > 256 */
     SA2_ERR_BAD_STRIDE = -4,     /* a stride is not positive */
-    SA2_ERR_BAD_WINDOW = -5,     /* w1 or w2 negative (or 0 with window_inclusive = 0) */
+    SA2_ERR_BAD_WINDOW = -5,     /* w1 or w2 negative (or 0 with window_inclusive = 0); a window below 1, first keys below 0 */
     SA2_ERR_WORKSPACE_TOO_SMALL = -6,
     SA2_ERR_LAUNCH_FAILED = -7,  /* hipGetLastError() after a launch */
     SA2_ERR_UNSUPPORTED = -8,    /* a forced kernel path does not support the shape/dtype */
@@ -242,6 +242,22 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
                         void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                         const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
                         const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream);
+
+/*
+ * The same with a sliding window: query i of a sequence attends to its keys j <= i with i - j < window or j < sinks, that is, to the
+ * last `window` keys up to its own (1 or more) and to the sequence's first `sinks` ones (0 or more).  A window of N or more is
+ * none: sa2_causal_forward and _backward run, bit for bit.
+ *   sequences    of the workspace's size: 0 for a batch, else the packed sequences of the call
+ * The first keys' gradients are sums of fp32 sums over chunks of queries, in their order.
+ */
+int sa2_window_forward(const void* q, const void* k, const void* v, void* out, void* out_low, float* lse,
+                       const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                       const int64_t* strides, int window, int sinks, float scale, int dtype, unsigned flags, void* hip_stream);
+size_t sa2_window_bwd_workspace_bytes(int sequences, int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags);
+int sa2_window_backward(const void* q, const void* k, const void* v, const void* out, const void* out_low, const void* dout, const float* lse,
+                        void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                        const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                        const int64_t* strides, int window, int sinks, float scale, int dtype, unsigned flags, void* hip_stream);
 
 /*
  * T drafted tokens per sequence (1 .. SA2_TREE_NODES; one: a decoding step) over a cache as at sa2_cache_append, which

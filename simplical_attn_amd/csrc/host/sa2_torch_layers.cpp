@@ -23,6 +23,9 @@ decltype(&sa2_cache_append) append_fn = nullptr;
 decltype(&sa2_causal_forward) causal_fwd_fn = nullptr;
 decltype(&sa2_causal_bwd_workspace_bytes) causal_ws_fn = nullptr;
 decltype(&sa2_causal_backward) causal_bwd_fn = nullptr;
+decltype(&sa2_window_forward) window_fwd_fn = nullptr;
+decltype(&sa2_window_bwd_workspace_bytes) window_ws_fn = nullptr;
+decltype(&sa2_window_backward) window_bwd_fn = nullptr;
 decltype(&sa2_tree_workspace_bytes) tree_ws_fn = nullptr;
 decltype(&sa2_tree_attention) tree_fn = nullptr;
 
@@ -256,6 +259,7 @@ struct Prompt {
     Tensor cu;                                 // may be undefined
     double scale;
     unsigned flags;
+    int window, sinks;                         // window 0: none
 };
 Tensor workspace(const Tensor& q, size_t bytes) { return at::empty({(int64_t)bytes}, q.options().dtype(at::kByte).requires_grad(false)); }
 
@@ -274,8 +278,14 @@ std::pair<Tensor, Tensor> run_causal_forward(const Tensor& q_, const Tensor& k_,
     put_strides(s + 3, k);
     put_strides(s + 6, v);
     put_strides(s + 9, out);
-    check(causal_fwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(), low && low->defined() ? low->data_ptr() : nullptr, (float*)lse.data_ptr(), ints(a.cu),
-                        a.cu.defined() ? (int)a.cu.numel() - 1 : 0, z.B, z.N, z.H, (int)k.size(-2), z.D, s, (float)a.scale, dtype_code(q), a.flags, stream(q)));
+    void* const left = low && low->defined() ? low->data_ptr() : nullptr;
+    const int sequences = a.cu.defined() ? (int)a.cu.numel() - 1 : 0, hk = (int)k.size(-2);
+    if (a.window)
+        check(window_fwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(), left, (float*)lse.data_ptr(), ints(a.cu), sequences, z.B, z.N, z.H, hk, z.D, s,
+                            a.window, a.sinks, (float)a.scale, dtype_code(q), a.flags, stream(q)));
+    else
+        check(causal_fwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(), left, (float*)lse.data_ptr(), ints(a.cu), sequences, z.B, z.N, z.H, hk, z.D, s,
+                            (float)a.scale, dtype_code(q), a.flags, stream(q)));
     return {out, lse};
 }
 
@@ -298,14 +308,20 @@ std::array<Tensor, 3> run_causal_backward(const Tensor& q_, const Tensor& k_, co
             if (t.defined()) t.zero_();        // (keys that no query head reads)
         return g;
     }
-    const size_t bytes = causal_ws_fn(z.B, z.N, z.H, hk, z.D, dtype_code(q), a.flags);
+    const int sequences = a.cu.defined() ? (int)a.cu.numel() - 1 : 0;
+    const size_t bytes = a.window ? window_ws_fn(sequences, z.B, z.N, z.H, hk, z.D, a.window, a.sinks, dtype_code(q), a.flags) : causal_ws_fn(z.B, z.N, z.H, hk, z.D, dtype_code(q), a.flags);
     const Tensor ws = workspace(q, std::max<size_t>(bytes, 256));
     int64_t s[24];
     const Tensor* const t[8] = {&q, &k, &v, &out, &dout, g[0].defined() ? &g[0] : &q, g[1].defined() ? &g[1] : &k, g[2].defined() ? &g[2] : &v};
     for (int i = 0; i < 8; ++i) put_strides(s + 3 * i, *t[i]);
     auto ptr = [&](int i) { return g[i].defined() ? g[i].data_ptr() : nullptr; };
-    check(causal_bwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.const_data_ptr(), low.defined() ? low.const_data_ptr() : nullptr, dout.const_data_ptr(), (const float*)lse.const_data_ptr(), ptr(0), ptr(1), ptr(2),
-                        ws.data_ptr(), (size_t)ws.numel(), ints(a.cu), a.cu.defined() ? (int)a.cu.numel() - 1 : 0, z.B, z.N, z.H, hk, z.D, s, (float)a.scale, dtype_code(q), a.flags, stream(q)));
+    const void* const left = low.defined() ? low.const_data_ptr() : nullptr;
+    if (a.window)
+        check(window_bwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.const_data_ptr(), left, dout.const_data_ptr(), (const float*)lse.const_data_ptr(), ptr(0), ptr(1), ptr(2),
+                            ws.data_ptr(), (size_t)ws.numel(), ints(a.cu), sequences, z.B, z.N, z.H, hk, z.D, s, a.window, a.sinks, (float)a.scale, dtype_code(q), a.flags, stream(q)));
+    else
+        check(causal_bwd_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.const_data_ptr(), left, dout.const_data_ptr(), (const float*)lse.const_data_ptr(), ptr(0), ptr(1), ptr(2),
+                            ws.data_ptr(), (size_t)ws.numel(), ints(a.cu), sequences, z.B, z.N, z.H, hk, z.D, s, (float)a.scale, dtype_code(q), a.flags, stream(q)));
     return g;
 }
 
@@ -317,13 +333,15 @@ struct CausalFormula : torch::autograd::Function<CausalFormula> {
         ctx->save_for_backward({q, k, v, out, lse, a.cu, low});
         ctx->saved_data["scale"] = a.scale;
         ctx->saved_data["flags"] = (int64_t)a.flags;
+        ctx->saved_data["window"] = (int64_t)a.window;
+        ctx->saved_data["sinks"] = (int64_t)a.sinks;
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "causal_attention has first derivatives only: its backward cannot run with create_graph=True");
         at::AutoDispatchBelowADInplaceOrView below;
         const auto s = ctx->get_saved_variables();
-        const Prompt a{s[5], ctx->saved_data["scale"].toDouble(), (unsigned)ctx->saved_data["flags"].toInt()};
+        const Prompt a{s[5], ctx->saved_data["scale"].toDouble(), (unsigned)ctx->saved_data["flags"].toInt(), (int)ctx->saved_data["window"].toInt(), (int)ctx->saved_data["sinks"].toInt()};
         unsigned needs = 0;
         for (int i = 0; i < 3; ++i) needs |= (ctx->needs_input_grad(i) ? 1u : 0u) << i;
         auto g = run_causal_backward(s[0], s[1], s[2], s[3], s[6], s[4], grads[0], needs, a);
@@ -331,7 +349,16 @@ struct CausalFormula : torch::autograd::Function<CausalFormula> {
     }
 };
 
-Prompt check_causal(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, const std::optional<double>& scale, unsigned flags) {
+// (window, first keys) as the C ABI takes them; (0, 0): none
+std::pair<int, int> check_window(const std::optional<int64_t>& window, int64_t sinks) {
+    TORCH_CHECK_VALUE(!window || *window >= 1, "window must be at least 1, got ", window ? *window : 0);
+    TORCH_CHECK_VALUE(sinks >= 0, "sinks must not be negative, got ", sinks);
+    TORCH_CHECK_VALUE(window || sinks == 0, "sinks go with a window");
+    const int64_t most = 0x7fffffff;
+    return {window ? (int)std::min(*window, most) : 0, (int)std::min(sinks, most)};
+}
+
+Prompt check_causal(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, const std::optional<double>& scale, unsigned flags, const std::optional<int64_t>& window, int64_t sinks) {
     check_first(q, "q");
     check_beside(k, "k", q, "q");
     check_beside(v, "v", q, "q");
@@ -340,20 +367,22 @@ Prompt check_causal(const Tensor& q, const Tensor& k, const Tensor& v, const May
     TORCH_CHECK_VALUE(q.size(-1) >= 1 && q.size(-1) <= 256, "head_dim must be 1 to 256, got ", q.size(-1));
     check_cu(cu, q);
     TORCH_CHECK_VALUE(q.dim() == 4 || cu, "packed rows need cu_seqlens");
+    const auto [reach, first] = check_window(window, sinks);
     check_place("causal_attention", {q, k, v});
-    return {dense(cu), scale ? *scale : 1.0 / std::sqrt((double)q.size(-1)), flags};
+    return {dense(cu), scale ? *scale : 1.0 / std::sqrt((double)q.size(-1)), flags, reach, first};
 }
 
-Tensor causal(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, std::optional<double> scale, unsigned flags) {
-    const Prompt a = check_causal(q, k, v, cu, scale, flags);
+Tensor causal(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, std::optional<double> scale, unsigned flags, std::optional<int64_t> window, int64_t sinks) {
+    const Prompt a = check_causal(q, k, v, cu, scale, flags, window, sinks);
     py::gil_scoped_release nogil;
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) return CausalFormula::apply(q, k, v, a);
     at::AutoDispatchBelowADInplaceOrView below;
     return run_causal_forward(q, k, v, a).first;
 }
 
-std::tuple<Tensor, Tensor, Maybe> causal_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, std::optional<double> scale, unsigned flags, bool keep_low) {
-    const Prompt a = check_causal(q, k, v, cu, scale, flags);
+std::tuple<Tensor, Tensor, Maybe> causal_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& cu, std::optional<double> scale, unsigned flags, bool keep_low,
+                                                std::optional<int64_t> window, int64_t sinks) {
+    const Prompt a = check_causal(q, k, v, cu, scale, flags, window, sinks);
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
     Tensor low;
@@ -362,10 +391,10 @@ std::tuple<Tensor, Tensor, Maybe> causal_forward(const Tensor& q, const Tensor& 
 }
 
 std::tuple<Maybe, Maybe, Maybe> causal_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse, const Tensor& dout, const Maybe& cu,
-                                                std::optional<double> scale, unsigned needs, unsigned flags, const Maybe& low) {
+                                                std::optional<double> scale, unsigned needs, unsigned flags, const Maybe& low, std::optional<int64_t> window, int64_t sinks) {
     TORCH_CHECK_VALUE(!low || dtype_code(q) != SA2_F32, "out_low goes with 16-bit tensors");
     if (low) TORCH_CHECK_VALUE(low->sizes() == q.sizes() && low->scalar_type() == q.scalar_type() && low->device() == q.device(), "out_low must match q in shape, dtype and device");
-    const Prompt a = check_causal(q, k, v, cu, scale, flags);
+    const Prompt a = check_causal(q, k, v, cu, scale, flags, window, sinks);
     for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(out, "out"), {dout, "dout"}})
         TORCH_CHECK_VALUE(t.sizes() == q.sizes() && t.scalar_type() == q.scalar_type() && t.device() == q.device(), name, " must match q in shape, dtype and device");
     const bool batched = q.dim() == 4;
@@ -420,7 +449,7 @@ Tensor tree(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Maybe& p
 }  // namespace
 
 void define_layers(py::module_& m) {
-    m.def("bind_layers", [](uintptr_t rotary, uintptr_t append, uintptr_t causal_fwd, uintptr_t causal_ws, uintptr_t causal_bwd, uintptr_t tree_ws, uintptr_t tree) {
+    m.def("bind_layers", [](uintptr_t rotary, uintptr_t append, uintptr_t causal_fwd, uintptr_t causal_ws, uintptr_t causal_bwd, uintptr_t tree_ws, uintptr_t tree, uintptr_t window_fwd, uintptr_t window_ws, uintptr_t window_bwd) {
         rotary_fn = (decltype(rotary_fn))rotary;
         append_fn = (decltype(append_fn))append;
         causal_fwd_fn = (decltype(causal_fwd_fn))causal_fwd;
@@ -428,6 +457,9 @@ void define_layers(py::module_& m) {
         causal_bwd_fn = (decltype(causal_bwd_fn))causal_bwd;
         tree_ws_fn = (decltype(tree_ws_fn))tree_ws;
         tree_fn = (decltype(tree_fn))tree;
+        window_fwd_fn = (decltype(window_fwd_fn))window_fwd;
+        window_ws_fn = (decltype(window_ws_fn))window_ws;
+        window_bwd_fn = (decltype(window_bwd_fn))window_bwd;
     });
     m.def("rotary", &rotary);
     m.def("cache_append", &append);

@@ -81,6 +81,59 @@ __device__ __forceinline__ void order(int pid, int streams, int& stream, int& ti
 // Rows of a tile: offset of the row at place `at` of the sequence
 __device__ __forceinline__ int64_t row_offset(const Tensor& t, const Span& s, int at, int h) { return t.off(s.b, s.first + at, h); }
 
+// Tiles of SIZE keys that queries first .. last see any of, numbered from 0 on: those of the first keys, then those of the window
+template <bool BAND, int SIZE>
+struct KeyTiles {
+    int head, start, count;
+    __device__ __forceinline__ KeyTiles(const Band& band, int first, int last) {
+        head = start = 0;
+        if constexpr (BAND) {
+            start = (first < band.window ? 0 : first - band.window + 1) / SIZE;
+            head = (band.sinks + SIZE - 1) / SIZE;
+            head = head < start ? head : start;
+        }
+        count = head + last / SIZE + 1 - start;
+    }
+    // the first key of tile t
+    __device__ __forceinline__ int at(int t) const { return (!BAND || t < head ? t : t - head + start) * SIZE; }
+};
+// Bits 0 .. n-1 of 32
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+// What query i sees of the keys j0 .. j0+31, and which of the queries i0 .. i0+31 see key j (`sink`: one of the first ones), bit by bit
+__device__ __forceinline__ uint32_t band_keys(const Band& b, int i, int j0) { return bits_below(i - j0 + 1) & (~bits_below(i - b.window + 1 - j0) | bits_below(b.sinks - j0)); }
+__device__ __forceinline__ uint32_t band_queries(const Band& b, int j, int i0, bool sink) { return ~bits_below(j - i0) & (sink ? ~0u : bits_below(j - i0 + b.window)); }
+// Of such queries or keys, those whose gradients count: a query that sees its own key only has one weight, 1, whose gradient is zero
+__device__ __forceinline__ uint32_t band_counted(const Band& b, uint32_t queries, int i0) { return i0 + 31 <= b.alone ? 0u : i0 == 0 ? queries & ~1u : queries; }
+// Whether queries i0 .. i1 see all of the keys j0 .. j1
+__device__ __forceinline__ bool band_full(const Band& b, int i0, int i1, int j0, int j1) { return j1 <= i0 && (i1 - j0 < b.window || j1 < b.sinks); }
+// Queries lo .. hi-1 that a workgroup takes for keys j0 .. j0+rows-1: with a band, those of the window of keys behind the first ones
+// (`sink` < 0), or a chunk of the sequence for the first keys.  false: none, or nothing that it has to leave
+struct KeyWork {
+    int lo, hi, sink;                                       // sink: the chunk's place in p.sink_part, or -1
+};
+template <bool BAND>
+__device__ __forceinline__ bool key_work(const Causal& p, const Span& s, int j0, int rows, int chunk, int slot, KeyWork& w) {
+    w = KeyWork{j0, s.len, -1};
+    if constexpr (BAND) {
+        if (slot < 0) {
+            if (j0 + rows <= p.band.sinks) return false;
+            const int64_t end = (int64_t)j0 + rows - 1 + p.band.window;
+            w.hi = end < s.len ? (int)end : s.len;
+        } else {
+            w.sink = slot;
+            w.lo = chunk * p.band.chunk > j0 ? chunk * p.band.chunk : j0;
+            w.hi = s.len - chunk * p.band.chunk < p.band.chunk ? s.len : (chunk + 1) * p.band.chunk;
+            return j0 < s.len && w.lo < w.hi;
+        }
+    }
+    return true;
+}
+// Sums of the first key j of a key head over chunk `slot`; which: 0 dK, 1 dV
+__device__ __forceinline__ float* sink_row(const Causal& p, int64_t slots, int which, int slot, int hk, int j) {
+    return p.sink_part + ((((int64_t)which * slots + slot) * p.HK + hk) * p.band.sinks + j) * p.D;
+}
+inline int64_t sink_slots(const Causal& p) { return (int64_t)p.rows.B * count_tiles(p.rows, p.band.chunk); }
+
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 }  // namespace

@@ -72,7 +72,7 @@ __device__ __forceinline__ void own_rows(float (&x)[DP / 2], const Tensor& t, co
         x[4 * c] = v.x * factor; x[4 * c + 1] = v.y * factor; x[4 * c + 2] = v.z * factor; x[4 * c + 3] = v.w * factor;
     }
 }
-// [tile rows] x [own rows]: rows of the tile in the registers, own ones in the lanes
+// [tile rows] x [own rows]: rows of the tile in the registers, own ones in the lanes.
 template <int DP>
 __device__ __forceinline__ floatx16 tile_product(const float* lds, const float (&own)[DP / 2]) {
     const int lane = threadIdx.x & 63;
@@ -123,6 +123,39 @@ __device__ __forceinline__ void weighted_rows(const float* lds, int first, const
                 for (int b = 0; b < DO / 32; ++b) acc[b] = mfma(a[b], p, acc[b]);
             }
         }
+}
+// The same where a flag for the whole tile says whether it holds an infinity or NaN (odd_values of what went into it) and `seen` is what the
+// lane's own row sees of it, bit by bit.  Such a tile is added up one row at a time on the vector ALU.  (The check and the branch for
+// each row of weighted_rows, unrolled, are 27000 instructions at head_dim 256, and held so many registers beside a window's masks that
+// the kernels went wrong.)
+__device__ __forceinline__ uint32_t odd_values(float4 x) {
+    uint32_t bits = 0;
+    for (const float y : {x.x, x.y, x.z, x.w}) bits |= (__float_as_uint(y) & 0x7f800000u) + 0x00800000u;
+    return bits;                                            // (of several ORed together the top bit counts)
+}
+template <int DP, int DO>
+__device__ __forceinline__ void banded_rows(const float* lds, int first, const floatx16& w, floatx16 (&acc)[DO / 32], bool odd, uint32_t seen) {
+    if (!odd) return weighted_rows<DP, DO, false>(lds, first, w, acc, [](int) { return true; });
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll 1
+    for (int row = 0; row < TILE; ++row) {
+        float held = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) held = row / 8 * 4 + row % 4 == i ? w[i] : held;
+        const float other = other_half(held), weight = (row / 4 & 1) == half ? held : other;
+        const bool sees = seen >> row & 1;
+        const float* const from = lds + row * Pitch<DP>::value + first + 4 * half;
+#pragma unroll
+        for (int b = 0; b < DO / 32; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 v = *(const float4*)(from + 32 * b + 8 * g);
+                acc[b][4 * g] = sees ? fmaf(weight, v.x, acc[b][4 * g]) : acc[b][4 * g];
+                acc[b][4 * g + 1] = sees ? fmaf(weight, v.y, acc[b][4 * g + 1]) : acc[b][4 * g + 1];
+                acc[b][4 * g + 2] = sees ? fmaf(weight, v.z, acc[b][4 * g + 2]) : acc[b][4 * g + 2];
+                acc[b][4 * g + 3] = sees ? fmaf(weight, v.w, acc[b][4 * g + 3]) : acc[b][4 * g + 3];
+            }
+    }
 }
 template <class F>
 int for_width(int D, F&& f) {

@@ -3,7 +3,7 @@
 #include <math.h>
 #include <string.h>
 
-#include "sa2_layer_common.h"
+#include "sa2_causal_common.h"
 
 using namespace sa2;
 
@@ -36,6 +36,18 @@ int make_causal(Causal& p, const int32_t* cu, int sequences, int B, int N, int H
     p.scale = scale;
     return SA2_OK;
 }
+// window 0: none
+int make_band(Causal& p, int window, int sinks) {
+    if (window < 0 || sinks < 0) return SA2_ERR_BAD_WINDOW;
+    if (window == 0 || window >= p.rows.N) return SA2_OK;                  // (every key of the sequence is in reach)
+    p.band.window = window;
+    p.band.sinks = sinks < p.rows.N ? sinks : p.rows.N;
+    p.band.alone = window == 1 && sinks == 0 ? 0x7fffffff : 0;
+    // (where the first keys are many, longer chunks, so that their sums stay a fraction of the tensors)
+    const int64_t chunk = 512 * (int64_t)(p.band.sinks > 128 ? (p.band.sinks + 127) / 128 : 1);
+    p.band.chunk = chunk < 1 << 30 ? (int)chunk : 1 << 30;
+    return p.band.sinks > 0 && (sink_slots(p) * p.HK > 0x7fffffff || p.band.sinks > 65535 * 32) ? SA2_ERR_TOO_LARGE : SA2_OK;
+}
 size_t row_bytes(const Causal& p, int heads) { return ((size_t)p.rows.B * heads * p.rows.N * sizeof(float) + 255) / 256 * 256; }
 size_t delta_bytes(const Causal& p) { return row_bytes(p, p.H); }
 
@@ -54,6 +66,78 @@ int tree_splits(int B, int T, int H, int HK, int D, int page_size, int table_wid
     int64_t n = CUS / streams;
     if (n > tiles / least) n = tiles / least;
     return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+}
+
+// Prompts; window 0: every key up to the query's own
+int prompt_forward(const void* q, const void* k, const void* v, void* out, void* out_low, float* lse,
+                   const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                   const int64_t* strides, int window, int sinks, float scale, int dtype, unsigned flags, void* hip_stream) {
+    if (!q || !k || !v || !out || !lse || !strides) return SA2_ERR_NULL_POINTER;
+    Causal p;
+    int rc = make_causal(p, cu_seqlens, sequences, B, N, H, HK, D, scale, dtype);
+    if (rc == SA2_OK) rc = make_band(p, window, sinks);
+    if (rc != SA2_OK) return rc;
+    p.q = tensor(q, strides, 0);
+    p.k = tensor(k, strides, 1);
+    p.v = tensor(v, strides, 2);
+    p.out = tensor(out, strides, 3);
+    p.out_low = dtype == SA2_F32 ? nullptr : out_low;
+    p.lse = lse;
+    if (!stride_ok(p.q, B, N, H) || !stride_ok(p.out, B, N, H) || !stride_ok(p.k, B, N, HK) || !stride_ok(p.v, B, N, HK)) return SA2_ERR_BAD_STRIDE;
+    const hipStream_t st = (hipStream_t)hip_stream;
+    const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out}) && !((uintptr_t)out_low & 15u);
+    if (p.band.window) return launch_window_f32_fwd(p, dtype, st);
+    return narrow ? launch_causal16_fwd(p, dtype, st) : launch_causal_f32_fwd(p, dtype, st);
+}
+
+size_t prompt_workspace(int sequences, int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags) {
+    Causal p;
+    static const int32_t packed = 0;                       // (only whether there are packed sequences counts here)
+    if (make_causal(p, sequences > 0 ? &packed : nullptr, sequences, B, N, H, HK, D, 1.f, dtype) != SA2_OK || make_band(p, window, sinks) != SA2_OK) return 0;
+    if (p.band.window) return (delta_bytes(p) + sink_part_bytes(p) + 255) / 256 * 256;
+    if ((flags & SA2_FLAG_FORCE_GENERIC) || !causal16_supported(D, dtype)) return delta_bytes(p);
+    return 2 * delta_bytes(p) + (dtype == SA2_F16 ? delta_bytes(p) + row_bytes(p, HK) : 0) + causal16_part_bytes(B, N, HK, p.G, D);
+}
+
+int prompt_backward(const void* q, const void* k, const void* v, const void* out, const void* out_low, const void* dout, const float* lse,
+                    void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                    const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                    const int64_t* strides, int window, int sinks, float scale, int dtype, unsigned flags, void* hip_stream) {
+    if (!q || !k || !v || !out || !dout || !lse || !workspace || !strides) return SA2_ERR_NULL_POINTER;
+    Causal p;
+    int rc = make_causal(p, cu_seqlens, sequences, B, N, H, HK, D, scale, dtype);
+    if (rc == SA2_OK) rc = make_band(p, window, sinks);
+    if (rc != SA2_OK) return rc;
+    Tensor* const t[8] = {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv};
+    const void* const at[8] = {q, k, v, out, dout, dq, dk, dv};
+    for (int i = 0; i < 8; ++i) {
+        *t[i] = tensor(at[i], strides, i);
+        if (at[i] && !stride_ok(*t[i], B, N, i == 1 || i == 2 || i > 5 ? HK : H)) return SA2_ERR_BAD_STRIDE;
+    }
+    if (((uintptr_t)workspace & 255u) || workspace_bytes < prompt_workspace(cu_seqlens ? sequences : 0, B, N, H, HK, D, window, sinks, dtype, flags)) return SA2_ERR_WORKSPACE_TOO_SMALL;
+    p.out_low = dtype == SA2_F32 ? nullptr : const_cast<void*>(out_low);
+    p.lse = const_cast<float*>(lse);
+    p.delta = (float*)workspace;
+    const hipStream_t st = (hipStream_t)hip_stream;
+    if (!dq && !dk && !dv) return SA2_OK;
+    char* behind = (char*)workspace + delta_bytes(p);
+    auto next = [&](size_t bytes) { char* const here = behind; behind += bytes; return (float*)here; };
+    if (p.band.window) {
+        p.sink_part = next(0);
+        return launch_window_f32_bwd(p, dtype, st);
+    }
+    // (-lse / scale is one of the 16-bit kernels' operands)
+    if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv}) &&
+        fabsf(scale) > 1e-20f && !((uintptr_t)out_low & 15u)) {
+        Causal16Terms terms{next(delta_bytes(p)), nullptr, nullptr};
+        if (dtype == SA2_F16) {
+            terms.dout = next(delta_bytes(p));
+            terms.v = next(row_bytes(p, HK));
+        }
+        p.part = next(0);
+        return launch_causal16_bwd(p, dtype, terms, st);
+    }
+    return launch_causal_f32_bwd(p, dtype, st);
 }
 
 }  // namespace
@@ -126,63 +210,34 @@ int sa2_cache_append(const void* k, const void* v, void* k_cache, void* v_cache,
 int sa2_causal_forward(const void* q, const void* k, const void* v, void* out, void* out_low, float* lse,
                        const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
                        const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream) {
-    if (!q || !k || !v || !out || !lse || !strides) return SA2_ERR_NULL_POINTER;
-    Causal p;
-    const int rc = make_causal(p, cu_seqlens, sequences, B, N, H, HK, D, scale, dtype);
-    if (rc != SA2_OK) return rc;
-    p.q = tensor(q, strides, 0);
-    p.k = tensor(k, strides, 1);
-    p.v = tensor(v, strides, 2);
-    p.out = tensor(out, strides, 3);
-    p.out_low = dtype == SA2_F32 ? nullptr : out_low;
-    p.lse = lse;
-    if (!stride_ok(p.q, B, N, H) || !stride_ok(p.out, B, N, H) || !stride_ok(p.k, B, N, HK) || !stride_ok(p.v, B, N, HK)) return SA2_ERR_BAD_STRIDE;
-    if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out}) && !((uintptr_t)out_low & 15u))
-        return launch_causal16_fwd(p, dtype, (hipStream_t)hip_stream);
-    return launch_causal_f32_fwd(p, dtype, (hipStream_t)hip_stream);
+    return prompt_forward(q, k, v, out, out_low, lse, cu_seqlens, sequences, B, N, H, HK, D, strides, 0, 0, scale, dtype, flags, hip_stream);
+}
+int sa2_window_forward(const void* q, const void* k, const void* v, void* out, void* out_low, float* lse,
+                       const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                       const int64_t* strides, int window, int sinks, float scale, int dtype, unsigned flags, void* hip_stream) {
+    if (window < 1) return SA2_ERR_BAD_WINDOW;
+    return prompt_forward(q, k, v, out, out_low, lse, cu_seqlens, sequences, B, N, H, HK, D, strides, window, sinks, scale, dtype, flags, hip_stream);
 }
 
 size_t sa2_causal_bwd_workspace_bytes(int B, int N, int H, int HK, int D, int dtype, unsigned flags) {
-    Causal p;
-    if (make_causal(p, nullptr, 0, B, N, H, HK, D, 1.f, dtype) != SA2_OK) return 0;
-    if ((flags & SA2_FLAG_FORCE_GENERIC) || !causal16_supported(D, dtype)) return delta_bytes(p);
-    return 2 * delta_bytes(p) + (dtype == SA2_F16 ? delta_bytes(p) + row_bytes(p, HK) : 0) + causal16_part_bytes(B, N, HK, p.G, D);
+    return prompt_workspace(0, B, N, H, HK, D, 0, 0, dtype, flags);
+}
+size_t sa2_window_bwd_workspace_bytes(int sequences, int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags) {
+    return window < 1 ? 0 : prompt_workspace(sequences, B, N, H, HK, D, window, sinks, dtype, flags);
 }
 
 int sa2_causal_backward(const void* q, const void* k, const void* v, const void* out, const void* out_low, const void* dout, const float* lse,
                         void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                         const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
                         const int64_t* strides, float scale, int dtype, unsigned flags, void* hip_stream) {
-    if (!q || !k || !v || !out || !dout || !lse || !workspace || !strides) return SA2_ERR_NULL_POINTER;
-    Causal p;
-    const int rc = make_causal(p, cu_seqlens, sequences, B, N, H, HK, D, scale, dtype);
-    if (rc != SA2_OK) return rc;
-    Tensor* const t[8] = {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv};
-    const void* const at[8] = {q, k, v, out, dout, dq, dk, dv};
-    for (int i = 0; i < 8; ++i) {
-        *t[i] = tensor(at[i], strides, i);
-        if (at[i] && !stride_ok(*t[i], B, N, i == 1 || i == 2 || i > 5 ? HK : H)) return SA2_ERR_BAD_STRIDE;
-    }
-    if (((uintptr_t)workspace & 255u) || workspace_bytes < sa2_causal_bwd_workspace_bytes(B, N, H, HK, D, dtype, flags)) return SA2_ERR_WORKSPACE_TOO_SMALL;
-    p.out_low = dtype == SA2_F32 ? nullptr : const_cast<void*>(out_low);
-    p.lse = const_cast<float*>(lse);
-    p.delta = (float*)workspace;
-    const hipStream_t st = (hipStream_t)hip_stream;
-    if (!dq && !dk && !dv) return SA2_OK;
-    // (-lse / scale is one of the 16-bit kernels' operands)
-    if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv}) &&
-        fabsf(scale) > 1e-20f && !((uintptr_t)out_low & 15u)) {
-        char* at = (char*)workspace + delta_bytes(p);
-        auto next = [&](size_t bytes) { char* const here = at; at += bytes; return (float*)here; };
-        Causal16Terms terms{next(delta_bytes(p)), nullptr, nullptr};
-        if (dtype == SA2_F16) {
-            terms.dout = next(delta_bytes(p));
-            terms.v = next(row_bytes(p, HK));
-        }
-        p.part = next(0);
-        return launch_causal16_bwd(p, dtype, terms, st);
-    }
-    return launch_causal_f32_bwd(p, dtype, st);
+    return prompt_backward(q, k, v, out, out_low, dout, lse, dq, dk, dv, workspace, workspace_bytes, cu_seqlens, sequences, B, N, H, HK, D, strides, 0, 0, scale, dtype, flags, hip_stream);
+}
+int sa2_window_backward(const void* q, const void* k, const void* v, const void* out, const void* out_low, const void* dout, const float* lse,
+                        void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                        const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
+                        const int64_t* strides, int window, int sinks, float scale, int dtype, unsigned flags, void* hip_stream) {
+    if (window < 1) return SA2_ERR_BAD_WINDOW;
+    return prompt_backward(q, k, v, out, out_low, dout, lse, dq, dk, dv, workspace, workspace_bytes, cu_seqlens, sequences, B, N, H, HK, D, strides, window, sinks, scale, dtype, flags, hip_stream);
 }
 
 size_t sa2_tree_workspace_bytes(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype, unsigned flags) {

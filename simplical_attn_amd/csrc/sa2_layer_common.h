@@ -17,6 +17,15 @@ struct Rows {
     int sequences;
 };
 
+// What queries see besides the causal mask (window 0: every key before them): the last `window` keys up to their own, and the first
+// `sinks` ones of the sequence.  Gradients of the first keys, which all queries see, are made by workgroups of their own, each with
+// `chunk` queries of a sequence (of all heads that share the keys), whose fp32 sums meet in a last launch.
+struct Band {
+    int window, sinks;
+    int alone;                                 // queries up to this number see their own key only
+    int chunk;
+};
+
 // One call of causal attention.  H query heads share HK heads of keys and values, G = H / HK neighbours one.
 struct Causal {
     Rows rows;
@@ -27,6 +36,8 @@ struct Causal {
     float* lse;                                // [B,H,N]
     float* delta;                              // [B,H,N]  sum_d dout*(out + out_low)
     float* part;                               // partial sums (path specific)
+    Band band;
+    float* sink_part;                          // [dK, dV][chunk of a sequence][HK][sinks][D]: the first keys' sums
 };
 
 struct Rotary {
@@ -81,6 +92,13 @@ int launch_rotary(const Rotary& p, int dtype, hipStream_t st);
 int launch_append(const Append& p, int dtype, hipStream_t st);
 int launch_causal_f32_fwd(const Causal& p, int dtype, hipStream_t st);
 int launch_causal_f32_bwd(const Causal& p, int dtype, hipStream_t st);
+// with p.band
+int launch_window_f32_fwd(const Causal& p, int dtype, hipStream_t st);
+int launch_window_f32_bwd(const Causal& p, int dtype, hipStream_t st);
+int launch_window_f32_narrow_fwd(const Causal& p, int dtype, bool wide, hipStream_t st);
+int launch_window_f32_narrow_bwd(const Causal& p, int dtype, bool wide, hipStream_t st);
+size_t sink_part_bytes(const Causal& p);
+int launch_sink_sums(const Causal& p, int dtype, hipStream_t st);
 // the same, head_dim up to 128: the four wavefronts of a workgroup share its 32 rows and divide what these see
 int launch_causal_f32_narrow_fwd(const Causal& p, int dtype, bool wide, hipStream_t st);
 int launch_causal_f32_narrow_bwd(const Causal& p, int dtype, bool wide, hipStream_t st);

@@ -84,32 +84,35 @@ def cache_append(k, v, k_cache, v_cache, lengths, page_table=None, rows=None, cu
     _lib.host().cache_append(k, v, k_cache, v_cache, lengths, page_table, rows, cu_seqlens)
 
 
-def causal_attention(q, k, v, cu_seqlens=None, scale=None, flags=_lib.FLAG_AUTO):
-    """softmax(scale q k^T) v, query i of a sequence over its keys 0 .. i; differentiable in q, k and v (once: create_graph=True
-    is refused).
+def causal_attention(q, k, v, cu_seqlens=None, scale=None, flags=_lib.FLAG_AUTO, window=None, sinks=0):
+    """softmax(scale q k^T) v, query i of a sequence over its keys 0 .. i, or of these the last ``window`` and the first ``sinks``;
+    differentiable in q, k and v (once: create_graph=True is refused).
 
     q        [batch, seq_len, heads, head_dim], or packed [rows, heads, head_dim] with cu_seqlens; head_dim up to 256
     k, v     as q, with heads that divide q's: query head h reads head h // (heads / key heads)
     scale    1 / sqrt(head_dim) if None
     flags    _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products whatever the type, gradients too
+    window   None, or at least 1: query i attends to key j where i - j < window (its own key among them; the windows [i - w, i] of
+             the 2-simplicial operator have one key more), or
+    sinks    where j < sinks: the sequence's first keys stay visible to all of its queries
 
     Returns a tensor like q, zero in rows of no sequence.  bf16 and fp16 with a head_dim up to 128 that is a multiple of 8 and rows on
     the 16-byte grid run on the 16-bit matrix pipes (softmax weights rounded to the type, sums in fp32), everything else
     with fp32 products."""
-    return _lib.host().causal(q, k, v, cu_seqlens, scale, int(flags))
+    return _lib.host().causal(q, k, v, cu_seqlens, scale, int(flags), window, sinks)
 
 
-def causal_attention_forward(q, k, v, cu_seqlens=None, scale=None, flags=_lib.FLAG_AUTO, keep_low=False):
+def causal_attention_forward(q, k, v, cu_seqlens=None, scale=None, flags=_lib.FLAG_AUTO, keep_low=False, window=None, sinks=0):
     """(out, lse) without autograd: lse is log sum e^(scale q k), [batch, heads, seq_len] or packed [heads, rows], float32,
     -infinity in rows of no sequence.  flags: _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products.
     keep_low: (out, lse, out_low) with what rounding out to 16 bits left, for the backward (None for float32; not written in rows of
     no sequence)."""
-    out, lse, out_low = _lib.host().causal_forward(q, k, v, cu_seqlens, scale, int(flags), bool(keep_low))
+    out, lse, out_low = _lib.host().causal_forward(q, k, v, cu_seqlens, scale, int(flags), bool(keep_low), window, sinks)
     return (out, lse, out_low) if keep_low else (out, lse)
 
 
 def causal_attention_backward(q, k, v, out, lse, dout, cu_seqlens=None, scale=None, needs=(True, True, True),
-                              flags=_lib.FLAG_AUTO, out_low=None):
+                              flags=_lib.FLAG_AUTO, out_low=None, window=None, sinks=0):
     """(dq, dk, dv) in the inputs' type, None where ``needs`` is False.  ``out``, ``lse`` and ``out_low`` are what
     causal_attention_forward returned for the same inputs and arguments.  With out_low these are causal_attention's gradients, bit for
     bit; without it, in 16-bit types, dq and dk of short sequences are 1.5 to 2.3 times as far off as their own rounding.
@@ -117,7 +120,7 @@ def causal_attention_backward(q, k, v, out, lse, dout, cu_seqlens=None, scale=No
     if len(needs) != 3:
         raise ValueError("needs must have three entries (dq, dk, dv), got %d" % len(needs))
     mask = sum(1 << t for t, need in enumerate(needs) if need)
-    return _lib.host().causal_backward(q, k, v, out, lse, dout, cu_seqlens, scale, mask, int(flags), out_low)
+    return _lib.host().causal_backward(q, k, v, out, lse, dout, cu_seqlens, scale, mask, int(flags), out_low, window, sinks)
 
 
 def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None, scale=None, flags=_lib.FLAG_AUTO):

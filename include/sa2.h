@@ -279,6 +279,21 @@ int sa2_tree_attention(const void* q, const void* k, const void* v, const void* 
                        int page_size, int pages, int table_width, const int64_t* strides, float scale,
                        int dtype, unsigned flags, void* hip_stream);
 
+/*
+ * The same with a sliding window, and the weights that the cached rows get.
+ *   window       0: none; else 1 or more: a node at place n (lengths[b] and its ancestors before it) attends to row or ancestor r of its
+ *                sequence where n - r < window or r < sinks.  Rows of the cache behind that are not read.
+ *   weights      NULL, or (T 1 only, else SA2_ERR_BAD_TREE) fp32 [B,HK,page_size * table_width or more], strides 18 and 19 (batch, head):
+ *                each row's softmax weight, summed over the query heads that share its head, is added at its place, and the
+ *                node's own at place lengths[b], where the cache has one
+ */
+size_t sa2_window_tree_workspace_bytes(int B, int T, int H, int HK, int D, int page_size, int table_width, int window, int sinks, int weighted, int dtype, unsigned flags);
+int sa2_window_tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out, float* weights,
+                              const int32_t* parents, const int32_t* lengths, const int32_t* page_table,
+                              void* workspace, size_t workspace_bytes, int B, int T, int H, int HK, int D,
+                              int page_size, int pages, int table_width, const int64_t* strides, int window, int sinks, float scale,
+                              int dtype, unsigned flags, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

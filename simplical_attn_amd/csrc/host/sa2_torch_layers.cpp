@@ -28,6 +28,8 @@ decltype(&sa2_window_bwd_workspace_bytes) window_ws_fn = nullptr;
 decltype(&sa2_window_backward) window_bwd_fn = nullptr;
 decltype(&sa2_tree_workspace_bytes) tree_ws_fn = nullptr;
 decltype(&sa2_tree_attention) tree_fn = nullptr;
+decltype(&sa2_window_tree_workspace_bytes) window_tree_ws_fn = nullptr;
+decltype(&sa2_window_tree_attention) window_tree_fn = nullptr;
 
 // ---- checks ----------------------------------------------------------------------------------------------------------
 // The first tensor of a call: [batch, rows, heads, head_dim], or packed [rows, heads, head_dim]
@@ -205,6 +207,18 @@ CacheView check_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor
     TORCH_CHECK_VALUE(!table || (table->size(0) == sequences && table->size(1) >= 1), "page_table ", table ? table->sizes() : at::IntArrayRef(), " must be [", sequences, ", pages of a sequence]");
     if (!table) TORCH_CHECK_VALUE(k_cache.size(0) == sequences, "without a page_table the cache is [sequences, capacity, heads, head_dim]: got ", k_cache.size(0), " pieces for ", sequences, " sequences");
     return {k_cache, v_cache, lengths.contiguous(), dense(table), (int)k_cache.size(1), (int)k_cache.size(0), table ? (int)table->size(1) : 1};
+}
+
+// The weights that the rows of a cache have gathered, of `heads` heads each: changed in place where `written`
+void check_weights(const Tensor& t, const CacheView& c, int64_t heads, bool written) {
+    const int64_t capacity = (int64_t)c.page_size * c.width;
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == c.lengths.numel() && t.size(1) == heads && t.size(2) >= capacity, "weights must be float32 [",
+                      c.lengths.numel(), ", ", heads, ", ", capacity, " or more], got ", t.scalar_type(), " ", t.sizes());
+    TORCH_CHECK_VALUE(t.device() == c.k.device(), "weights must be on the device of the other tensors");
+    TORCH_CHECK_VALUE(strided(t), "weights need unit stride along the places and positive strides");
+    if (!written) return;
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "weights are added to in place and have no gradient: call it under torch.no_grad() or on detached tensors");
+    TORCH_CHECK(c10::InferenceMode::is_enabled() || !t.is_inference(), "weights are changed in place, which inference tensors allow in inference mode only");
 }
 
 // Whether the memory from a tensor's first element to its last meets the other's
@@ -411,7 +425,7 @@ std::tuple<Maybe, Maybe, Maybe> causal_backward(const Tensor& q, const Tensor& k
 
 // ---- drafted trees -----------------------------------------------------------------------------------------------------
 Tensor tree(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Maybe& parents, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths, const Maybe& table,
-            std::optional<double> scale, unsigned flags) {
+            std::optional<double> scale, unsigned flags, std::optional<int64_t> window, int64_t sinks, const Maybe& weights) {
     TORCH_CHECK_VALUE(q_.dim() == 4, "q: expected [batch, nodes, heads, head_dim], got ", q_.sizes());
     check_first(q_, "q");
     check_beside(k_, "k", q_, "q");
@@ -425,6 +439,12 @@ Tensor tree(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Maybe& p
     const CacheView c = check_cache(k_cache, v_cache, lengths, table, k_, q_.size(0));
     TORCH_CHECK(!(at::GradMode::is_enabled() && (q_.requires_grad() || k_.requires_grad() || v_.requires_grad() || k_cache.requires_grad() || v_cache.requires_grad())),
                 "tree_attention has no gradient: call it under torch.no_grad() or on detached tensors");
+    const auto [reach, first] = check_window(window, sinks);
+    if (weights) {
+        TORCH_CHECK_VALUE(q_.size(1) == 1, "weights are gathered from single tokens: a tree has ", q_.size(1), " nodes");
+        check_weights(*weights, c, k_.size(2), true);
+        check_place("tree_attention", {*weights});
+    }
     check_place("tree_attention", {q_, k_, v_, k_cache, v_cache});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
@@ -435,21 +455,35 @@ Tensor tree(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Maybe& p
     if (out.numel() == 0) return out;
     const Sizes z = sizes(q);
     const int hk = (int)k.size(2);
-    const size_t bytes = tree_ws_fn(z.B, z.N, z.H, hk, z.D, c.page_size, c.width, dtype_code(q), flags);
+    const bool banded = reach > 0 || weights;
+    const size_t bytes = banded ? window_tree_ws_fn(z.B, z.N, z.H, hk, z.D, c.page_size, c.width, reach, first, weights.has_value(), dtype_code(q), flags)
+                                : tree_ws_fn(z.B, z.N, z.H, hk, z.D, c.page_size, c.width, dtype_code(q), flags);
     const Tensor ws = bytes ? workspace(q, bytes) : Tensor();
-    int64_t s[18];
+    int64_t s[20] = {};
     const Tensor* const t[6] = {&q, &k, &v, &c.k, &c.v, &out};
     for (int i = 0; i < 6; ++i) put_strides(s + 3 * i, *t[i]);
-    check(tree_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), c.k.const_data_ptr(), c.v.const_data_ptr(), out.data_ptr(), ints(up), ints(c.lengths), ints(c.table),
-                  bytes ? ws.data_ptr() : nullptr, bytes, z.B, z.N, z.H, hk, z.D, c.page_size, c.pages, c.width, s, (float)(scale ? *scale : 1.0 / std::sqrt((double)z.D)), dtype_code(q),
-                  flags, stream(q)));
+    void* const space = bytes ? ws.data_ptr() : nullptr;
+    const float factor = (float)(scale ? *scale : 1.0 / std::sqrt((double)z.D));
+    if (banded) {
+        if (weights) {
+            s[18] = weights->stride(0);
+            s[19] = weights->stride(1);
+        }
+        check(window_tree_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), c.k.const_data_ptr(), c.v.const_data_ptr(), out.data_ptr(), weights ? (float*)weights->data_ptr() : nullptr, ints(up),
+                             ints(c.lengths), ints(c.table), space, bytes, z.B, z.N, z.H, hk, z.D, c.page_size, c.pages, c.width, s, reach, first, factor, dtype_code(q), flags, stream(q)));
+        if (weights) torch::autograd::impl::bump_version(*weights);
+    } else {
+        check(tree_fn(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), c.k.const_data_ptr(), c.v.const_data_ptr(), out.data_ptr(), ints(up), ints(c.lengths), ints(c.table), space, bytes,
+                      z.B, z.N, z.H, hk, z.D, c.page_size, c.pages, c.width, s, factor, dtype_code(q), flags, stream(q)));
+    }
     return out;
 }
 
 }  // namespace
 
 void define_layers(py::module_& m) {
-    m.def("bind_layers", [](uintptr_t rotary, uintptr_t append, uintptr_t causal_fwd, uintptr_t causal_ws, uintptr_t causal_bwd, uintptr_t tree_ws, uintptr_t tree, uintptr_t window_fwd, uintptr_t window_ws, uintptr_t window_bwd) {
+    m.def("bind_layers", [](uintptr_t rotary, uintptr_t append, uintptr_t causal_fwd, uintptr_t causal_ws, uintptr_t causal_bwd, uintptr_t tree_ws, uintptr_t tree, uintptr_t window_fwd, uintptr_t window_ws, uintptr_t window_bwd,
+                             uintptr_t window_tree_ws, uintptr_t window_tree) {
         rotary_fn = (decltype(rotary_fn))rotary;
         append_fn = (decltype(append_fn))append;
         causal_fwd_fn = (decltype(causal_fwd_fn))causal_fwd;
@@ -460,6 +494,8 @@ void define_layers(py::module_& m) {
         window_fwd_fn = (decltype(window_fwd_fn))window_fwd;
         window_ws_fn = (decltype(window_ws_fn))window_ws;
         window_bwd_fn = (decltype(window_bwd_fn))window_bwd;
+        window_tree_ws_fn = (decltype(window_tree_ws_fn))window_tree_ws;
+        window_tree_fn = (decltype(window_tree_fn))window_tree;
     });
     m.def("rotary", &rotary);
     m.def("cache_append", &append);

@@ -59,10 +59,10 @@ int check_tree(int B, int T, int H, int HK, int D, int dtype) {
 }
 // Workgroups that share a sequence's keys: as many as are on the chip at once, one per CU, each with at least four tiles of 32
 // keys (one per wavefront; eight where the wavefronts share them) of what a sequence may hold, at most 64 (how many it does hold is known on the device only)
-int tree_splits(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype) {
-    const int64_t keys = (int64_t)B * HK * page_size * table_width;
+int tree_splits(int B, int T, int H, int HK, int D, int page_size, int table_width, int window, int sinks, int dtype) {
+    const int64_t reach = tree_reach((int64_t)page_size * table_width, T, window, sinks), keys = (int64_t)B * HK * reach;
     const int rows = T * (H / HK), block = dtype == SA2_F32 ? 32 : tree16_rows(rows, keys), least = block > 64 ? 8 : 4;
-    const int64_t streams = (int64_t)B * HK * ((rows + block - 1) / block), tiles = ((int64_t)page_size * table_width + 31) / 32;
+    const int64_t streams = (int64_t)B * HK * ((rows + block - 1) / block), tiles = (reach + 31) / 32;
     int64_t n = CUS / streams;
     if (n > tiles / least) n = tiles / least;
     return n < 1 ? 1 : n > 64 ? 64 : (int)n;
@@ -138,6 +138,74 @@ int prompt_backward(const void* q, const void* k, const void* v, const void* out
         return launch_causal16_bwd(p, dtype, terms, st);
     }
     return launch_causal_f32_bwd(p, dtype, st);
+}
+
+// Tiles of 32 scores that a row of query leaves at most, its own node's among them
+int64_t tree_span(int T, int page_size, int table_width, int window, int sinks) {
+    const int64_t all = ((int64_t)page_size * table_width + 31) / 32, seen = ((int64_t)window + sinks) / 32 + 4;
+    return 32 * ((window && seen < all ? seen : all) + 1);
+}
+// A window that every cached row is in is none
+int tree_window_of(int T, int page_size, int table_width, int window) { return window >= (int64_t)page_size * table_width + T ? 0 : window; }
+size_t tree_parts(int B, int T, int H, int D, int nsplit, bool weighted) { return (tree_part_bytes(B, T, H, D, nsplit, weighted) + 255) / 256 * 256; }
+
+size_t tree_workspace(int B, int T, int H, int HK, int D, int page_size, int table_width, int window, int sinks, bool weighted, int dtype) {
+    if (check_tree(B, T, H, HK, D, dtype) != SA2_OK || page_size < 1 || table_width < 1 || window < 0 || sinks < 0 || (weighted && T != 1)) return 0;
+    window = tree_window_of(T, page_size, table_width, window);
+    const int nsplit = tree_splits(B, T, H, HK, D, page_size, table_width, window, sinks, dtype);
+    if (!weighted) return tree_part_bytes(B, T, H, D, nsplit);
+    return tree_parts(B, T, H, D, nsplit, true) + (size_t)B * H * tree_span(T, page_size, table_width, window, sinks) * sizeof(float);
+}
+
+// window 0: none; weights: wanted or nullptr, with their strides behind those of the tensors
+int tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out, float* weights,
+                   const int32_t* parents, const int32_t* lengths, const int32_t* page_table,
+                   void* workspace, size_t workspace_bytes, int B, int T, int H, int HK, int D,
+                   int page_size, int pages, int table_width, const int64_t* strides, int window, int sinks, float scale,
+                   int dtype, unsigned flags, void* hip_stream) {
+    if (!q || !k || !v || !k_cache || !v_cache || !out || !lengths || !strides) return SA2_ERR_NULL_POINTER;
+    const int rc = check_tree(B, T, H, HK, D, dtype);
+    if (rc != SA2_OK) return rc;
+    if (weights && T != 1) return SA2_ERR_BAD_TREE;
+    if (page_size < 1 || pages < 1 || table_width < 1 || (!page_table && (pages < B || table_width != 1)) || (int64_t)page_size * table_width > 0x7fffffff - 64)
+        return SA2_ERR_BAD_CACHE;
+    window = tree_window_of(T, page_size, table_width, window);
+    Tree p;
+    memset(&p, 0, sizeof(p));
+    p.B = B; p.T = T; p.H = H; p.HK = HK; p.G = H / HK; p.D = D;
+    p.scale = scale;
+    p.q = tensor(q, strides, 0);
+    p.k = tensor(k, strides, 1);
+    p.v = tensor(v, strides, 2);
+    p.cache = Cache{tensor(k_cache, strides, 3), tensor(v_cache, strides, 4), page_table, lengths, page_size, pages, table_width};
+    p.out = tensor(out, strides, 5);
+    if (!stride_ok(p.q, B, T, H) || !stride_ok(p.out, B, T, H) || !stride_ok(p.k, B, T, HK) || !stride_ok(p.v, B, T, HK) ||
+        !stride_ok(p.cache.k, pages, page_size, HK) || !stride_ok(p.cache.v, pages, page_size, HK))
+        return SA2_ERR_BAD_STRIDE;
+    p.parents = parents;
+    p.nsplit = tree_splits(B, T, H, HK, D, page_size, table_width, window, sinks, dtype);
+    p.part = (float*)workspace;
+    const bool banded = window > 0 || weights;
+    const size_t need = tree_workspace(B, T, H, HK, D, page_size, table_width, window, sinks, weights != nullptr, dtype);
+    if (need && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < need)) return SA2_ERR_WORKSPACE_TOO_SMALL;
+    if (banded) {
+        p.window = window > 0 ? window : 0x7fffffff;
+        p.sinks = window > 0 ? sinks : 0;
+    }
+    if (weights) {
+        p.weights = weights;
+        p.weights_sb = strides[18];
+        p.weights_sh = strides[19];
+        if ((B > 1 && p.weights_sb < 1) || (HK > 1 && p.weights_sh < 1)) return SA2_ERR_BAD_STRIDE;
+        p.scores = (float*)((char*)workspace + tree_parts(B, T, H, D, p.nsplit, true));
+        p.span = tree_span(T, page_size, table_width, window, sinks);
+        if ((int64_t)B * HK * ((p.span + 1023) / 1024) > 0x7fffffff) return SA2_ERR_TOO_LARGE;
+    }
+    const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && (banded ? tree16_layout(p, dtype) : tree16_supported(p, dtype));
+    p.dealt = B > 1 && p.nsplit >= 8 && (!narrow || (tree16_rows(p) > 64 && !weights));      // (sa2_tree16.h takes equal shares; 32 sequences at most)
+    const hipStream_t st = (hipStream_t)hip_stream;
+    if (banded) return narrow ? launch_window_tree16(p, dtype, st) : launch_window_tree_f32(p, dtype, st);
+    return narrow ? launch_tree16(p, dtype, st) : launch_tree_f32(p, dtype, st);
 }
 
 }  // namespace
@@ -241,8 +309,10 @@ int sa2_window_backward(const void* q, const void* k, const void* v, const void*
 }
 
 size_t sa2_tree_workspace_bytes(int B, int T, int H, int HK, int D, int page_size, int table_width, int dtype, unsigned flags) {
-    if (check_tree(B, T, H, HK, D, dtype) != SA2_OK || page_size < 1 || table_width < 1) return 0;
-    return tree_part_bytes(B, T, H, D, tree_splits(B, T, H, HK, D, page_size, table_width, dtype));
+    return tree_workspace(B, T, H, HK, D, page_size, table_width, 0, 0, false, dtype);
+}
+size_t sa2_window_tree_workspace_bytes(int B, int T, int H, int HK, int D, int page_size, int table_width, int window, int sinks, int weighted, int dtype, unsigned flags) {
+    return tree_workspace(B, T, H, HK, D, page_size, table_width, window, sinks, weighted != 0, dtype);
 }
 
 int sa2_tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out,
@@ -250,32 +320,17 @@ int sa2_tree_attention(const void* q, const void* k, const void* v, const void* 
                        void* workspace, size_t workspace_bytes, int B, int T, int H, int HK, int D,
                        int page_size, int pages, int table_width, const int64_t* strides, float scale,
                        int dtype, unsigned flags, void* hip_stream) {
-    if (!q || !k || !v || !k_cache || !v_cache || !out || !lengths || !strides) return SA2_ERR_NULL_POINTER;
-    const int rc = check_tree(B, T, H, HK, D, dtype);
-    if (rc != SA2_OK) return rc;
-    if (page_size < 1 || pages < 1 || table_width < 1 || (!page_table && (pages < B || table_width != 1)) || (int64_t)page_size * table_width > 0x7fffffff - 64)
-        return SA2_ERR_BAD_CACHE;
-    Tree p;
-    memset(&p, 0, sizeof(p));
-    p.B = B; p.T = T; p.H = H; p.HK = HK; p.G = H / HK; p.D = D;
-    p.scale = scale;
-    p.q = tensor(q, strides, 0);
-    p.k = tensor(k, strides, 1);
-    p.v = tensor(v, strides, 2);
-    p.cache = Cache{tensor(k_cache, strides, 3), tensor(v_cache, strides, 4), page_table, lengths, page_size, pages, table_width};
-    p.out = tensor(out, strides, 5);
-    if (!stride_ok(p.q, B, T, H) || !stride_ok(p.out, B, T, H) || !stride_ok(p.k, B, T, HK) || !stride_ok(p.v, B, T, HK) ||
-        !stride_ok(p.cache.k, pages, page_size, HK) || !stride_ok(p.cache.v, pages, page_size, HK))
-        return SA2_ERR_BAD_STRIDE;
-    p.parents = parents;
-    p.nsplit = tree_splits(B, T, H, HK, D, page_size, table_width, dtype);
-    p.part = (float*)workspace;
-    if (p.nsplit > 1 && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < tree_part_bytes(B, T, H, D, p.nsplit)))
-        return SA2_ERR_WORKSPACE_TOO_SMALL;
-    const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && tree16_supported(p, dtype);
-    p.dealt = B > 1 && p.nsplit >= 8 && (!narrow || tree16_rows(p) > 64);      // (sa2_tree16.hip takes equal shares; 32 sequences at most)
-    if (narrow) return launch_tree16(p, dtype, (hipStream_t)hip_stream);
-    return launch_tree_f32(p, dtype, (hipStream_t)hip_stream);
+    return tree_attention(q, k, v, k_cache, v_cache, out, nullptr, parents, lengths, page_table, workspace, workspace_bytes, B, T, H, HK, D, page_size, pages, table_width, strides, 0, 0, scale, dtype,
+                          flags, hip_stream);
+}
+int sa2_window_tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out, float* weights,
+                              const int32_t* parents, const int32_t* lengths, const int32_t* page_table,
+                              void* workspace, size_t workspace_bytes, int B, int T, int H, int HK, int D,
+                              int page_size, int pages, int table_width, const int64_t* strides, int window, int sinks, float scale,
+                              int dtype, unsigned flags, void* hip_stream) {
+    if (window < 0 || sinks < 0) return SA2_ERR_BAD_WINDOW;
+    return tree_attention(q, k, v, k_cache, v_cache, out, weights, parents, lengths, page_table, workspace, workspace_bytes, B, T, H, HK, D, page_size, pages, table_width, strides, window, sinks,
+                          scale, dtype, flags, hip_stream);
 }
 
 }  // extern "C"

@@ -82,10 +82,16 @@ struct Tree {
     float* part;
     int nsplit;
     bool dealt;                                // shares by the sequences' lengths
+    // Kernels with BAND only.  A node sees of the cached rows and of its ancestors the last `window` up to itself, and the first `sinks`
+    // ones; where `weights` are wanted (trees of one node), the scores of all rows go to `scores`, [B][HK][R][span] by the numbers
+    // that the sweep gives the rows, and a second launch adds what they weigh to weights[b, hk, place].
+    int window, sinks;
+    float *weights, *scores;
+    int64_t weights_sb, weights_sh, span;
 };
 __host__ __device__ constexpr int tree_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-inline size_t tree_part_bytes(int B, int T, int H, int D, int nsplit) {
-    return nsplit > 1 ? (size_t)nsplit * B * T * H * (tree_width(D) + 2) * sizeof(float) : 0;
+inline size_t tree_part_bytes(int B, int T, int H, int D, int nsplit, bool always = false) {
+    return nsplit > 1 || always ? (size_t)nsplit * B * T * H * (tree_width(D) + 2) * sizeof(float) : 0;
 }
 
 int launch_rotary(const Rotary& p, int dtype, hipStream_t st);
@@ -118,15 +124,24 @@ int causal16_splits(int B, int N, int HK, int G);
 size_t causal16_part_bytes(int B, int N, int HK, int G, int D);
 int launch_causal16_bwd(const Causal& p, int dtype, const Causal16Terms& terms, hipStream_t st);
 int launch_causal16_dq(const Causal& p, int dtype, const Causal16Terms& terms, hipStream_t st);
+// rows of the cache that a sequence's nodes see at most
+inline int64_t tree_reach(int64_t capacity, int T, int window, int sinks) {
+    const int64_t reach = (int64_t)window + sinks + T;
+    return window && reach < capacity ? reach : capacity;
+}
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
+int launch_window_tree_f32(const Tree& p, int dtype, hipStream_t st);
+int launch_window_tree16(const Tree& p, int dtype, hipStream_t st);
+int launch_window_tree_rows16(const Tree& p, int dtype, hipStream_t st);
 // 16-bit kernels: rows that a workgroup has of R; up to 64 its wavefronts share them and divide the keys, beyond it is the other
 // way round (16/4 heads, 4 x 65536 cached rows, head_dim 128, 192 rows: 398 us dividing keys, 161 dividing rows).  From 33 to 64
 // it is the other way round too where a CU has 1024 keys or more (64 rows of head_dim 128: 4 x 65536 rows 148 us and 98, 32 x 2048
 // 63 and 54; 8 x 2048 26.5 and 27.6, 512 rows 19 and 23).  `keys`: those that the cache may hold, of all sequences and key heads.
 inline int tree16_rows(int R, int64_t keys) { return R <= 32 ? 32 : R <= 64 && keys < 1024 * CUS ? 64 : R <= 128 ? 128 : 256; }
-inline int tree16_rows(const Tree& p) { return tree16_rows(p.T * p.G, (int64_t)p.B * p.HK * p.cache.page_size * p.cache.width); }
+inline int tree16_rows(const Tree& p) { return tree16_rows(p.T * p.G, (int64_t)p.B * p.HK * tree_reach((int64_t)p.cache.page_size * p.cache.width, p.T, p.window, p.sinks)); }
 constexpr int TREE16_ENTRIES = 4096;                       // of the page table that a workgroup keeps in LDS
 int launch_tree_rows16(const Tree& p, int dtype, hipStream_t st);
+bool tree16_layout(const Tree& p, int dtype);
 bool tree16_supported(const Tree& p, int dtype);
 int launch_tree16(const Tree& p, int dtype, hipStream_t st);
 

@@ -36,6 +36,51 @@ __device__ __forceinline__ int tree_held(const Tree& p, int b) {
     const int n = p.cache.lengths[b];
     return n < 0 ? 0 : n > room ? (int)room : n;
 }
+// The cached rows that the nodes of a sequence see any of, in tiles of SIZE that the sweep numbers: first those that all nodes see whole,
+// the last rows behind them, then with a band those at the window's start (two or three), then the first rows'.
+template <bool BAND, int SIZE>
+struct TreeRows {
+    int held, whole, edge, near, cached;                    // whole, edge: the first tile that all nodes see, that any node sees
+    __device__ __forceinline__ TreeRows(const Tree& p, int b) {
+        held = tree_held(p, b);
+        near = cached = (held + SIZE - 1) / SIZE;
+        whole = edge = 0;
+        if constexpr (BAND) {
+            // node depths are 0 .. T - 1: rows from held + depth - window + 1 on
+            const int64_t low = (int64_t)held - p.window + 1, high = low + p.T - 1;
+            edge = low > 0 ? (int)(low / SIZE) : 0;
+            whole = high > 0 ? (int)((high + SIZE - 1) / SIZE) : 0;
+            whole = whole < near ? whole : near;
+            edge = edge < whole ? edge : whole;
+            const int first = (p.sinks - 1) / SIZE + (p.sinks > 0), head = first < edge ? first : edge;
+            near -= whole;
+            cached = near + whole - edge + head;
+        }
+    }
+    // the first row of tile t
+    __device__ __forceinline__ int row(int t) const {
+        if (!BAND || t < near) return (whole + t) * SIZE;
+        return (t - near < whole - edge ? edge + t - near : t - near - (whole - edge)) * SIZE;
+    }
+};
+// What a node at place `at` sees of the rows r0 .. r0+31
+__device__ __forceinline__ uint32_t tree_window(const Tree& p, int64_t at, int r0) {
+    const int64_t low = at - p.window + 1 - r0;
+    return (low <= 0 ? ~0u : ~bits_below(low < 32 ? (int)low : 32)) | bits_below(p.sinks - r0);
+}
+// Bits of tree_ancestors that are in the window of the lane's node, which is the last of them; a chain's nodes stand in the order of
+// their depths
+__device__ __forceinline__ uint64_t tree_banded(const Tree& p, int held, uint64_t ancestors) {
+    const int depth = __popcll(ancestors) - 1, drop = depth - p.window + 1, keep = p.sinks - held;
+    if (!__any(drop > 0)) return ancestors;
+    uint64_t left = ancestors, out = ancestors;
+    for (int k = 0; k < drop; ++k) {
+        const uint64_t lowest = left & (0 - left);
+        left ^= lowest;
+        if (k >= keep) out ^= lowest;
+    }
+    return out;
+}
 // Page and place of cached row r; false where the table names no page of the cache
 __device__ __forceinline__ bool tree_place(const Cache& c, int b, int r, int& page, int& at) {
     if (!c.table) {
@@ -62,7 +107,8 @@ struct TreeShare {
 template <class F>
 __device__ __forceinline__ bool tree_deal(const Tree& p, F&& is, TreeShare& s) {
     const int lane = threadIdx.x & 63;
-    const double keys = lane < p.B ? (double)tree_held(p, lane) + p.T : 0.0;
+    double keys = lane < p.B ? (double)tree_held(p, lane) + p.T : 0.0;
+    if (p.window) keys = fmin(keys, (double)p.window + p.sinks + p.T);
     double total = keys;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
@@ -116,5 +162,6 @@ __device__ __forceinline__ float* tree_values(const Tree& p, int unit, int hk, i
 }  // namespace
 
 int launch_tree_join(const Tree& p, int dtype, hipStream_t st);
+int launch_tree_weights(const Tree& p, int dtype, float lift, hipStream_t st);
 
 }  // namespace sa2

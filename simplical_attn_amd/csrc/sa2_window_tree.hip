@@ -1,0 +1,60 @@
+// Launches of attention of drafted tokens with a window, or with the cached rows' weights, with fp32 products; and the kernel that adds
+// up weights.
+#include "sa2_tree_f32.h"
+
+namespace sa2 {
+namespace {
+
+// weights[b, hk, place of row] += sum over the G query heads of e^(score - lse), from the scores that the sweep left and the reference
+// points and sums of its shares.  A workgroup has 1024 rows; every wavefront joins the shares for itself.
+// `lift`: sums are 2^lift times as large as their reference points say
+__global__ __launch_bounds__(256) void tree_weights_kernel(Tree p, float lift) {
+    constexpr int EACH = 4;
+    const int64_t per = (p.span + 256 * EACH - 1) / (256 * EACH), stream = blockIdx.x / per;
+    const int hk = (int)(stream % p.HK), b = (int)(stream / p.HK), lane = threadIdx.x & 63;
+    const TreeRows<true, 32> cache(p, b);
+    const int64_t first = (blockIdx.x - stream * per) * 256 * EACH, number = first + threadIdx.x * EACH;
+    const int tile = (int)(number / 32), rows = cache.cached * 32;
+    if (first > rows) return;                               // (the tile behind the cached ones has the node itself)
+    TreeShare share;
+    tree_shares_of(p, b, share);
+    const float c = fabsf(p.scale) * LOG2E;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < p.G; ++r) {
+        const TreePart s = lane < share.count ? *tree_stat(p, share.first + lane, hk, r) : TreePart{-INFINITY, 0.f};
+        const float top = wave_max(s.top), f = s.sum == 0.f ? 0.f : s.top == -INFINITY ? 1.f : exp2f((s.top - top) * c), total = wave_sum(f * s.sum);
+        if (total == 0.f || number > rows) continue;
+        const float4 x = *(const float4*)(p.scores + (stream * p.G + r) * p.span + number);
+        const float over = 1.f / total, off = lift - (top == -INFINITY ? 0.f : top * c);
+        // (hidden rows and those that are not there have -infinity)
+        auto weight = [&](float y) { return y == -INFINITY ? 0.f : exp2f(fmaf(y, c, off)) * over; };
+        sum.x += weight(x.x); sum.y += weight(x.y); sum.z += weight(x.z); sum.w += weight(x.w);
+    }
+    if (number > rows) return;
+    const int64_t room = p.cache.table ? (int64_t)p.cache.width * p.cache.page_size : p.cache.page_size;
+    const int64_t place = number == rows ? cache.held : cache.row(tile) + number % 32;
+    float* const to = p.weights + b * p.weights_sb + hk * p.weights_sh + place;
+    const float* const add = &sum.x;
+    for (int i = 0; i < EACH; ++i) {
+        if (number == rows ? i > 0 || place >= room : place + i >= cache.held) break;
+        to[i] += add[i];
+    }
+}
+
+}  // namespace
+
+int launch_tree_weights(const Tree& p, int dtype, float lift, hipStream_t st) {
+    const int64_t grid = (int64_t)p.B * p.HK * ((p.span + 1023) / 1024);
+    if (grid > 0x7fffffff) return SA2_ERR_TOO_LARGE;
+    tree_weights_kernel<<<dim3((unsigned)grid), dim3(256), 0, st>>>(p, lift);
+    return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
+}
+
+int launch_window_tree_f32(const Tree& p, int dtype, hipStream_t st) {
+    const int rc = launch_tree_f32_of<true>(p, dtype, st);
+    if (rc != SA2_OK || (p.nsplit == 1 && !p.scores)) return rc;
+    const int joined = launch_tree_join(p, dtype, st);
+    return joined == SA2_OK && p.scores ? launch_tree_weights(p, dtype, 0.f, st) : joined;
+}
+
+}  // namespace sa2

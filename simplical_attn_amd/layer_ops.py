@@ -123,9 +123,10 @@ def causal_attention_backward(q, k, v, out, lse, dout, cu_seqlens=None, scale=No
     return _lib.host().causal_backward(q, k, v, out, lse, dout, cu_seqlens, scale, mask, int(flags), out_low, window, sinks)
 
 
-def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None, scale=None, flags=_lib.FLAG_AUTO):
+def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None, scale=None, flags=_lib.FLAG_AUTO, window=None,
+                   sinks=0, weights=None):
     """Attention of drafted tokens over a cache: node i of a sequence attends to the ``lengths`` rows that the cache holds, to
-    itself and to its ancestors in the draft.  One node is a decoding step.
+    itself and to its ancestors in the draft, or of these to the last ``window`` and the first ``sinks``.  One node is a decoding step.
 
     q                 [batch, nodes, heads, head_dim], 1 to 64 nodes
     k, v              [batch, nodes, key heads, head_dim]: the drafted tokens' own, not yet in the cache
@@ -135,7 +136,12 @@ def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None,
     k_cache, v_cache, lengths, page_table   as at cache_append, which brings the accepted nodes into the cache
     scale             1 / sqrt(head_dim) if None
     flags             _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products whatever the type
+    window, sinks     as at causal_attention: a node's place is lengths plus the number of its ancestors, a cached row's is where it
+                      stands.  Rows out of the window are not read
+    weights           float32 [batch, key heads, places], at least a place for each row that the cache may hold; single tokens only.
+                      The softmax weight of each cached row, summed over the query heads that share its head, is added at the row's
+                      place, the token's own at place ``lengths`` (where cache_append will put it): what cache_evict goes by
 
     No gradients.  Returns a tensor like q.  bf16 and fp16 with a head_dim up to 128 that is a multiple of 8 and rows on the 16-byte
     grid run on the 16-bit matrix pipes (softmax weights rounded to the type, sums in fp32), everything else with fp32 products."""
-    return _lib.host().tree(q, k, v, parents, k_cache, v_cache, lengths, page_table, scale, int(flags))
+    return _lib.host().tree(q, k, v, parents, k_cache, v_cache, lengths, page_table, scale, int(flags), window, sinks, weights)

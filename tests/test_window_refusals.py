@@ -63,3 +63,46 @@ def test_c_entries_of_prompts(lib):
 
     assert backward(window=0) == backward(sinks=-2) == -5
     assert backward(workspace=None) == -1 and backward(nbytes=8) == -6
+
+
+def _tree(q=(2, 1, 4, 8), k=(2, 1, 2, 8), cache=(6, 16, 2, 8), **kw):
+    return sa.tree_attention(t(*q), t(*k), t(*k), None, t(*cache), t(*cache), ints(3, 4), ints(*range(6)).view(2, 3), **kw)
+
+
+@pytest.mark.parametrize("error,kw", [
+    (ValueError, dict(window=0)), (ValueError, dict(window=2, sinks=-1)), (ValueError, dict(sinks=1)),
+    (ValueError, dict(weights=t(2, 2, 47))), (ValueError, dict(weights=t(2, 4, 48))), (ValueError, dict(weights=t(1, 2, 48))), (ValueError, dict(weights=t(2, 48))),
+    (ValueError, dict(weights=t(2, 2, 48, dtype=torch.float16))), (ValueError, dict(weights=t(2, 48, 2).transpose(1, 2))),
+    (ValueError, dict(weights=t(1, 1, 1).expand(2, 2, 48))),
+    (ValueError, dict(q=(2, 3, 4, 8), k=(2, 3, 2, 8), weights=t(2, 2, 48))),
+    (RuntimeError, dict(weights=t(2, 2, 48).requires_grad_(True))),
+    (RuntimeError, dict(weights=t(2, 2, 48))), (RuntimeError, dict(window=5))])
+def test_trees(lib, error, kw):
+    with pytest.raises(error):
+        _tree(**kw)
+
+
+def test_inference_tensors_gather_no_weights_outside_of_inference_mode(lib):
+    with torch.inference_mode():
+        weights = t(2, 2, 48)
+    with pytest.raises(RuntimeError, match="inference"):
+        _tree(weights=weights)
+
+
+def test_c_entries_of_trees(lib):
+    s = _lib.stride_array([(4096, 64, 8)] * 6 + [(128, 64, 0)])
+
+    def tree(window=4, sinks=1, weights=None, T=1, workspace=ONE, nbytes=1 << 30, strides=s):
+        return lib.sa2_window_tree_attention(ONE, ONE, ONE, ONE, ONE, ONE, weights, None, ONE, None, workspace, nbytes, 2, T, 4, 2, 8, 4096, 4, 1, strides, window, sinks, 1.0, 0, 0, None)
+
+    assert tree(window=-1) == tree(sinks=-1) == -5
+    assert tree(weights=ONE, T=2) == -14 and tree(T=65) == -14
+    assert tree(weights=ONE, nbytes=100) == tree(weights=ONE, workspace=None) == -6
+    assert tree(weights=ONE, strides=_lib.stride_array([(4096, 64, 8)] * 6 + [(0, 64, 0)])) == -4
+
+    def size(window=0, sinks=0, weighted=0, T=1, width=64):
+        return lib.sa2_window_tree_workspace_bytes(2, T, 4, 2, 64, 64, width, window, sinks, weighted, 1, 0)
+
+    assert size(window=-1) == size(weighted=1, T=2) == 0
+    assert size() == lib.sa2_tree_workspace_bytes(2, 1, 4, 2, 64, 64, 64, 1, 0)
+    assert size(window=200) < size() < size(weighted=1) and size(window=200, weighted=1) < size(weighted=1)

@@ -46,7 +46,8 @@ typedef enum sa2_status {
     SA2_ERR_BAD_HEADS = -11,     /* query heads are not a multiple of the heads of keys and values */
     SA2_ERR_BAD_ROTARY = -12,    /* rotary_dim is odd, < 2 or > D, or positions are neither 4 nor 8 bytes */
     SA2_ERR_BAD_CACHE = -13,     /* page size, page count or table width < 1, or (trees) page size times width >= 2^31 - 64 */
-    SA2_ERR_BAD_TREE = -14       /* a tree of fewer than 1 or more than SA2_TREE_NODES nodes */
+    SA2_ERR_BAD_TREE = -14,      /* a tree of fewer than 1 or more than SA2_TREE_NODES nodes; weights from trees of several nodes */
+    SA2_ERR_BAD_EVICTION = -15   /* keep < 1, first or recent < 0, first + recent > keep, or fewer places than the cache has rows */
 } sa2_status;
 
 typedef enum sa2_dtype { SA2_F32 = 0, SA2_BF16 = 1, SA2_F16 = 2 } sa2_dtype;
@@ -293,6 +294,36 @@ int sa2_window_tree_attention(const void* q, const void* k, const void* v, const
                               void* workspace, size_t workspace_bytes, int B, int T, int H, int HK, int D,
                               int page_size, int pages, int table_width, const int64_t* strides, int window, int sinks, float scale,
                               int dtype, unsigned flags, void* hip_stream);
+
+/*
+ * What each key of a prompt got: w_j = sum over the query heads that share its head and the queries i that see it (as at
+ * sa2_window_forward; window 0: all from its own on) of e^(scale q_i k_j - lse_i).
+ *   lse          as the forward left it
+ *   lengths      NULL: weights [B,HK,N] (packed: [HK,N], zero for rows of no sequence) are overwritten.  Else weights
+ *                [sequences,HK,places], and key a of sequence b is added at place lengths[b] + a, where that is below `places`
+ *   strides      q, k (3 int64 each), then weights' batch (or sequence) and head
+ *   workspace    sa2_key_weights_workspace_bytes(...) bytes, 256-byte aligned (0 bytes: may be NULL); contents on entry ignored
+ * No atomics: two calls on the same inputs give identical bits.
+ */
+size_t sa2_key_weights_workspace_bytes(int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags);
+int sa2_key_weights(const void* q, const void* k, const float* lse, float* weights, const int32_t* lengths, int64_t places, void* workspace, size_t workspace_bytes,
+                    const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D, const int64_t* strides, int window, int sinks, float scale,
+                    int dtype, unsigned flags, void* hip_stream);
+
+/*
+ * Eviction: of the lengths[b] rows of each sequence (clamped to the capacity) and key head, `keep` stay: the first `first`, the last
+ * `recent` and of the others those of the largest weights (of equal ones the first; NaN is below all numbers).  They keep their order
+ * and move to the places 0 .. keep-1, in place.  Sequences of no more than `keep` rows are left as they are.  lengths are not changed.
+ *   weights      [B,heads,places] fp32, places >= page_size * table_width; heads HK, or 1: one choice for all heads
+ *   left         [B,heads,places] contiguous: the weights of the rows that stay, at their new places, zeros behind
+ *   kept         [B,heads,keep] contiguous: the places that the rows had, ascending, -1 behind them
+ *   strides      k_cache, v_cache (page, row, head), then weights' batch and head
+ * Rows in pages that are not in 0 .. pages-1 are chosen like others; what would come from or go there is left out.  What the places
+ * from keep on hold is as it was.
+ */
+int sa2_cache_evict(void* k_cache, void* v_cache, const float* weights, float* left, int32_t* kept, const int32_t* lengths, const int32_t* page_table,
+                    int B, int HK, int heads, int D, int page_size, int pages, int table_width, int64_t places, int keep, int first, int recent,
+                    const int64_t* strides, int dtype, void* hip_stream);
 
 #ifdef __cplusplus
 }

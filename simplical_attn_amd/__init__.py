@@ -14,9 +14,11 @@ from .simplicial_attn import (  # noqa: F401
 from .compiled_op import two_simplicial_attention  # noqa: F401,E402
 from .layer_ops import (  # noqa: F401,E402
     cache_append,
+    cache_evict,
     causal_attention,
     causal_attention_backward,
     causal_attention_forward,
+    key_weights,
     rotary_embedding,
     rotary_frequencies,
     tree_attention,
@@ -39,6 +41,8 @@ __all__ = [
     "causal_attention_forward",
     "causal_attention_backward",
     "tree_attention",
+    "key_weights",
+    "cache_evict",
 ]
 
 # Names the reference package exports (simplicial/__init__.py:12-27) that have no

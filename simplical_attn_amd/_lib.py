@@ -13,7 +13,8 @@ EXPORTED_SYMBOLS = (
     "sa2_rotary", "sa2_cache_append", "sa2_causal_forward", "sa2_causal_bwd_workspace_bytes", "sa2_causal_backward",
     "sa2_tree_workspace_bytes", "sa2_tree_attention",
     "sa2_window_forward", "sa2_window_bwd_workspace_bytes", "sa2_window_backward",
-    "sa2_window_tree_workspace_bytes", "sa2_window_tree_attention",
+    "sa2_window_tree_workspace_bytes", "sa2_window_tree_attention", "sa2_key_weights_workspace_bytes", "sa2_key_weights",
+    "sa2_cache_evict",
 )
 STATIC_WORKSPACE_BYTES = 64 << 20
 
@@ -93,6 +94,12 @@ def load():
     lib.sa2_window_tree_workspace_bytes.argtypes = [c_int] * 11 + [c_uint]
     lib.sa2_window_tree_attention.restype = c_int
     lib.sa2_window_tree_attention.argtypes = ([c_void_p] * 11 + [c_size_t] + [c_int] * 8 + [i64p, c_int, c_int, c_float, c_int, c_uint, c_void_p])
+    lib.sa2_key_weights_workspace_bytes.restype = c_size_t
+    lib.sa2_key_weights_workspace_bytes.argtypes = [c_int] * 8 + [c_uint]
+    lib.sa2_key_weights.restype = c_int
+    lib.sa2_key_weights.argtypes = ([c_void_p] * 5 + [ctypes.c_int64, c_void_p, c_size_t, c_void_p] + [c_int] * 6 + [i64p, c_int, c_int, c_float, c_int, c_uint, c_void_p])
+    lib.sa2_cache_evict.restype = c_int
+    lib.sa2_cache_evict.argtypes = [c_void_p] * 7 + [c_int] * 7 + [ctypes.c_int64] + [c_int] * 3 + [i64p, c_int, c_void_p]
     _lib = lib
     return lib
 

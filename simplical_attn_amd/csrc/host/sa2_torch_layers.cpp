@@ -30,6 +30,9 @@ decltype(&sa2_tree_workspace_bytes) tree_ws_fn = nullptr;
 decltype(&sa2_tree_attention) tree_fn = nullptr;
 decltype(&sa2_window_tree_workspace_bytes) window_tree_ws_fn = nullptr;
 decltype(&sa2_window_tree_attention) window_tree_fn = nullptr;
+decltype(&sa2_key_weights_workspace_bytes) key_weights_ws_fn = nullptr;
+decltype(&sa2_key_weights) key_weights_fn = nullptr;
+decltype(&sa2_cache_evict) evict_fn = nullptr;
 
 // ---- checks ----------------------------------------------------------------------------------------------------------
 // The first tensor of a call: [batch, rows, heads, head_dim], or packed [rows, heads, head_dim]
@@ -209,6 +212,11 @@ CacheView check_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor
     return {k_cache, v_cache, lengths.contiguous(), dense(table), (int)k_cache.size(1), (int)k_cache.size(0), table ? (int)table->size(1) : 1};
 }
 
+void check_added(const Tensor& t) {
+    TORCH_CHECK_VALUE(strided(t), "weights need unit stride along the places and positive strides: they are added to in place");
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "weights are added to in place and have no gradient: call it under torch.no_grad() or on detached tensors");
+    TORCH_CHECK(c10::InferenceMode::is_enabled() || !t.is_inference(), "weights are changed in place, which inference tensors allow in inference mode only");
+}
 // The weights that the rows of a cache have gathered, of `heads` heads each: changed in place where `written`
 void check_weights(const Tensor& t, const CacheView& c, int64_t heads, bool written) {
     const int64_t capacity = (int64_t)c.page_size * c.width;
@@ -216,9 +224,7 @@ void check_weights(const Tensor& t, const CacheView& c, int64_t heads, bool writ
                       c.lengths.numel(), ", ", heads, ", ", capacity, " or more], got ", t.scalar_type(), " ", t.sizes());
     TORCH_CHECK_VALUE(t.device() == c.k.device(), "weights must be on the device of the other tensors");
     TORCH_CHECK_VALUE(strided(t), "weights need unit stride along the places and positive strides");
-    if (!written) return;
-    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "weights are added to in place and have no gradient: call it under torch.no_grad() or on detached tensors");
-    TORCH_CHECK(c10::InferenceMode::is_enabled() || !t.is_inference(), "weights are changed in place, which inference tensors allow in inference mode only");
+    if (written) check_added(t);
 }
 
 // Whether the memory from a tensor's first element to its last meets the other's
@@ -479,11 +485,95 @@ Tensor tree(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Maybe& p
     return out;
 }
 
+// ---- gathered weights ---------------------------------------------------------------------------------------------------
+Maybe key_weights(const Tensor& q_, const Tensor& k_, const Tensor& lse, const Maybe& cu, std::optional<double> scale, std::optional<int64_t> window, int64_t sinks, const Maybe& weights,
+                  const Maybe& lengths, unsigned flags) {
+    check_first(q_, "q");
+    check_beside(k_, "k", q_, "q");
+    check_heads(q_, k_);
+    TORCH_CHECK_VALUE(q_.size(-1) >= 1 && q_.size(-1) <= 256, "head_dim must be 1 to 256, got ", q_.size(-1));
+    check_cu(cu, q_);
+    TORCH_CHECK_VALUE(q_.dim() == 4 || cu, "packed rows need cu_seqlens");
+    const bool batched = q_.dim() == 4;
+    TORCH_CHECK_VALUE(lse.scalar_type() == at::kFloat && lse.device() == q_.device() && lse.is_contiguous() && lse.dim() == q_.dim() - 1 && lse.size(-1) == q_.size(-3) && lse.size(-2) == q_.size(-2) &&
+                          (!batched || lse.size(0) == q_.size(0)), "lse must be the contiguous float32 tensor that the forward returned, got ", lse.scalar_type(), " ", lse.sizes());
+    const auto [reach, first] = check_window(window, sinks);
+    const int64_t sequences = cu ? cu->numel() - 1 : q_.size(0), hk64 = k_.size(-2);
+    TORCH_CHECK_VALUE(weights.has_value() == lengths.has_value(), "weights and lengths go together");
+    if (weights) {
+        check_ints(lengths, "lengths", q_, 1);
+        TORCH_CHECK_VALUE(lengths->numel() == sequences, "lengths has ", lengths->numel(), " entries for ", sequences, " sequences");
+        TORCH_CHECK_VALUE(weights->scalar_type() == at::kFloat && weights->dim() == 3 && weights->size(0) == sequences && weights->size(1) == hk64 && weights->size(2) >= 1 && weights->device() == q_.device(),
+                          "weights must be float32 [", sequences, ", ", hk64, ", places] on the device of the other tensors, got ", weights->scalar_type(), " ", weights->sizes());
+        check_added(*weights);
+        check_place("key_weights", {*weights});
+    }
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (q_.requires_grad() || k_.requires_grad() || lse.requires_grad())), "key_weights has no gradient: call it under torch.no_grad() or on detached tensors");
+    check_place("key_weights", {q_, k_, lse});
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Unseen unseen("key_weights");
+    const Tensor q = rows(q_), k = rows(k_), ends = dense(cu), held = dense(lengths);
+    const c10::DeviceGuard guard(q.device());
+    const Sizes z = sizes(q);
+    const int hk = (int)hk64;
+    const auto fp32 = q.options().dtype(at::kFloat).requires_grad(false);
+    const Tensor out = weights ? *weights : batched ? at::empty({z.B, hk, z.N}, fp32) : at::empty({hk, z.N}, fp32);
+    const Maybe result = weights ? Maybe() : Maybe(out);
+    if (z.B == 0 || z.N == 0 || hk == 0 || z.H == 0) {
+        if (!weights) out.zero_();                 // (keys that no query head reads)
+        return result;
+    }
+    const size_t bytes = key_weights_ws_fn(z.B, z.N, z.H, hk, z.D, reach, first, dtype_code(q), flags);
+    const Tensor ws = bytes ? workspace(q, bytes) : Tensor();
+    int64_t s[8];
+    put_strides(s, q);
+    put_strides(s + 3, k);
+    s[6] = out.dim() == 3 ? out.stride(0) : 0;
+    s[7] = out.stride(-2);
+    check(key_weights_fn(q.const_data_ptr(), k.const_data_ptr(), (const float*)lse.const_data_ptr(), (float*)out.data_ptr(), ints(held), weights ? weights->size(2) : 0, bytes ? ws.data_ptr() : nullptr, bytes,
+                         ints(ends), ends.defined() ? (int)ends.numel() - 1 : 0, z.B, z.N, z.H, hk, z.D, s, reach, first, (float)(scale ? *scale : 1.0 / std::sqrt((double)z.D)), dtype_code(q), flags,
+                         stream(q)));
+    if (weights) torch::autograd::impl::bump_version(*weights);
+    return result;
+}
+
+std::pair<Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_cache, const Tensor& weights, const Tensor& lengths, int64_t keep, int64_t first, int64_t recent, const Maybe& table) {
+    TORCH_CHECK_VALUE(k_cache.dim() == 4 && k_cache.size(3) >= 1 && k_cache.size(3) <= 256 && k_cache.size(2) >= 1, "k_cache: expected [pages, page_size, heads, head_dim], head_dim 1 to 256, got ", k_cache.sizes());
+    TORCH_CHECK_TYPE(dtype_code(k_cache) >= 0, "k_cache: unsupported dtype ", k_cache.scalar_type(), " (float32, bfloat16, float16)");
+    TORCH_CHECK_VALUE(lengths.dim() == 1, "lengths must be an int32 tensor of 1 dimension, got ", lengths.sizes());
+    const CacheView c = check_cache(k_cache, v_cache, lengths, table, k_cache, lengths.numel());
+    TORCH_CHECK_VALUE((int64_t)c.page_size * c.width <= 0x7fffffff - 64, "a cache of 2^31 - 64 rows per sequence or more");
+    TORCH_CHECK_VALUE(weights.dim() == 3, "weights must be float32 [batch, heads, places], got ", weights.sizes());
+    check_weights(weights, c, weights.size(1) == 1 ? 1 : k_cache.size(2), false);
+    TORCH_CHECK_VALUE(keep >= 1 && first >= 0 && recent >= 0 && keep < ((int64_t)1 << 31) && first + recent <= keep, "keep must be at least 1, first and recent at least 0 and together at most keep, got ", keep, ", ", first, ", ", recent);
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (k_cache.requires_grad() || v_cache.requires_grad() || weights.requires_grad())), "cache_evict has no gradient: call it under torch.no_grad() or on detached tensors");
+    TORCH_CHECK(c10::InferenceMode::is_enabled() || !(k_cache.is_inference() || v_cache.is_inference()), "cache_evict changes the cache in place, which inference tensors allow in inference mode only");
+    check_place("cache_evict", {k_cache, v_cache, weights});
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Unseen unseen("cache_evict");
+    const c10::DeviceGuard guard(k_cache.device());
+    const auto options = weights.options().requires_grad(false);
+    const Tensor kept = at::empty({weights.size(0), weights.size(1), keep}, options.dtype(at::kInt)), left = at::empty(weights.sizes(), options.memory_format(at::MemoryFormat::Contiguous));
+    if (weights.size(0) == 0) return {kept, left};
+    int64_t s[8];
+    put_strides(s, c.k);
+    put_strides(s + 3, c.v);
+    s[6] = weights.stride(0);
+    s[7] = weights.stride(1);
+    check(evict_fn(c.k.data_ptr(), c.v.data_ptr(), (const float*)weights.const_data_ptr(), (float*)left.data_ptr(), kept.data_ptr<int32_t>(), ints(c.lengths), ints(c.table), (int)weights.size(0),
+                   (int)c.k.size(2), (int)weights.size(1), (int)c.k.size(3), c.page_size, c.pages, c.width, weights.size(2), (int)keep, (int)first, (int)recent, s, dtype_code(c.k), stream(c.k)));
+    torch::autograd::impl::bump_version(c.k);
+    torch::autograd::impl::bump_version(c.v);
+    return {kept, left};
+}
+
 }  // namespace
 
 void define_layers(py::module_& m) {
     m.def("bind_layers", [](uintptr_t rotary, uintptr_t append, uintptr_t causal_fwd, uintptr_t causal_ws, uintptr_t causal_bwd, uintptr_t tree_ws, uintptr_t tree, uintptr_t window_fwd, uintptr_t window_ws, uintptr_t window_bwd,
-                             uintptr_t window_tree_ws, uintptr_t window_tree) {
+                             uintptr_t window_tree_ws, uintptr_t window_tree, uintptr_t key_weights_ws, uintptr_t key_weights, uintptr_t evict) {
         rotary_fn = (decltype(rotary_fn))rotary;
         append_fn = (decltype(append_fn))append;
         causal_fwd_fn = (decltype(causal_fwd_fn))causal_fwd;
@@ -496,6 +586,9 @@ void define_layers(py::module_& m) {
         window_bwd_fn = (decltype(window_bwd_fn))window_bwd;
         window_tree_ws_fn = (decltype(window_tree_ws_fn))window_tree_ws;
         window_tree_fn = (decltype(window_tree_fn))window_tree;
+        key_weights_ws_fn = (decltype(key_weights_ws_fn))key_weights_ws;
+        key_weights_fn = (decltype(key_weights_fn))key_weights;
+        evict_fn = (decltype(evict_fn))evict;
     });
     m.def("rotary", &rotary);
     m.def("cache_append", &append);
@@ -503,6 +596,8 @@ void define_layers(py::module_& m) {
     m.def("causal_forward", &causal_forward);
     m.def("causal_backward", &causal_backward);
     m.def("tree", &tree);
+    m.def("key_weights", &key_weights);
+    m.def("cache_evict", &evict);
 }
 
 }  // namespace sa2_host

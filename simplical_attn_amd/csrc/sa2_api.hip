@@ -228,7 +228,7 @@ const char* sa2_strerror(int status) {
         case SA2_ERR_BAD_DTYPE: return "unknown dtype (0 = fp32, 1 = bf16, 2 = fp16)";
         case SA2_ERR_BAD_SHAPE: return "bad shape: B, N, H, D must be >= 1 and D <= 256";
         case SA2_ERR_BAD_STRIDE: return "bad stride: batch/sequence/head strides must be positive (D stride is 1)";
-        case SA2_ERR_BAD_WINDOW: return "bad window: w1 and w2 must be >= 0 (>= 1 for the half-open convention)";
+        case SA2_ERR_BAD_WINDOW: return "bad window: w1 and w2 must be >= 0 (>= 1 for the half-open convention); a window of keys >= 1, first keys >= 0";
         case SA2_ERR_WORKSPACE_TOO_SMALL: return "workspace is smaller than sa2_bwd_workspace_bytes() (forward: sa2_fwd_workspace_bytes()) or not 256-byte aligned";
         case SA2_ERR_LAUNCH_FAILED: return "a HIP kernel launch failed";
         case SA2_ERR_UNSUPPORTED: return "the forced kernel path does not support this shape, dtype or layout";
@@ -239,7 +239,8 @@ const char* sa2_strerror(int status) {
         case SA2_ERR_BAD_ROTARY: return "rotary_dim must be even and in 2 .. D, positions int32 or int64";
         case SA2_ERR_BAD_CACHE: return "a cache needs a page size, a page count and a table width of at least 1, and for tree attention "
                                        "page size times table width below 2^31 - 64";
-        case SA2_ERR_BAD_TREE: return "a drafted tree must have 1 to 64 nodes";
+        case SA2_ERR_BAD_TREE: return "a drafted tree must have 1 to 64 nodes, one where weights are gathered";
+        case SA2_ERR_BAD_EVICTION: return "bad eviction: at least one row must stay, first and recent >= 0 and together at most as many, and weights must have a place for each row of the cache";
     }
     return "unknown sa2 status";
 }

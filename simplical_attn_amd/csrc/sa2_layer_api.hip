@@ -208,6 +208,30 @@ int tree_attention(const void* q, const void* k, const void* v, const void* k_ca
     return narrow ? launch_tree16(p, dtype, st) : launch_tree_f32(p, dtype, st);
 }
 
+// Shares of the streams of blocks of `block` keys in tiles of `tile` queries: about 1024 in all, of 16 tiles at least
+void key_shares(KeySums& p, int block, int tile) {
+    const int64_t longest = p.band.window && p.band.sinks == 0 && p.band.window + block < p.rows.N ? p.band.window + block : p.rows.N;
+    const int64_t blocks = (int64_t)p.rows.B * p.HK * ((p.rows.N + block - 1) / block), tiles = (longest + tile - 1) / tile * p.G, each = (blocks * tiles / 2 + 1023) / 1024;
+    p.chunk = (int)(each < 16 ? 16 : each < tiles ? each : tiles);
+    p.shares = (int)((tiles + p.chunk - 1) / p.chunk);
+}
+size_t key_part_bytes(const KeySums& p) { return p.shares > 1 ? (size_t)p.shares * p.rows.B * p.HK * p.rows.N * sizeof(float) : 0; }
+
+int make_key_sums(KeySums& p, const int32_t* cu, int sequences, int B, int N, int H, int HK, int D, int window, int sinks, float scale, int dtype) {
+    Causal c;
+    int rc = make_causal(c, cu, sequences, B, N, H, HK, D, scale, dtype);
+    if (rc != SA2_OK) return rc;
+    if (window < 0 || sinks < 0) return SA2_ERR_BAD_WINDOW;
+    memset(&p, 0, sizeof(p));
+    p.rows = c.rows;
+    p.H = H; p.HK = HK; p.G = c.G; p.D = D;
+    p.scale = scale;
+    p.band.window = window < N ? window : 0;
+    p.band.sinks = p.band.window ? (sinks < N ? sinks : N) : 0;
+    key_shares(p, 128, 32);
+    return SA2_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -331,6 +355,59 @@ int sa2_window_tree_attention(const void* q, const void* k, const void* v, const
     if (window < 0 || sinks < 0) return SA2_ERR_BAD_WINDOW;
     return tree_attention(q, k, v, k_cache, v_cache, out, weights, parents, lengths, page_table, workspace, workspace_bytes, B, T, H, HK, D, page_size, pages, table_width, strides, window, sinks,
                           scale, dtype, flags, hip_stream);
+}
+
+size_t sa2_key_weights_workspace_bytes(int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags) {
+    KeySums p;
+    return make_key_sums(p, nullptr, 0, B, N, H, HK, D, window, sinks, 1.f, dtype) == SA2_OK ? key_part_bytes(p) : 0;
+}
+int sa2_key_weights(const void* q, const void* k, const float* lse, float* weights, const int32_t* lengths, int64_t places, void* workspace, size_t workspace_bytes,
+                    const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D, const int64_t* strides, int window, int sinks, float scale,
+                    int dtype, unsigned flags, void* hip_stream) {
+    if (!q || !k || !lse || !weights || !strides) return SA2_ERR_NULL_POINTER;
+    KeySums p;
+    const int rc = make_key_sums(p, cu_seqlens, sequences, B, N, H, HK, D, window, sinks, scale, dtype);
+    if (rc != SA2_OK) return rc;
+    p.q = tensor(q, strides, 0);
+    p.k = tensor(k, strides, 1);
+    p.lse = lse;
+    p.out = weights;
+    p.sb = strides[6];
+    p.sh = strides[7];
+    p.lengths = lengths;
+    p.places = places;
+    const int outer = cu_seqlens && lengths ? sequences : B;
+    if (!stride_ok(p.q, B, N, H) || !stride_ok(p.k, B, N, HK) || (outer > 1 && p.sb < 1) || (HK > 1 && p.sh < 1)) return SA2_ERR_BAD_STRIDE;
+    if (lengths && places < 1) return SA2_ERR_BAD_SHAPE;
+    const size_t need = key_part_bytes(p);
+    if (need && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < need)) return SA2_ERR_WORKSPACE_TOO_SMALL;
+    p.part = (float*)workspace;
+    return launch_key_sums_f32(p, dtype, (hipStream_t)hip_stream);
+}
+
+int sa2_cache_evict(void* k_cache, void* v_cache, const float* weights, float* left, int32_t* kept, const int32_t* lengths, const int32_t* page_table,
+                    int B, int HK, int heads, int D, int page_size, int pages, int table_width, int64_t places, int keep, int first, int recent,
+                    const int64_t* strides, int dtype, void* hip_stream) {
+    if (!k_cache || !v_cache || !weights || !left || !kept || !lengths || !strides) return SA2_ERR_NULL_POINTER;
+    if (!valid_dtype(dtype)) return SA2_ERR_BAD_DTYPE;
+    if (B < 1 || HK < 1 || D < 1 || D > 256) return SA2_ERR_BAD_SHAPE;
+    if (heads != HK && heads != 1) return SA2_ERR_BAD_HEADS;
+    if (page_size < 1 || pages < 1 || table_width < 1 || (!page_table && (pages < B || table_width != 1)) || (int64_t)page_size * table_width > 0x7fffffff - 64) return SA2_ERR_BAD_CACHE;
+    if (keep < 1 || first < 0 || recent < 0 || (int64_t)first + recent > keep || places < (int64_t)page_size * table_width) return SA2_ERR_BAD_EVICTION;
+    Evict p;
+    memset(&p, 0, sizeof(p));
+    p.cache = Cache{tensor(k_cache, strides, 0), tensor(v_cache, strides, 1), page_table, lengths, page_size, pages, table_width};
+    if (!stride_ok(p.cache.k, pages, page_size, HK) || !stride_ok(p.cache.v, pages, page_size, HK)) return SA2_ERR_BAD_STRIDE;
+    p.B = B; p.HK = HK; p.heads = heads; p.D = D;
+    p.weights = weights;
+    p.sb = strides[6];
+    p.sh = strides[7];
+    if ((B > 1 && p.sb < 1) || (heads > 1 && p.sh < 1)) return SA2_ERR_BAD_STRIDE;
+    p.places = places;
+    p.left = left;
+    p.kept = kept;
+    p.keep = keep; p.first = first; p.recent = recent;
+    return launch_evict(p, dtype, (hipStream_t)hip_stream);
 }
 
 }  // extern "C"

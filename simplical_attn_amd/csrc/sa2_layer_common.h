@@ -94,6 +94,40 @@ inline size_t tree_part_bytes(int B, int T, int H, int D, int nsplit, bool alway
     return nsplit > 1 || always ? (size_t)nsplit * B * T * H * (tree_width(D) + 2) * sizeof(float) : 0;
 }
 
+// What each key of a prompt got from the queries that see it: sums of e^(scale q k - lse) over them and over the G query heads.  The stream
+// of a block of keys, tiles of queries of one head after the other, is cut into shares of `chunk` tiles, whose sums lie in `part`:
+// [share][B][HK][N].
+struct KeySums {
+    Rows rows;
+    int H, HK, G, D;
+    float scale;
+    Tensor q, k;
+    const float* lse;                          // [B,H,N]
+    Band band;                                 // (window, sinks)
+    float* part;
+    int shares, chunk;
+    // out[b * sb + hk * sh + n]; or with `lengths`, added to place lengths[b] + (n in its sequence b) where that is below `places`
+    float* out;
+    int64_t sb, sh;
+    const int32_t* lengths;
+    int64_t places;
+};
+
+// Rows of a cache that stay: kept[b, head, i] (ascending, -1 behind them) goes to place i.  One choice for each key head, or (heads 1) one for
+// all of them.
+struct Evict {
+    Cache cache;
+    int B, HK, heads, D;
+    const float* weights;                      // [B][heads][..places], strides sb, sh
+    int64_t sb, sh, places;
+    float* left;                               // [B][heads][places]: of the rows that stay, zeros behind
+    int32_t* kept;                             // [B][heads][keep]
+    int keep, first, recent;
+};
+
+int launch_key_sums_f32(const KeySums& p, int dtype, hipStream_t st);
+int launch_key_sums_join(const KeySums& p, int block, int tile, hipStream_t st);
+int launch_evict(const Evict& p, int dtype, hipStream_t st);
 int launch_rotary(const Rotary& p, int dtype, hipStream_t st);
 int launch_append(const Append& p, int dtype, hipStream_t st);
 int launch_causal_f32_fwd(const Causal& p, int dtype, hipStream_t st);

@@ -145,3 +145,31 @@ def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None,
     No gradients.  Returns a tensor like q.  bf16 and fp16 with a head_dim up to 128 that is a multiple of 8 and rows on the 16-byte
     grid run on the 16-bit matrix pipes (softmax weights rounded to the type, sums in fp32), everything else with fp32 products."""
     return _lib.host().tree(q, k, v, parents, k_cache, v_cache, lengths, page_table, scale, int(flags), window, sinks, weights)
+
+
+def key_weights(q, k, lse, cu_seqlens=None, scale=None, window=None, sinks=0, weights=None, lengths=None, flags=_lib.FLAG_AUTO):
+    """The softmax weight that each key of a prompt got, summed over the queries that see it and the query heads that share its head:
+    float32 [batch, key heads, seq_len], or packed [key heads, rows] (zero in rows of no sequence).
+
+    q, k, lse        of causal_attention_forward, with its cu_seqlens, scale, window and sinks
+    weights, lengths given: the sums are added to weights (float32 [batch, key heads, places], in place), key a of a sequence at place
+                     lengths + a, as cache_append puts its row there; keys whose place lies beyond are left out.  Returns None then
+    flags            _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products whatever the type
+
+    No gradients.  Deterministic.  Sums and weights are float32 throughout."""
+    return _lib.host().key_weights(q, k, lse, cu_seqlens, scale, window, sinks, weights, lengths, int(flags))
+
+
+def cache_evict(k_cache, v_cache, weights, lengths, keep, first=0, recent=0, page_table=None):
+    """Drops rows of a cache: of each sequence and key head ``keep`` stay, in their order, at the places 0 .. keep-1 (in place): the
+    ``first`` first, the ``recent`` last ones, and of the others those of the largest weights, of equal ones the first.
+
+    k_cache, v_cache, lengths, page_table   as at cache_append
+    weights   float32 [batch, key heads, places], at least a place for each row that the cache may hold (tree_attention and
+              key_weights add to them), not changed; NaN counts as less than any number.  [batch, 1, places]: one choice for all heads
+
+    Returns (kept, weights): kept int32 [batch, heads, keep], the places that the rows had, ascending, -1 behind them; and a new
+    tensor with the weights of the rows that stay, at their new places, zeros behind.  Sequences of at most ``keep`` rows stay as
+    they are.  lengths are the caller's: torch.minimum(lengths, keep) of them are left.  From then on a row's place is not its position:
+    rotary positions go on from the old lengths, and a window of tree_attention counts places."""
+    return _lib.host().cache_evict(k_cache, v_cache, weights, lengths, int(keep), int(first), int(recent), page_table)

@@ -106,3 +106,56 @@ def test_c_entries_of_trees(lib):
     assert size(window=-1) == size(weighted=1, T=2) == 0
     assert size() == lib.sa2_tree_workspace_bytes(2, 1, 4, 2, 64, 64, 64, 1, 0)
     assert size(window=200) < size() < size(weighted=1) and size(window=200, weighted=1) < size(weighted=1)
+
+
+def _sums(q=(1, 5, 4, 8), k=(1, 5, 2, 8), lse=(1, 4, 5), **kw):
+    return sa.key_weights(t(*q), t(*k), lse if isinstance(lse, torch.Tensor) else t(*lse), **kw)
+
+
+@pytest.mark.parametrize("error,kw", [
+    (ValueError, dict(k=(1, 4, 2, 8))), (ValueError, dict(k=(1, 5, 3, 8))), (ValueError, dict(lse=(1, 5, 4))), (ValueError, dict(lse=t(1, 4, 5, dtype=torch.float64))),
+    (ValueError, dict(lse=t(1, 5, 4).transpose(1, 2))), (ValueError, dict(q=(5, 4, 8), k=(5, 2, 8), lse=(4, 5))), (ValueError, dict(window=0)), (ValueError, dict(sinks=2)),
+    (ValueError, dict(weights=t(1, 2, 9))), (ValueError, dict(lengths=ints(0))), (ValueError, dict(weights=t(1, 4, 9), lengths=ints(0))),
+    (ValueError, dict(weights=t(1, 2, 9), lengths=ints(0, 0))), (ValueError, dict(weights=t(1, 2, 9, dtype=torch.float16), lengths=ints(0))),
+    (ValueError, dict(weights=t(1, 9, 2).transpose(1, 2), lengths=ints(0))), (RuntimeError, dict(weights=t(1, 2, 9).requires_grad_(True), lengths=ints(0))),
+    (RuntimeError, dict(lse=t(1, 4, 5).requires_grad_(True))), (RuntimeError, dict())])
+def test_key_weights(lib, error, kw):
+    with pytest.raises(error):
+        _sums(**kw)
+
+
+def _evict(cache=(6, 16, 2, 8), weights=(2, 2, 48), lengths=ints(3, 4), keep=5, table=ints(*range(6)).view(2, 3), **kw):
+    make = lambda x: x if isinstance(x, torch.Tensor) else t(*x)  # noqa: E731
+    cache = make(cache)
+    return sa.cache_evict(cache, cache.clone(), make(weights), lengths, keep, page_table=table, **kw)
+
+
+@pytest.mark.parametrize("error,kw", [
+    (ValueError, dict(keep=0)), (ValueError, dict(first=-1)), (ValueError, dict(recent=-1)), (ValueError, dict(first=3, recent=3)), (ValueError, dict(keep=1 << 31)),
+    (ValueError, dict(weights=(2, 2, 47))), (ValueError, dict(weights=(2, 3, 48))), (ValueError, dict(weights=(3, 2, 48))), (ValueError, dict(weights=(2, 48))),
+    (ValueError, dict(weights=t(2, 2, 48, dtype=torch.bfloat16))), (ValueError, dict(weights=t(2, 48, 2).transpose(1, 2))), (ValueError, dict(lengths=ints(1, 2, 3))),
+    (ValueError, dict(lengths=ints(1, 2).long())), (ValueError, dict(table=None)), (ValueError, dict(cache=(6, 0, 2, 8))), (ValueError, dict(cache=(6, 16, 2, 264))),
+    (TypeError, dict(cache=t(6, 16, 2, 8, dtype=torch.float64))), (RuntimeError, dict(cache=t(6, 16, 2, 8).requires_grad_(True))), (RuntimeError, dict())])
+def test_evict(lib, error, kw):
+    with pytest.raises(error):
+        _evict(**kw)
+
+
+def test_c_entries_of_weights_and_eviction(lib):
+    s = _lib.stride_array([(4096, 64, 8)] * 3)
+
+    def sums(q=ONE, window=0, sinks=0, B=1, N=64, H=4, HK=2, D=8, dtype=0, lengths=None, places=0, workspace=ONE, nbytes=1 << 30, strides=s):
+        return lib.sa2_key_weights(q, ONE, ONE, ONE, lengths, places, workspace, nbytes, None, 0, B, N, H, HK, D, strides, window, sinks, 1.0, dtype, 0, None)
+
+    assert sums(q=None) == -1 and sums(dtype=5) == -2 and sums(D=0) == -3 and sums(HK=3) == -11 and sums(window=-1) == sums(window=3, sinks=-1) == -5
+    assert sums(lengths=ONE, places=0) == -3 and sums(N=4096, nbytes=4) == -6
+    assert sums(B=2, strides=_lib.stride_array([(4096, 64, 8), (4096, 64, 8), (0, 64, 8)])) == -4
+    assert lib.sa2_key_weights_workspace_bytes(1, 4096, 4, 2, 64, 0, 0, 1, 0) > 0 == lib.sa2_key_weights_workspace_bytes(1, 4096, 4, 3, 64, 0, 0, 1, 0)
+
+    def evict(k=ONE, B=2, HK=2, heads=2, D=8, page=16, pages=6, width=1, places=16, keep=5, first=0, recent=0, dtype=0, strides=s):
+        return lib.sa2_cache_evict(k, ONE, ONE, ONE, ONE, ONE, None, B, HK, heads, D, page, pages, width, places, keep, first, recent, strides, dtype, None)
+
+    assert evict(k=None) == -1 and evict(dtype=7) == -2 and evict(B=0) == evict(D=257) == -3 and evict(heads=3) == -11
+    assert evict(page=0) == evict(pages=1) == evict(width=2) == evict(page=(1 << 31) - 64, places=1 << 40) == -13
+    assert evict(keep=0) == evict(first=-1) == evict(recent=-1) == evict(first=3, recent=3) == evict(places=15) == -15
+    assert evict(strides=_lib.stride_array([(0, 64, 8)] * 3)) == -4

@@ -132,6 +132,9 @@ __device__ __forceinline__ bool key_work(const Causal& p, const Span& s, int j0,
 __device__ __forceinline__ float* sink_row(const Causal& p, int64_t slots, int which, int slot, int hk, int j) {
     return p.sink_part + ((((int64_t)which * slots + slot) * p.HK + hk) * p.band.sinks + j) * p.D;
 }
+// Windows: query heads that a workgroup's four wavefronts have, and whether a wavefront has two blocks of 32 queries (as causal16_two)
+inline int window_heads(const Causal& p) { return p.G % 4 == 0 ? 4 : p.G % 2 == 0 ? 2 : 1; }
+inline bool window_two(const Causal& p, int heads) { return (int64_t)p.rows.B * (p.H / heads) * count_tiles(p.rows, 256 / heads) >= 2 * CUS; }
 inline int64_t sink_slots(const Causal& p) { return (int64_t)p.rows.B * count_tiles(p.rows, p.band.chunk); }
 
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }

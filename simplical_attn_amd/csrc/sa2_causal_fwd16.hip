@@ -14,6 +14,7 @@ namespace {
 // The keys of a workgroup's block of queries, as the sweep takes them (sa2_sweep16.h)
 template <int D>
 struct CausalKeys {
+    static constexpr bool SLIDING = false;
     Fetch<D> fetch;
     bool padded, active;
     int last, mine, tiles, full, pieces;

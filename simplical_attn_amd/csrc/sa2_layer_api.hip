@@ -86,7 +86,7 @@ int prompt_forward(const void* q, const void* k, const void* v, void* out, void*
     if (!stride_ok(p.q, B, N, H) || !stride_ok(p.out, B, N, H) || !stride_ok(p.k, B, N, HK) || !stride_ok(p.v, B, N, HK)) return SA2_ERR_BAD_STRIDE;
     const hipStream_t st = (hipStream_t)hip_stream;
     const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out}) && !((uintptr_t)out_low & 15u);
-    if (p.band.window) return launch_window_f32_fwd(p, dtype, st);
+    if (p.band.window) return narrow ? launch_window16_fwd(p, dtype, st) : launch_window_f32_fwd(p, dtype, st);
     return narrow ? launch_causal16_fwd(p, dtype, st) : launch_causal_f32_fwd(p, dtype, st);
 }
 

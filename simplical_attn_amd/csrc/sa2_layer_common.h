@@ -148,6 +148,7 @@ bool causal16_layout(const Causal& p, std::initializer_list<const Tensor*> ts);
 // whether a wavefront owns two blocks of 32 queries (forward, dQ)
 bool causal16_two(const Causal& p);
 int launch_causal16_fwd(const Causal& p, int dtype, hipStream_t st);
+int launch_window16_fwd(const Causal& p, int dtype, hipStream_t st);
 // Their backward.  Row terms: p.delta receives -delta; fp16: the Euclidean norms of rows bound dS
 struct Causal16Terms {
     float* minus_lse;                          // [B,H,N]  -lse / scale; fp16: what weights are lifted by added (sa2_causal_dkv16.hip)

@@ -21,6 +21,8 @@ namespace sa2 {
 namespace {
 
 constexpr int BUFFERS = 3;
+template <class SRC, int NQ>
+constexpr int SWEEP_BUFFERS = SRC::SLIDING && NQ == 1 ? 4 : BUFFERS;  // (see `sliding`)
 
 template <class E> struct RefLimit;
 template <> struct RefLimit<ElemBF16> { static constexpr float value = 1.152921504606847e18f; };   // 2^60
@@ -51,8 +53,15 @@ struct SweepRegs : Lone<(D * NQ > 128 ? 192 : 96)> {
 //   sees(n, piece)              what the lane's row of block n sees of a piece, bit by key
 //   guarded(piece)              values that some row does not see may be infinite or NaN
 //   lower                       lowered_by of the keys
+// SLIDING: in the place of full and pieces
+//   window, a, b                the leading tiles that hold windows, latest keys first, and those of them that the wavefront's rows see; the
+//                               others, which every row sees or does not as sees() says, hold first keys
+//   before                      1: the first tile stands before those and is looked at for reference points only
+//   clear, clear_end            tiles from clear to clear_end - 1, before b - 1, are seen whole by all rows, and so is the one behind each
+//   any(piece)                  some row sees some of a piece
+//   narrow                      some row may see no key of the first piece of tile a
 // Queries lie in their registers; outputs are left in theirs, in units of e^(scale m), with the lane's part of their sums in l.
-// LDS holds BUFFERS tiles from `base` on (with a fourth, and requests two tiles ahead, times were the same).
+// LDS holds SWEEP_BUFFERS tiles from `base` on (with a fourth, and requests two tiles ahead, times were the same).
 // c: |scale| log2(e).  All wavefronts of the workgroup call it.
 template <class E, int D, int NQ, class SRC>
 __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, float (&m)[NQ], float (&l)[NQ]) {
@@ -62,7 +71,9 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
     constexpr int KK = D / 16, DT = D / 32, O0 = L::O0, Q0 = L::Q0;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const uint32_t row_lane = T::row_lane(lane), column_lane = T::column_lane(lane);
-    auto after = [&](uint32_t buf) { return buf == base + (BUFFERS - 1) * Buffer<D>::BYTES ? base : buf + Buffer<D>::BYTES; };
+    constexpr int RING = SWEEP_BUFFERS<SRC, NQ>;
+    auto after = [&](uint32_t buf) { return buf == base + (RING - 1) * Buffer<D>::BYTES ? base : buf + Buffer<D>::BYTES; };
+    auto buffer_of = [&](int t) { return base + (uint32_t)(t % RING) * Buffer<D>::BYTES; };
 
     constexpr int UNITS = 2 * NQ;                                          // of a tile: unit v is piece v / NQ, block v % NQ
     floatx16 st[2];                                                        // logits
@@ -144,8 +155,10 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
     };
     // One step of the pipeline: logits of unit V + 2, output of unit V, weights of unit V + 1; operands of the units after
     // those, from kat and vat, as soon as the ones before have been read for the last time (two MFMAs later)
-    auto step = [&](auto VV, uint32_t kat, uint32_t vat) __attribute__((always_inline)) {
+    // (MASKED: bit k of `seen` says whether the lane's row sees key k of unit V + 1)
+    auto step = [&](auto VV, uint32_t kat, uint32_t vat, auto MASKED, uint32_t seen) __attribute__((always_inline)) {
         constexpr int V = decltype(VV)::value, SLOTS = 4 * DT, LAG = SLOTS - 4;
+        const uint32_t own = decltype(MASKED)::value ? seen >> 4 * half : 0u;
         constexpr bool NEXT_K = (V + 3) % NQ == 0, NEXT_V = (V + VB) % NQ == 0;
         constexpr int set = V / NQ % VB, next_set = (V + VB) / NQ % VB;    // of V operands
         constexpr int mid = (V + 1) % NQ;
@@ -161,6 +174,7 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
             deal<16, i - 2, LAG>([&](auto X) __attribute__((always_inline)) { e[decltype(X)::value] = fast_exp2(e[decltype(X)::value]); });
             deal<16, i - 3, LAG>([&](auto X) __attribute__((always_inline)) {
                 constexpr int j = decltype(X)::value;
+                if constexpr (decltype(MASKED)::value) e[j] = __uint_as_float(__float_as_uint(e[j]) & (uint32_t)__builtin_amdgcn_sbfe((int)own, 8 * (j / 4) + j % 4, 1));
                 sum += e[j];
                 if constexpr (j % 2) z.u[j / 2] = pack2<E>(e[j - 1], e[j]);
             });
@@ -244,6 +258,108 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
         asm volatile("s_nop 7" ::: "memory");                              // (the last MFMA has read its operands)
     };
     constexpr int LOOK = NQ == 1 ? 2 : 1;                                  // tiles ahead that a round of steps reads keys of
+    const std::false_type whole{};
+    const std::true_type some{};
+    // SLIDING: the tiles of src.a .. src.b - 1 go through the pipeline to the last, with masks where some row does not see all of
+    // a tile or the next; then the first keys' tiles, piece by piece.  Tile `t` is worked on when the one LOOK behind it is there (what
+    // the steps read ahead of a wavefront's last tile is not used).  Rows' reference points come from the first of these tiles, the one
+    // with their own keys; in fp16, whose weights have less room above it, from the next one and the first keys as well.
+    auto sliding = [&](const auto& src, bool safe) {
+        auto tops = [&](int t, int sub) {
+            load_keys(keys_at(buffer_of(t), sub));
+            L::keep_out();
+            static_for<NQ>([&](auto N) __attribute__((always_inline)) {
+                constexpr int n = decltype(N)::value;
+                logits(N, st[n]);
+                ready(st[n]);
+                m[n] = fmaxf(m[n], top_of(st[n], src.sees(n, 2 * t + sub)) - src.lower);
+            });
+        };
+        auto advance = [&](int t) __attribute__((always_inline)) {
+            const int to = t < src.tiles ? t : src.tiles - 1;
+#pragma unroll 1
+            while (released < to) arrive();
+        };
+        const bool active = src.a < src.b;
+        if (!safe && active) {
+            int t = src.a;
+            if (E::DTYPE == SA2_F16 && src.before) tops(0, 0);
+            advance(t + LOOK);
+            if (src.narrow) tops(t, 1);
+            if (E::DTYPE == SA2_F16 && t + 1 < src.b) tops(t + 1, 1);
+            uint32_t here = buffer_of(t);
+            load_keys(keys_at(here, 0));
+            L::keep_out();
+            static_for<NQ>([&](auto N) __attribute__((always_inline)) {
+                constexpr int n = decltype(N)::value;
+                logits(N, st[n]);
+                ready(st[n]);
+                m[n] = fmaxf(m[n], top_of(st[n], src.sees(n, 2 * t)) - src.lower);
+                if (m[n] == -INFINITY) {
+                    m[n] = 0.f;
+                    worst = INFINITY;
+                }
+            });
+            load_keys(keys_at(here, 1));
+            L::keep_out();
+            if constexpr (NQ == 1) {
+                logits(LONE_C(0), st[1]);
+                ready(st[1]);
+                load_keys(keys_at(after(here), 0));
+            }
+            load_values(values_at(here, 0));
+            L::keep_out();
+            float sum;
+            weights(st[0], m[0], sum, w[0], some, src.sees(0, 2 * t));
+            worst = fmaxf(worst, sum);
+            l[0] += sum;
+            asm volatile("s_nop 3" : "+v"(w[0][0]), "+v"(w[0][1]));
+            // Runs of rounds with and without masks (the last tile is in the first kind); true: that was the last one
+            auto rounds = [&](auto MASKED) __attribute__((always_inline)) {
+                constexpr bool SOME = decltype(MASKED)::value;
+                auto seen = [&](int n, int piece) { return SOME ? src.sees(n, piece) : 0u; };
+#pragma unroll 1
+                do {
+                    advance(t + LOOK);
+                    const bool last = t + 1 == src.b;
+                    const uint32_t next = after(here);
+                    L::keep_out();
+                    if constexpr (NQ == 1) {
+                        step(LONE_C(0), keys_at(next, 1), values_at(here, 1), MASKED, seen(0, 2 * t + 1));
+                        if (SOME && last) return true;
+                        step(LONE_C(1), keys_at(after(next), 0), values_at(next, 0), MASKED, seen(0, 2 * t + 2));
+                    } else {
+                        step(LONE_C(0), 0u, VB == 2 ? values_at(here, 1) : 0u, MASKED, seen(1, 2 * t));
+                        step(LONE_C(1), keys_at(next, 0), VB == 2 ? 0u : values_at(here, 1), MASKED, seen(0, 2 * t + 1));
+                        step(LONE_C(2), 0u, VB == 2 ? values_at(next, 0) : 0u, MASKED, seen(1, 2 * t + 1));
+                        if (SOME && last) return true;
+                        step(LONE_C(3), keys_at(next, 1), VB == 2 ? 0u : values_at(next, 0), MASKED, seen(0, 2 * t + 2));
+                    }
+                    here = next;
+                    ++t;
+                } while ((t >= src.clear && t < src.clear_end) != SOME);
+                return false;
+            };
+#pragma unroll 1
+            while (!rounds(some)) {
+                if (t < src.clear_end) rounds(whole);
+            }
+            L::keep_out();
+            rest();
+            asm volatile("s_nop 3" : "+v"(w[1][0]), "+v"(w[1][1]));
+            static_for<2 * DT>([&](auto J) __attribute__((always_inline)) { output_mfma(LONE_C(NQ - 1), J, w[1], LONE_C(VB - 1)); });
+            rest();
+        }
+        // (up to and with the last tile, which every wavefront waits for)
+#pragma unroll 1
+        for (int t = safe ? src.before : src.window; t <= src.tiles; ++t) {
+            advance(t + LOOK);
+            if (!active || t == src.tiles || (t < src.window && (t < src.a || t >= src.b))) continue;
+#pragma unroll 1
+            for (int sub = 0; sub < 2; ++sub)
+                if (src.any(2 * t + sub)) piece(buffer_of(t), sub, 2 * t + sub, safe);
+        }
+    };
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
         released = -1;
@@ -258,86 +374,98 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
             l[n] = 0.f;
             m[n] = -INFINITY;
         }
-        int done = 0;                                                      // pieces of 32 keys
-        uint32_t here = base;
-        if (pass == 0 && src.full > LOOK) {
-            load_keys(keys_at(base, 0));
-            static_for<NQ>([&](auto N) __attribute__((always_inline)) {
-                constexpr int n = decltype(N)::value;
-                logits(N, st[n]);
-                ready(st[n]);
-                m[n] = top_of(st[n], ~0u) - src.lower;
-                if (m[n] == -INFINITY) {                                   // (scores of minus infinity say nothing about the others)
-                    m[n] = 0.f;
-                    worst = INFINITY;
-                }
+        if constexpr (SRC::SLIDING) {
+            sliding(src, pass != 0);
+            // (a weight of zero does not keep an infinity or NaN out: outputs with one are made again, by pieces that do)
+            rest();
+            float poison = 0.f;
+            static_for<NQ * DT * 4>([&](auto X) __attribute__((always_inline)) {
+                const float4 o = L::template get_regs<O0 + 4 * decltype(X)::value>();
+                poison = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, fmaf(o.w, 0.f, poison))));
             });
-            if constexpr (NQ == 1) {
-                load_keys(keys_at(base, 1));
-                logits(LONE_C(0), st[1]);
-                ready(st[1]);
-                arrive();
-                load_keys(keys_at(after(base), 0));
-            } else {
-                load_keys(keys_at(base, 1));
-            }
-            load_values(values_at(base, 0));
-            weigh(st[0], 0, w[0]);
-            asm volatile("s_nop 3" : "+v"(w[0][0]), "+v"(w[0][1]));
-            int t = 0;
-            for (; t + LOOK < src.full; ++t) {
-                const uint32_t next = after(here);
-                L::keep_out();
-                if constexpr (VB == 2) {
-                    step(LONE_C(0), 0u, values_at(here, 1));
-                    arrive();
-                    step(LONE_C(1), keys_at(next, 0), 0u);
-                    step(LONE_C(2), 0u, values_at(next, 0));
-                    step(LONE_C(3), keys_at(next, 1), 0u);
-                } else if constexpr (NQ == 2) {
-                    step(LONE_C(0), 0u, 0u);
-                    arrive();
-                    step(LONE_C(1), keys_at(next, 0), values_at(here, 1));
-                    step(LONE_C(2), 0u, 0u);
-                    step(LONE_C(3), keys_at(next, 1), values_at(next, 0));
-                } else {
-                    step(LONE_C(0), keys_at(next, 1), values_at(here, 1));
-                    arrive();
-                    step(LONE_C(1), keys_at(after(next), 0), values_at(next, 0));
-                }
-                here = next;
-            }
-            // the two units that are under way
-            rest();
-            output(LONE_C(0), w[0]);
-            weigh(st[1], NQ - 1, w[1]);
-            if constexpr (NQ == 1) load_values(values_at(here, 1));
-            output(LONE_C(NQ - 1), w[1]);
-            rest();
-            done = 2 * t + (NQ == 1 ? 2 : 1);
-            if constexpr (NQ == 1) here = after(here);
-        }
-        // the rest by itself; in the second pass all
-        for (int t = done / 2; t < src.tiles; ++t, here = after(here)) {
-            if (t > released) arrive();
-#pragma unroll 1
-            for (int sub = t == done / 2 ? done % 2 : 0; sub < 2; ++sub)
-                if (2 * t + sub < src.pieces) piece(here, sub, 2 * t + sub, pass != 0);
-        }
-        bool again = worst > RefLimit<E>::value;
-        if constexpr (E::DTYPE == SA2_BF16) {
-            // (with smaller weights a second sweep would come no further; fp16 values times weights up to the limit are far from fp32's end)
-            if (pass == 0 && __any(worst > OUTPUT_CHECK)) {
-                rest();
-                uint32_t bits = 0;
-                static_for<NQ * DT * 4>([&](auto X) __attribute__((always_inline)) {
-                    const float4 o = L::template get_regs<O0 + 4 * decltype(X)::value>();
-                    for (const float y : {o.x, o.y, o.z, o.w}) bits |= (__float_as_uint(y) & 0x7f800000u) + 0x00800000u;
+            if (pass != 0 || !__syncthreads_or(worst > RefLimit<E>::value || poison != 0.f)) break;
+        } else {
+            int done = 0;                                                      // pieces of 32 keys
+            uint32_t here = base;
+            if (pass == 0 && src.full > LOOK) {
+                load_keys(keys_at(base, 0));
+                static_for<NQ>([&](auto N) __attribute__((always_inline)) {
+                    constexpr int n = decltype(N)::value;
+                    logits(N, st[n]);
+                    ready(st[n]);
+                    m[n] = top_of(st[n], ~0u) - src.lower;
+                    if (m[n] == -INFINITY) {                                   // (scores of minus infinity say nothing about the others)
+                        m[n] = 0.f;
+                        worst = INFINITY;
+                    }
                 });
-                again = again || bits >> 31;
+                if constexpr (NQ == 1) {
+                    load_keys(keys_at(base, 1));
+                    logits(LONE_C(0), st[1]);
+                    ready(st[1]);
+                    arrive();
+                    load_keys(keys_at(after(base), 0));
+                } else {
+                    load_keys(keys_at(base, 1));
+                }
+                load_values(values_at(base, 0));
+                weigh(st[0], 0, w[0]);
+                asm volatile("s_nop 3" : "+v"(w[0][0]), "+v"(w[0][1]));
+                int t = 0;
+                for (; t + LOOK < src.full; ++t) {
+                    const uint32_t next = after(here);
+                    L::keep_out();
+                    if constexpr (VB == 2) {
+                        step(LONE_C(0), 0u, values_at(here, 1), whole, 0u);
+                        arrive();
+                        step(LONE_C(1), keys_at(next, 0), 0u, whole, 0u);
+                        step(LONE_C(2), 0u, values_at(next, 0), whole, 0u);
+                        step(LONE_C(3), keys_at(next, 1), 0u, whole, 0u);
+                    } else if constexpr (NQ == 2) {
+                        step(LONE_C(0), 0u, 0u, whole, 0u);
+                        arrive();
+                        step(LONE_C(1), keys_at(next, 0), values_at(here, 1), whole, 0u);
+                        step(LONE_C(2), 0u, 0u, whole, 0u);
+                        step(LONE_C(3), keys_at(next, 1), values_at(next, 0), whole, 0u);
+                    } else {
+                        step(LONE_C(0), keys_at(next, 1), values_at(here, 1), whole, 0u);
+                        arrive();
+                        step(LONE_C(1), keys_at(after(next), 0), values_at(next, 0), whole, 0u);
+                    }
+                    here = next;
+                }
+                // the two units that are under way
+                rest();
+                output(LONE_C(0), w[0]);
+                weigh(st[1], NQ - 1, w[1]);
+                if constexpr (NQ == 1) load_values(values_at(here, 1));
+                output(LONE_C(NQ - 1), w[1]);
+                rest();
+                done = 2 * t + (NQ == 1 ? 2 : 1);
+                if constexpr (NQ == 1) here = after(here);
             }
+            // the rest by itself; in the second pass all
+            for (int t = done / 2; t < src.tiles; ++t, here = after(here)) {
+                if (t > released) arrive();
+    #pragma unroll 1
+                for (int sub = t == done / 2 ? done % 2 : 0; sub < 2; ++sub)
+                    if (2 * t + sub < src.pieces) piece(here, sub, 2 * t + sub, pass != 0);
+            }
+            bool again = worst > RefLimit<E>::value;
+            if constexpr (E::DTYPE == SA2_BF16) {
+                // (with smaller weights a second sweep would come no further; fp16 values times weights up to the limit are far from fp32's end)
+                if (pass == 0 && __any(worst > OUTPUT_CHECK)) {
+                    rest();
+                    uint32_t bits = 0;
+                    static_for<NQ * DT * 4>([&](auto X) __attribute__((always_inline)) {
+                        const float4 o = L::template get_regs<O0 + 4 * decltype(X)::value>();
+                        for (const float y : {o.x, o.y, o.z, o.w}) bits |= (__float_as_uint(y) & 0x7f800000u) + 0x00800000u;
+                    });
+                    again = again || bits >> 31;
+                }
+            }
+            if (!__syncthreads_or(again)) break;
         }
-        if (!__syncthreads_or(again)) break;
     }
     rest();
 }

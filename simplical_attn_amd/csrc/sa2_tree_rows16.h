@@ -16,6 +16,7 @@ namespace {
 
 template <int D, int NQ, bool BAND>
 struct TreeKeys {
+    static constexpr bool SLIDING = false;                 // (all tiles but the leading ones go piece by piece)
     using T = QuadTile<D>;
     const Tree& p;
     const int32_t* pages;                                  // of the share, the first of them page0 (with a band: see sa2_tree16.h)

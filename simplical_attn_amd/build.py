@@ -44,7 +44,8 @@ _WFWD = tuple((pattern.replace("causal", "window"), owned) for pattern, owned in
 _CTREE = tuple((pattern.replace("causal_fwd16", "tree_rows16"), owned) for pattern, owned in _CFWD)
 _CDQ = (("causal_dq16_kernel.*Li128ELi2E", 256), ("causal_dq16_kernel.*(Li128ELi1E|Li64ELi2E)", 192), ("causal_dq16_kernel.*Li64ELi1E", 96))
 _CDKV = (("causal_(dkv|bwd)16_kernel.*Li128E", 192), ("causal_(dkv|bwd)16_kernel.*Li64E", 96))
-HAND_PLACED = {"sa2_causal_fwd16.hip": _CFWD, "sa2_window_fwd16.hip": _WFWD, "sa2_tree_rows16.hip": _CTREE, "sa2_window_tree_rows16.hip": _CTREE, "sa2_causal_dq16.hip": _CDQ, "sa2_causal_dkv16.hip": _CDKV,
+_WBWD = (("window_dq16_kernel.*Li128E", 256), ("window_dkv16_kernel.*Li128E", 192), ("window_bwd16_kernel.*Li64ELi2E", 192), ("window_bwd16_kernel.*Li64ELi1E", 96))
+HAND_PLACED = {"sa2_causal_fwd16.hip": _CFWD, "sa2_window_fwd16.hip": _WFWD, "sa2_window_bwd16.hip": _WBWD, "sa2_tree_rows16.hip": _CTREE, "sa2_window_tree_rows16.hip": _CTREE, "sa2_causal_dq16.hip": _CDQ, "sa2_causal_dkv16.hip": _CDKV,
                "sa2_mfma_bwd_kv_bf16.hip": _KV, "sa2_mfma_bwd_kv_fp16.hip": _KV,
                "sa2_mfma_bwd_kp_lone_bf16.hip": _KP, "sa2_mfma_bwd_kp_lone_fp16.hip": _KP,
                "sa2_mfma_fwd_lone_bf16.hip": _FWD, "sa2_mfma_fwd_lone_fp16.hip": _FWD,

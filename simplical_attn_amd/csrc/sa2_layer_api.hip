@@ -43,8 +43,8 @@ int make_band(Causal& p, int window, int sinks) {
     p.band.window = window;
     p.band.sinks = sinks < p.rows.N ? sinks : p.rows.N;
     p.band.alone = window == 1 && sinks == 0 ? 0x7fffffff : 0;
-    // (where the first keys are many, longer chunks, so that their sums stay a fraction of the tensors)
-    const int64_t chunk = 512 * (int64_t)(p.band.sinks > 128 ? (p.band.sinks + 127) / 128 : 1);
+    // (where the first keys are many, longer chunks, so that their sums stay of the tensors' size)
+    const int64_t chunk = 128 * (int64_t)(p.band.sinks > 128 ? (p.band.sinks + 127) / 128 : 1);
     p.band.chunk = chunk < 1 << 30 ? (int)chunk : 1 << 30;
     return p.band.sinks > 0 && (sink_slots(p) * p.HK > 0x7fffffff || p.band.sinks > 65535 * 32) ? SA2_ERR_TOO_LARGE : SA2_OK;
 }
@@ -94,7 +94,11 @@ size_t prompt_workspace(int sequences, int B, int N, int H, int HK, int D, int w
     Causal p;
     static const int32_t packed = 0;                       // (only whether there are packed sequences counts here)
     if (make_causal(p, sequences > 0 ? &packed : nullptr, sequences, B, N, H, HK, D, 1.f, dtype) != SA2_OK || make_band(p, window, sinks) != SA2_OK) return 0;
-    if (p.band.window) return (delta_bytes(p) + sink_part_bytes(p) + 255) / 256 * 256;
+    if (p.band.window) {
+        const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype);
+        const size_t terms = narrow ? delta_bytes(p) + (dtype == SA2_F16 ? 2 * delta_bytes(p) + 2 * row_bytes(p, HK) : 0) + window16_part_bytes(p) : 0;
+        return (delta_bytes(p) + terms + sink_part_bytes(p) + 255) / 256 * 256;
+    }
     if ((flags & SA2_FLAG_FORCE_GENERIC) || !causal16_supported(D, dtype)) return delta_bytes(p);
     return 2 * delta_bytes(p) + (dtype == SA2_F16 ? delta_bytes(p) + row_bytes(p, HK) : 0) + causal16_part_bytes(B, N, HK, p.G, D);
 }
@@ -122,13 +126,25 @@ int prompt_backward(const void* q, const void* k, const void* v, const void* out
     if (!dq && !dk && !dv) return SA2_OK;
     char* behind = (char*)workspace + delta_bytes(p);
     auto next = [&](size_t bytes) { char* const here = behind; behind += bytes; return (float*)here; };
-    if (p.band.window) {
-        p.sink_part = next(0);
-        return launch_window_f32_bwd(p, dtype, st);
-    }
     // (-lse / scale is one of the 16-bit kernels' operands)
-    if (!(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv}) &&
-        fabsf(scale) > 1e-20f && !((uintptr_t)out_low & 15u)) {
+    const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && causal16_supported(D, dtype) && causal16_layout(p, {&p.q, &p.k, &p.v, &p.out, &p.dout, &p.dq, &p.dk, &p.dv}) &&
+                        fabsf(scale) > 1e-20f && !((uintptr_t)out_low & 15u);
+    if (p.band.window) {
+        Causal16Terms terms{};
+        if (narrow) {
+            terms.minus_lse = next(delta_bytes(p));
+            if (dtype == SA2_F16) {
+                terms.dout = next(delta_bytes(p));
+                terms.queries = next(delta_bytes(p));
+                terms.v = next(row_bytes(p, HK));
+                terms.keys = next(row_bytes(p, HK));
+            }
+            p.part = next(window16_part_bytes(p));
+        }
+        p.sink_part = next(0);
+        return narrow ? launch_window16_bwd(p, dtype, terms, st) : launch_window_f32_bwd(p, dtype, st);
+    }
+    if (narrow) {
         Causal16Terms terms{next(delta_bytes(p)), nullptr, nullptr};
         if (dtype == SA2_F16) {
             terms.dout = next(delta_bytes(p));

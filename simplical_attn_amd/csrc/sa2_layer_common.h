@@ -154,6 +154,7 @@ struct Causal16Terms {
     float* minus_lse;                          // [B,H,N]  -lse / scale; fp16: what weights are lifted by added (sa2_causal_dkv16.hip)
     float* dout;                               // [B,H,N]  |dout|, fp16 only
     float* v;                                  // [B,HK,N] |v|, fp16 only
+    float *queries, *keys;                     // [B,H,N], [B,HK,N]: the factors of rows of dQ and of keys (sa2_causal16.h), fp16 with a band only
 };
 int causal16_splits(int B, int N, int HK, int G);
 size_t causal16_part_bytes(int B, int N, int HK, int G, int D);
@@ -164,6 +165,10 @@ inline int64_t tree_reach(int64_t capacity, int T, int window, int sinks) {
     const int64_t reach = (int64_t)window + sinks + T;
     return window && reach < capacity ? reach : capacity;
 }
+// With p.band: shares of the key blocks' streams, the largest number of their sums' bytes; the whole backward
+int window16_splits(const Causal& p);
+size_t window16_part_bytes(const Causal& p);
+int launch_window16_bwd(const Causal& p, int dtype, const Causal16Terms& terms, hipStream_t st);
 int launch_tree_f32(const Tree& p, int dtype, hipStream_t st);
 int launch_window_tree_f32(const Tree& p, int dtype, hipStream_t st);
 int launch_window_tree16(const Tree& p, int dtype, hipStream_t st);

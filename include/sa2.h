@@ -246,8 +246,8 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
 
 /*
  * The same with a sliding window: query i of a sequence attends to its keys j <= i with i - j < window or j < sinks, that is, to the
- * last `window` keys up to its own (1 or more) and to the sequence's first `sinks` ones (0 or more).  A window of N or more is
- * none: sa2_causal_forward and _backward run, bit for bit.
+ * last `window` keys up to its own (1 or more) and to the sequence's first `sinks` ones (0 to 65535; more: SA2_ERR_TOO_LARGE).
+ * A window of N or more is none: sa2_causal_forward and _backward run, bit for bit.
  *   sequences    of the workspace's size: 0 for a batch, else the packed sequences of the call
  * The first keys' gradients are sums of fp32 sums over chunks of queries, in their order.
  */

@@ -426,8 +426,10 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
         // no number: a weight of zero does not keep an infinity or NaN out.  Windows under two tiles go by pieces alone.
         const std::true_type yes{};
         const std::false_type no{};
+        // A block's own rows by pieces too, which carry what rounding dS leaves, at the start of a sequence, whose rows are short
         constexpr int OWN = BLOCK / TILE_ROWS;
-        const int own = t0 * TILE_ROWS == j0 ? OWN : 0;                    // (a chunk behind the block has none of its rows)
+        const bool diagonal = t0 * TILE_ROWS == j0;                        // (a chunk behind the block has none of its rows)
+        const int own = diagonal && j0 == 0 ? OWN : 0, run = sink && !diagonal ? hi - lo : per;
         const bool active = lo < hi && mine < (sink ? p.band.sinks : s.len) && (sink || mine + SUB > p.band.sinks);
         const Fetch<D> start = fetch;
         const int rg0 = rg, rt0 = rt;
@@ -452,7 +454,7 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
             };
 #pragma unroll 1
             for (int at = lo; at < hi;) {
-                const int g = at / per, i0 = at - g * per, i1 = hi - at < per - i0 ? i0 + hi - at : per;
+                const int g = at / run, i0 = at - g * run, i1 = hi - at < run - i0 ? i0 + hi - at : run;
                 int i = i0;
                 const int slow = !active || !fast ? i1 : own < i1 ? own : i1;
 #pragma unroll 1
@@ -466,9 +468,9 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
                     }
                 }
                 if (i < i1) {
-                    // tiles before `clear` are seen whole
-                    const int reach = (mine + p.band.window) / TILE_ROWS - t0, clear = sink ? i1 : reach;
-                    auto row = [&](int x, int sub) { return (t0 + x) * TILE_ROWS + sub * SUB; };
+                    // (32 MFMAs for 16 weights leave room for masks in every step; of the first keys' queries behind their block, all of
+                    // which see them, one run over all heads)
+                    auto seen = [&](int x, int sub) { return sink && !diagonal ? ~0u : sees((t0 + x) * TILE_ROWS + sub * SUB); };
                     advance(at + i - i0 + 1);
                     L::keep_out();
                     static_for<8>([&](auto X) __attribute__((always_inline)) { load_stat(X, stats_at(here, 0), st[0], dp[0]); });
@@ -483,23 +485,18 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
                     L::keep_out();
                     // (where no tile follows, `next` is read and its products are not used)
                     uint32_t next = after(here);
-                    step(LONE_C(0), yes, no, rows_at(here, 1), rows_at(next, 0), stats_at(next, 0), 0u, cols_at(here, 0), yes, sees(row(i, 0)));
+                    step(LONE_C(0), yes, no, rows_at(here, 1), rows_at(next, 0), stats_at(next, 0), 0u, cols_at(here, 0), yes, seen(i, 0));
                     ++i;
-                    auto rounds = [&](auto MASKED, int end) __attribute__((always_inline)) {
-                        auto seen = [&](int x, int sub) { return decltype(MASKED)::value ? sees(row(x, sub)) : 0u; };
 #pragma unroll 1
-                        for (; i < end; ++i) {
-                            const uint32_t last = here;
-                            here = next;
-                            next = after(here);
-                            advance(at + i - i0 + 1);
-                            step(LONE_C(1), yes, yes, rows_at(here, 0), rows_at(here, 1), stats_at(here, 1), cols_at(last, 0), cols_at(last, 1), MASKED, seen(i - 1, 1));
-                            step(LONE_C(0), yes, yes, rows_at(here, 1), rows_at(next, 0), stats_at(next, 0), cols_at(last, 1), cols_at(here, 0), MASKED, seen(i, 0));
-                        }
-                    };
-                    rounds(no, clear < i1 ? clear : i1);
-                    rounds(yes, i1);
-                    step(LONE_C(1), no, yes, 0u, 0u, 0u, cols_at(here, 0), cols_at(here, 1), yes, sees(row(i1 - 1, 1)));
+                    for (; i < i1; ++i) {
+                        const uint32_t last = here;
+                        here = next;
+                        next = after(here);
+                        advance(at + i - i0 + 1);
+                        step(LONE_C(1), yes, yes, rows_at(here, 0), rows_at(here, 1), stats_at(here, 1), cols_at(last, 0), cols_at(last, 1), yes, seen(i - 1, 1));
+                        step(LONE_C(0), yes, yes, rows_at(here, 1), rows_at(next, 0), stats_at(next, 0), cols_at(last, 1), cols_at(here, 0), yes, seen(i, 0));
+                    }
+                    step(LONE_C(1), no, yes, 0u, 0u, 0u, cols_at(here, 0), cols_at(here, 1), yes, seen(i1 - 1, 1));
                     static_for<4 * DT - LEAD>([&](auto C) __attribute__((always_inline)) { load_col(LONE_C(decltype(C)::value + LEAD), cols_at(here, 1)); });
                     asm volatile("s_nop 3" : "+v"(pw[1][0]), "+v"(pw[1][1]), "+v"(dw[1][0]), "+v"(dw[1][1]));
                     L::keep_out();

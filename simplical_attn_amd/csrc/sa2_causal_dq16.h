@@ -91,6 +91,10 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const Causal
     Fetch<D> fetch;
     fetch.init(p.k, p.v, s, hk, p.D);
 
+    if (BAND) {                                                            // (the first two tiles' latencies with those of the queries)
+        fetch.request(key(0), last, base, padded);
+        if (tiles > 1) fetch.request(key(1), last, base + Buffer<D>::BYTES, padded);
+    }
     const float c = p.scale * LOG2E;
     float lse2[NQ], f[NQ], df[NQ];                                         // f: the rows' factors, df: delta times them
     if constexpr (E::DTYPE == SA2_F16 && !BAND) query_factors<NQ>(p, terms, s, h, q0, f, (float*)lds);
@@ -243,11 +247,16 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const Causal
         fetch.request(key(t), last, arriving, padded);
         arriving = after(arriving);
     };
+    int begun = 0;                                                         // with a band: tiles that have been requested
     auto arrive = [&]() {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         ++released;
-        if (released + 1 < tiles) request(released + 1);
+        if constexpr (BAND) {
+            if (begun == released + 1 && begun < tiles) request(begun++);
+        } else {
+            if (released + 1 < tiles) request(released + 1);
+        }
     };
     // what the lane's row of block n sees of the keys from .. from + 31, with a band
     auto sees = [&](int n, int from) {
@@ -288,12 +297,13 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const Causal
     constexpr int LOOK = NQ == 1 ? 2 : 1;
     const std::false_type no{};
     if constexpr (BAND) {
-        // Tiles from .. own - 1 through the pipeline, as in sa2_sweep16.h, with masks up to tile `clear`; the one with the own keys and those of the
-        // first keys piece by piece.  Windows under two tiles, whose rows are as short as a short sequence's, all by pieces, which carry
-        // what rounding dS leaves; so does a second pass where a sum is no number: a weight of zero does not keep an infinity or NaN out.
+        // Tiles from .. end - 1 through the pipeline, as in sa2_sweep16.h, with masks up to tile `clear` and in the last one, which has the own keys;
+        // those of the first keys piece by piece.  Windows under two tiles, and rows at the start of a sequence, all by pieces, which carry
+        // what rounding dS leaves: rows are short there.  So does a second pass where a sum is no number: a weight of zero does not keep an
+        // infinity or NaN out.
         const bool joined = (p.band.sinks + TILE_ROWS - 1) / TILE_ROWS > reach.start;      // (first keys that the windows reach into)
         const int low = mine < p.band.window ? 0 : mine - p.band.window + 1, edge = mine + ROWS - p.band.window;
-        const int from = joined ? 0 : low / TILE_ROWS - reach.start, own = mine / TILE_ROWS - reach.start;
+        const int from = joined ? 0 : low / TILE_ROWS - reach.start, end = mine / TILE_ROWS - reach.start + 1;
         const int clear = edge > 0 ? (edge + TILE_ROWS - 1) / TILE_ROWS - reach.start : 0;
         const std::true_type some{};
         auto advance = [&](int t) __attribute__((always_inline)) {
@@ -304,10 +314,11 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const Causal
 #pragma unroll 1
         for (int pass = 0; pass < 2; ++pass) {
             released = -1;
-            arriving = base;
-            request(0);
+            begun = pass ? 1 : tiles < 2 ? tiles : 2;
+            arriving = pass ? base : buffer_of(begun);
+            if (pass) request(0);
             arrive();
-            const bool fast = pass == 0 && active && p.band.window >= 2 * TILE_ROWS && from < own;
+            const bool fast = pass == 0 && active && p.band.window >= 2 * TILE_ROWS && mine >= 2 * TILE_ROWS;
             if (fast) {
                 int t = from;
                 advance(t + LOOK);
@@ -335,29 +346,29 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const Causal
 #pragma unroll 1
                     do {
                         advance(t + LOOK);
-                        const bool end = t + 1 == own;
+                        const bool last_one = t + 1 == end;
                         const uint32_t next = after(here);
                         const int k0 = key(t), k1 = key(t + 1);
                         L::keep_out();
                         if constexpr (NQ == 1) {
                             step(LONE_C(0), rows_at(next, 1), cols_at(here, 1), MASKED, seen(0, k0 + SUB));
-                            if (SOME && end) return true;
+                            if (SOME && last_one) return true;
                             step(LONE_C(1), rows_at(after(next), 0), cols_at(next, 0), MASKED, seen(0, k1));
                         } else {
                             step(LONE_C(0), 0u, 0u, MASKED, seen(1, k0));
                             step(LONE_C(1), rows_at(next, 0), cols_at(here, 1), MASKED, seen(0, k0 + SUB));
                             step(LONE_C(2), 0u, 0u, MASKED, seen(1, k0 + SUB));
-                            if (SOME && end) return true;
+                            if (SOME && last_one) return true;
                             step(LONE_C(3), rows_at(next, 1), cols_at(next, 0), MASKED, seen(0, k1));
                         }
                         here = next;
                         ++t;
-                    } while ((t >= clear && t + 1 < own) != SOME);
+                    } while ((t >= clear && t + 2 < end) != SOME);
                     return false;
                 };
 #pragma unroll 1
                 while (!rounds(some)) {
-                    if (t + 1 < own) rounds(no);
+                    if (t + 2 < end) rounds(no);
                 }
                 L::keep_out();
                 rest();
@@ -365,7 +376,7 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const Causal
             }
             // (up to and with the last tile, which every wavefront waits for)
 #pragma unroll 1
-            for (int t = fast ? own : 0; t <= tiles; ++t) {
+            for (int t = fast ? near : 0; t <= tiles; ++t) {
                 advance(t + LOOK);
                 if (!active || t == tiles) continue;
 #pragma unroll 1

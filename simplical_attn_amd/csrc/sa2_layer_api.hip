@@ -46,7 +46,7 @@ int make_band(Causal& p, int window, int sinks) {
     // (where the first keys are many, longer chunks, so that their sums stay of the tensors' size)
     const int64_t chunk = 128 * (int64_t)(p.band.sinks > 128 ? (p.band.sinks + 127) / 128 : 1);
     p.band.chunk = chunk < 1 << 30 ? (int)chunk : 1 << 30;
-    return p.band.sinks > 0 && (sink_slots(p) * p.HK > 0x7fffffff || p.band.sinks > 65535 * 32) ? SA2_ERR_TOO_LARGE : SA2_OK;
+    return p.band.sinks > 0 && (sink_slots(p) * p.HK > 0x7fffffff || p.band.sinks > 65535) ? SA2_ERR_TOO_LARGE : SA2_OK;
 }
 size_t row_bytes(const Causal& p, int heads) { return ((size_t)p.rows.B * heads * p.rows.N * sizeof(float) + 255) / 256 * 256; }
 size_t delta_bytes(const Causal& p) { return row_bytes(p, p.H); }

@@ -59,6 +59,7 @@ struct SweepRegs : Lone<(D * NQ > 128 ? 192 : 96)> {
 //   before                      1: the first tile stands before those and is looked at for reference points only
 //   clear, clear_end            tiles from clear to clear_end - 1, before b - 1, are seen whole by all rows, and so is the one behind each
 //   any(piece)                  some row sees some of a piece
+//   begin(base)                 requests of the first two tiles, which the caller makes before it brings the queries (their latencies together)
 //   narrow                      some row may see no key of the first piece of tile a
 // Queries lie in their registers; outputs are left in theirs, in units of e^(scale m), with the lane's part of their sums in l.
 // LDS holds SWEEP_BUFFERS tiles from `base` on (with a fourth, and requests two tiles ahead, times were the same).
@@ -204,11 +205,16 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
         src.request(t, arriving);
         arriving = after(arriving);
     };
+    int begun = 0;                                                         // SLIDING: tiles that have been requested
     auto arrive = [&]() {                                                  // the next one too; its successor is on its way
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         ++released;
-        if (released + 1 < src.tiles) request(released + 1);
+        if constexpr (SRC::SLIDING) {
+            if (begun == released + 1 && begun < src.tiles) request(begun++);
+        } else {
+            if (released + 1 < src.tiles) request(released + 1);
+        }
     };
     // One piece of 32 keys by itself, with masks, and values that a weight of zero would not keep out.  Rows that have no reference point
     // take their maximum here; `safe`: all rows do, as the running one.  The weights of a block stand between the MFMAs of the other.
@@ -364,7 +370,17 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
     for (int pass = 0; pass < 2; ++pass) {
         released = -1;
         arriving = base;
-        request(0);
+        if constexpr (SRC::SLIDING) {
+            if (pass == 0) {                                               // (the caller has begun with two)
+                begun = src.tiles < 2 ? src.tiles : 2;
+                arriving = buffer_of(begun);
+            } else {
+                begun = 1;
+                request(0);
+            }
+        } else {
+            request(0);
+        }
         arrive();
         rest();
         static_for<NQ * DT * 4>([&](auto X) __attribute__((always_inline)) { L::template set_regs<O0 + 4 * decltype(X)::value>(0u, 0u, 0u, 0u); });

@@ -23,6 +23,10 @@ struct WindowKeys {
     // the first key of tile t
     __device__ __forceinline__ int key(int t) const { return (t < before ? 0 : t < window ? top - (t - before) : head - 1 - (t - window)) * TILE_ROWS; }
     __device__ __forceinline__ void request(int t, uint32_t buffer) const { fetch.request(key(t), len, buffer, padded); }
+    __device__ __forceinline__ void begin(uint32_t base) const {
+        request(0, base);
+        if (tiles > 1) request(1, base + Buffer<D>::BYTES);
+    }
     __device__ __forceinline__ bool any(int piece) const {
         const int k0 = key(piece / 2) + piece % 2 * SUB;
         return k0 < mine + 32 * NQ && (mine - (k0 + SUB - 1) < band.window || k0 < band.sinks);
@@ -64,23 +68,6 @@ __global__ __launch_bounds__(THREADS, D == 64 && NQ == 2 ? 2 : 1) void window_fw
     }
     const int q0 = s.block * block, mine = q0 + wave / heads * ROWS, last = q0 + block < s.len ? q0 + block : s.len;
     const float c = fabsf(p.scale) * LOG2E;
-    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-    static_for<NQ>([&](auto N) __attribute__((always_inline)) {
-        constexpr int n = decltype(N)::value;
-        const int at = mine + 32 * n + (lane & 31);
-        const uint16_t* row = (const uint16_t*)p.q.p + row_offset(p.q, s, at < s.len ? at : 0, h);
-        uint4 x[KK];
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const int col = 16 * kk + 8 * half;
-            x[kk] = make_uint4(0, 0, 0, 0);
-            if (at < s.len && col < p.D) x[kk] = *(const uint4*)(row + col);
-        }
-        static_for<KK>([&](auto K) __attribute__((always_inline)) {
-            constexpr int kk = decltype(K)::value;
-            L::template set_regs<Q0 + (n * KK + kk) * 4>(x[kk].x ^ flip, x[kk].y ^ flip, x[kk].z ^ flip, x[kk].w ^ flip);
-        });
-    });
     const KeyTiles<true, TILE_ROWS> reach(p.band, q0, last - 1);
     WindowKeys<D, NQ> keys;
     keys.fetch.init(p.k, p.v, s, hk, p.D);
@@ -109,6 +96,24 @@ __global__ __launch_bounds__(THREADS, D == 64 && NQ == 2 ? 2 : 1) void window_fw
     // (weights that are lost below 2^-25 of a row's largest: of the keys that it sees)
     const int64_t most = (int64_t)p.band.window + p.band.sinks;
     keys.lower = lowered_by<E>(most < last ? (int)most : last, c);
+    keys.begin(base);
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+    static_for<NQ>([&](auto N) __attribute__((always_inline)) {
+        constexpr int n = decltype(N)::value;
+        const int at = mine + 32 * n + (lane & 31);
+        const uint16_t* row = (const uint16_t*)p.q.p + row_offset(p.q, s, at < s.len ? at : 0, h);
+        uint4 x[KK];
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int col = 16 * kk + 8 * half;
+            x[kk] = make_uint4(0, 0, 0, 0);
+            if (at < s.len && col < p.D) x[kk] = *(const uint4*)(row + col);
+        }
+        static_for<KK>([&](auto K) __attribute__((always_inline)) {
+            constexpr int kk = decltype(K)::value;
+            L::template set_regs<Q0 + (n * KK + kk) * 4>(x[kk].x ^ flip, x[kk].y ^ flip, x[kk].z ^ flip, x[kk].w ^ flip);
+        });
+    });
     float m[NQ], l[NQ];
     sweep16<E, D, NQ>(keys, base, c, m, l);
     static_for<NQ>([&](auto N) __attribute__((always_inline)) {

@@ -224,11 +224,12 @@ int tree_attention(const void* q, const void* k, const void* v, const void* k_ca
     return narrow ? launch_tree16(p, dtype, st) : launch_tree_f32(p, dtype, st);
 }
 
-// Shares of the streams of blocks of `block` keys in tiles of `tile` queries: about 1024 in all, of 16 tiles at least
+// Shares of the streams of blocks of `block` keys in tiles of `tile` queries: about 1024 in all, of 16 tiles at least (8 of 64 queries)
 void key_shares(KeySums& p, int block, int tile) {
     const int64_t longest = p.band.window && p.band.sinks == 0 && p.band.window + block < p.rows.N ? p.band.window + block : p.rows.N;
     const int64_t blocks = (int64_t)p.rows.B * p.HK * ((p.rows.N + block - 1) / block), tiles = (longest + tile - 1) / tile * p.G, each = (blocks * tiles / 2 + 1023) / 1024;
-    p.chunk = (int)(each < 16 ? 16 : each < tiles ? each : tiles);
+    const int64_t least = tile > 32 ? 8 : 16;
+    p.chunk = (int)(each < least ? least : each < tiles ? each : tiles);
     p.shares = (int)((tiles + p.chunk - 1) / p.chunk);
 }
 size_t key_part_bytes(const KeySums& p) { return p.shares > 1 ? (size_t)p.shares * p.rows.B * p.HK * p.rows.N * sizeof(float) : 0; }
@@ -246,6 +247,15 @@ int make_key_sums(KeySums& p, const int32_t* cu, int sequences, int B, int N, in
     p.band.sinks = p.band.window ? (sinks < N ? sinks : N) : 0;
     key_shares(p, 128, 32);
     return SA2_OK;
+}
+// for the kernels on the 16-bit MFMA
+KeySums narrow_sums(KeySums p) {
+    key_shares(p, KEY_SUMS16_BLOCK, 64);
+    return p;
+}
+size_t key_sums_workspace(const KeySums& p, int dtype, unsigned flags) {
+    const size_t wide = key_part_bytes(p), narrow = causal16_supported(p.D, dtype) && !(flags & SA2_FLAG_FORCE_GENERIC) ? key_part_bytes(narrow_sums(p)) : 0;
+    return wide > narrow ? wide : narrow;                  // (which it is goes by the tensors' alignment)
 }
 
 }  // namespace
@@ -375,7 +385,7 @@ int sa2_window_tree_attention(const void* q, const void* k, const void* v, const
 
 size_t sa2_key_weights_workspace_bytes(int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags) {
     KeySums p;
-    return make_key_sums(p, nullptr, 0, B, N, H, HK, D, window, sinks, 1.f, dtype) == SA2_OK ? key_part_bytes(p) : 0;
+    return make_key_sums(p, nullptr, 0, B, N, H, HK, D, window, sinks, 1.f, dtype) == SA2_OK ? key_sums_workspace(p, dtype, flags) : 0;
 }
 int sa2_key_weights(const void* q, const void* k, const float* lse, float* weights, const int32_t* lengths, int64_t places, void* workspace, size_t workspace_bytes,
                     const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D, const int64_t* strides, int window, int sinks, float scale,
@@ -395,9 +405,10 @@ int sa2_key_weights(const void* q, const void* k, const float* lse, float* weigh
     const int outer = cu_seqlens && lengths ? sequences : B;
     if (!stride_ok(p.q, B, N, H) || !stride_ok(p.k, B, N, HK) || (outer > 1 && p.sb < 1) || (HK > 1 && p.sh < 1)) return SA2_ERR_BAD_STRIDE;
     if (lengths && places < 1) return SA2_ERR_BAD_SHAPE;
-    const size_t need = key_part_bytes(p);
+    const size_t need = key_sums_workspace(p, dtype, flags);
     if (need && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < need)) return SA2_ERR_WORKSPACE_TOO_SMALL;
     p.part = (float*)workspace;
+    if (!(flags & SA2_FLAG_FORCE_GENERIC) && key_sums16_supported(p, dtype)) return launch_key_sums16(narrow_sums(p), dtype, (hipStream_t)hip_stream);
     return launch_key_sums_f32(p, dtype, (hipStream_t)hip_stream);
 }
 

@@ -125,6 +125,9 @@ struct Evict {
     int keep, first, recent;
 };
 
+constexpr int KEY_SUMS16_BLOCK = 256;                      // keys of a workgroup
+bool key_sums16_supported(const KeySums& p, int dtype);
+int launch_key_sums16(const KeySums& p, int dtype, hipStream_t st);
 int launch_key_sums_f32(const KeySums& p, int dtype, hipStream_t st);
 int launch_key_sums_join(const KeySums& p, int block, int tile, hipStream_t st);
 int launch_evict(const Evict& p, int dtype, hipStream_t st);

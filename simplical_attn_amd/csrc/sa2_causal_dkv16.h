@@ -468,8 +468,7 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
                     }
                 }
                 if (i < i1) {
-                    // (32 MFMAs for 16 weights leave room for masks in every step; of the first keys' queries behind their block, all of
-                    // which see them, one run over all heads)
+                    // (of the first keys' queries behind their block, all of which see them, one run over all heads)
                     auto seen = [&](int x, int sub) { return sink && !diagonal ? ~0u : sees((t0 + x) * TILE_ROWS + sub * SUB); };
                     advance(at + i - i0 + 1);
                     L::keep_out();
@@ -487,15 +486,23 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
                     uint32_t next = after(here);
                     step(LONE_C(0), yes, no, rows_at(here, 1), rows_at(next, 0), stats_at(next, 0), 0u, cols_at(here, 0), yes, seen(i, 0));
                     ++i;
+                    auto rounds = [&](auto MASKED, int to) __attribute__((always_inline)) {
+                        auto bits = [&](int x, int sub) { return decltype(MASKED)::value ? seen(x, sub) : 0u; };
 #pragma unroll 1
-                    for (; i < i1; ++i) {
-                        const uint32_t last = here;
-                        here = next;
-                        next = after(here);
-                        advance(at + i - i0 + 1);
-                        step(LONE_C(1), yes, yes, rows_at(here, 0), rows_at(here, 1), stats_at(here, 1), cols_at(last, 0), cols_at(last, 1), yes, seen(i - 1, 1));
-                        step(LONE_C(0), yes, yes, rows_at(here, 1), rows_at(next, 0), stats_at(next, 0), cols_at(last, 1), cols_at(here, 0), yes, seen(i, 0));
-                    }
+                        for (; i < to; ++i) {
+                            const uint32_t last = here;
+                            here = next;
+                            next = after(here);
+                            advance(at + i - i0 + 1);
+                            step(LONE_C(1), yes, yes, rows_at(here, 0), rows_at(here, 1), stats_at(here, 1), cols_at(last, 0), cols_at(last, 1), MASKED, bits(i - 1, 1));
+                            step(LONE_C(0), yes, yes, rows_at(here, 1), rows_at(next, 0), stats_at(next, 0), cols_at(last, 1), cols_at(here, 0), MASKED, bits(i, 0));
+                        }
+                    };
+                    // (tiles from the block's own on and before `clear` are seen whole)
+                    const int reach = sink ? i1 : (mine + p.band.window) / TILE_ROWS - t0, clear = reach < i1 ? reach : i1, whole = diagonal ? OWN + 1 : 0;
+                    rounds(yes, whole < i1 ? whole : i1);
+                    rounds(no, clear);
+                    rounds(yes, i1);
                     step(LONE_C(1), no, yes, 0u, 0u, 0u, cols_at(here, 0), cols_at(here, 1), yes, seen(i1 - 1, 1));
                     static_for<4 * DT - LEAD>([&](auto C) __attribute__((always_inline)) { load_col(LONE_C(decltype(C)::value + LEAD), cols_at(here, 1)); });
                     asm volatile("s_nop 3" : "+v"(pw[1][0]), "+v"(pw[1][1]), "+v"(dw[1][0]), "+v"(dw[1][1]));

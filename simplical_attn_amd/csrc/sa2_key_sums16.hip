@@ -6,22 +6,24 @@
 // A wavefront owns KB blocks of 32 keys: S = Q K^T leaves lane l with key l % 32 and 16 of 32 queries, so that a key's sum is arithmetic within the
 // lane.  Q comes by direct global->LDS loads in tiles of 64 rows, which the four wavefronts and their blocks share; the operands of
 // a product are read once for KB of them.  Scores, exponentials and sums are fp32.
-// Bound by the exponentials: 16 of them, 16 products with the scale and 16 additions take 384 cycles for 32 x 32 scores, the MFMAs 256 (head_dim
-// 128), beside each other where two wavefronts share a SIMD.
+// Bound by issue: a 32 x 32 of scores (head_dim 128) takes 8 MFMAs, 16 exponentials, 16 products with the scale and 16 additions, which run beside
+// each other only where wavefronts share a SIMD; three do (168 registers).  16 heads over 4 key heads, 8192 queries, head_dim 128, bf16: 190 us
+// without a window (0.7 PFLOP/s), 43 us with one of 512.  Tried: both blocks' chains of MFMAs side by side (191 us; 216 where that leaves two
+// wavefronts on a SIMD), requests two tiles ahead (no change).
 #include "sa2_causal16.h"
 #include "sa2_key_sums.h"
 
 namespace sa2 {
 namespace {
 
-constexpr int RING = 3;
+constexpr int RING = 2;
 template <int D>
 struct QueryTile {                                          // 64 rows of Q, and their lse
     static constexpr int STATS = 2 * QuadTile<D>::BYTES, BYTES = STATS + TILE_ROWS * 4;
 };
 
 template <class E, int D, int KB>
-__global__ __launch_bounds__(THREADS, 2) void key_sums16_kernel(KeySums p, bool padded) {
+__global__ __launch_bounds__(THREADS, 3) void key_sums16_kernel(KeySums p, bool padded) {
     using T = QuadTile<D>;
     using X8 = typename E::x8;
     constexpr int KK = D / 16, INSTR = TILE_ROWS / T::RPW / WAVES, BLOCK = 32 * KB * WAVES;
@@ -29,9 +31,9 @@ __global__ __launch_bounds__(THREADS, 2) void key_sums16_kernel(KeySums p, bool 
     const uint32_t base = lds_address(lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int stream, tile;
-    order(blockIdx.x, p.rows.B * p.HK * p.shares, stream, tile);
-    const int share = stream % p.shares;
-    stream /= p.shares;
+    order(blockIdx.x, p.rows.B * p.HK, stream, tile);       // (a block's shares behind each other, so that no XCD has only late, empty ones)
+    const int share = tile % p.shares;
+    tile /= p.shares;
     const int b = stream / p.HK, hk = stream % p.HK;
     Span s;
     if (!find_tile(p.rows, b, tile, BLOCK, s)) return;

@@ -20,9 +20,9 @@ __global__ __launch_bounds__(THREADS) void key_sums_f32_kernel(KeySums p) {
     float* const stats = lds + TILE * Pitch<DP>::value;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     int stream, tile;
-    order(blockIdx.x, p.rows.B * p.HK * p.shares, stream, tile);
-    const int share = stream % p.shares;
-    stream /= p.shares;
+    order(blockIdx.x, p.rows.B * p.HK, stream, tile);       // (a block's shares behind each other, so that no XCD has only late, empty ones)
+    const int share = tile % p.shares;
+    tile /= p.shares;
     const int b = stream / p.HK, hk = stream % p.HK;
     Span s;
     if (!find_tile(p.rows, b, tile, BLOCK, s)) return;

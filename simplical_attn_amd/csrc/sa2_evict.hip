@@ -7,7 +7,8 @@
 namespace sa2 {
 namespace {
 
-constexpr int THREADS = 1024, BINS = 2048;
+constexpr int THREADS = 1024, BINS = 2048, COPIES = 8;      // (lanes count in one of 8 copies: weights of few magnitudes fall into few bins)
+constexpr int CREW = THREADS / 64;
 
 // Weights as integers of the same order; NaN is below all, zeros are equal
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -43,8 +44,8 @@ __device__ __forceinline__ int before_me(int x, int* lds, int& total) {
 }
 
 __global__ __launch_bounds__(THREADS) void choose_kernel(Evict p) {
-    __shared__ int bins[BINS];
-    __shared__ int sums[2][THREADS / 64];
+    __shared__ __attribute__((aligned(16))) int bins[BINS * COPIES];
+    __shared__ int sums[2 * CREW];
     __shared__ int found[2];
     const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, n = evict_held(p, b);
     const float* const w = p.weights + b * p.sb + h * p.sh;
@@ -61,26 +62,42 @@ __global__ __launch_bounds__(THREADS) void choose_kernel(Evict p) {
         return;
     }
     // the smallest weight of the rows from .. to - 1 that stays, and how many of that weight do
-    const int from = p.first, to = n - p.recent;
+    const int from = p.first, to = n - p.recent, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int need = p.keep - p.first - p.recent;
+    const bool any = need > 0;
     uint32_t prefix = 0;
-    if (need > 0) {
+    if (any) {
 #pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass < 2 ? 11 : 10;
-            for (int i = threadIdx.x; i < BINS; i += THREADS) bins[i] = 0;
+            for (int i = threadIdx.x; i < BINS * COPIES / 4; i += THREADS) ((int4*)bins)[i] = make_int4(0, 0, 0, 0);
             __syncthreads();
-            for (int i = from + threadIdx.x; i < to; i += THREADS) {
-                const uint32_t u = ordered(w[i]);
-                if (pass == 0 || u >> (shift + width) == prefix) atomicAdd(&bins[u >> shift & ((1u << width) - 1)], 1);
+            const auto tally = [&](float x) {
+                const uint32_t u = ordered(x);
+                if (pass == 0 || u >> (shift + width) == prefix) atomicAdd(&bins[(u >> shift & ((1u << width) - 1)) * COPIES + threadIdx.x % COPIES], 1);
+            };
+            int64_t i = from + (int)threadIdx.x;
+#pragma unroll 1
+            for (; i + 7 * THREADS < to; i += 8 * THREADS) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = w[i + j * THREADS];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) tally(x[j]);
             }
+#pragma unroll 1
+            for (; i < to; i += THREADS) tally(w[i]);
             __syncthreads();
             // from the highest bin down: the one in which the number that is needed is reached
             const int size = 1 << width, mine = size / THREADS;          // 2 or 1
             int count[2], total;
-            count[0] = bins[size - 1 - mine * threadIdx.x];
-            count[1] = mine == 2 ? bins[size - 2 - 2 * threadIdx.x] : 0;
-            int above = before_me(count[0] + count[1], sums[0], total);
+            const auto of = [&](int bin) {
+                const int4 l = ((const int4*)bins)[2 * bin], h = ((const int4*)bins)[2 * bin + 1];
+                return l.x + l.y + l.z + l.w + h.x + h.y + h.z + h.w;
+            };
+            count[0] = of(size - 1 - mine * threadIdx.x);
+            count[1] = mine == 2 ? of(size - 2 - 2 * threadIdx.x) : 0;
+            int above = before_me(count[0] + count[1], sums, total);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if (j < mine && above < need && above + count[j] >= need) {
@@ -94,86 +111,163 @@ __global__ __launch_bounds__(THREADS) void choose_kernel(Evict p) {
             need = found[1];
         }
     }
-    const bool any = p.keep > p.first + p.recent;
-    // in their order: each thread four rows in a row
-    constexpr int EACH = 4;
-    int placed = 0, equal = 0;
-    for (int base = 0; base < n; base += THREADS * EACH) {
-        const int i0 = base + threadIdx.x * EACH;
-        float x[EACH];
-        bool sure[EACH], same[EACH];
-        int ties = 0;
+    // In their order, 4096 rows at a time: before a row stand the sure ones before it and, of equal weights, no more than are needed.  Within a
+    // wavefront these are bits of ballots, the wavefronts' numbers (sure ones and, 16 bits up, equal ones) go over LDS.
+    const uint64_t lower = ((uint64_t)1 << lane) - 1;
+    int sure_before = 0, same_before = 0;
+    float x[4], next[4];
+    const auto load = [&](int64_t base, float (&to)[4]) {
+        const int64_t i = base + 4 * (int)threadIdx.x;
 #pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-            const int i = i0 + j;
-            x[j] = i < n ? w[i] : 0.f;
+        for (int j = 0; j < 4; ++j) to[j] = i + j < n ? w[i + j] : 0.f;
+    };
+    load(0, x);
+    int turn = 0;
+#pragma unroll 1
+    for (int64_t base = 0; base < n; base += 4 * THREADS, turn ^= 1) {
+        load(base + 4 * THREADS, next);
+        const int64_t i = base + 4 * (int)threadIdx.x;
+        bool sure[4], same[4];
+        int before = 0, all = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
             const uint32_t u = ordered(x[j]);
-            const bool free = i >= from && i < to;
-            sure[j] = i < n && (!free || (any && u > prefix));
+            const bool free = i + j >= from && i + j < to;
+            sure[j] = i + j < n && (!free || (any && u > prefix));
             same[j] = free && any && u == prefix;
-            ties += same[j];
+            const uint64_t of_sure = __ballot(sure[j]), of_same = __ballot(same[j]);
+            before += __popcll(of_sure & lower) + (__popcll(of_same & lower) << 16);
+            all += __popcll(of_sure) + (__popcll(of_same) << 16);
         }
-        int total;
-        int rank = equal + before_me(ties, sums[0], total);
-        equal += total;
-        int count = 0;
+        if (lane == 0) sums[turn * CREW + wave] = all;
+        __syncthreads();
+        all = 0;
 #pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-            if (same[j] && rank++ < need) sure[j] = true;
-            count += sure[j];
+        for (int c = 0; c < CREW; ++c) {
+            const int y = sums[turn * CREW + c];
+            before += c < wave ? y : 0;
+            all += y;
         }
-        int to_place = placed + before_me(count, sums[1], total);
-        placed += total;
+        int place = sure_before + (before & 0xffff), equal = same_before + (before >> 16);
 #pragma unroll
-        for (int j = 0; j < EACH; ++j)
-            if (sure[j]) {
-                left[to_place] = x[j];
-                kept[to_place++] = i0 + j;
+        for (int j = 0; j < 4; ++j) {
+            if (sure[j] || (same[j] && equal < need)) {
+                const int64_t to = place + (int64_t)(equal < need ? equal : need);
+                left[to] = x[j];
+                kept[to] = (int)i + j;
             }
+            place += sure[j];
+            equal += same[j];
+            x[j] = next[j];
+        }
+        sure_before += all & 0xffff;
+        same_before += all >> 16;
     }
 }
 
-// Rows to their new places.  A workgroup has `SLICE` pieces of every row of one tensor of a sequence's head and takes the rows in steps:
-// reads of a step end before its writes begin, and what later steps read lies behind what this one writes (kept[i] >= i).
-constexpr int MOVERS = 256, SLICE = 4, STEP = 8 * MOVERS / SLICE;
+// Rows to their new places.  A workgroup has `SLICE` pieces of every row of one tensor of a sequence's head and takes the rows in steps.  What
+// the rows of a step lie behind is not written before them (kept[i] >= i), so that reads may run ahead of writes, never behind: each step's
+// rows are asked for a step early, their pages two and their numbers three, and a step's writes begin when all of its reads have ended.
+typedef uint32_t Quad __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint32_t word(Quad x) { return x.x; }
+__device__ __forceinline__ uint32_t word(uint32_t x) { return x; }
+constexpr int MOVERS = 512, SLICE = 4, EACH = 8, STEP = EACH * MOVERS / SLICE;
+// r / d = r * factor >> shift for r < 2^31: with 2^l >= d, factor d = 2^(31 + l) + e, 0 < e <= 2^l, the product's error is below 1 / d
+struct Quotient {
+    uint32_t factor;
+    int shift;
+};
+Quotient quotient(uint32_t d) {
+    int l = 0;
+    while ((uint64_t)1 << l < d) ++l;
+    return Quotient{(uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), 31 + l};
+}
+__device__ const Quad nothing = {0, 0, 0, 0};
 template <class UNIT>
-__global__ __launch_bounds__(MOVERS) void move_kernel(Evict p, int size, int pieces, int slices) {
-    const int slice = blockIdx.x % slices, which = blockIdx.x / slices % 2, stream = blockIdx.x / slices / 2, b = stream / p.HK, hk = stream % p.HK;
+__global__ __launch_bounds__(MOVERS) void move_kernel(Evict p, Quotient pages_in, int size, int pieces, int slices) {
+    int slice, stream;                                      // slices of the same rows on the same XCD, whose cache lines they share
+    const int streams = p.B * p.HK * 2, pid = blockIdx.x;
+    if (streams % 8 == 0) {
+        slice = (pid >> 3) % slices;
+        stream = (pid >> 3) / slices * 8 + (pid & 7);
+    } else {
+        slice = pid / streams;
+        stream = pid % streams;
+    }
+    const int which = stream & 1, b = (stream >> 1) / p.HK, hk = (stream >> 1) % p.HK;
     const int n = evict_held(p, b), piece = slice * SLICE + threadIdx.x % SLICE, mine = threadIdx.x / SLICE;
     if (n <= p.keep) return;
     const int32_t* const kept = p.kept + ((int64_t)b * p.heads + (p.heads > 1 ? hk : 0)) * p.keep;
+    const int32_t* const table = p.cache.table ? p.cache.table + (int64_t)b * p.cache.width : nullptr;
     const Tensor& t = which ? p.cache.v : p.cache.k;
-    auto row = [&](int r) -> UNIT* {
-        int64_t page = b;
-        int at = r;
-        if (p.cache.table) {
-            const int i = (int)((unsigned)r / (unsigned)p.cache.page_size);
-            page = p.cache.table[(int64_t)b * p.cache.width + i];
-            at = r - i * p.cache.page_size;
-            if (page < 0 || page >= p.cache.pages) return nullptr;
-        }
-        return (UNIT*)((char*)t.p + t.off(page, at, hk) * size) + piece;
-    };
-    for (int i0 = 0; i0 < p.keep; i0 += STEP) {
-        UNIT x[8];
-        UNIT* to[8];
+    char* const origin = (char*)t.p + (hk * t.sh + (int64_t)piece * (sizeof(UNIT) / size)) * size;
+    const bool has = piece < pieces;
+    const unsigned keep = p.keep;
+    const auto place = [&](int step, int u) { return (unsigned)step * STEP + u * (MOVERS / SLICE) + mine; };        // (may pass 31 bits behind the last row)
+    const auto page_of = [&](unsigned r) { return table ? (int)((uint64_t)r * pages_in.factor >> pages_in.shift) : 0; };
+    const auto numbers = [&](int step, int (&from)[EACH]) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int i = i0 + u * (MOVERS / SLICE) + mine, from = i < p.keep ? kept[i] : -1;
-            to[u] = nullptr;
-            if (from > i && piece < pieces) {
-                const UNIT* const src = row(from);
-                if (src) {
-                    to[u] = row(i);
-                    x[u] = *src;
-                }
-            }
+        for (int u = 0; u < EACH; ++u) {
+            const unsigned i = place(step, u);
+            from[u] = kept[i < keep ? i : keep - 1];
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    const auto pages = [&](int step, const int (&from)[EACH], int (&src)[EACH], int (&dst)[EACH]) {
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            const unsigned i = place(step, u);
+            src[u] = table ? table[page_of(from[u])] : b;
+            dst[u] = table ? table[page_of(i < keep ? i : keep - 1)] : b;
+        }
+    };
+    const auto at = [&](int page, unsigned r) { return origin + ((int64_t)page * t.sb + (int64_t)(int)(r - page_of(r) * p.cache.page_size) * t.sn) * size; };
+    const auto moves = [&](int step, int u, int from, int src, int dst) {
+        const unsigned i = place(step, u);
+        return has && i < keep && (unsigned)from > i && (unsigned)src < (unsigned)p.cache.pages && (unsigned)dst < (unsigned)p.cache.pages;
+    };
+    const auto reads = [&](int step, const int (&from)[EACH], const int (&src)[EACH], const int (&dst)[EACH], UNIT (&x)[EACH], UNIT* (&to)[EACH]) {
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            const bool go = moves(step, u, from[u], src[u], dst[u]);
+            x[u] = *(go ? (const UNIT*)at(src[u], from[u]) : (const UNIT*)&nothing);
+            to[u] = go ? (UNIT*)at(dst[u], place(step, u)) : nullptr;
+        }
+    };
+    const int steps = (p.keep + STEP - 1) / STEP;
+    int from0[EACH], from1[EACH], from2[EACH], src1[EACH], dst1[EACH];
+    UNIT x[EACH];
+    UNIT* to[EACH];
+    numbers(0, from0);
+    numbers(1, from1);
+    numbers(2, from2);
+    {
+        int src0[EACH], dst0[EACH];
+        pages(0, from0, src0, dst0);
+        pages(1, from1, src1, dst1);
+        reads(0, from0, src0, dst0, x, to);
+    }
+    for (int step = 0; step < steps; ++step) {
+        int from3[EACH], src2[EACH], dst2[EACH];
+        UNIT next[EACH];
+        UNIT* next_to[EACH];
+        numbers(step + 3, from3);
+        pages(step + 2, from2, src2, dst2);
+        reads(step + 1, from1, src1, dst1, next, next_to);
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) asm volatile("" ::"v"(word(x[u])) : "memory");       // (has come)
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < EACH; ++u)
             if (to[u]) *to[u] = x[u];
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            x[u] = next[u];
+            to[u] = next_to[u];
+            from1[u] = from2[u];
+            from2[u] = from3[u];
+            src1[u] = src2[u];
+            dst1[u] = dst2[u];
+        }
     }
 }
 
@@ -188,9 +282,10 @@ int launch_evict(const Evict& p, int dtype, hipStream_t st) {
     choose_kernel<<<dim3((unsigned)(p.B * p.heads)), dim3(THREADS), 0, st>>>(p);
     if (hipGetLastError() != hipSuccess) return SA2_ERR_LAUNCH_FAILED;
     const dim3 blocks((unsigned)grid), block(MOVERS);
-    if (wide) move_kernel<uint4><<<blocks, block, 0, st>>>(p, size, pieces, slices);
-    else if (size == 4) move_kernel<uint32_t><<<blocks, block, 0, st>>>(p, size, pieces, slices);
-    else move_kernel<uint16_t><<<blocks, block, 0, st>>>(p, size, pieces, slices);
+    const Quotient pages_in = quotient(p.cache.page_size);
+    if (wide) move_kernel<Quad><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
+    else if (size == 4) move_kernel<uint32_t><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
+    else move_kernel<uint16_t><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 

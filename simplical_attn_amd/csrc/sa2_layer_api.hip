@@ -224,7 +224,9 @@ int tree_attention(const void* q, const void* k, const void* v, const void* k_ca
     return narrow ? launch_tree16(p, dtype, st) : launch_tree_f32(p, dtype, st);
 }
 
-// Shares of the streams of blocks of `block` keys in tiles of `tile` queries: about `all` of them, of `least` tiles or more
+// Shares of the streams of blocks of `block` keys in tiles of `tile` queries: about `all` of them, of `least` tiles or more.  Short prompts in many
+// short shares: 512 queries of 16 heads over 4 key heads (head_dim 128) take 16 us with 4 tiles of 64 and 24 with 8, in fp32 23 with 2 tiles of
+// 32 and 52 with 16; below these numbers the workgroups' starts and the join cost as much as they save.
 void key_shares(KeySums& p, int block, int tile, int all, int least) {
     const int64_t longest = p.band.window && p.band.sinks == 0 && p.band.window + block < p.rows.N ? p.band.window + block : p.rows.N;
     const int64_t blocks = (int64_t)p.rows.B * p.HK * ((p.rows.N + block - 1) / block), tiles = (longest + tile - 1) / tile * p.G, each = (blocks * tiles / 2 + all - 1) / all;
@@ -244,13 +246,13 @@ int make_key_sums(KeySums& p, const int32_t* cu, int sequences, int B, int N, in
     p.scale = scale;
     p.band.window = window < N ? window : 0;
     p.band.sinks = p.band.window ? (sinks < N ? sinks : N) : 0;
-    key_shares(p, 128, 32, 1024, 16);
+    key_shares(p, 128, 32, 1024, 2);
     return SA2_OK;
 }
 // for the kernels on the 16-bit MFMA.  4096 shares are more than fit on the card at once, so that the short ones of packed prompts fill the gaps:
 // six of 8100 queries in all 97 us (1024: 158, 2048: 112)
 KeySums narrow_sums(KeySums p) {
-    key_shares(p, KEY_SUMS16_BLOCK, 64, 4096, 8);
+    key_shares(p, KEY_SUMS16_BLOCK, 64, 4096, 4);
     return p;
 }
 size_t key_sums_workspace(const KeySums& p, int dtype, unsigned flags) {

@@ -7,8 +7,7 @@ int launch_window_tree16(const Tree& p, int dtype, hipStream_t st) {
     // (the kernel for large trees leaves no scores; a tree of one node is large from 65 query heads per key head on)
     const int rc = tree16_rows(p) > 64 && !p.scores ? launch_window_tree_rows16(p, dtype, st) : launch_tree16_of<true>(p, dtype, st);
     if (rc != SA2_OK || (p.nsplit == 1 && !p.scores)) return rc;
-    const int joined = launch_tree_join(p, dtype, st);
-    return joined == SA2_OK && p.scores ? launch_tree_weights(p, dtype, dtype == SA2_F16 ? 15.f : 0.f, st) : joined;
+    return p.scores ? launch_tree_weights(p, dtype, dtype == SA2_F16 ? 15.f : 0.f, st) : launch_tree_join(p, dtype, st);
 }
 
 }  // namespace sa2

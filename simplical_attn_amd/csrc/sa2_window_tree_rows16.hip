@@ -1,4 +1,4 @@
-// Launches of large drafted trees with a window on the 16-bit MFMA (sa2_tree_rows16.h).
+// Launches of large drafted trees with a window on the 16-bit MFMA (sa2_tree_rows16.h): work and bounds are those of the kernel without a window, over the tiles in reach.
 #include "sa2_tree_rows16.h"
 
 namespace sa2 {

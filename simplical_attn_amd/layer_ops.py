@@ -1,5 +1,6 @@
 """Operators of the ordinary attention layers that stand between 2-simplicial ones: rotary positions, causal attention
-over whole prompts, rows of a cache of keys and values, and attention of drafted tokens over it.
+over whole prompts, rows of a cache of keys and values, and attention of drafted tokens over it; windows with first keys
+that stay visible, and the eviction of cached rows by the attention weight they gathered.
 
 The kernels are the HIP library's (include/sa2.h), reached by the native host path (csrc/host/sa2_torch_layers.cpp), which
 checks every argument, makes outputs and workspaces and holds the autograd formulas.  Like the rest of the package they

@@ -302,10 +302,11 @@ int sa2_window_tree_attention(const void* q, const void* k, const void* v, const
  *   lengths      NULL: weights [B,HK,N] (packed: [HK,N], zero for rows of no sequence) are overwritten.  Else weights
  *                [sequences,HK,places], and key a of sequence b is added at place lengths[b] + a, where that is below `places`
  *   strides      q, k (3 int64 each), then weights' batch (or sequence) and head
- *   workspace    sa2_key_weights_workspace_bytes(...) bytes, 256-byte aligned (0 bytes: may be NULL); contents on entry ignored
+ *   sinks        at most 65535 (or the rows): SA2_ERR_TOO_LARGE
+ *   workspace    sa2_key_weights_workspace_bytes(...) bytes (sequences 0: not packed), 256-byte aligned (0 bytes: may be NULL); contents on entry ignored
  * No atomics: two calls on the same inputs give identical bits.
  */
-size_t sa2_key_weights_workspace_bytes(int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags);
+size_t sa2_key_weights_workspace_bytes(int sequences, int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags);
 int sa2_key_weights(const void* q, const void* k, const float* lse, float* weights, const int32_t* lengths, int64_t places, void* workspace, size_t workspace_bytes,
                     const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D, const int64_t* strides, int window, int sinks, float scale,
                     int dtype, unsigned flags, void* hip_stream);
@@ -318,7 +319,7 @@ int sa2_key_weights(const void* q, const void* k, const float* lse, float* weigh
  *   left         [B,heads,places] contiguous: the weights of the rows that stay, at their new places, zeros behind
  *   kept         [B,heads,keep] contiguous: the places that the rows had, ascending, -1 behind them
  *   strides      k_cache, v_cache (page, row, head), then weights' batch and head
- * Rows in pages that are not in 0 .. pages-1 are chosen like others; what would come from or go there is left out.  What the places
+ * No two sequences share a page, and no memory is both cache's.  Rows in pages that are not in 0 .. pages-1 are chosen like others; what would come from or go there is left out.  What the places
  * from keep on hold is as it was.
  */
 int sa2_cache_evict(void* k_cache, void* v_cache, const float* weights, float* left, int32_t* kept, const int32_t* lengths, const int32_t* page_table,

@@ -95,7 +95,7 @@ def load():
     lib.sa2_window_tree_attention.restype = c_int
     lib.sa2_window_tree_attention.argtypes = ([c_void_p] * 11 + [c_size_t] + [c_int] * 8 + [i64p, c_int, c_int, c_float, c_int, c_uint, c_void_p])
     lib.sa2_key_weights_workspace_bytes.restype = c_size_t
-    lib.sa2_key_weights_workspace_bytes.argtypes = [c_int] * 8 + [c_uint]
+    lib.sa2_key_weights_workspace_bytes.argtypes = [c_int] * 9 + [c_uint]
     lib.sa2_key_weights.restype = c_int
     lib.sa2_key_weights.argtypes = ([c_void_p] * 5 + [ctypes.c_int64, c_void_p, c_size_t, c_void_p] + [c_int] * 6 + [i64p, c_int, c_int, c_float, c_int, c_uint, c_void_p])
     lib.sa2_cache_evict.restype = c_int

@@ -524,7 +524,7 @@ Maybe key_weights(const Tensor& q_, const Tensor& k_, const Tensor& lse, const M
         if (!weights) out.zero_();                 // (keys that no query head reads)
         return result;
     }
-    const size_t bytes = key_weights_ws_fn(z.B, z.N, z.H, hk, z.D, reach, first, dtype_code(q), flags);
+    const size_t bytes = key_weights_ws_fn(ends.defined() ? (int)ends.numel() - 1 : 0, z.B, z.N, z.H, hk, z.D, reach, first, dtype_code(q), flags);
     const Tensor ws = bytes ? workspace(q, bytes) : Tensor();
     int64_t s[8];
     put_strides(s, q);
@@ -549,6 +549,7 @@ std::pair<Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_cache, co
     TORCH_CHECK_VALUE(keep >= 1 && first >= 0 && recent >= 0 && keep < ((int64_t)1 << 31) && first + recent <= keep, "keep must be at least 1, first and recent at least 0 and together at most keep, got ", keep, ", ", first, ", ", recent);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (k_cache.requires_grad() || v_cache.requires_grad() || weights.requires_grad())), "cache_evict has no gradient: call it under torch.no_grad() or on detached tensors");
     TORCH_CHECK(c10::InferenceMode::is_enabled() || !(k_cache.is_inference() || v_cache.is_inference()), "cache_evict changes the cache in place, which inference tensors allow in inference mode only");
+    TORCH_CHECK_VALUE(k_cache.numel() == 0 || k_cache.const_data_ptr() != v_cache.const_data_ptr(), "k_cache and v_cache are the same memory, whose rows would move twice");
     check_place("cache_evict", {k_cache, v_cache, weights});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;

@@ -30,13 +30,10 @@ __global__ __launch_bounds__(THREADS, 3) void key_sums16_kernel(KeySums p, bool 
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t base = lds_address(lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    int stream, tile;
-    order(blockIdx.x, p.rows.B * p.HK, stream, tile);       // (a block's shares behind each other, so that no XCD has only late, empty ones)
-    const int share = tile % p.shares;
-    tile /= p.shares;
-    const int b = stream / p.HK, hk = stream % p.HK;
-    Span s;
-    if (!find_tile(p.rows, b, tile, BLOCK, s)) return;
+    KeyBlock w;
+    if (!key_block(p, blockIdx.x, BLOCK, w)) return;
+    const Span& s = w.s;
+    const int hk = w.hk, share = w.share;
     if (s.fill) {
         if (share == 0)
             for (int i = threadIdx.x; i < s.len; i += THREADS) put_key_sum(p, s, hk, i, 0.f);
@@ -45,7 +42,7 @@ __global__ __launch_bounds__(THREADS, 3) void key_sums16_kernel(KeySums p, bool 
     const int j0 = s.block * BLOCK, mine = j0 + wave * 32 * KB;
     const KeyStream of = key_stream(p, s, j0, BLOCK, TILE_ROWS);
     const int64_t all = (int64_t)of.per * p.G;
-    const int lo = share * p.chunk, hi = all - lo < p.chunk ? (int)all : lo + p.chunk;
+    const int lo = share * w.chunk, hi = all - lo < w.chunk ? (int)all : lo + w.chunk;
     if (lo >= hi) return;
 
     // tiles of the stream to LDS, each wavefront a quarter
@@ -80,10 +77,10 @@ __global__ __launch_bounds__(THREADS, 3) void key_sums16_kernel(KeySums p, bool 
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
             const int col = 16 * kk + 8 * half;
-            union { uint4 u; X8 x; } w;
-            w.u = make_uint4(0, 0, 0, 0);
-            if (key < s.len && col < p.D) w.u = *(const uint4*)(row + col);
-            k[n][kk] = w.x;
+            union { uint4 u; X8 x; } word;
+            word.u = make_uint4(0, 0, 0, 0);
+            if (key < s.len && col < p.D) word.u = *(const uint4*)(row + col);
+            k[n][kk] = word.x;
         }
     }
     const float c = p.scale * LOG2E;
@@ -139,15 +136,15 @@ __global__ __launch_bounds__(THREADS, 3) void key_sums16_kernel(KeySums p, bool 
         const float both = sum[n] + other_half(sum[n]);
         const int key = mine + 32 * n + (lane & 31);
         if (half || key >= s.len) continue;
-        if (p.shares == 1) put_key_sum(p, s, hk, key, both);
-        else p.part[(((int64_t)share * p.rows.B + s.b) * p.HK + hk) * p.rows.N + s.first + key] = both;
+        if (w.to) w.to[key] = both;
+        else put_key_sum(p, s, hk, key, both);
     }
 }
 
 template <class E, int D, int KB>
 int launch(const KeySums& p, hipStream_t st) {
     const auto kernel = key_sums16_kernel<E, D, KB>;
-    const int64_t grid = (int64_t)p.rows.B * p.HK * p.shares * count_tiles(p.rows, 32 * KB * WAVES);
+    const int64_t grid = p.front_grid + key_blocks(p, 32 * KB * WAVES);
     if (grid > 0x7fffffff) return SA2_ERR_TOO_LARGE;
     if (!allow_full_lds((const void*)kernel)) return SA2_ERR_LAUNCH_FAILED;
     kernel<<<dim3((unsigned)grid), dim3(THREADS), RING * QueryTile<D>::BYTES, st>>>(p, p.D != D);
@@ -167,7 +164,7 @@ int launch_key_sums16(const KeySums& p, int dtype, hipStream_t st) {
         return p.D <= 64 ? launch<E, 64, KEY_SUMS16_BLOCK / 128>(p, st) : launch<E, 128, KEY_SUMS16_BLOCK / 128>(p, st);
     };
     const int rc = dtype == SA2_F16 ? of(ElemF16{}) : of(ElemBF16{});
-    return rc == SA2_OK && p.shares > 1 ? launch_key_sums_join(p, KEY_SUMS16_BLOCK, TILE_ROWS, st) : rc;
+    return rc == SA2_OK && (p.shares > 1 || p.front_shares > 1) ? launch_key_sums_join(p, KEY_SUMS16_BLOCK, TILE_ROWS, st) : rc;
 }
 
 }  // namespace sa2

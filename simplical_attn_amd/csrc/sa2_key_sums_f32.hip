@@ -20,13 +20,10 @@ __global__ __launch_bounds__(THREADS) void key_sums_f32_kernel(KeySums p) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float* const stats = lds + TILE * Pitch<DP>::value;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    int stream, tile;
-    order(blockIdx.x, p.rows.B * p.HK, stream, tile);       // (a block's shares behind each other, so that no XCD has only late, empty ones)
-    const int share = tile % p.shares;
-    tile /= p.shares;
-    const int b = stream / p.HK, hk = stream % p.HK;
-    Span s;
-    if (!find_tile(p.rows, b, tile, BLOCK, s)) return;
+    KeyBlock w;
+    if (!key_block(p, blockIdx.x, BLOCK, w)) return;
+    const Span& s = w.s;
+    const int hk = w.hk, share = w.share;
     if (s.fill) {
         if (share == 0)
             for (int i = threadIdx.x; i < s.len; i += THREADS) put_key_sum(p, s, hk, i, 0.f);
@@ -35,7 +32,7 @@ __global__ __launch_bounds__(THREADS) void key_sums_f32_kernel(KeySums p) {
     const int j0 = s.block * BLOCK, mine = j0 + wave * TILE, key = mine + (lane & 31);
     const KeyStream of = key_stream(p, s, j0, BLOCK, TILE);
     const int64_t all = (int64_t)of.per * p.G;
-    const int lo = share * p.chunk, hi = all - lo < p.chunk ? (int)all : lo + p.chunk;
+    const int lo = share * w.chunk, hi = all - lo < w.chunk ? (int)all : lo + w.chunk;
     if (lo >= hi) return;
     float k[DP / 2];
     own_rows<T, DP>(k, p.k, s, mine, hk, p.D, WIDE, 1.f);
@@ -68,22 +65,22 @@ __global__ __launch_bounds__(THREADS) void key_sums_f32_kernel(KeySums p) {
         const int q0 = of.lo + it % of.per * TILE;
         const uint32_t seen = key_all_seen(p, s, q0, q0 + TILE - 1, mine, mine + TILE - 1) ? ~0u : key_seen_by(p, s, key, q0);
         if (!__any(seen != 0)) continue;
-        const floatx16 w = tile_product<DP>(lds, k);
+        const floatx16 x = tile_product<DP>(lds, k);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const float4 l = *(const float4*)(stats + 8 * g + 4 * half);
             const float* const ls = &l.x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float e = exp2f(fmaf(w[4 * g + r], c, -ls[r]));
+                const float e = exp2f(fmaf(x[4 * g + r], c, -ls[r]));
                 sum += seen >> (8 * g + 4 * half + r) & 1 ? e : 0.f;
             }
         }
     }
     sum += other_half(sum);
     if (half || key >= s.len) return;
-    if (p.shares == 1) put_key_sum(p, s, hk, key, sum);
-    else p.part[(((int64_t)share * p.rows.B + s.b) * p.HK + hk) * p.rows.N + s.first + key] = sum;
+    if (w.to) w.to[key] = sum;
+    else put_key_sum(p, s, hk, key, sum);
 }
 
 // The sums of the shares, in their order: a thread per key
@@ -95,9 +92,18 @@ __global__ __launch_bounds__(THREADS) void key_sums_join_kernel(KeySums p, int b
     if (!find_tile(p.rows, b, at, THREADS, s) || s.fill) return;
     const int key = s.block * THREADS + threadIdx.x;
     if (key >= s.len) return;
-    const int64_t all = (int64_t)key_stream(p, s, key / block * block, block, tile).per * p.G, step = (int64_t)p.rows.B * p.HK * p.rows.N;
-    const int n = (int)((all + p.chunk - 1) / p.chunk);
-    const float* const from = p.part + ((int64_t)s.b * p.HK + hk) * p.rows.N + s.first + key;
+    const bool front = key < p.front;
+    if ((front ? p.front_shares : p.shares) == 1) return;   // (is where it belongs)
+    const int64_t all = (int64_t)key_stream(p, s, key / block * block, block, tile).per * p.G;
+    const int chunk = front ? p.front_chunk : p.chunk, n = (int)((all + chunk - 1) / chunk);
+    int64_t step = (int64_t)p.rows.B * p.HK * p.rows.N;
+    const float* from = p.part + ((int64_t)s.b * p.HK + hk) * p.rows.N + s.first + key;
+    if (front) {
+        const int sequence = p.rows.cu ? sequence_of(p.rows, s.first) : s.b;
+        if (sequence < 0) return;
+        step = (int64_t)(p.rows.cu ? p.rows.sequences : p.rows.B) * p.HK * p.front;
+        from = p.front_part + ((int64_t)sequence * p.HK + hk) * p.front + key;
+    }
     float sum = 0.f;
     for (int i = 0; i < n; i += 8) {                        // (eight reads under way, added in order)
         float x[8];
@@ -126,7 +132,7 @@ int launch_key_sums_f32(const KeySums& p, int dtype, hipStream_t st) {
         for (const Tensor* t : {&p.q, &p.k}) wide = wide && (uintptr_t)t->p % BYTES == 0 && t->sn % 4 == 0 && t->sh % 4 == 0 && (p.rows.B == 1 || t->sb % 4 == 0);
         return for_width(p.D, [&](auto w) {
             constexpr int DP = decltype(w)::value;
-            const int64_t grid = (int64_t)p.rows.B * p.HK * p.shares * count_tiles(p.rows, BLOCK);
+            const int64_t grid = p.front_grid + key_blocks(p, BLOCK);
             if (grid > 0x7fffffff) return (int)SA2_ERR_TOO_LARGE;
             const auto kernel = wide ? key_sums_f32_kernel<T, DP, true> : key_sums_f32_kernel<T, DP, false>;
             if (!allow_full_lds((const void*)kernel)) return (int)SA2_ERR_LAUNCH_FAILED;
@@ -134,7 +140,7 @@ int launch_key_sums_f32(const KeySums& p, int dtype, hipStream_t st) {
             return (int)(hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED);
         });
     });
-    return rc == SA2_OK && p.shares > 1 ? launch_key_sums_join(p, BLOCK, TILE, st) : rc;
+    return rc == SA2_OK && (p.shares > 1 || p.front_shares > 1) ? launch_key_sums_join(p, BLOCK, TILE, st) : rc;
 }
 
 }  // namespace sa2

@@ -228,12 +228,30 @@ int tree_attention(const void* q, const void* k, const void* v, const void* k_ca
 // short shares: 512 queries of 16 heads over 4 key heads (head_dim 128) take 16 us with 4 tiles of 64 and 24 with 8, in fp32 23 with 2 tiles of
 // 32 and 52 with 16; below these numbers the workgroups' starts and the join cost as much as they save.
 void key_shares(KeySums& p, int block, int tile, int all, int least) {
-    const int64_t longest = p.band.window && p.band.sinks == 0 && p.band.window + block < p.rows.N ? p.band.window + block : p.rows.N;
-    const int64_t blocks = (int64_t)p.rows.B * p.HK * ((p.rows.N + block - 1) / block), tiles = (longest + tile - 1) / tile * p.G, each = (blocks * tiles / 2 + all - 1) / all;
-    p.chunk = (int)(each < least ? least : each < tiles ? each : tiles);
-    p.shares = (int)((tiles + p.chunk - 1) / p.chunk);
+    const int64_t N = p.rows.N, streams = (int64_t)p.rows.B * p.HK, longest = p.band.window && p.band.window + block < N ? p.band.window + block : N;
+    const auto cut = [&](int64_t tiles, int64_t each) { return (int)(each < least ? least : each < tiles ? each : tiles); };
+    const auto shares = [](int64_t tiles, int chunk) { return (int)((tiles + chunk - 1) / chunk); };
+    const int64_t tiles = (longest + tile - 1) / tile * p.G, work = streams * ((N + block - 1) / block) * tiles / (p.band.window ? 1 : 2);
+    p.chunk = cut(tiles, (work + all - 1) / all);
+    p.shares = shares(tiles, p.chunk);
+    p.front_shares = 1;
+    if (!p.band.sinks) return;
+    // (a block of the first keys: of every sequence, whatever its length)
+    const int64_t blocks = (p.band.sinks + block - 1) / block, whole = (N + tile - 1) / tile * p.G, of_all = (int64_t)(p.rows.sequences ? p.rows.sequences : p.rows.B) * p.HK * blocks;
+    p.front = (int)(blocks * block);
+    p.front_chunk = cut(whole, (streams * blocks * whole + 1023) / 1024);
+    p.front_shares = shares(whole, p.front_chunk);
+    if (of_all * p.front_shares > 65536) {
+        p.front_shares = of_all >= 65536 ? 1 : (int)(65536 / of_all);
+        p.front_chunk = shares(whole, p.front_shares);
+    }
+    const int64_t grid = (of_all * p.front_shares + 7) / 8 * 8;
+    p.front_grid = grid > 0x7fffffff ? -1 : (int)grid;
 }
-size_t key_part_bytes(const KeySums& p) { return p.shares > 1 ? (size_t)p.shares * p.rows.B * p.HK * p.rows.N * sizeof(float) : 0; }
+size_t key_part_bytes(const KeySums& p) { return p.shares > 1 ? ((size_t)p.shares * p.rows.B * p.HK * p.rows.N * sizeof(float) + 255) / 256 * 256 : 0; }
+size_t key_parts_bytes(const KeySums& p) {
+    return key_part_bytes(p) + (p.front_shares > 1 ? (size_t)p.front_shares * (p.rows.sequences ? p.rows.sequences : p.rows.B) * p.HK * p.front * sizeof(float) : 0);
+}
 
 int make_key_sums(KeySums& p, const int32_t* cu, int sequences, int B, int N, int H, int HK, int D, int window, int sinks, float scale, int dtype) {
     Causal c;
@@ -246,6 +264,7 @@ int make_key_sums(KeySums& p, const int32_t* cu, int sequences, int B, int N, in
     p.scale = scale;
     p.band.window = window < N ? window : 0;
     p.band.sinks = p.band.window ? (sinks < N ? sinks : N) : 0;
+    if (p.band.sinks > 65535) return SA2_ERR_TOO_LARGE;
     key_shares(p, 128, 32, 1024, 2);
     return SA2_OK;
 }
@@ -256,7 +275,7 @@ KeySums narrow_sums(KeySums p) {
     return p;
 }
 size_t key_sums_workspace(const KeySums& p, int dtype, unsigned flags) {
-    const size_t wide = key_part_bytes(p), narrow = causal16_supported(p.D, dtype) && !(flags & SA2_FLAG_FORCE_GENERIC) ? key_part_bytes(narrow_sums(p)) : 0;
+    const size_t wide = key_parts_bytes(p), narrow = causal16_supported(p.D, dtype) && !(flags & SA2_FLAG_FORCE_GENERIC) ? key_parts_bytes(narrow_sums(p)) : 0;
     return wide > narrow ? wide : narrow;                  // (which it is goes by the tensors' alignment)
 }
 
@@ -385,9 +404,10 @@ int sa2_window_tree_attention(const void* q, const void* k, const void* v, const
                           scale, dtype, flags, hip_stream);
 }
 
-size_t sa2_key_weights_workspace_bytes(int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags) {
+size_t sa2_key_weights_workspace_bytes(int sequences, int B, int N, int H, int HK, int D, int window, int sinks, int dtype, unsigned flags) {
     KeySums p;
-    return make_key_sums(p, nullptr, 0, B, N, H, HK, D, window, sinks, 1.f, dtype) == SA2_OK ? key_sums_workspace(p, dtype, flags) : 0;
+    static const int32_t packed = 0;                       // (only whether there are packed sequences counts here)
+    return make_key_sums(p, sequences > 0 ? &packed : nullptr, sequences, B, N, H, HK, D, window, sinks, 1.f, dtype) == SA2_OK ? key_sums_workspace(p, dtype, flags) : 0;
 }
 int sa2_key_weights(const void* q, const void* k, const float* lse, float* weights, const int32_t* lengths, int64_t places, void* workspace, size_t workspace_bytes,
                     const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D, const int64_t* strides, int window, int sinks, float scale,
@@ -409,8 +429,12 @@ int sa2_key_weights(const void* q, const void* k, const float* lse, float* weigh
     if (lengths && places < 1) return SA2_ERR_BAD_SHAPE;
     const size_t need = key_sums_workspace(p, dtype, flags);
     if (need && (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < need)) return SA2_ERR_WORKSPACE_TOO_SMALL;
+    const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && key_sums16_supported(p, dtype);
+    if (narrow) p = narrow_sums(p);
+    if (p.front_grid < 0) return SA2_ERR_TOO_LARGE;
     p.part = (float*)workspace;
-    if (!(flags & SA2_FLAG_FORCE_GENERIC) && key_sums16_supported(p, dtype)) return launch_key_sums16(narrow_sums(p), dtype, (hipStream_t)hip_stream);
+    p.front_part = (float*)((char*)workspace + key_part_bytes(p));
+    if (narrow) return launch_key_sums16(p, dtype, (hipStream_t)hip_stream);
     return launch_key_sums_f32(p, dtype, (hipStream_t)hip_stream);
 }
 

@@ -106,6 +106,10 @@ struct KeySums {
     Band band;                                 // (window, sinks)
     float* part;
     int shares, chunk;
+    // With a window, the blocks of the first keys, which all queries see: `front` keys of every sequence, in shares of their own
+    int front, front_shares, front_chunk;
+    float* front_part;                         // [front_shares][sequence][HK][front]
+    int front_grid;
     // out[b * sb + hk * sh + n]; or with `lengths`, added to place lengths[b] + (n in its sequence b) where that is below `places`
     float* out;
     int64_t sb, sh;

@@ -171,6 +171,7 @@ def cache_evict(k_cache, v_cache, weights, lengths, keep, first=0, recent=0, pag
 
     Returns (kept, weights): kept int32 [batch, heads, keep], the places that the rows had, ascending, -1 behind them; and a new
     tensor with the weights of the rows that stay, at their new places, zeros behind.  Sequences of at most ``keep`` rows stay as
-    they are.  lengths are the caller's: torch.minimum(lengths, keep) of them are left.  From then on a row's place is not its position:
+    they are.  Rows move within a sequence's own pages: one that two sequences share has to be copied first.  lengths are the caller's:
+    torch.minimum(lengths, keep) of them are left.  From then on a row's place is not its position:
     rotary positions go on from the old lengths, and a window of tree_attention counts places."""
     return _lib.host().cache_evict(k_cache, v_cache, weights, lengths, int(keep), int(first), int(recent), page_table)

@@ -145,3 +145,40 @@ def test_views_scales_streams_and_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, sa.key_weights(q, k, lse))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("sinks", [1, 128, 257, 600])
+@pytest.mark.parametrize("ends,add", [([0, 700, 700, 1100, 1101, 2000], False), ([0, 700, 700, 1100, 1101, 2000], True), ([5 * i for i in range(101)], True)])
+def test_many_first_keys(ends, add, sinks, dtype):
+    """Blocks of first keys, whose streams are cut by themselves: of sequences shorter than a block, than the first keys, and longer."""
+    H, HK, D, window = 4, 2, 64, 33
+    T = ends[-1] + 3
+    q, k = _inputs((T,), H, HK, D, dtype, sinks)
+    cu = torch.tensor(ends, dtype=torch.int32, device=DEV)
+    lse = _lse(q, k, cu, window, sinks)
+    got = sa.key_weights(q, k, lse, cu, window=window, sinks=sinks)
+    if add:
+        places = torch.zeros(len(ends) - 1, HK, 1000, device=DEV)
+        sa.key_weights(q, k, lse, cu, window=window, sinks=sinks, weights=places, lengths=torch.zeros(len(ends) - 1, dtype=torch.int32, device=DEV))
+    for i, (a, b) in enumerate(zip(ends, ends[1:])):
+        for hk in range(HK):
+            hs = slice(2 * hk, 2 * hk + 2)
+            if b > a:
+                _check(got[hk, a:b], _exact(q[a:b, hs], k[a:b, hk], lse[hs, a:b], D ** -0.5, window, sinks))
+            if add:
+                assert torch.equal(places[i, hk, :b - a], got[hk, a:b]) and places[i, hk, b - a:].count_nonzero() == 0
+    assert got[:, ends[-1]:].count_nonzero() == 0
+
+
+def test_bounds_out_of_order():
+    """No defined sums, but no access outside of the tensors either: what stands around the places stays."""
+    q, k = _inputs((400,), 2, 1, 64, BF16, 3)
+    for ends in ([0, 100, 200, 50], [-7, 500, 300, 90], [300, 200, 100, 0], [0, 399, 10, 380]):
+        cu = torch.tensor(ends, dtype=torch.int32, device=DEV)
+        for window, sinks in ((None, 0), (20, 3)):
+            lse = torch.zeros(2, 400, device=DEV)
+            wide = torch.full((9, 1, 128), -1.0, device=DEV)
+            held = torch.zeros(9, dtype=torch.int32, device=DEV)
+            sa.key_weights(q, k, lse, cu, window=window, sinks=sinks, weights=wide[3:6], lengths=held[3:6])
+            assert (wide[:3] == -1).all() and (wide[6:] == -1).all()

@@ -150,7 +150,7 @@ def test_c_entries_of_weights_and_eviction(lib):
     assert sums(q=None) == -1 and sums(dtype=5) == -2 and sums(D=0) == -3 and sums(HK=3) == -11 and sums(window=-1) == sums(window=3, sinks=-1) == -5
     assert sums(lengths=ONE, places=0) == -3 and sums(N=4096, nbytes=4) == -6
     assert sums(B=2, strides=_lib.stride_array([(4096, 64, 8), (4096, 64, 8), (0, 64, 8)])) == -4
-    assert lib.sa2_key_weights_workspace_bytes(1, 4096, 4, 2, 64, 0, 0, 1, 0) > 0 == lib.sa2_key_weights_workspace_bytes(1, 4096, 4, 3, 64, 0, 0, 1, 0)
+    assert lib.sa2_key_weights_workspace_bytes(0, 1, 4096, 4, 2, 64, 0, 0, 1, 0) > 0 == lib.sa2_key_weights_workspace_bytes(0, 1, 4096, 4, 3, 64, 0, 0, 1, 0)
 
     def evict(k=ONE, B=2, HK=2, heads=2, D=8, page=16, pages=6, width=1, places=16, keep=5, first=0, recent=0, dtype=0, strides=s):
         return lib.sa2_cache_evict(k, ONE, ONE, ONE, ONE, ONE, None, B, HK, heads, D, page, pages, width, places, keep, first, recent, strides, dtype, None)
@@ -159,3 +159,15 @@ def test_c_entries_of_weights_and_eviction(lib):
     assert evict(page=0) == evict(pages=1) == evict(width=2) == evict(page=(1 << 31) - 64, places=1 << 40) == -13
     assert evict(keep=0) == evict(first=-1) == evict(recent=-1) == evict(first=3, recent=3) == evict(places=15) == -15
     assert evict(strides=_lib.stride_array([(0, 64, 8)] * 3)) == -4
+
+
+def test_one_cache_twice(lib):
+    cache = t(6, 16, 2, 8)
+    with pytest.raises(ValueError, match="same memory"):
+        sa.cache_evict(cache, cache, t(2, 2, 48), ints(3, 4), 5, page_table=ints(*range(6)).view(2, 3))
+
+
+def test_first_keys_that_are_too_many(lib):
+    s = _lib.stride_array([(1 << 20, 8, 8)] * 3)
+    assert lib.sa2_key_weights(ONE, ONE, ONE, ONE, None, 0, ONE, 1 << 40, None, 0, 1, 1 << 17, 1, 1, 8, s, 3, 65536, 1.0, 0, 0, None) == -9
+    assert lib.sa2_key_weights_workspace_bytes(0, 1, 1 << 17, 1, 1, 8, 3, 65536, 0, 0) == 0

@@ -1,8 +1,8 @@
 // Eviction from a cache: of each sequence's rows the first ones, the latest ones and those that gathered most weight stay, in their order.
 //
 // Which ones: a workgroup per sequence and head finds the smallest weight that stays digit by digit (11, 11 and 10 bits of the weights
-// as ordered integers, counted in LDS), then numbers the rows that stay, of equal ones the first.  One CU's vector ALU has four readings of
-// the weights: 65536 of them take 64 us, 2000 10 (the unrolled form that keeps them in registers is fetched cold: 31).  Moving them: see
+// as ordered integers, counted in LDS), then numbers the rows that stay, of equal ones the first.  Bound by a CU's vector ALU, which
+// has four readings of the weights: 65536 of them take 50 us, 2000 10 (the unrolled form that keeps them in registers is fetched cold: 31).  Moving them: see
 // move_kernel.
 #include "sa2_layer_common.h"
 
@@ -45,21 +45,21 @@ __device__ __forceinline__ int before_me(int x, int* lds, int& total) {
     return base + sum - x;
 }
 
-__global__ __launch_bounds__(THREADS) void choose_kernel(Evict p) {
+__global__ __launch_bounds__(THREADS) void choose_kernel(Evict p, int parts) {
     __shared__ __attribute__((aligned(16))) int bins[BINS * COPIES];
     __shared__ int sums[2 * CREW];
     __shared__ int found[2];
-    const int b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, n = evict_held(p, b);
+    const int stream = blockIdx.x / parts, part = blockIdx.x % parts, b = stream / p.heads, h = stream % p.heads, n = evict_held(p, b), me = part * THREADS + threadIdx.x, all_of_us = parts * THREADS;
     const float* const w = p.weights + b * p.sb + h * p.sh;
-    float* const left = p.left + (int64_t)blockIdx.x * p.places;
-    int32_t* const kept = p.kept + (int64_t)blockIdx.x * p.keep;
+    float* const left = p.left + (int64_t)stream * p.places;
+    int32_t* const kept = p.kept + (int64_t)stream * p.keep;
     const int stay = n < p.keep ? n : p.keep;
-    for (int64_t i = stay + threadIdx.x; i < p.places; i += THREADS) left[i] = 0.f;
-    for (int i = stay + threadIdx.x; i < p.keep; i += THREADS) kept[i] = -1;
+    for (int64_t i = (int64_t)stay + me; i < p.places; i += all_of_us) left[i] = 0.f;
+    for (int64_t i = (int64_t)stay + me; i < p.keep; i += all_of_us) kept[i] = -1;
     if (n <= p.keep) {
-        for (int i = threadIdx.x; i < n; i += THREADS) {
+        for (int64_t i = me; i < n; i += all_of_us) {
             left[i] = w[i];
-            kept[i] = i;
+            kept[i] = (int)i;
         }
         return;
     }
@@ -115,28 +115,46 @@ __global__ __launch_bounds__(THREADS) void choose_kernel(Evict p) {
     }
     // In their order, 4096 rows at a time: before a row stand the sure ones before it and, of equal weights, no more than are needed.  Within a
     // wavefront these are bits of ballots, the wavefronts' numbers (sure ones and, 16 bits up, equal ones) go over LDS.
-    const uint64_t lower = ((uint64_t)1 << lane) - 1;
+    // Each of the workgroups that share a head numbers its part, and counts what stands before that.
+    const auto kind = [&](int64_t i, float weight) {       // 2: stays, 1: of the smallest weight that does
+        const uint32_t u = ordered(weight);
+        return i >= n ? 0 : i < from || i >= to ? 2 : !any ? 0 : u > prefix ? 2 : u == prefix ? 1 : 0;
+    };
+    const int steps = (int)(((int64_t)n + 4 * THREADS - 1) / (4 * THREADS));
+    const int64_t begin = (int64_t)steps * part / parts * 4 * THREADS, end = (int64_t)steps * (part + 1) / parts * 4 * THREADS;
     int sure_before = 0, same_before = 0;
+    if (begin) {
+        int sure = 0, same = 0;
+#pragma unroll 8
+        for (int64_t i = threadIdx.x; i < begin; i += THREADS) {         // (all before n)
+            const int what = kind(i, w[i]);
+            sure += what == 2;
+            same += what == 1;
+        }
+        before_me(sure, sums, sure_before);
+        before_me(same, sums + CREW, same_before);
+        __syncthreads();
+    }
+    const uint64_t lower = ((uint64_t)1 << lane) - 1;
     float x[4], next[4];
     const auto load = [&](int64_t base, float (&to)[4]) {
         const int64_t i = base + 4 * (int)threadIdx.x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) to[j] = i + j < n ? w[i + j] : 0.f;
     };
-    load(0, x);
+    load(begin, x);
     int turn = 0;
 #pragma unroll 1
-    for (int64_t base = 0; base < n; base += 4 * THREADS, turn ^= 1) {
+    for (int64_t base = begin; base < end; base += 4 * THREADS, turn ^= 1) {
         load(base + 4 * THREADS, next);
         const int64_t i = base + 4 * (int)threadIdx.x;
         bool sure[4], same[4];
         int before = 0, all = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t u = ordered(x[j]);
-            const bool free = i + j >= from && i + j < to;
-            sure[j] = i + j < n && (!free || (any && u > prefix));
-            same[j] = free && any && u == prefix;
+            const int what = kind(i + j, x[j]);
+            sure[j] = what == 2;
+            same[j] = what == 1;
             const uint64_t of_sure = __ballot(sure[j]), of_same = __ballot(same[j]);
             before += __popcll(of_sure & lower) + (__popcll(of_same & lower) << 16);
             all += __popcll(of_sure) + (__popcll(of_same) << 16);
@@ -170,12 +188,12 @@ __global__ __launch_bounds__(THREADS) void choose_kernel(Evict p) {
 // Rows to their new places.  A workgroup has `SLICE` pieces of every row of one tensor of a sequence's head and takes the rows in steps.  What
 // the rows of a step lie behind is not written before them (kept[i] >= i), so that reads may run ahead of writes, never behind: each step's
 // rows are asked for a step early, their pages two and their numbers three, and a step's writes begin when all of its reads have ended.
-// 16384 rows of 256 bytes of 16 heads: 98 us (2.7 TB/s read and written) by 128 workgroups, 1024 rows of 32 heads 10 us; narrower slices (two
-// pieces) 88 and 15, one step at a time without the reads ahead 380 and 26.
+// 16384 rows of 256 bytes of 16 heads: 88 us (3.0 TB/s read and written) by 256 workgroups with two pieces, 98 by 128 with four; 1024 rows of 32
+// heads: 10 us with four pieces, 15 with two.  One step at a time, without the reads ahead, 380 and 26.
 typedef uint32_t Quad __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint32_t word(Quad x) { return x.x; }
 __device__ __forceinline__ uint32_t word(uint32_t x) { return x; }
-constexpr int MOVERS = 512, SLICE = 4, EACH = 8, STEP = EACH * MOVERS / SLICE;
+constexpr int MOVERS = 512, EACH = 8;
 // r / d = r * factor >> shift for r < 2^31: with 2^l >= d, factor d = 2^(31 + l) + e, 0 < e <= 2^l, the product's error is below 1 / d
 struct Quotient {
     uint32_t factor;
@@ -187,8 +205,9 @@ Quotient quotient(uint32_t d) {
     return Quotient{(uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), 31 + l};
 }
 __device__ const Quad nothing = {0, 0, 0, 0};
-template <class UNIT>
+template <class UNIT, int SLICE>
 __global__ __launch_bounds__(MOVERS) void move_kernel(Evict p, Quotient pages_in, int size, int pieces, int slices) {
+    constexpr int STEP = EACH * MOVERS / SLICE;
     int slice, stream;                                      // slices of the same rows on the same XCD, whose cache lines they share
     const int streams = p.B * p.HK * 2, pid = blockIdx.x;
     if (streams % 8 == 0) {
@@ -280,16 +299,28 @@ __global__ __launch_bounds__(MOVERS) void move_kernel(Evict p, Quotient pages_in
 int launch_evict(const Evict& p, int dtype, hipStream_t st) {
     const int size = dtype == SA2_F32 ? 4 : 2;
     const bool wide = (p.D * size) % 16 == 0 && aligned16(p.cache.k, size, true) && aligned16(p.cache.v, size, true);
-    const int pieces = wide ? p.D * size / 16 : p.D, slices = (pieces + SLICE - 1) / SLICE;
-    const int64_t grid = (int64_t)p.B * p.HK * 2 * slices;
-    if ((int64_t)p.B * p.heads > 0x7fffffff || grid > 0x7fffffff) return SA2_ERR_TOO_LARGE;
-    choose_kernel<<<dim3((unsigned)(p.B * p.heads)), dim3(THREADS), 0, st>>>(p);
+    const int pieces = wide ? p.D * size / 16 : p.D;
+    const auto slices_of = [&](int slice) { return (int64_t)p.B * p.HK * 2 * ((pieces + slice - 1) / slice); };
+    const bool narrow = slices_of(4) < CUS;                 // half as wide where that leaves CUs without any
+    const int64_t grid = slices_of(narrow ? 2 : 4);
+    // workgroups that number a head's rows (each finds the smallest weight for itself): four of 65536 rows
+    // 50 us, one 64; of 2000 rows one takes 10
+    const int64_t room = (int64_t)p.cache.page_size * (p.cache.table ? p.cache.width : 1), streams = (int64_t)p.B * p.heads;
+    const int parts = room < 32768 || streams * 2 > CUS ? 1 : streams * 4 > CUS ? 2 : 4;
+    if (streams * parts > 0x7fffffff || grid > 0x7fffffff) return SA2_ERR_TOO_LARGE;
+    choose_kernel<<<dim3((unsigned)(p.B * p.heads * parts)), dim3(THREADS), 0, st>>>(p, parts);
     if (hipGetLastError() != hipSuccess) return SA2_ERR_LAUNCH_FAILED;
     const dim3 blocks((unsigned)grid), block(MOVERS);
     const Quotient pages_in = quotient(p.cache.page_size);
-    if (wide) move_kernel<Quad><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
-    else if (size == 4) move_kernel<uint32_t><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
-    else move_kernel<uint16_t><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
+    const auto move = [&](auto slice) {
+        constexpr int SLICE = decltype(slice)::value;
+        const int slices = (pieces + SLICE - 1) / SLICE;
+        if (wide) move_kernel<Quad, SLICE><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
+        else if (size == 4) move_kernel<uint32_t, SLICE><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
+        else move_kernel<uint16_t, SLICE><<<blocks, block, 0, st>>>(p, pages_in, size, pieces, slices);
+    };
+    if (narrow) move(std::integral_constant<int, 2>{});
+    else move(std::integral_constant<int, 4>{});
     return hipGetLastError() == hipSuccess ? SA2_OK : SA2_ERR_LAUNCH_FAILED;
 }
 

@@ -14,7 +14,7 @@ namespace {
 // ---- fp16: factors of the rows of dQ and of the keys (sa2_causal16.h), from the rows that meet there alone --------------------------------
 constexpr int FACTOR_ROWS = 256;
 
-// max of x(n - window + 1) .. x(n) for the lane's n = n0 + threadIdx.x; x(i) is 0 where i < 0.  `lds`: 4 * FACTOR_ROWS + 4 floats, and every
+// max of x(n - window + 1) .. x(n) for the lane's n = n0 + threadIdx.x; x(i) is 0 where i < 0.  `lds`: 2 * FACTOR_ROWS floats, and every
 // thread calls it.  Windows up to 256 double up to the largest power of two, two of which overlap; longer ones are the 256 up to n, the
 // 256 from the window's start, and what all windows of the block share between them.
 template <class X>

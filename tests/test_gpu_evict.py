@@ -36,6 +36,9 @@ def _expect(kc, vc, w, lengths, table, keep, first, recent):
             stay = _chosen(w[b, h], n, keep, first, recent)
             kept[b, h, :len(stay)] = torch.tensor(stay, dtype=torch.int32)
             left[b, h, :len(stay)] = w[b, h, stay]
+            if table is None:
+                kc[b, :len(stay), hk], vc[b, :len(stay), hk] = old[0][b, stay, hk], old[1][b, stay, hk]
+                continue
             for i, r in enumerate(stay):
                 src, dst = ((b, x) if table is None else (int(table[b, x // page]), x % page) for x in (r, i))
                 if r != i and 0 <= src[0] < kc.shape[0] and 0 <= dst[0] < kc.shape[0]:
@@ -100,6 +103,23 @@ def test_weights_of_any_kind(values):
         got = _run(kc, vc, w, lengths, table, keep, first, recent)
         want = _expect(kc, vc, w, lengths, table, keep, first, recent)
         assert torch.equal(got[0].cpu(), want[0]) and _same(got[1].cpu(), want[1]) and all(torch.equal(a.cpu(), b) for a, b in zip(got[2:], want[2:]))
+
+
+@pytest.mark.parametrize("values", ["drawn", "equal", "few"])
+@pytest.mark.parametrize("heads,paged", [(2, True), (1, True), (2, False)])
+def test_workgroups_that_share_a_head(heads, paged, values):
+    """Caches of 32768 rows on: the weights that are equal, the first and the last rows fall into any of the parts, or into none."""
+    kc, vc, w, lengths, table = _case(6, 2, heads, 8, 300, 110, FP16, 7, paged, 1)
+    g = torch.Generator().manual_seed(8)
+    if values == "equal":
+        w = torch.ones_like(w)
+    elif values == "few":
+        w = torch.randint(0, 3, w.shape, generator=g).float().to(DEV)
+    lengths = torch.tensor([33000, 32768, 4097, 100, 0, 17000], dtype=torch.int32)
+    for keep, first, recent in ((8300, 4, 4000), (90, 0, 50), (32999, 20000, 10), (16500, 0, 16500)):
+        got = _run(kc, vc, w, lengths, table, keep, first, recent)
+        want = _expect(kc, vc, w, lengths, table, keep, first, recent)
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
 
 
 def test_pages_and_lengths_outside_of_the_cache():

@@ -221,3 +221,20 @@ def test_results_are_deterministic():
     first = _all(q, k, v, dout, 256, 4)
     second = _all(q, k, v, dout, 256, 4)
     assert all(torch.equal(a, b) for a, b in zip((*first[:2], *first[2]), (*second[:2], *second[2])))
+
+
+def test_tensors_of_more_than_2_to_31_elements():
+    """The last rows of a long sequence against those rows by themselves: without first keys they see nothing else."""
+    N, H, HK, D, window, rows = 270_000, 64, 8, 128, 100, 300
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q, k, v, dout = (torch.empty(1, N, h, D, dtype=BF16, device=DEV).normal_(generator=g) for h in (H, HK, HK, H))
+    out, lse, grads = _all(q, k, v, dout, window, 0)
+    near, at = slice(N - rows - window + 1, N), slice(window - 1, None)
+    for hk in (0, HK - 1):
+        hs = slice(8 * hk, 8 * hk + 8)
+        want = exact(q[0, near, hs], k[0, near, hk], v[0, near, hk], dout[0, near, hs], D ** -0.5, BF16, True, window, 0)
+        check(out[0, near, hs][at], [x[at] for x in want["out"]], "out")
+        check(lse[0, hs, near].transpose(0, 1)[at], [x[at] for x in want["lse"]], "lse")
+        check(grads[0][0, near, hs][at], [x[at] for x in want["dq"]], "dq")
+        check(grads[1][0, near, hk:hk + 1][at], [x[at] for x in want["dk"]], "dk")
+        check(grads[2][0, near, hk:hk + 1][at], [x[at] for x in want["dv"]], "dv")

@@ -546,7 +546,7 @@ std::pair<Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_cache, co
     TORCH_CHECK_VALUE((int64_t)c.page_size * c.width <= 0x7fffffff - 64, "a cache of 2^31 - 64 rows per sequence or more");
     TORCH_CHECK_VALUE(weights.dim() == 3, "weights must be float32 [batch, heads, places], got ", weights.sizes());
     check_weights(weights, c, weights.size(1) == 1 ? 1 : k_cache.size(2), false);
-    TORCH_CHECK_VALUE(keep >= 1 && first >= 0 && recent >= 0 && keep < ((int64_t)1 << 31) && first + recent <= keep, "keep must be at least 1, first and recent at least 0 and together at most keep, got ", keep, ", ", first, ", ", recent);
+    TORCH_CHECK_VALUE(keep >= 1 && first >= 0 && recent >= 0 && keep < ((int64_t)1 << 31) && first <= keep && recent <= keep - first, "keep must be at least 1, first and recent at least 0 and together at most keep, got ", keep, ", ", first, ", ", recent);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (k_cache.requires_grad() || v_cache.requires_grad() || weights.requires_grad())), "cache_evict has no gradient: call it under torch.no_grad() or on detached tensors");
     TORCH_CHECK(c10::InferenceMode::is_enabled() || !(k_cache.is_inference() || v_cache.is_inference()), "cache_evict changes the cache in place, which inference tensors allow in inference mode only");
     TORCH_CHECK_VALUE(k_cache.numel() == 0 || k_cache.const_data_ptr() != v_cache.const_data_ptr(), "k_cache and v_cache are the same memory, whose rows would move twice");

@@ -6,8 +6,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
+#include <vector>
 
 #include "sa2_torch.h"
 
@@ -235,6 +237,47 @@ bool meet(const Tensor& a, const Tensor& b) {
         return (const char*)t.const_data_ptr() + (last + 1) * t.element_size();
     };
     return (const char*)a.const_data_ptr() < end(b) && (const char*)b.const_data_ptr() < end(a);
+}
+
+// Bytes from one element to another are sums of these: `stride` times any number from lo to hi
+struct Steps {
+    int64_t stride, lo, hi;
+};
+// Whether the steps from `i` on (longest first) can add up to `bytes`; a search of too many turns, of axes that reach over one another, counts as yes
+bool reaches(const std::vector<Steps>& steps, size_t i, int64_t bytes, int& turns) {
+    if (i == steps.size()) return bytes == 0;
+    int64_t least = 0, most = 0;               // of the others
+    for (size_t j = i + 1; j < steps.size(); ++j) {
+        least += steps[j].stride * steps[j].lo;
+        most += steps[j].stride * steps[j].hi;
+    }
+    const Steps& s = steps[i];
+    const auto down = [&](int64_t x) { return x / s.stride - (x % s.stride < 0); };
+    for (int64_t n = std::max(s.lo, -down(most - bytes)); n <= std::min(s.hi, down(bytes - least)); ++n)
+        if (--turns < 0 || reaches(steps, i + 1, bytes - n * s.stride, turns)) return true;
+    return false;
+}
+// Whether two tensors with positive strides have a byte in common.  Halves of one buffer, whose elements lie between each other, have none.
+bool share(const Tensor& a, const Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0 || !meet(a, b)) return false;
+    const int64_t size = a.element_size();
+    std::vector<Steps> steps{{1, 1 - size, size - 1}};
+    const auto add = [&](int64_t stride, int64_t lo, int64_t hi) {
+        for (Steps& s : steps)
+            if (s.stride == stride) {
+                s.lo += lo;
+                s.hi += hi;
+                return;
+            }
+        steps.push_back({stride, lo, hi});
+    };
+    for (int64_t i = 0; i < a.dim(); ++i)
+        if (a.size(i) > 1) add(a.stride(i) * size, 0, a.size(i) - 1);
+    for (int64_t i = 0; i < b.dim(); ++i)
+        if (b.size(i) > 1) add(b.stride(i) * size, 1 - b.size(i), 0);
+    std::sort(steps.begin(), steps.end(), [](const Steps& x, const Steps& y) { return x.stride > y.stride; });
+    int turns = 4096;
+    return reaches(steps, 0, (const char*)b.const_data_ptr() - (const char*)a.const_data_ptr(), turns);
 }
 
 void append(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths, const Maybe& table, const Maybe& chosen, const Maybe& cu) {
@@ -549,7 +592,7 @@ std::pair<Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_cache, co
     TORCH_CHECK_VALUE(keep >= 1 && first >= 0 && recent >= 0 && keep < ((int64_t)1 << 31) && first <= keep && recent <= keep - first, "keep must be at least 1, first and recent at least 0 and together at most keep, got ", keep, ", ", first, ", ", recent);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (k_cache.requires_grad() || v_cache.requires_grad() || weights.requires_grad())), "cache_evict has no gradient: call it under torch.no_grad() or on detached tensors");
     TORCH_CHECK(c10::InferenceMode::is_enabled() || !(k_cache.is_inference() || v_cache.is_inference()), "cache_evict changes the cache in place, which inference tensors allow in inference mode only");
-    TORCH_CHECK_VALUE(k_cache.numel() == 0 || k_cache.const_data_ptr() != v_cache.const_data_ptr(), "k_cache and v_cache are the same memory, whose rows would move twice");
+    TORCH_CHECK_VALUE(!share(k_cache, v_cache), "k_cache and v_cache have rows in the same memory, which would move twice");
     check_place("cache_evict", {k_cache, v_cache, weights});
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;

@@ -165,7 +165,7 @@ def cache_evict(k_cache, v_cache, weights, lengths, keep, first=0, recent=0, pag
     """Drops rows of a cache: of each sequence and key head ``keep`` stay, in their order, at the places 0 .. keep-1 (in place): the
     ``first`` first, the ``recent`` last ones, and of the others those of the largest weights, of equal ones the first.
 
-    k_cache, v_cache, lengths, page_table   as at cache_append
+    k_cache, v_cache, lengths, page_table   as at cache_append; the two caches have no memory in common (halves of one buffer are fine)
     weights   float32 [batch, key heads, places], at least a place for each row that the cache may hold (tree_attention and
               key_weights add to them), not changed; NaN counts as less than any number.  [batch, 1, places]: one choice for all heads
 

@@ -214,21 +214,6 @@ CacheView check_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor
     return {k_cache, v_cache, lengths.contiguous(), dense(table), (int)k_cache.size(1), (int)k_cache.size(0), table ? (int)table->size(1) : 1};
 }
 
-void check_added(const Tensor& t) {
-    TORCH_CHECK_VALUE(strided(t), "weights need unit stride along the places and positive strides: they are added to in place");
-    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "weights are added to in place and have no gradient: call it under torch.no_grad() or on detached tensors");
-    TORCH_CHECK(c10::InferenceMode::is_enabled() || !t.is_inference(), "weights are changed in place, which inference tensors allow in inference mode only");
-}
-// The weights that the rows of a cache have gathered, of `heads` heads each: changed in place where `written`
-void check_weights(const Tensor& t, const CacheView& c, int64_t heads, bool written) {
-    const int64_t capacity = (int64_t)c.page_size * c.width;
-    TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == c.lengths.numel() && t.size(1) == heads && t.size(2) >= capacity, "weights must be float32 [",
-                      c.lengths.numel(), ", ", heads, ", ", capacity, " or more], got ", t.scalar_type(), " ", t.sizes());
-    TORCH_CHECK_VALUE(t.device() == c.k.device(), "weights must be on the device of the other tensors");
-    TORCH_CHECK_VALUE(strided(t), "weights need unit stride along the places and positive strides");
-    if (written) check_added(t);
-}
-
 // Whether the memory from a tensor's first element to its last meets the other's
 bool meet(const Tensor& a, const Tensor& b) {
     auto end = [](const Tensor& t) {
@@ -278,6 +263,38 @@ bool share(const Tensor& a, const Tensor& b) {
     std::sort(steps.begin(), steps.end(), [](const Steps& x, const Steps& y) { return x.stride > y.stride; });
     int turns = 4096;
     return reaches(steps, 0, (const char*)b.const_data_ptr() - (const char*)a.const_data_ptr(), turns);
+}
+// Whether two elements of one tensor (with positive strides) have memory in common
+bool folded(const Tensor& t) {
+    std::vector<Steps> steps;
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1) steps.push_back({t.stride(i), 1 - t.size(i), t.size(i) - 1});
+    std::sort(steps.begin(), steps.end(), [](const Steps& x, const Steps& y) { return x.stride > y.stride; });
+    int turns = 4096;
+    int64_t inner = 0;                         // what the shorter steps reach
+    for (size_t i = steps.size(); i-- > 0;) {
+        const Steps& s = steps[i];
+        for (int64_t n = 1; n <= std::min(s.hi, inner / s.stride); ++n)
+            if (--turns < 0 || reaches(steps, i + 1, n * s.stride, turns)) return true;
+        inner += s.hi * s.stride;
+    }
+    return false;
+}
+
+void check_added(const Tensor& t) {
+    TORCH_CHECK_VALUE(strided(t), "weights need unit stride along the places and positive strides: they are added to in place");
+    TORCH_CHECK_VALUE(t.numel() == 0 || !folded(t), "weights of different places share memory: they are added to in place");
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "weights are added to in place and have no gradient: call it under torch.no_grad() or on detached tensors");
+    TORCH_CHECK(c10::InferenceMode::is_enabled() || !t.is_inference(), "weights are changed in place, which inference tensors allow in inference mode only");
+}
+// The weights that the rows of a cache have gathered, of `heads` heads each: changed in place where `written`
+void check_weights(const Tensor& t, const CacheView& c, int64_t heads, bool written) {
+    const int64_t capacity = (int64_t)c.page_size * c.width;
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == c.lengths.numel() && t.size(1) == heads && t.size(2) >= capacity, "weights must be float32 [",
+                      c.lengths.numel(), ", ", heads, ", ", capacity, " or more], got ", t.scalar_type(), " ", t.sizes());
+    TORCH_CHECK_VALUE(t.device() == c.k.device(), "weights must be on the device of the other tensors");
+    TORCH_CHECK_VALUE(strided(t), "weights need unit stride along the places and positive strides");
+    if (written) check_added(t);
 }
 
 void append(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths, const Maybe& table, const Maybe& chosen, const Maybe& cu) {
@@ -592,6 +609,7 @@ std::pair<Tensor, Tensor> evict(const Tensor& k_cache, const Tensor& v_cache, co
     TORCH_CHECK_VALUE(keep >= 1 && first >= 0 && recent >= 0 && keep < ((int64_t)1 << 31) && first <= keep && recent <= keep - first, "keep must be at least 1, first and recent at least 0 and together at most keep, got ", keep, ", ", first, ", ", recent);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (k_cache.requires_grad() || v_cache.requires_grad() || weights.requires_grad())), "cache_evict has no gradient: call it under torch.no_grad() or on detached tensors");
     TORCH_CHECK(c10::InferenceMode::is_enabled() || !(k_cache.is_inference() || v_cache.is_inference()), "cache_evict changes the cache in place, which inference tensors allow in inference mode only");
+    TORCH_CHECK_VALUE(k_cache.numel() == 0 || !(folded(k_cache) || folded(v_cache)), "rows of a cache share memory with one another: they move in place");
     TORCH_CHECK_VALUE(!share(k_cache, v_cache), "k_cache and v_cache have rows in the same memory, which would move twice");
     check_place("cache_evict", {k_cache, v_cache, weights});
     py::gil_scoped_release nogil;

@@ -78,7 +78,7 @@ __global__ __launch_bounds__(THREADS) void choose_kernel(Evict p, int parts) {
                 const uint32_t u = ordered(x);
                 if (pass == 0 || u >> (shift + width) == prefix) atomicAdd(&bins[(u >> shift & ((1u << width) - 1)) * COPIES + threadIdx.x % COPIES], 1);
             };
-            int64_t i = from + (int)threadIdx.x;
+            int64_t i = (int64_t)from + threadIdx.x;
 #pragma unroll 1
             for (; i + 7 * THREADS < to; i += 8 * THREADS) {
                 float x[8];
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(MOVERS) void move_kernel(Evict p, Quotient pages_in
             to[u] = go ? (UNIT*)at(dst[u], place(step, u)) : nullptr;
         }
     };
-    const int steps = (p.keep + STEP - 1) / STEP;
+    const int steps = (int)(((int64_t)p.keep + STEP - 1) / STEP);
     int from0[EACH], from1[EACH], from2[EACH], src1[EACH], dst1[EACH];
     UNIT x[EACH];
     UNIT* to[EACH];

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
     if (BAND && p.cache.table) {
         page0 = (int)((unsigned)(cache.edge * 32) / (unsigned)page_size);
         near_pages = held > cache.edge * 32 ? (int)((unsigned)(held - 1) / (unsigned)page_size) - page0 + 1 : 0;
-        const int head = cached - cache.near - (cache.whole - cache.edge), first_pages = (head * 32 + page_size - 1) / page_size;
+        const int head = cached - cache.near - (cache.whole - cache.edge), first_pages = (int)(((unsigned)(head * 32) + page_size - 1) / page_size);
         kept = (int64_t)near_pages + first_pages <= TREE16_ENTRIES;
         if (kept)
             for (int i = threadIdx.x; i < near_pages + first_pages; i += THREADS) {

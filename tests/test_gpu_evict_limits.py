@@ -22,10 +22,14 @@ def test_the_longest_cache(keep, first, recent, heavy, dropped):
     weights = torch.zeros(1, 1, ROWS, device=DEV)
     weights[..., heavy] = 2.0
     kept, left = sa.cache_evict(k_cache, v_cache, weights, torch.tensor([ROWS], dtype=torch.int32, device=DEV), keep, first, recent)
-    stay = torch.ones(ROWS, dtype=torch.bool, device=DEV)
-    stay[dropped] = False
-    assert torch.equal(kept[0, 0], torch.arange(ROWS, dtype=torch.int32, device=DEV)[stay])
-    assert torch.equal(left[0, 0, :keep], weights[0, 0][stay]) and left[0, 0, keep:].count_nonzero() == 0
+    assert left[0, 0, keep:].count_nonzero() == 0
     for bits, cache in ((k_bits, k_cache), (v_bits, v_cache)):
-        now = cache.view(torch.int16).flatten()
-        assert torch.equal(now[:keep], bits[stay]) and torch.equal(now[keep:], bits[keep:])
+        assert torch.equal(cache.view(torch.int16).flatten()[keep:], bits[keep:])
+    at = 0
+    for a, b in zip([0] + [x + 1 for x in dropped], dropped + [ROWS]):       # runs of rows that stay
+        to = slice(at, at + b - a)
+        at += b - a
+        assert torch.equal(kept[0, 0, to], torch.arange(a, b, dtype=torch.int32, device=DEV)) and torch.equal(left[0, 0, to], weights[0, 0, a:b])
+        for bits, cache in ((k_bits, k_cache), (v_bits, v_cache)):
+            assert torch.equal(cache.view(torch.int16).flatten()[to], bits[a:b])
+    assert at == keep

@@ -106,36 +106,53 @@ __device__ __forceinline__ uint32_t band_queries(const Band& b, int j, int i0, b
 __device__ __forceinline__ uint32_t band_counted(const Band& b, uint32_t queries, int i0) { return i0 + 31 <= b.alone ? 0u : i0 == 0 ? queries & ~1u : queries; }
 // Whether queries i0 .. i1 see all of the keys j0 .. j1
 __device__ __forceinline__ bool band_full(const Band& b, int i0, int i1, int j0, int j1) { return j1 <= i0 && (i1 - j0 < b.window || j1 < b.sinks); }
-// Queries lo .. hi-1 that a workgroup takes for keys j0 .. j0+rows-1: with a band, those of the window of keys behind the first ones
-// (`sink` < 0), or a chunk of the sequence for the first keys.  false: none, or nothing that it has to leave
+// Keys j0 .. j0+rows-1 of a workgroup and the queries lo .. hi-1 that it takes for them: with a band, those of the window of keys behind the
+// first ones (`extra` < 0), or a chunk of the sequence for the first keys.  The workgroups of these come in groups, of which `extra` is the
+// number in the group: a group has a chunk (`s` is the `tile`-th of them), its members a block of the first keys each; or (by_rows) a group
+// of two a block of `rows` rows, of which a sequence has half as many at least as pairs of a chunk and a block of first keys.
+// false: none, or nothing that it has to leave
 struct KeyWork {
-    int lo, hi, sink;                                       // sink: the chunk's place in p.sink_part, or -1
+    int j0, lo, hi;
+    int64_t sink;                                           // the chunk's first row of sums, or -1
 };
 template <bool BAND>
-__device__ __forceinline__ bool key_work(const Causal& p, const Span& s, int j0, int rows, int chunk, int slot, KeyWork& w) {
-    w = KeyWork{j0, s.len, -1};
+__device__ __forceinline__ bool key_work(const Causal& p, const Span& s, int rows, int tile, int extra, KeyWork& w) {
+    w = KeyWork{s.block * rows, s.block * rows, s.len, -1};
     if constexpr (BAND) {
-        if (slot < 0) {
-            if (j0 + rows <= p.band.sinks) return false;
-            const int64_t end = (int64_t)j0 + rows - 1 + p.band.window;
+        if (extra < 0) {
+            if (w.j0 + rows <= p.band.sinks) return false;
+            const int64_t end = (int64_t)w.j0 + rows - 1 + p.band.window;
             w.hi = end < s.len ? (int)end : s.len;
         } else {
-            w.sink = slot;
-            w.lo = chunk * p.band.chunk > j0 ? chunk * p.band.chunk : j0;
-            w.hi = s.len - chunk * p.band.chunk < p.band.chunk ? s.len : (chunk + 1) * p.band.chunk;
-            return j0 < s.len && w.lo < w.hi;
+            int chunk = s.block;
+            w.j0 = extra * rows;
+            w.sink = s.b * (p.band.sink_rows / p.rows.B) + (int64_t)tile * p.band.sinks;
+            if (p.band.by_rows) {
+                const int held = p.band.sinks < s.len ? p.band.sinks : s.len, blocks = (held + rows - 1) / rows;
+                const int64_t pair = 2 * (int64_t)s.block + extra;
+                chunk = (int)(pair / blocks);
+                w.j0 = (int)(pair % blocks) * rows;
+                w.sink = 2 * (int64_t)s.first + (int64_t)chunk * held;
+            }
+            const int64_t from = (int64_t)chunk * p.band.chunk;
+            if (from >= s.len) return false;
+            w.lo = from > w.j0 ? (int)from : w.j0;
+            w.hi = s.len - from < p.band.chunk ? s.len : (int)from + p.band.chunk;
+            return w.j0 < s.len && w.lo < w.hi;
         }
     }
     return true;
 }
-// Sums of the first key j of a key head over chunk `slot`; which: 0 dK, 1 dV
-__device__ __forceinline__ float* sink_row(const Causal& p, int64_t slots, int which, int slot, int hk, int j) {
-    return p.sink_part + ((((int64_t)which * slots + slot) * p.HK + hk) * p.band.sinks + j) * p.D;
+// Sums of the first key j of a key head over the chunk whose rows begin at `sink`; which: 0 dK, 1 dV
+__device__ __forceinline__ float* sink_row(const Causal& p, int which, int64_t sink, int hk, int j) {
+    return p.sink_part + (((int64_t)which * p.HK + hk) * p.band.sink_rows + sink + j) * p.D;
 }
+// Members of a group of workgroups of the first keys, and the groups, of a key head
+inline int sink_members(const Causal& p, int rows) { return p.band.by_rows ? 2 : (p.band.sinks + rows - 1) / rows; }
+inline int64_t sink_groups(const Causal& p, int rows) { return (int64_t)p.rows.B * count_tiles(p.rows, p.band.by_rows ? rows : p.band.chunk); }
 // Windows: query heads that a workgroup's four wavefronts have, and whether a wavefront has two blocks of 32 queries (as causal16_two)
 inline int window_heads(const Causal& p) { return p.G % 4 == 0 ? 4 : p.G % 2 == 0 ? 2 : 1; }
 inline bool window_two(const Causal& p, int heads) { return (int64_t)p.rows.B * (p.H / heads) * count_tiles(p.rows, 256 / heads) >= 2 * CUS; }
-inline int64_t sink_slots(const Causal& p) { return (int64_t)p.rows.B * count_tiles(p.rows, p.band.chunk); }
 
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 

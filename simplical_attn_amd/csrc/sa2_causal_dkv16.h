@@ -166,9 +166,9 @@ __device__ __forceinline__ float key_factor(const Causal& p, const Causal16Terms
 }
 
 // ---- dK, dV ------------------------------------------------------------------------------------------------------------
-// With a band, workgroups from `main` on have the first keys (Band), `blocks` of them for a chunk of queries, and leave fp32 sums
+// With a band, workgroups from `main` on have the first keys (key_work), in groups of `members`, and leave fp32 sums
 template <class E, int D, bool BAND = false>
-__device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16Terms& terms, int nsplit, bool padded, int id, char* lds, int main = 0, int blocks = 1, int64_t slots = 0) {
+__device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16Terms& terms, int nsplit, bool padded, int id, char* lds, int main = 0, int members = 1) {
     using T = QuadTile<D>;
     using X8 = typename E::x8;
     using L = Lone<(D == 128 ? 192 : 96)>;
@@ -176,11 +176,11 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
     constexpr int V0 = 0, K0 = DT * 16, KEY0 = 2 * DT * 16, VALUE0 = KEY0 + KK * 4;      // sums of dV and dK, keys, values
     const uint32_t base = lds_address(lds), stats = base + BUFFERS * Buffer<D>::BYTES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    int stream, tile, j0 = 0;
+    int stream, tile, extra = -1;
     const bool sink = BAND && id >= main;
     if (sink) {
-        j0 = (id - main) % blocks * BLOCK;
-        id = (id - main) / blocks;
+        extra = (id - main) % members;
+        id = (id - main) / members;
         nsplit = 1;
     }
     order(id, p.rows.B * p.HK * nsplit, stream, tile);
@@ -188,7 +188,7 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
     stream /= nsplit;
     const int b = stream / p.HK, hk = stream % p.HK;
     Span s;
-    if (!find_tile(p.rows, b, tile, sink ? p.band.chunk : BLOCK, s)) return;
+    if (!find_tile(p.rows, b, tile, sink && !p.band.by_rows ? p.band.chunk : BLOCK, s)) return;
     typedef typename E::scalar scalar;
     if (s.fill) {
         if (nsplit == 1 && !sink)
@@ -198,10 +198,9 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
             }
         return;
     }
-    if (!sink) j0 = s.block * BLOCK;
     KeyWork work;
-    if (!key_work<BAND>(p, s, j0, BLOCK, s.block, sink ? (int)(b * (slots / p.rows.B)) + tile : -1, work)) return;
-    const int mine = j0 + wave * SUB, key = mine + (lane & 31);
+    if (!key_work<BAND>(p, s, BLOCK, tile, extra, work)) return;
+    const int j0 = work.j0, mine = j0 + wave * SUB, key = mine + (lane & 31);
     const float c = p.scale * LOG2E;
     // the stream: tiles of 64 queries, from the one with the block's first key on, of one head after the other
     const int t0 = work.lo / TILE_ROWS, per = (work.hi + TILE_ROWS - 1) / TILE_ROWS - t0;
@@ -596,8 +595,8 @@ __device__ __forceinline__ void keys_gradients16(const Causal& p, const Causal16
             k.x *= to; k.y *= to; k.z *= to; k.w *= to;
             if (col < p.D) {
                 if (sink) {
-                    if (p.dk.p) *(float4*)(sink_row(p, slots, 0, work.sink, hk, key) + col) = k;
-                    if (p.dv.p) *(float4*)(sink_row(p, slots, 1, work.sink, hk, key) + col) = v;
+                    if (p.dk.p) *(float4*)(sink_row(p, 0, work.sink, hk, key) + col) = k;
+                    if (p.dv.p) *(float4*)(sink_row(p, 1, work.sink, hk, key) + col) = v;
                 } else if (nsplit > 1) {
                     *(float4*)(part + col) = k;
                     *(float4*)(part + total * p.D + col) = v;

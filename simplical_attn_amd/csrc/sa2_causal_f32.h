@@ -252,34 +252,33 @@ __global__ __launch_bounds__(THREADS) void causal_f32_dq_kernel(Causal p) {
 
 // dK and dV: the wavefront owns 32 keys and sweeps the queries of all G heads that see them.  Columns `first` .. + DO of the
 // gradients: at head_dim 256 two workgroups share them, each with all of the two first products (the registers hold no more).
-// With a band, workgroups from `main` on have the first keys (Band), `blocks` of them for a chunk of queries.
+// With a band, workgroups from `main` on have the first keys (key_work), in groups of `members`.
 template <class T, int DP, int DO, bool WIDE, bool BAND>
-__global__ __launch_bounds__(THREADS) void causal_f32_dkv_kernel(Causal p, int main, int blocks, int64_t slots) {
+__global__ __launch_bounds__(THREADS) void causal_f32_dkv_kernel(Causal p, int main, int members) {
     constexpr bool wide = WIDE;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float *qt = lds, *dt = lds + TILE * Pitch<DP>::value, *stats = dt + TILE * Pitch<DP>::value;     // lse * log2(e), delta
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    int stream, tile, id = blockIdx.x, j0 = 0;
+    int stream, tile, id = blockIdx.x, extra = -1;
     const bool sink = BAND && id >= main;
     if (sink) {
-        j0 = (id - main) % blocks * BLOCK;
-        id = (id - main) / blocks;
+        extra = (id - main) % members;
+        id = (id - main) / members;
     }
     order(id, p.rows.B * p.HK * (DP / DO), stream, tile);
     const int first = stream % (DP / DO) * DO;
     stream /= DP / DO;
     const int b = stream / p.HK, hk = stream % p.HK;
     Span s;
-    if (!find_tile(p.rows, b, tile, sink ? p.band.chunk : BLOCK, s)) return;
+    if (!find_tile(p.rows, b, tile, sink && !p.band.by_rows ? p.band.chunk : BLOCK, s)) return;
     if (s.fill) {
         if (first || sink) return;
         fill_rows<T>(p.dk, s, hk, p.D);
         return fill_rows<T>(p.dv, s, hk, p.D);
     }
-    if (!sink) j0 = s.block * BLOCK;
     KeyWork work;
-    if (!key_work<BAND>(p, s, j0, BLOCK, s.block, sink ? (int)(b * (slots / p.rows.B)) + tile : -1, work)) return;
-    const int mine = j0 + wave * TILE, ki = mine + (lane & 31);
+    if (!key_work<BAND>(p, s, BLOCK, tile, extra, work)) return;
+    const int j0 = work.j0, mine = j0 + wave * TILE, ki = mine + (lane & 31);
     float k[DP / 2], v[DP / 2];
     own_rows<T, DP>(k, p.k, s, mine, hk, p.D, wide, 1.f);
     own_rows<T, DP>(v, p.v, s, mine, hk, p.D, wide, 1.f);
@@ -348,7 +347,7 @@ __global__ __launch_bounds__(THREADS) void causal_f32_dkv_kernel(Causal p, int m
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             if (!(which ? p.dv.p : p.dk.p)) continue;
-            float* const row = sink_row(p, slots, which, work.sink, hk, ki);
+            float* const row = sink_row(p, which, work.sink, hk, ki);
 #pragma unroll
             for (int i = 0; i < DO / 32; ++i)
 #pragma unroll
@@ -410,11 +409,12 @@ int f32_backward(const Causal& p, int dtype, hipStream_t st) {
         } else {
             constexpr int SHARES = 2;
             const int64_t tiles = (int64_t)p.rows.B * count_tiles(p.rows, BLOCK), main = tiles * p.HK * SHARES;
-            const int64_t slots = sink ? sink_slots(p) : 0, blocks = sink ? (p.band.sinks + BLOCK - 1) / BLOCK : 0;
+            const int members = sink ? sink_members(p, BLOCK) : 1;
+            const int64_t first = sink ? sink_groups(p, BLOCK) * members * p.HK * SHARES : 0;
             if (main > 0x7fffffff) return (int)SA2_ERR_TOO_LARGE;
             if (p.dk.p || p.dv.p)
-                rc = launch(wide ? causal_f32_dkv_kernel<T, 256, 128, true, BAND> : causal_f32_dkv_kernel<T, 256, 128, false, BAND>, p, main + slots * p.HK * SHARES * blocks,
-                            2 * TILE * Pitch<256>::value + 64, st, (int)main, (int)blocks, slots);
+                rc = launch(wide ? causal_f32_dkv_kernel<T, 256, 128, true, BAND> : causal_f32_dkv_kernel<T, 256, 128, false, BAND>, p, main + first,
+                            2 * TILE * Pitch<256>::value + 64, st, (int)main, members);
             if (rc == SA2_OK && p.dq.p)
                 rc = launch(wide ? causal_f32_dq_kernel<T, 256, true, BAND> : causal_f32_dq_kernel<T, 256, false, BAND>, p, tiles * p.H, 2 * TILE * Pitch<256>::value, st);
         }

@@ -268,34 +268,33 @@ __device__ __forceinline__ void queries_gradient(const Causal& p, int id, float*
     add_up<T, DP>(lds, REGION, p.dq, s, q0, h, p.D, wide, p.scale);
 }
 
-// KEYS, VALUES: which of dK and dV a workgroup makes.  With a band, workgroups from `main` on have the first keys (Band), `blocks` of them
-// for a chunk of queries
+// KEYS, VALUES: which of dK and dV a workgroup makes.  With a band, workgroups from `main` on have the first keys (key_work), in groups of
+// `members`
 template <class T, int DP, bool WIDE, bool KEYS, bool VALUES, bool BAND>
-__device__ __forceinline__ void keys_gradients(const Causal& p, int id, float* lds, int main, int blocks, int64_t slots) {
+__device__ __forceinline__ void keys_gradients(const Causal& p, int id, float* lds, int main, int members) {
     constexpr bool wide = WIDE;
     constexpr int REGION = 2 * TILE * Pitch<DP>::value;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     float *qt = lds + wave * REGION, *dt = qt + TILE * Pitch<DP>::value, *stats = lds + WAVES * REGION + wave * 64;
     const bool sink = BAND && id >= main;
-    int stream, tile, j0 = 0;
+    int stream, tile, extra = -1;
     if (sink) {
-        j0 = (id - main) % blocks * TILE;
-        id = (id - main) / blocks;
+        extra = (id - main) % members;
+        id = (id - main) / members;
     }
     order(id, p.rows.B * p.HK, stream, tile);
     const int b = stream / p.HK, hk = stream % p.HK;
     Span s;
-    if (!find_tile(p.rows, b, tile, sink ? p.band.chunk : TILE, s)) return;
+    if (!find_tile(p.rows, b, tile, sink && !p.band.by_rows ? p.band.chunk : TILE, s)) return;
     if (s.fill) {
         if (sink) return;
         if (KEYS) zeros<T>(p.dk, s, hk, p.D);
         if (VALUES) zeros<T>(p.dv, s, hk, p.D);
         return;
     }
-    if (!sink) j0 = s.block * TILE;
     KeyWork work;
-    if (!key_work<BAND>(p, s, j0, TILE, s.block, sink ? (int)(b * (slots / p.rows.B)) + tile : -1, work)) return;
-    const int ki = j0 + (lane & 31), per = (work.hi - work.lo + TILE - 1) / TILE;
+    if (!key_work<BAND>(p, s, TILE, tile, extra, work)) return;
+    const int j0 = work.j0, ki = j0 + (lane & 31), per = (work.hi - work.lo + TILE - 1) / TILE;
     float k[DP / 2], v[DP / 2];
     own_rows<T, DP>(k, p.k, s, j0, hk, p.D, wide, 1.f);
     if constexpr (KEYS) own_rows<T, DP>(v, p.v, s, j0, hk, p.D, wide, 1.f);
@@ -358,8 +357,8 @@ __device__ __forceinline__ void keys_gradients(const Causal& p, int id, float* l
     const float* const values = lds + TILE * Pitch<DP>::value;
     if (BAND && work.sink >= 0) {
         const int left = p.band.sinks < s.len ? p.band.sinks - j0 : s.len - j0;
-        if (KEYS && p.dk.p) add_up_to<DP>(lds, REGION, sink_row(p, slots, 0, work.sink, hk, j0), left, p.D, p.scale);
-        if (VALUES && p.dv.p) add_up_to<DP>(values, REGION, sink_row(p, slots, 1, work.sink, hk, j0), left, p.D, 1.f);
+        if (KEYS && p.dk.p) add_up_to<DP>(lds, REGION, sink_row(p, 0, work.sink, hk, j0), left, p.D, p.scale);
+        if (VALUES && p.dv.p) add_up_to<DP>(values, REGION, sink_row(p, 1, work.sink, hk, j0), left, p.D, 1.f);
         return;
     }
     const int skip = BAND ? p.band.sinks - j0 : 0;
@@ -372,13 +371,13 @@ __device__ __forceinline__ void keys_gradients(const Causal& p, int id, float* l
 // APART: dK and dV from workgroups of their own, with the logits twice (five products instead of four).  At head_dim 128 always, because
 // keys, values and both sums take 256 registers and what did not fit went to memory (N 8192, 4/1 heads: 5.8 ms together, 4.7 apart);
 // below where there are CUs for both (217 rows of 4/2 heads of 64: 41 us together, 32 apart; B2 N1024 H8/8: 156 and 181).
-// `main` and `blocks`: see keys_gradients
+// `main` and `members`: see keys_gradients
 template <class T, int DP, bool WIDE, bool APART, bool BAND>
-__global__ __launch_bounds__(THREADS) void causal_f32_narrow_bwd_kernel(Causal p, int keys, int values, int main, int blocks, int64_t slots) {
+__global__ __launch_bounds__(THREADS) void causal_f32_narrow_bwd_kernel(Causal p, int keys, int values, int main, int members) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int id = blockIdx.x;
-    if (id < keys) keys_gradients<T, DP, WIDE, true, !APART, BAND>(p, id, lds, main, blocks, slots);
-    else if (APART && id < keys + values) keys_gradients<T, DP, WIDE, false, true, BAND>(p, id - keys, lds, main, blocks, slots);
+    if (id < keys) keys_gradients<T, DP, WIDE, true, !APART, BAND>(p, id, lds, main, members);
+    else if (APART && id < keys + values) keys_gradients<T, DP, WIDE, false, true, BAND>(p, id - keys, lds, main, members);
     else queries_gradient<T, DP, WIDE, BAND>(p, id - keys - values, lds);
 }
 
@@ -415,8 +414,8 @@ int narrow_backward(const Causal& p, int dtype, bool wide, hipStream_t st) {
         return for_narrow_width(p.D, [&](auto w) {
             constexpr int DP = decltype(w)::value;
             const bool any = p.dk.p || p.dv.p, sink = BAND && any && p.band.sinks > 0;
-            const int64_t slots = sink ? sink_slots(p) : 0, blocks = sink ? (p.band.sinks + TILE - 1) / TILE : 0;
-            const int64_t tiles = (int64_t)p.rows.B * count_tiles(p.rows, TILE), main = tiles * p.HK, each = main + slots * p.HK * blocks;
+            const int members = sink ? sink_members(p, TILE) : 1;
+            const int64_t tiles = (int64_t)p.rows.B * count_tiles(p.rows, TILE), main = tiles * p.HK, each = main + (sink ? sink_groups(p, TILE) * members * p.HK : 0);
             const bool apart = DP == 128 || 2 * each <= CUS;
             const int64_t keys = (apart ? p.dk.p != nullptr : any) ? each : 0, values = apart && p.dv.p ? each : 0, grid = keys + values + (p.dq.p ? tiles * p.H : 0);
             if (grid == 0) return (int)SA2_OK;
@@ -424,9 +423,9 @@ int narrow_backward(const Causal& p, int dtype, bool wide, hipStream_t st) {
             if constexpr (DP < 128)
                 if (!apart)
                     return launch(wide ? causal_f32_narrow_bwd_kernel<T, DP, true, false, BAND> : causal_f32_narrow_bwd_kernel<T, DP, false, false, BAND>, p, grid, DP, st, (int)keys, (int)values,
-                                  (int)main, (int)blocks, slots);
+                                  (int)main, members);
             return launch(wide ? causal_f32_narrow_bwd_kernel<T, DP, true, true, BAND> : causal_f32_narrow_bwd_kernel<T, DP, false, true, BAND>, p, grid, DP, st, (int)keys, (int)values, (int)main,
-                          (int)blocks, slots);
+                          members);
         });
     });
 }

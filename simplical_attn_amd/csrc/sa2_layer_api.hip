@@ -43,10 +43,13 @@ int make_band(Causal& p, int window, int sinks) {
     p.band.window = window;
     p.band.sinks = sinks < p.rows.N ? sinks : p.rows.N;
     p.band.alone = window == 1 && sinks == 0 ? 0x7fffffff : 0;
-    // (where the first keys are many, longer chunks, so that their sums stay of the tensors' size)
-    const int64_t chunk = 128 * (int64_t)(p.band.sinks > 128 ? (p.band.sinks + 127) / 128 : 1);
-    p.band.chunk = chunk < 1 << 30 ? (int)chunk : 1 << 30;
-    return p.band.sinks > 0 && (sink_slots(p) * p.HK > 0x7fffffff || p.band.sinks > 65535) ? SA2_ERR_TOO_LARGE : SA2_OK;
+    if (p.band.sinks > 65535) return SA2_ERR_TOO_LARGE;
+    // (where the first keys are many, longer chunks, so that their sums stay of the tensors' size; of many short sequences: see Band)
+    p.band.chunk = 128 * (p.band.sinks > 128 ? (p.band.sinks + 127) / 128 : 1);
+    const int64_t chunks = sink_groups(p, 0), rows = 2 * (int64_t)p.rows.B * p.rows.N;
+    p.band.by_rows = chunks * p.band.sinks > rows;         // (of a batch never: ceil(N / chunk) sinks <= N + sinks)
+    p.band.sink_rows = p.band.by_rows ? rows : chunks * p.band.sinks;
+    return SA2_OK;
 }
 size_t row_bytes(const Causal& p, int heads) { return ((size_t)p.rows.B * heads * p.rows.N * sizeof(float) + 255) / 256 * 256; }
 size_t delta_bytes(const Causal& p) { return row_bytes(p, p.H); }

@@ -19,11 +19,15 @@ struct Rows {
 
 // What queries see besides the causal mask (window 0: every key before them): the last `window` keys up to their own, and the first
 // `sinks` ones of the sequence.  Gradients of the first keys, which all queries see, are made by workgroups of their own, each with
-// `chunk` queries of a sequence (of all heads that share the keys), whose fp32 sums meet in a last launch.
+// `chunk` queries of a sequence (of all heads that share the keys), whose fp32 sums meet in a last launch.  A chunk has `sinks` rows of sums,
+// or (`by_rows`), where those of many short packed sequences would be more than twice the tensors' rows, as many as its sequence has first keys: chunk c
+// of the sequence whose rows begin at n has those from 2 n + c min(sinks, its length) on.  (chunk is sinks or more, so that 2 len rows are enough.)
 struct Band {
     int window, sinks;
     int alone;                                 // queries up to this number see their own key only
     int chunk;
+    bool by_rows;
+    int64_t sink_rows;                         // in all, of a key head
 };
 
 // One call of causal attention.  H query heads share HK heads of keys and values, G = H / HK neighbours one.
@@ -37,7 +41,7 @@ struct Causal {
     float* delta;                              // [B,H,N]  sum_d dout*(out + out_low)
     float* part;                               // partial sums (path specific)
     Band band;
-    float* sink_part;                          // [dK, dV][chunk of a sequence][HK][sinks][D]: the first keys' sums
+    float* sink_part;                          // [dK, dV][HK][sink_rows][D]: the first keys' sums
 };
 
 struct Rotary {

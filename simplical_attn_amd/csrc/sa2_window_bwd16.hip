@@ -99,17 +99,17 @@ __global__ __launch_bounds__(FACTOR_ROWS) void window_factors_kernel(Causal p, C
 
 // `queries` workgroups for dQ, then those for dK and dV
 template <class E, int D, int NQ>
-__global__ __launch_bounds__(THREADS, 1) void window_bwd16_kernel(Causal p, Causal16Terms terms, int nsplit, int queries, int heads, int main, int blocks, int64_t slots, bool padded) {
+__global__ __launch_bounds__(THREADS, 1) void window_bwd16_kernel(Causal p, Causal16Terms terms, int nsplit, int queries, int heads, int main, int members, bool padded) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     if ((int)blockIdx.x < queries) queries_gradient16<E, D, NQ, true>(p, terms, padded, blockIdx.x, lds, heads);
-    else keys_gradients16<E, D, true>(p, terms, nsplit, padded, blockIdx.x - queries, lds, main, blocks, slots);
+    else keys_gradients16<E, D, true>(p, terms, nsplit, padded, blockIdx.x - queries, lds, main, members);
 }
 // At head_dim 128 one launch after the other, and two blocks of queries per wavefront whatever their number: dQ's sums and operands beside
 // the masks and the other kernel's needs left no registers (with one block, its operands moved between the files in front of the MFMAs)
 template <class E, int D>
-__global__ __launch_bounds__(THREADS, 1) void window_dkv16_kernel(Causal p, Causal16Terms terms, int nsplit, int main, int blocks, int64_t slots, bool padded) {
+__global__ __launch_bounds__(THREADS, 1) void window_dkv16_kernel(Causal p, Causal16Terms terms, int nsplit, int main, int members, bool padded) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    keys_gradients16<E, D, true>(p, terms, nsplit, padded, blockIdx.x, lds, main, blocks, slots);
+    keys_gradients16<E, D, true>(p, terms, nsplit, padded, blockIdx.x, lds, main, members);
 }
 template <class E, int D, int NQ>
 __global__ __launch_bounds__(THREADS, 1) void window_dq16_kernel(Causal p, Causal16Terms terms, int heads, bool padded) {
@@ -123,7 +123,8 @@ int launch_of(const Causal& p, const Causal16Terms& terms, int heads, hipStream_
     const int nsplit = window16_splits(p);
     const int64_t queries = p.dq.p ? (int64_t)p.rows.B * (p.H / heads) * count_tiles(p.rows, 32 * NQ * WAVES / heads) : 0;
     const int64_t main = any ? (int64_t)p.rows.B * p.HK * nsplit * count_tiles(p.rows, BLOCK) : 0;
-    const int64_t slots = sink ? sink_slots(p) : 0, blocks = sink ? (p.band.sinks + BLOCK - 1) / BLOCK : 1, keys = main + slots * p.HK * blocks;
+    const int members = sink ? sink_members(p, BLOCK) : 1;
+    const int64_t keys = main + (sink ? sink_groups(p, BLOCK) * members * p.HK : 0);
     constexpr int LDS = BUFFERS * (Buffer<D>::BYTES + STATS), QUERY_LDS = QUERY_BUFFERS<NQ, true> * Buffer<D>::BYTES;
     static_assert(LDS >= QUERY_LDS, "");
     if (queries + keys > 0x7fffffff) return SA2_ERR_TOO_LARGE;
@@ -131,12 +132,12 @@ int launch_of(const Causal& p, const Causal16Terms& terms, int heads, hipStream_
     if constexpr (D == 64) {
         const auto kernel = window_bwd16_kernel<E, D, NQ>;
         if (!allow_full_lds((const void*)kernel)) return SA2_ERR_LAUNCH_FAILED;
-        kernel<<<dim3((unsigned)(queries + keys)), block, LDS, st>>>(p, terms, nsplit, (int)queries, heads, (int)main, (int)blocks, slots, padded);
+        kernel<<<dim3((unsigned)(queries + keys)), block, LDS, st>>>(p, terms, nsplit, (int)queries, heads, (int)main, members, padded);
     } else {
         const auto to_keys = window_dkv16_kernel<E, D>;
         const auto to_queries = window_dq16_kernel<E, D, NQ>;
         if (!allow_full_lds((const void*)to_keys) || !allow_full_lds((const void*)to_queries)) return SA2_ERR_LAUNCH_FAILED;
-        if (keys) to_keys<<<dim3((unsigned)keys), block, LDS, st>>>(p, terms, nsplit, (int)main, (int)blocks, slots, padded);
+        if (keys) to_keys<<<dim3((unsigned)keys), block, LDS, st>>>(p, terms, nsplit, (int)main, members, padded);
         if (queries) to_queries<<<dim3((unsigned)queries), block, QUERY_LDS, st>>>(p, terms, heads, padded);
     }
     if (hipGetLastError() != hipSuccess) return SA2_ERR_LAUNCH_FAILED;

@@ -246,7 +246,8 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
 
 /*
  * The same with a sliding window: query i of a sequence attends to its keys j <= i with i - j < window or j < sinks, that is, to the
- * last `window` keys up to its own (1 or more) and to the sequence's first `sinks` ones (0 to 65535; more: SA2_ERR_TOO_LARGE).
+ * last `window` keys up to its own (1 or more) and to the sequence's first `sinks` ones (0 to 65535; more, or N above 2^31 - 1024:
+ * SA2_ERR_TOO_LARGE).
  * A window of N or more is none: sa2_causal_forward and _backward run, bit for bit.
  *   sequences    of the workspace's size: 0 for a batch, else the packed sequences of the call
  * The first keys' gradients are sums of fp32 sums over chunks of queries, in their order.
@@ -302,7 +303,7 @@ int sa2_window_tree_attention(const void* q, const void* k, const void* v, const
  *   lengths      NULL: weights [B,HK,N] (packed: [HK,N], zero for rows of no sequence) are overwritten.  Else weights
  *                [sequences,HK,places], and key a of sequence b is added at place lengths[b] + a, where that is below `places`
  *   strides      q, k (3 int64 each), then weights' batch (or sequence) and head
- *   sinks        at most 65535 (or the rows): SA2_ERR_TOO_LARGE
+ *   sinks        at most 65535 (or the rows), and N at most 2^31 - 1024: SA2_ERR_TOO_LARGE
  *   workspace    sa2_key_weights_workspace_bytes(...) bytes (sequences 0: not packed), 256-byte aligned (0 bytes: may be NULL); contents on entry ignored
  * No atomics: two calls on the same inputs give identical bits.
  */

@@ -36,6 +36,8 @@ int make_causal(Causal& p, const int32_t* cu, int sequences, int B, int N, int H
     p.scale = scale;
     return SA2_OK;
 }
+// Rows that the kernels of windows and of keys' weights take: row numbers up to two blocks of 256 behind the last row fit 31 bits
+constexpr int BAND_ROWS = 0x7fffffff - 1023;
 // window 0: none
 int make_band(Causal& p, int window, int sinks) {
     if (window < 0 || sinks < 0) return SA2_ERR_BAD_WINDOW;
@@ -43,7 +45,7 @@ int make_band(Causal& p, int window, int sinks) {
     p.band.window = window;
     p.band.sinks = sinks < p.rows.N ? sinks : p.rows.N;
     p.band.alone = window == 1 && sinks == 0 ? 0x7fffffff : 0;
-    if (p.band.sinks > 65535) return SA2_ERR_TOO_LARGE;
+    if (p.rows.N > BAND_ROWS || p.band.sinks > 65535) return SA2_ERR_TOO_LARGE;
     // (where the first keys are many, longer chunks, so that their sums stay of the tensors' size; of many short sequences: see Band)
     p.band.chunk = 128 * (p.band.sinks > 128 ? (p.band.sinks + 127) / 128 : 1);
     const int64_t chunks = sink_groups(p, 0), rows = 2 * (int64_t)p.rows.B * p.rows.N;
@@ -261,6 +263,7 @@ int make_key_sums(KeySums& p, const int32_t* cu, int sequences, int B, int N, in
     int rc = make_causal(c, cu, sequences, B, N, H, HK, D, scale, dtype);
     if (rc != SA2_OK) return rc;
     if (window < 0 || sinks < 0) return SA2_ERR_BAD_WINDOW;
+    if (N > BAND_ROWS) return SA2_ERR_TOO_LARGE;
     memset(&p, 0, sizeof(p));
     p.rows = c.rows;
     p.H = H; p.HK = HK; p.G = c.G; p.D = D;

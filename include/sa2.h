@@ -250,7 +250,8 @@ int sa2_causal_backward(const void* q, const void* k, const void* v, const void*
  * SA2_ERR_TOO_LARGE).
  * A window of N or more is none: sa2_causal_forward and _backward run, bit for bit.
  *   sequences    of the workspace's size: 0 for a batch, else the packed sequences of the call
- * The first keys' gradients are sums of fp32 sums over chunks of queries, in their order.
+ * The first keys' gradients are sums of fp32 sums over chunks of queries, in their order, for which the workspace has at most two rows for
+ * each row of dK and of dV.
  */
 int sa2_window_forward(const void* q, const void* k, const void* v, void* out, void* out_low, float* lse,
                        const int32_t* cu_seqlens, int sequences, int B, int N, int H, int HK, int D,
@@ -320,8 +321,9 @@ int sa2_key_weights(const void* q, const void* k, const float* lse, float* weigh
  *   left         [B,heads,places] contiguous: the weights of the rows that stay, at their new places, zeros behind
  *   kept         [B,heads,keep] contiguous: the places that the rows had, ascending, -1 behind them
  *   strides      k_cache, v_cache (page, row, head), then weights' batch and head
- * No two sequences share a page, and no memory is both cache's.  Rows in pages that are not in 0 .. pages-1 are chosen like others; what would come from or go there is left out.  What the places
- * from keep on hold is as it was.
+ * No two sequences share a page, and no element of memory is in both caches or twice in one (the Python operator refuses such tensors).  Rows in
+ * pages that are not in 0 .. pages-1 are chosen like others; what would come from or go there is left out.  What the places from keep on hold
+ * is as it was.
  */
 int sa2_cache_evict(void* k_cache, void* v_cache, const float* weights, float* left, int32_t* kept, const int32_t* lengths, const int32_t* page_table,
                     int B, int HK, int heads, int D, int page_size, int pages, int table_width, int64_t places, int keep, int first, int recent,

@@ -1,4 +1,4 @@
-// Causal attention, gradient of the queries, bf16 and fp16 on the 16-bit MFMA (row terms: sa2_causal_dkv16.hip).
+// Causal attention, gradient of the queries, bf16 and fp16 on the 16-bit MFMA (row terms: sa2_causal_dkv16.h).
 //
 //   P = e^(scale q k - lse), dP = dO V^T, dS = P (dP - delta), dQ_i = scale sum_j dS_ij k_j
 //
@@ -174,7 +174,7 @@ __device__ __forceinline__ void queries_gradient16(const Causal& p, const Causal
         static_for<2 * DT>([&](auto J) __attribute__((always_inline)) { second_mfma(N, J, x); });
         rest();
     };
-    // dS of a unit, and what its rounding left (for the pieces of the own tile: see sa2_causal_dkv16.hip); masked: the lane's query sees the piece's keys 0 .. seen, with a band those
+    // dS of a unit, and what its rounding left (for the pieces of the own tile: see sa2_causal_dkv16.h); masked: the lane's query sees the piece's keys 0 .. seen, with a band those
     // whose bits are set
     auto weigh = [&](const floatx16& x, const floatx16& y, int n, X8 (&z)[2], X8 (&rest)[2], auto masked, int seen) {
         union { uint32_t u[8]; X8 v[2]; } o, low;

@@ -8,7 +8,7 @@
 // query l % 32 and the keys 8g + 4(l/32) + r in register 4g + r, so that softmax is arithmetic within a lane and one exchange
 // of halves, and these registers are, as they are, the second operand of the next product.
 // Here: the kernels for a head_dim above 128, whose accumulators leave no room for a wavefront to have tiles of its own (four share
-// each tile and have 32 rows apiece); the row terms; the choice.  Up to 128: sa2_causal_f32_narrow.hip.
+// each tile and have 32 rows apiece); the row terms; the choice.  Up to 128: sa2_causal_f32_narrow.h.
 // Bound by the matrix pipe: an MFMA takes 64 cycles, for which one LDS read of 4 or 16 bytes per lane is enough.  N4096 H8/2, forward and
 // backward: head_dim 256 bf16 2.3 and 15.4 ms, fp32 3.3 and 19.5; 192 (on 256 columns) as long.
 #pragma once

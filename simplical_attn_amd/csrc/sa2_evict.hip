@@ -1,9 +1,9 @@
 // Eviction from a cache: of each sequence's rows the first ones, the latest ones and those that gathered most weight stay, in their order.
 //
-// Which ones: a workgroup per sequence and head finds the smallest weight that stays digit by digit (11, 11 and 10 bits of the weights
-// as ordered integers, counted in LDS), then numbers the rows that stay, of equal ones the first.  Bound by a CU's vector ALU, which
-// has four readings of the weights: 65536 of them take 50 us, 2000 10 (the unrolled form that keeps them in registers is fetched cold: 31).  Moving them: see
-// move_kernel.
+// Which ones: up to four workgroups per sequence and head find the smallest weight that stays digit by digit (11, 11 and 10 bits of the weights
+// as ordered integers, counted in LDS), each for itself, then number a part of the rows that stay, of equal ones the first.  Bound by a CU's vector
+// ALU, which has all weights three times and its part once more: 65536 of them take 50 us with four workgroups (56 where they come from memory) and 64
+// with one, 2000 10 with one (the unrolled form that keeps them in registers is fetched cold: 31).  Moving them: see move_kernel.
 #include "sa2_layer_common.h"
 
 namespace sa2 {
@@ -188,8 +188,9 @@ __global__ __launch_bounds__(THREADS) void choose_kernel(Evict p, int parts) {
 // Rows to their new places.  A workgroup has `SLICE` pieces of every row of one tensor of a sequence's head and takes the rows in steps.  What
 // the rows of a step lie behind is not written before them (kept[i] >= i), so that reads may run ahead of writes, never behind: each step's
 // rows are asked for a step early, their pages two and their numbers three, and a step's writes begin when all of its reads have ended.
-// 16384 rows of 256 bytes of 16 heads: 88 us (3.0 TB/s read and written) by 256 workgroups with two pieces, 98 by 128 with four; 1024 rows of 32
-// heads: 10 us with four pieces, 15 with two.  One step at a time, without the reads ahead, 380 and 26.
+// 16384 rows of 256 bytes of 16 heads: 104 us (2.6 TB/s read and written) by 256 workgroups with two pieces, and where the call before left these
+// rows in the card's last cache 88, by 128 workgroups with four pieces 98; 1024 rows of 32 heads: 10 us with four pieces, 15 with two.  One step at a
+// time, without the reads ahead, 380 and 26.
 typedef uint32_t Quad __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint32_t word(Quad x) { return x.x; }
 __device__ __forceinline__ uint32_t word(uint32_t x) { return x; }

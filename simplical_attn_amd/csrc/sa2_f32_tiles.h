@@ -125,9 +125,10 @@ __device__ __forceinline__ void weighted_rows(const float* lds, int first, const
         }
 }
 // The same where a flag for the whole tile says whether it holds an infinity or NaN (odd_values of what went into it) and `seen` is what the
-// lane's own row sees of it, bit by bit.  Such a tile is added up one row at a time on the vector ALU.  (The check and the branch for
-// each row of weighted_rows, unrolled, are 27000 instructions at head_dim 256, and held so many registers beside a window's masks that
-// the kernels went wrong.)
+// lane's own row sees of it, bit by bit.  Such a tile is added up one row at a time on the vector ALU.  (weighted_rows, with a check and a branch for
+// each row, unrolled, makes kernels of 24000 instructions at head_dim 256, beyond the reach of a short branch, this one 7600.  A form of the
+// banded kernels with it gave wrong dK for some keys at head_dim 136, fp32, and was given up; why is not known.  In the listing of such a form long
+// branches, spilled registers and the waits behind MFMAs are in order.)
 __device__ __forceinline__ uint32_t odd_values(float4 x) {
     uint32_t bits = 0;
     for (const float y : {x.x, x.y, x.z, x.w}) bits |= (__float_as_uint(y) & 0x7f800000u) + 0x00800000u;

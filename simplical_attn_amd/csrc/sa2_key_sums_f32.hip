@@ -4,8 +4,9 @@
 //   w_j = sum over heads g and queries i that see j of e^(scale q_gi k_j - lse_gi)
 //
 // A wavefront owns 32 keys, whose products with a tile of 32 queries in LDS leave a lane one key and 16 queries: its sum is arithmetic
-// within the lane.  Bound by the matrix pipe (64 cycles for two columns of 32 x 32 products): 4096 queries of 16 heads over
-// 4 key heads, head_dim 128: 462 us, 74 TFLOP/s of 154.  Short prompts by the start of workgroups and the second launch (217 queries, 4 heads: 11.6 us).
+// within the lane.  4096 queries of 16 heads over 4 key heads, head_dim 128: 460 us, 75 TFLOP/s of the 154 that a large product reaches.  An MFMA
+// has the matrix pipe for 64 cycles (two columns of 32 x 32 products); a tile's chain of them, its exponentials and masks, and the two barriers
+// around the next tile's way to LDS stand one after the other, which only other wavefronts fill.  Short prompts are bound by the start of workgroups and the second launch (217 queries, 4 heads: 11.6 us).
 #include "sa2_f32_tiles.h"
 #include "sa2_key_sums.h"
 

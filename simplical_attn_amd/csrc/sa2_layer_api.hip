@@ -162,7 +162,7 @@ int prompt_backward(const void* q, const void* k, const void* v, const void* out
 }
 
 // Tiles of 32 scores that a row of query leaves at most, its own node's among them
-int64_t tree_span(int T, int page_size, int table_width, int window, int sinks) {
+int64_t tree_span(int page_size, int table_width, int window, int sinks) {
     const int64_t all = ((int64_t)page_size * table_width + 31) / 32, seen = ((int64_t)window + sinks) / 32 + 4;
     return 32 * ((window && seen < all ? seen : all) + 1);
 }
@@ -175,7 +175,7 @@ size_t tree_workspace(int B, int T, int H, int HK, int D, int page_size, int tab
     window = tree_window_of(T, page_size, table_width, window);
     const int nsplit = tree_splits(B, T, H, HK, D, page_size, table_width, window, sinks, dtype);
     if (!weighted) return tree_part_bytes(B, T, H, D, nsplit);
-    return tree_parts(B, T, H, D, nsplit, true) + (size_t)B * H * tree_span(T, page_size, table_width, window, sinks) * sizeof(float);
+    return tree_parts(B, T, H, D, nsplit, true) + (size_t)B * H * tree_span(page_size, table_width, window, sinks) * sizeof(float);
 }
 
 // window 0: none; weights: wanted or nullptr, with their strides behind those of the tensors
@@ -219,7 +219,7 @@ int tree_attention(const void* q, const void* k, const void* v, const void* k_ca
         p.weights_sh = strides[19];
         if ((B > 1 && p.weights_sb < 1) || (HK > 1 && p.weights_sh < 1)) return SA2_ERR_BAD_STRIDE;
         p.scores = (float*)((char*)workspace + tree_parts(B, T, H, D, p.nsplit, true));
-        p.span = tree_span(T, page_size, table_width, window, sinks);
+        p.span = tree_span(page_size, table_width, window, sinks);
         if ((int64_t)B * HK * ((p.span + 1023) / 1024) > 0x7fffffff) return SA2_ERR_TOO_LARGE;
     }
     const bool narrow = !(flags & SA2_FLAG_FORCE_GENERIC) && (banded ? tree16_layout(p, dtype) : tree16_supported(p, dtype));

@@ -162,7 +162,7 @@ int launch_causal16_fwd(const Causal& p, int dtype, hipStream_t st);
 int launch_window16_fwd(const Causal& p, int dtype, hipStream_t st);
 // Their backward.  Row terms: p.delta receives -delta; fp16: the Euclidean norms of rows bound dS
 struct Causal16Terms {
-    float* minus_lse;                          // [B,H,N]  -lse / scale; fp16: what weights are lifted by added (sa2_causal_dkv16.hip)
+    float* minus_lse;                          // [B,H,N]  -lse / scale; fp16: what weights are lifted by added (sa2_causal_dkv16.h)
     float* dout;                               // [B,H,N]  |dout|, fp16 only
     float* v;                                  // [B,HK,N] |v|, fp16 only
     float *queries, *keys;                     // [B,H,N], [B,HK,N]: the factors of rows of dQ and of keys (sa2_causal16.h), fp16 with a band only

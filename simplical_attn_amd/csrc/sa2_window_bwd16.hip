@@ -3,9 +3,11 @@
 //
 // The keys behind the first ones are seen by the queries of their windows, a stream of (window + 127) rows per head and block of 128; the
 // first keys by all queries, in chunks of these whose fp32 sums meet in a last launch.
-// 16 heads over 4 key heads, 8192 queries, head_dim 128, bf16, window 512 with 4 first keys: dQ 145 us, dK and dV 135 (0.24 and 0.51 PFLOP/s of the
+// 16 heads over 4 key heads, 8192 queries, head_dim 128, bf16, window 512 with 4 first keys: dQ 145 us, dK and dV 135 (0.35 and 0.50 PFLOP/s of the
 // three and four products that each forms), row terms 20 (memory), the first keys' sums 12.  Ten tiles per workgroup, so that starts and ends weigh as
-// much as the sweep.  8 heads, batch 2, 2048 queries, head_dim 64, window 512: 42 us in one launch, one workgroup per CU.
+// much as the sweep.  8 heads, batch 2, 2048 queries, head_dim 64, window 512: 42 us in one launch of 512 workgroups, half of them for dQ, of which a
+// CU has one at a time: two rounds of such chains.  fp16: 46 us more than bf16 in the first case (all gradients 340 us and 294), factors and row terms;
+// with many first keys the factors cost more, since every row goes through all of these.
 #include "sa2_causal_dkv16.h"
 
 namespace sa2 {

@@ -6,7 +6,7 @@
 // 32 NQ queries; where heads share keys, they are the same queries of two or four of these heads, so that all wavefronts need the same
 // tiles: with the blocks of one head one behind the other, as without a window, a workgroup of 256 queries fetches 768 keys for a window
 // of 512 of which a wavefront needs 576.
-// 16 heads over 4 key heads, 8192 queries, head_dim 128, bf16, window 512 with 4 first keys: 105 us (0.33 PFLOP/s); 8 heads over 2, 32768 queries,
+// 16 heads over 4 key heads, 8192 queries, head_dim 128, bf16, window 512 with 4 first keys: 105 us (0.32 PFLOP/s); 8 heads over 2, 32768 queries,
 // window 4096, fp16: 540 us (0.96, 78 % of a large product's rate).  A tile of 64 keys takes 1.35 us, a workgroup's start and end 17: first
 // loads, queries to accumulation registers, masks, the join of the first keys, the output.
 #include "sa2_sweep16.h"

@@ -95,7 +95,7 @@ def causal_attention(q, k, v, cu_seqlens=None, scale=None, flags=_lib.FLAG_AUTO,
     flags    _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products whatever the type, gradients too
     window   None, or at least 1: query i attends to key j where i - j < window (its own key among them; the windows [i - w, i] of
              the 2-simplicial operator have one key more), or
-    sinks    where j < sinks: the sequence's first keys stay visible to all of its queries
+    sinks    where j < sinks: the sequence's first keys stay visible to all of its queries; at most 65535, or as many as there are rows
 
     Returns a tensor like q, zero in rows of no sequence.  bf16 and fp16 with a head_dim up to 128 that is a multiple of 8 and rows on
     the 16-byte grid run on the 16-bit matrix pipes (softmax weights rounded to the type, sums in fp32), everything else
@@ -141,7 +141,8 @@ def tree_attention(q, k, v, parents, k_cache, v_cache, lengths, page_table=None,
                       stands.  Rows out of the window are not read
     weights           float32 [batch, key heads, places], at least a place for each row that the cache may hold; single tokens only.
                       The softmax weight of each cached row, summed over the query heads that share its head, is added at the row's
-                      place, the token's own at place ``lengths`` (where cache_append will put it): what cache_evict goes by
+                      place, the token's own at place ``lengths`` (where cache_append will put it): what cache_evict goes by.  No two
+                      places share memory
 
     No gradients.  Returns a tensor like q.  bf16 and fp16 with a head_dim up to 128 that is a multiple of 8 and rows on the 16-byte
     grid run on the 16-bit matrix pipes (softmax weights rounded to the type, sums in fp32), everything else with fp32 products."""
@@ -154,7 +155,8 @@ def key_weights(q, k, lse, cu_seqlens=None, scale=None, window=None, sinks=0, we
 
     q, k, lse        of causal_attention_forward, with its cu_seqlens, scale, window and sinks
     weights, lengths given: the sums are added to weights (float32 [batch, key heads, places], in place), key a of a sequence at place
-                     lengths + a, as cache_append puts its row there; keys whose place lies beyond are left out.  Returns None then
+                     lengths + a, as cache_append puts its row there; keys whose place lies beyond are left out.  Returns None then.
+                     No two places share memory
     flags            _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products whatever the type
 
     No gradients.  Deterministic.  Sums and weights are float32 throughout."""

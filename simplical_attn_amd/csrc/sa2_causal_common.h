@@ -154,6 +154,9 @@ inline int64_t sink_groups(const Causal& p, int rows) { return (int64_t)p.rows.B
 inline int window_heads(const Causal& p) { return p.G % 4 == 0 ? 4 : p.G % 2 == 0 ? 2 : 1; }
 inline bool window_two(const Causal& p, int heads) { return (int64_t)p.rows.B * (p.H / heads) * count_tiles(p.rows, 256 / heads) >= 2 * CUS; }
 
+// Whether the exponent x c - at c of a score near the reference point `at` is not to be had from at c, whose rounding, half a unit of 2^-24 of it, is more
+// than half a power of two: x - at comes first then
+__device__ __forceinline__ bool far_from_zero(float at, float c) { return fabsf(at) * c > 16777216.f; }
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 }  // namespace

@@ -10,8 +10,8 @@
 // The weights are e^(s - m) with m the row's maximum over its first 32 keys: no maximum and no scaling of the output in the
 // sweep.  Rounding weights to bf16 costs half a step of each, whatever m, to fp16 half a step or 2^-25, which is why there m is lower than
 // that (lowered_by).  A unit whose sum passes RefLimit, or first keys whose scores
-// are all minus infinity, have the workgroup sweep its keys a second time, with the running maximum; in bf16, whose values reach the end
-// of fp32's range, an output that is no number does so too once weights are above 1.
+// are all minus infinity, or so far from zero that s c - m c is not to be had from a rounded m c, have the workgroup sweep its keys a second time,
+// with the running maximum; in bf16, whose values reach the end of fp32's range, an output that is no number does so too once weights are above 1.
 // K and V come by direct global->LDS loads into three buffers of 64 keys, so that one barrier per 64 keys is enough.
 #pragma once
 
@@ -250,8 +250,12 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
                     m[n] = m[n] == -INFINITY ? top : m[n];                 // (nothing has been added up in its units)
                 }
             }
-            const float at = m[n] == -INFINITY ? 0.f : m[n];
-            float sum;
+            float at = m[n] == -INFINITY ? 0.f : m[n], sum;
+            if (safe && __any(far_from_zero(at, c))) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) st[n][r] -= at;
+                at = 0.f;
+            }
             if (__all(seen == ~0u)) weights(st[n], at, sum, w[n], std::false_type{}, 0);
             else weights(st[n], at, sum, w[n], std::true_type{}, seen);
             if (!safe) worst = fmaxf(worst, sum);
@@ -266,6 +270,13 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
     constexpr int LOOK = NQ == 1 ? 2 : 1;                                  // tiles ahead that a round of steps reads keys of
     const std::false_type whole{};
     const std::true_type some{};
+    // after the first pass: a row's reference point is too far from zero for it
+    auto far = [&]() {
+        bool any = false;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) any = any || (is_finite(m[n]) && far_from_zero(m[n], c));
+        return any;
+    };
     // SLIDING: the tiles of src.a .. src.b - 1 go through the pipeline to the last, with masks where some row does not see all of
     // a tile or the next; then the first keys' tiles, piece by piece.  Tile `t` is worked on when the one LOOK behind it is there (what
     // the steps read ahead of a wavefront's last tile is not used).  Rows' reference points come from the first of these tiles, the one
@@ -399,7 +410,7 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
                 const float4 o = L::template get_regs<O0 + 4 * decltype(X)::value>();
                 poison = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, fmaf(o.w, 0.f, poison))));
             });
-            if (pass != 0 || !__syncthreads_or(worst > RefLimit<E>::value || poison != 0.f)) break;
+            if (pass != 0 || !__syncthreads_or(worst > RefLimit<E>::value || poison != 0.f || far())) break;
         } else {
             int done = 0;                                                      // pieces of 32 keys
             uint32_t here = base;
@@ -467,7 +478,7 @@ __device__ __forceinline__ void sweep16(const SRC& src, uint32_t base, float c, 
                 for (int sub = t == done / 2 ? done % 2 : 0; sub < 2; ++sub)
                     if (2 * t + sub < src.pieces) piece(here, sub, 2 * t + sub, pass != 0);
             }
-            bool again = worst > RefLimit<E>::value;
+            bool again = worst > RefLimit<E>::value || (pass == 0 && far());
             if constexpr (E::DTYPE == SA2_BF16) {
                 // (with smaller weights a second sweep would come no further; fp16 values times weights up to the limit are far from fp32's end)
                 if (pass == 0 && __any(worst > OUTPUT_CHECK)) {

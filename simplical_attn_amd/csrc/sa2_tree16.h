@@ -210,7 +210,13 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
             }
             union { uint32_t u[8]; X8 v[2]; } w;
             // (fp16: weights of up to 2^15 instead of 1, in all shares alike, so that many far below the largest are not lost)
-            const float off = fmaf(-ref, c, E::DTYPE == SA2_F16 ? 15.f : 0.f);
+            constexpr float lift = E::DTYPE == SA2_F16 ? 15.f : 0.f;
+            float off = fmaf(-ref, c, lift);
+            if (__any(far_from_zero(ref, c))) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[n][i] -= ref;
+                off = lift;
+            }
             float part[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {

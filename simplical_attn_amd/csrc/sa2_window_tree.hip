@@ -33,9 +33,9 @@ __global__ __launch_bounds__(256) void tree_weights_kernel(Tree p, float lift, b
         const float top = wave_max(s.top), f = s.sum == 0.f ? 0.f : s.top == -INFINITY ? 1.f : exp2f((s.top - top) * c), total = wave_sum(f * s.sum);
         if (total == 0.f || number > rows) continue;
         const float4 x = *(const float4*)(p.scores + (stream * p.G + r) * p.span + number);
-        const float over = 1.f / total, off = lift - (top == -INFINITY ? 0.f : top * c);
+        const float over = 1.f / total, from = top == -INFINITY ? 0.f : top;
         // (hidden rows and those that are not there have -infinity)
-        auto weight = [&](float y) { return y == -INFINITY ? 0.f : exp2f(fmaf(y, c, off)) * over; };
+        auto weight = [&](float y) { return y == -INFINITY ? 0.f : exp2f(fmaf(y - from, c, lift)) * over; };
         sum.x += weight(x.x); sum.y += weight(x.y); sum.z += weight(x.z); sum.w += weight(x.w);
     }
     if (number > rows) return;

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
     // lane that found its row.
     const int chunk = T::dma_chunk(lane), sub = T::dma_row(lane);
     const bool pad = chunk * 8 >= p.D, together = p.D == D && (!p.cache.table || page_size % T::RPW == 0);
-    auto request = [&](int t, uint32_t to) {
+    auto request = [&](int t, uint32_t to) __attribute__((always_inline)) {
         const bool drafted = t >= cached;
         const int first = drafted ? (t - cached) * 32 : cache.row(t), r = first + (lane & 31);
         const Tensor &K = drafted ? p.k : p.cache.k, &V = drafted ? p.v : p.cache.v;
@@ -106,8 +106,11 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
     };
     int t = lo + wave;
     uint32_t there[2] = {0, 0};
-    if (t < hi) there[0] = request(t, mine);
-    if (t + WAVES < hi) there[1] = request(t + WAVES, mine + STAGE);
+    auto begin = [&]() __attribute__((always_inline)) {
+        if (t < hi) there[0] = request(t, mine);
+        if (t + WAVES < hi) there[1] = request(t + WAVES, mine + STAGE);
+    };
+    begin();
 
     // what the lane's rows are and see
     uint64_t ancestors = tree_ancestors(p, b);
@@ -141,17 +144,22 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
         for (int kk = 0; kk < KK; ++kk) stays(q[n][kk]);                   // (their wait is here and not in the sweep)
     floatx16 o[NQ][DT];
     float m[NQ], l[NQ];
+    bool look[NQ] = {};                                                    // some row's m is far from zero (the same in all lanes)
+    auto nothing_yet = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        m[n] = -INFINITY;
-        l[n] = 0.f;
+        for (int n = 0; n < NQ; ++n) {
+            m[n] = -INFINITY;
+            l[n] = 0.f;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[n][d][i] = 0.f;
-    }
+                for (int i = 0; i < 16; ++i) o[n][d][i] = 0.f;
+        }
+    };
+    nothing_yet();
     const uint32_t row_lane = T::row_lane(lane), column_lane = T::column_lane(lane);
-    auto tile = [&](uint32_t at, bool drafted, int first, uint32_t here, int number) {
+    // FAR: scores less their reference point come first (far_from_zero): 0 never, 1 always, 2 where one is far from zero
+    auto tile = [&](uint32_t at, bool drafted, int first, uint32_t here, int number, auto FAR) __attribute__((always_inline)) {
         X8 kf[KK], vf[2][DT];
         uint32_t ka = at + row_lane, va = at + T::BYTES + column_lane;
         stays(ka);
@@ -207,12 +215,13 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[n][d][i] *= f;
                 m[n] = m2;
+                if (decltype(FAR)::value == 2) look[n] = __any(far_from_zero(ref, c));
             }
             union { uint32_t u[8]; X8 v[2]; } w;
             // (fp16: weights of up to 2^15 instead of 1, in all shares alike, so that many far below the largest are not lost)
             constexpr float lift = E::DTYPE == SA2_F16 ? 15.f : 0.f;
             float off = fmaf(-ref, c, lift);
-            if (__any(far_from_zero(ref, c))) {
+            if (decltype(FAR)::value == 1 || (decltype(FAR)::value == 2 && look[n])) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[n][i] -= ref;
                 off = lift;
@@ -264,15 +273,34 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
             }
         }
     };
-    for (int s = 0; t < hi; t += WAVES, s ^= 1) {
-        if (t + WAVES < hi) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * T::NGROUP) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        tile(mine + s * STAGE, t >= cached, t >= cached ? (t - cached) * 32 : BAND ? cache.row(t) : 0, s ? there[1] : there[0], t);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (t + 2 * WAVES < hi) {
-            const uint32_t next = request(t + 2 * WAVES, mine + s * STAGE);
-            if (s) there[1] = next;
-            else there[0] = next;
+    auto sweep = [&](auto FAR) __attribute__((always_inline)) {
+        for (int s = 0; t < hi; t += WAVES, s ^= 1) {
+            if (t + WAVES < hi) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * T::NGROUP) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            tile(mine + s * STAGE, t >= cached, t >= cached ? (t - cached) * 32 : BAND ? cache.row(t) : 0, s ? there[1] : there[0], t, FAR);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (t + 2 * WAVES < hi) {
+                const uint32_t next = request(t + 2 * WAVES, mine + s * STAGE);
+                if (s) there[1] = next;
+                else there[0] = next;
+            }
+        }
+    };
+    // A wavefront with a row so far from zero that its weights are not to be had the short way sweeps its tiles again: a look in every tile takes
+    // 1.6 % of a call (16 x 16384 rows, 108 us).  Two blocks of 128 columns look all the same (48 rows over 8 x 2048: 25.9 -> 26.4 us), because a second
+    // sweep's code takes registers that they lack (27.4).
+    if constexpr (D * NQ > 128) {
+        sweep(std::integral_constant<int, 2>{});
+    } else {
+        sweep(std::integral_constant<int, 0>{});
+        bool far = false;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) far = far || (is_finite(m[n]) && far_from_zero(m[n], c));
+        if (__any(far)) {
+            t = lo + wave;
+            begin();
+            nothing_yet();
+            sweep(std::integral_constant<int, 1>{});
         }
     }
 

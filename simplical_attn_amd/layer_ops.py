@@ -159,7 +159,7 @@ def key_weights(q, k, lse, cu_seqlens=None, scale=None, window=None, sinks=0, we
                      No two places share memory
     flags            _lib.FLAG_FORCE_GENERIC runs the kernels with fp32 products whatever the type
 
-    No gradients.  Deterministic.  Sums and weights are float32 throughout."""
+    No gradients.  Deterministic.  Sums and weights are float32 throughout; scores are to stay within some 10^7, where lse's 24 bits end."""
     return _lib.host().key_weights(q, k, lse, cu_seqlens, scale, window, sinks, weights, lengths, int(flags))
 
 

@@ -71,7 +71,7 @@ def test_prompts(B, N, D, window, sinks, dtype, size):
 
 
 @pytest.mark.parametrize("window,sinks", [(None, 0), (20, 2), (90, 2)])
-@pytest.mark.parametrize("T,H", [(1, 4), (5, 4), (40, 4), (1, 70)])
+@pytest.mark.parametrize("T,H", [(1, 4), (5, 4), (12, 4), (40, 4), (1, 70)])
 @pytest.mark.parametrize("dtype,D", [(BF16, 64), (FP16, 128), (FP32, 64), (BF16, 136)])
 @pytest.mark.parametrize("size", [0, 1])
 def test_trees(T, H, dtype, D, window, sinks, size):

@@ -109,7 +109,7 @@ __device__ __forceinline__ bool band_full(const Band& b, int i0, int i1, int j0,
 // Keys j0 .. j0+rows-1 of a workgroup and the queries lo .. hi-1 that it takes for them: with a band, those of the window of keys behind the
 // first ones (`extra` < 0), or a chunk of the sequence for the first keys.  The workgroups of these come in groups, of which `extra` is the
 // number in the group: a group has a chunk (`s` is the `tile`-th of them), its members a block of the first keys each; or (by_rows) a group
-// of two a block of `rows` rows, of which a sequence has half as many at least as pairs of a chunk and a block of first keys.
+// of two a block of `rows` rows, and its members two of the sequence's pairs of a chunk and a block of first keys (which are never more than that).
 // false: none, or nothing that it has to leave
 struct KeyWork {
     int j0, lo, hi;

@@ -145,6 +145,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
     floatx16 o[NQ][DT];
     float m[NQ], l[NQ];
     bool look[NQ] = {};                                                    // some row's m is far from zero (the same in all lanes)
+    float farthest = 0.f;                                                  // of the reference points that the lane's rows have had
     auto nothing_yet = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -216,6 +217,7 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
                     for (int i = 0; i < 16; ++i) o[n][d][i] *= f;
                 m[n] = m2;
                 if (decltype(FAR)::value == 2) look[n] = __any(far_from_zero(ref, c));
+                if (decltype(FAR)::value == 0) farthest = fmaxf(farthest, fabsf(ref));
             }
             union { uint32_t u[8]; X8 v[2]; } w;
             // (fp16: weights of up to 2^15 instead of 1, in all shares alike, so that many far below the largest are not lost)
@@ -286,17 +288,14 @@ __global__ __launch_bounds__(THREADS, 1) void tree16_kernel(Tree p, int blocks) 
             }
         }
     };
-    // A wavefront with a row so far from zero that its weights are not to be had the short way sweeps its tiles again: a look in every tile takes
+    // A wavefront with a row that was so far from zero that its weights are not to be had the short way sweeps its tiles again: a look in every tile takes
     // 1.6 % of a call (16 x 16384 rows, 108 us).  Two blocks of 128 columns look all the same (48 rows over 8 x 2048: 25.9 -> 26.4 us), because a second
     // sweep's code takes registers that they lack (27.4).
     if constexpr (D * NQ > 128) {
         sweep(std::integral_constant<int, 2>{});
     } else {
         sweep(std::integral_constant<int, 0>{});
-        bool far = false;
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) far = far || (is_finite(m[n]) && far_from_zero(m[n], c));
-        if (__any(far)) {
+        if (__any(far_from_zero(farthest, c))) {
             t = lo + wave;
             begin();
             nothing_yet();

@@ -70,7 +70,7 @@ def test_prompts(B, N, D, window, sinks, dtype, size):
             _check(out[i, :, h], lse[i, h], q[i, :, h], k[i, :, 0], v[i, :, 0], visible, D ** -0.5, dtype, dtype != FP32 and D <= 128)
 
 
-@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 2), (90, 2)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 2), (90, 2), (1400, 2), (300, 100)])
 @pytest.mark.parametrize("T,H", [(1, 4), (5, 4), (12, 4), (40, 4), (1, 70)])
 @pytest.mark.parametrize("dtype,D", [(BF16, 64), (FP16, 128), (FP32, 64), (BF16, 136)])
 @pytest.mark.parametrize("size", [0, 1])
@@ -86,6 +86,8 @@ def test_trees(T, H, dtype, D, window, sinks, size):
     kc[0, ..., 0] = -b                                      # the first sequence has only low rows, the second such ones at its end
     kc[1, 1250:] = 0.0
     kc[1, 1250:, :, 0] = -b
+    kc[1, 300:700] = 0.0                                    # (and in tiles before and behind others)
+    kc[1, 300:700, :, 0] = -b
     weights = torch.zeros(2, 1, rows, device=DEV) if T == 1 else None
     out = sa.tree_attention(q, k, v, None, kc, vc, torch.tensor(held, dtype=torch.int32, device=DEV), window=window, sinks=sinks, weights=weights)
     for i, n in enumerate(held):
